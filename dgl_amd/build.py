@@ -19,6 +19,7 @@ FLAGS = [
     "-fno-fast-math",
     "-fhip-fp32-correctly-rounded-divide-sqrt",
     "-fvisibility=hidden", "-Wall", "-Wno-unused-function",
+    "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",   # no v_pk_*_f32: two scalar operations instead, the same bits
     "-x", "hip",
 ]
 
@@ -38,8 +39,8 @@ def build_peaks(force: bool = False) -> str:
     if not force and os.path.exists(PEAKS_LIB) and os.path.getmtime(PEAKS_LIB) >= os.path.getmtime(PEAKS_SRC):
         return PEAKS_LIB
     os.makedirs(os.path.dirname(PEAKS_LIB), exist_ok=True)
-    cmd = [hipcc(), "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", "-x", "hip",
-           PEAKS_SRC, "-o", PEAKS_LIB]
+    cmd = [hipcc(), "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
+           "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops", "-x", "hip", PEAKS_SRC, "-o", PEAKS_LIB]
     res = subprocess.run(cmd, capture_output=True, text=True)
     if res.returncode != 0:
         sys.stderr.write(res.stdout + res.stderr)
