@@ -20,6 +20,8 @@ PROBLEM_TSP = 0
 PROBLEM_CVRP = 1
 ARITH_SPLIT_F16 = 0    # f16 split-operand matrix cores, f32 accumulate (default)
 ARITH_F32 = 1          # f32-input matrix instructions (bitwise FMA chains)
+DTYPE_F32, DTYPE_F16, DTYPE_BF16 = 0, 1, 2
+ATTENTION_MAX_LENGTH = 1 << 24   # DGL_ATTENTION_MAX_LENGTH
 
 
 class TspState(Structure):
@@ -52,6 +54,21 @@ class PolicyIO(Structure):
                 ("tile", c_void_p), ("idx_last", c_void_p), ("idx_depot", c_void_p), ("infeasible", c_void_p),
                 ("logits_out", c_void_p), ("prob_out", c_void_p), ("selected_out", c_void_p),
                 ("overflow_out", c_void_p)]
+
+
+class Attention(Structure):
+    _fields_ = [("dtype", c_int32), ("B", c_int32), ("Hq", c_int32), ("Hkv", c_int32), ("Lq", c_int32), ("Lk", c_int32),
+                ("D", c_int32), ("causal", c_int32), ("scale", c_float), ("cap", c_float),
+                ("q_stride", c_int64 * 3), ("k_stride", c_int64 * 3), ("v_stride", c_int64 * 3), ("o_stride", c_int64 * 3),
+                ("q", c_void_p), ("k", c_void_p), ("v", c_void_p), ("out", c_void_p), ("lse", c_void_p),
+                ("slope", c_void_p), ("pos_q", c_void_p), ("pos_k", c_void_p), ("pos_q_stride", c_int64),
+                ("pos_k_stride", c_int64), ("doc_q", c_void_p), ("doc_k", c_void_p), ("doc_q_stride", c_int64),
+                ("doc_k_stride", c_int64), ("prefix", c_void_p)]
+
+
+class AttentionGrad(Structure):
+    _fields_ = [("dout", c_void_p), ("dq", c_void_p), ("dk", c_void_p), ("dv", c_void_p), ("dout_stride", c_int64 * 3),
+                ("dq_stride", c_int64 * 3), ("dk_stride", c_int64 * 3), ("dv_stride", c_int64 * 3), ("dslope", c_void_p)]
 
 
 # name -> (restype, argtypes); every symbol include/dgl_amd.h declares
@@ -99,6 +116,9 @@ SIGNATURES = {
                                    c_void_p]),
     "dgl_beam_advance_compact": (c_int32, [POINTER(PolicyIO), c_void_p, c_void_p, c_int32, c_int32, c_int32,
                                            c_int32, c_void_p, c_void_p, c_void_p]),
+    "dgl_attention_forward": (c_int32, [POINTER(Attention), c_void_p]),
+    "dgl_attention_backward": (c_int32, [POINTER(Attention), POINTER(AttentionGrad), c_void_p, c_void_p]),
+    "dgl_attention_backward_workspace_floats": (c_int64, [POINTER(Attention)]),
     "dgl_set_sqrt_model": (c_int32, [c_int32]),
     "dgl_sqrt_apply": (c_int32, [c_void_p, c_void_p, c_int64, c_void_p]),
 }

@@ -1,0 +1,250 @@
+"""Attention over the nodes of an instance or the positions of a sequence, as an operator of its own.
+
+The policy network evaluates its attention inside fused kernels over the neighbourhood of one node (at most 256 tokens,
+TSP/TSPModel.py:420-441).  Here it is for whole instances and long sequences, with capped scores, a bias that falls with
+distance, document / causal / prefix masks, and its gradients (include/dgl_amd.h, dgl_attention_t):
+
+    s_ij = cap tanh(scale q_i.k_j / cap) - slope[h] dist(i, j),     out_i = sum_j softmax_j(s_ij) v_j
+
+Tensors are [batch, heads, tokens, head size] views of any strides whose last axis is consecutive (16-byte aligned; others
+are copied), float32, float16 or bfloat16.  The computation runs in libdgl_amd on the current stream of the tensors' device.
+"""
+from __future__ import annotations
+
+import ctypes
+from typing import Optional, Tuple
+
+import torch
+
+from . import _lib
+from ._lib import check, ptr
+
+_DTYPES = {torch.float32: _lib.DTYPE_F32, torch.float16: _lib.DTYPE_F16, torch.bfloat16: _lib.DTYPE_BF16}
+
+
+def _stream(device) -> int:
+    return torch.cuda.current_stream(device).cuda_stream
+
+
+class _on:
+    """Make a tensor's device current for a launch (nothing to do where it already is)."""
+
+    def __init__(self, device):
+        self.device, self.guard = device, None
+
+    def __enter__(self):
+        if self.device.index != torch.cuda.current_device():
+            self.guard = torch.cuda.device(self.device)
+            self.guard.__enter__()
+
+    def __exit__(self, *exc):
+        if self.guard is not None:
+            self.guard.__exit__(*exc)
+
+
+def _usable(t: torch.Tensor) -> torch.Tensor:
+    """The tensor itself where the kernels can address it, else a contiguous copy."""
+    vec = 16 // t.element_size()
+    st = t.stride()
+    if (st[-1] == 1 or t.shape[-1] <= 1) and t.data_ptr() % 16 == 0 and all(x % vec == 0 for x in st[:-1]):
+        return t
+    return t.clone(memory_format=torch.contiguous_format)
+
+
+def _stride3(t: torch.Tensor):
+    return (ctypes.c_int64 * 3)(*t.stride()[:3])
+
+
+def _check_qkv(q, k, v):
+    for name, t in (("q", q), ("k", k), ("v", v)):
+        if t.dim() != 4:
+            raise ValueError(f"{name} has shape {tuple(t.shape)}: expected [batch, heads, tokens, head size]")
+        if not t.is_cuda or t.device != q.device:
+            raise ValueError(f"{name} is on {t.device}: q, k and v belong on one GPU")
+        if t.dtype != q.dtype:
+            raise ValueError(f"{name} is {t.dtype}, q is {q.dtype}")
+    if q.dtype not in _DTYPES:
+        raise ValueError(f"{q.dtype}: float32, float16 or bfloat16 is expected")
+    B, H, _, D = q.shape
+    if k.shape != v.shape or k.shape[0] != B or k.shape[3] != D:
+        raise ValueError(f"q {tuple(q.shape)}, k {tuple(k.shape)} and v {tuple(v.shape)} do not fit")
+    if k.shape[1] < 1 or H % k.shape[1]:
+        raise ValueError(f"{H} query heads over {k.shape[1]} key heads")
+
+
+def _side(t: Optional[torch.Tensor], name, shape, dtype, device) -> Optional[torch.Tensor]:
+    """A float32 / int32 side input, broadcast over the batch where it may be, inner axes consecutive."""
+    if t is None:
+        return None
+    if t.device != device:
+        raise ValueError(f"{name} is on {t.device}, q on {device}")
+    if tuple(t.shape) != shape:
+        raise ValueError(f"{name} has shape {tuple(t.shape)}, expected {shape}")
+    if t.dtype != dtype:
+        if dtype == torch.int32 and t.is_floating_point() or dtype == torch.float32 and not t.is_floating_point():
+            raise ValueError(f"{name} is {t.dtype}, expected {dtype}")
+        t = t.to(dtype)
+    inner, want = t.stride()[1:], []
+    n = 1
+    for s in reversed(shape[1:]):
+        want.insert(0, n)
+        n *= s
+    if any(a != b and s > 1 for a, b, s in zip(inner, want, shape[1:])) or (t.dim() == 1 and shape[0] > 1 and t.stride(0) != 1):
+        t = t.contiguous()
+    return t
+
+
+class _Call:
+    """Arguments of one operator call: the ABI struct and the tensors it points to."""
+
+    def __init__(self, q, k, v, scale, cap, slope, pos_q, pos_k, doc_q, doc_k, causal, prefix):
+        _check_qkv(q, k, v)
+        B, H, L, D = q.shape
+        M = k.shape[2]
+        dev = q.device
+        cap = float(cap)
+        if not 0.0 <= cap < float("inf"):
+            raise ValueError(f"cap {cap}: a number >= 0 is expected (0: no cap)")
+        if (pos_q is None) != (pos_k is None) or (doc_q is None) != (doc_k is None):
+            raise ValueError("coordinates and document ids are given for both sides or for neither")
+        if pos_q is not None and slope is None:
+            raise ValueError("coordinates without a slope")
+        if prefix is not None and not causal:
+            raise ValueError("a prefix belongs to a causal mask")
+        self.q, self.k, self.v = _usable(q), _usable(k), _usable(v)
+        self.slope = _side(slope, "slope", (H,), torch.float32, dev)
+        self.pos_q = _side(pos_q, "pos_q", (B, L, 2), torch.float32, dev)
+        self.pos_k = _side(pos_k, "pos_k", (B, M, 2), torch.float32, dev)
+        self.doc_q = _side(doc_q, "doc_q", (B, L), torch.int32, dev)
+        self.doc_k = _side(doc_k, "doc_k", (B, M), torch.int32, dev)
+        self.prefix = _side(prefix, "prefix", (B,), torch.int32, dev)
+        a = self.a = _lib.Attention()
+        a.dtype, a.B, a.Hq, a.Hkv, a.Lq, a.Lk, a.D = _DTYPES[q.dtype], B, H, k.shape[1], L, M, D
+        a.causal, a.cap = int(bool(causal)), cap
+        a.scale = D ** -0.5 if scale is None else float(scale)
+        a.q_stride, a.k_stride, a.v_stride = _stride3(self.q), _stride3(self.k), _stride3(self.v)
+        a.q, a.k, a.v = ptr(self.q), ptr(self.k), ptr(self.v)
+        a.slope, a.prefix = ptr(self.slope), ptr(self.prefix)
+        if pos_q is not None:
+            a.pos_q, a.pos_k = ptr(self.pos_q), ptr(self.pos_k)
+            a.pos_q_stride, a.pos_k_stride = self.pos_q.stride(0), self.pos_k.stride(0)
+        if doc_q is not None:
+            a.doc_q, a.doc_k = ptr(self.doc_q), ptr(self.doc_k)
+            a.doc_q_stride, a.doc_k_stride = self.doc_q.stride(0), self.doc_k.stride(0)
+
+    def set_out(self, out, lse):
+        self.out, self.lse = out, lse
+        self.a.out, self.a.o_stride, self.a.lse = ptr(out), _stride3(out), ptr(lse)
+
+
+def _like_heads(t: torch.Tensor) -> torch.Tensor:
+    """An empty [batch, heads, tokens, size] tensor stored token by token (as the linear layer after the operator reads
+    it) where its model is, head by head otherwise."""
+    B, H, L, D = t.shape
+    if t.stride(1) < t.stride(2):
+        return torch.empty(B, L, H, D, dtype=t.dtype, device=t.device).transpose(1, 2)
+    return torch.empty(B, H, L, D, dtype=t.dtype, device=t.device)
+
+
+def _forward(call: _Call, want_lse: bool):
+    q = call.q
+    out = _like_heads(q)
+    lse = torch.empty(q.shape[:3], dtype=torch.float32, device=q.device) if want_lse else None
+    call.set_out(out, lse)
+    if out.numel():
+        with _on(q.device):
+            check(_lib.load().dgl_attention_forward(ctypes.byref(call.a), _stream(q.device)), "dgl_attention_forward")
+    return out, lse
+
+
+def _backward(call: _Call, dout: torch.Tensor, want_slope: bool):
+    lib, q = _lib.load(), call.q
+    if dout.shape != q.shape or dout.dtype != q.dtype or dout.device != q.device:
+        raise ValueError(f"dout is {tuple(dout.shape)} {dout.dtype} on {dout.device}, expected out's "
+                         f"{tuple(q.shape)} {q.dtype} on {q.device}")
+    dout = _usable(dout)
+    dq, dk, dv = _like_heads(q), _like_heads(call.k), _like_heads(call.v)
+    dslope = torch.empty(q.shape[1], dtype=torch.float32, device=q.device) if want_slope else None
+    if q.shape[0] == 0:
+        return dq, dk, dv, None if dslope is None else dslope.zero_()
+    g = _lib.AttentionGrad()
+    g.dout, g.dq, g.dk, g.dv, g.dslope = ptr(dout), ptr(dq), ptr(dk), ptr(dv), ptr(dslope)
+    g.dout_stride, g.dq_stride, g.dk_stride, g.dv_stride = _stride3(dout), _stride3(dq), _stride3(dk), _stride3(dv)
+    need = lib.dgl_attention_backward_workspace_floats(ctypes.byref(call.a))
+    with _on(q.device):
+        ws = torch.empty(max(need, 1), dtype=torch.float32, device=q.device)
+        check(lib.dgl_attention_backward(ctypes.byref(call.a), ctypes.byref(g), ptr(ws), _stream(q.device)),
+              "dgl_attention_backward")
+    return dq, dk, dv, dslope
+
+
+def attention_forward(q, k, v, *, scale=None, cap=0.0, slope=None, pos_q=None, pos_k=None, doc_q=None, doc_k=None,
+                      causal=False, prefix=None) -> Tuple[torch.Tensor, torch.Tensor]:
+    """(out, lse) without autograd: the pair of calls to use where the backward pass is driven by hand, for instance
+    inside a captured graph."""
+    with torch.no_grad():
+        return _forward(_Call(q, k, v, scale, cap, slope, pos_q, pos_k, doc_q, doc_k, causal, prefix), True)
+
+
+def attention_backward(dout, q, k, v, out, lse, *, scale=None, cap=0.0, slope=None, pos_q=None, pos_k=None, doc_q=None,
+                       doc_k=None, causal=False, prefix=None):
+    """(dq, dk, dv, dslope or None) of the forward call with the same arguments, given its out and lse."""
+    with torch.no_grad():
+        call = _Call(q, k, v, scale, cap, slope, pos_q, pos_k, doc_q, doc_k, causal, prefix)
+        if out.shape != q.shape or out.dtype != q.dtype or out.device != q.device:
+            raise ValueError(f"out is {tuple(out.shape)} {out.dtype}, expected {tuple(q.shape)} {q.dtype}")
+        if tuple(lse.shape) != tuple(q.shape[:3]) or lse.dtype != torch.float32 or lse.device != q.device:
+            raise ValueError(f"lse is {tuple(lse.shape)} {lse.dtype}, expected {tuple(q.shape[:3])} float32")
+        call.set_out(_usable(out), lse.contiguous())
+        return _backward(call, dout, slope is not None)
+
+
+class _Attention(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, slope, scale, cap, pos_q, pos_k, doc_q, doc_k, causal, prefix):
+        call = _Call(q, k, v, scale, cap, slope, pos_q, pos_k, doc_q, doc_k, causal, prefix)
+        need = any(ctx.needs_input_grad[:4])
+        out, lse = _forward(call, need)
+        if need:
+            # (the saved inputs are the caller's: autograd notices a change in place between the two passes)
+            ctx.save_for_backward(q, k, v, slope, pos_q, pos_k, doc_q, doc_k, prefix, out, lse)
+            ctx.scalars = (scale, cap, causal)
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dout):
+        q, k, v, slope, pos_q, pos_k, doc_q, doc_k, prefix, out, lse = ctx.saved_tensors
+        scale, cap, causal = ctx.scalars
+        call = _Call(q, k, v, scale, cap, slope, pos_q, pos_k, doc_q, doc_k, causal, prefix)
+        call.set_out(out, lse)
+        dq, dk, dv, dslope = _backward(call, dout, slope is not None and ctx.needs_input_grad[3])
+        if dslope is not None and slope.dtype != torch.float32:
+            dslope = dslope.to(slope.dtype)
+        return dq, dk, dv, dslope, None, None, None, None, None, None, None, None
+
+
+def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, scale: Optional[float] = None, cap: float = 0.0,
+              slope: Optional[torch.Tensor] = None, pos_q: Optional[torch.Tensor] = None,
+              pos_k: Optional[torch.Tensor] = None, doc_q: Optional[torch.Tensor] = None,
+              doc_k: Optional[torch.Tensor] = None, causal: bool = False,
+              prefix: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Attention of q [B, H, Lq, D] over k, v [B, Hkv, Lk, D] (H a multiple of Hkv), differentiable in q, k, v and slope.
+
+    ``scale``: default D ** -0.5.  ``cap`` > 0: scores pass through cap tanh(. / cap).  ``slope`` [H]: bias -slope dist,
+    between the coordinates ``pos_q`` [B, Lq, 2] and ``pos_k`` [B, Lk, 2], or, without them, between positions
+    (|i + Lk - Lq - j|).  ``doc_q`` [B, Lq] / ``doc_k`` [B, Lk]: whole numbers; tokens see their own document, negative ids
+    are padding (such rows give zeros).  ``causal``: j <= i + Lk - Lq, and in front of ``prefix`` [B] everything.
+
+    Under graph capture, leaves that collect gradients are refused: a leaf's accumulation belongs to the stream on which
+    it was first used, and a captured backward pass that meets an eager graph of the same leaf ends the process.  Capture
+    attention_forward and attention_backward instead."""
+    if torch.is_grad_enabled() and torch.cuda.is_available() and torch.cuda.is_current_stream_capturing():
+        for t in (q, k, v, slope):
+            if t is not None and t.requires_grad and t.is_leaf:
+                raise RuntimeError("attention: a leaf that requires grad inside a graph capture; capture attention_forward "
+                                   "and attention_backward, or pass a tensor computed from the leaf")
+    for name, t in (("pos_q", pos_q), ("pos_k", pos_k)):
+        if t is not None and t.requires_grad and torch.is_grad_enabled():
+            raise ValueError(f"{name} requires grad: the operator is not differentiable in the coordinates")
+    return _Attention.apply(q, k, v, slope, scale, cap, pos_q, pos_k, doc_q, doc_k, causal, prefix)

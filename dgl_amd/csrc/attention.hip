@@ -1,0 +1,1135 @@
+// Attention over nodes or sequence positions, forward and backward.
+//
+//   s_ij = cap tanh(scale q_i . k_j / cap) - slope_h dist(i, j)          (cap = 0: no tanh; slope = NULL: no bias)
+//   p_ij = softmax over the allowed j;   o_i = sum_j p_ij v_j;   lse_i = log sum_j exp(s_ij)
+//   dp = do v^T;  ds = p (dp - do . o);  dslope = - sum ds dist;  du = ds (1 - tanh^2);
+//   dq = scale du k;  dk = scale du^T q;  dv = p^T do
+//
+// dist is the Euclidean distance of 2-D coordinates, or |i + Lk - Lq - j|; a pair is allowed when both sides carry the same
+// document id >= 0 and, under `causal`, j <= i + Lk - Lq or j < prefix.  A row without an allowed pair gives zeros.
+//
+// One pass over the keys with a running maximum and sum (scores never leave registers); the backward pass recomputes the
+// scores from lse in two kernels - one owns query rows (dq, delta, dslope), one owns key rows (dk, dv, summed over the
+// query heads that share them) - so no gradient needs atomics and every call gives the same bits.
+//
+// A pair that is masked contributes nothing, whatever its operands hold: the products of the matrix instructions would
+// carry a NaN or infinity of a masked row into its tile neighbours (0 * NaN), so a result that is not finite at the end is
+// recomputed pair by pair (careful_*), which costs nothing where all is finite.
+#include "attention_tile.h"
+
+#include <cfloat>
+
+namespace {
+
+#define ATTN_THREADS 256
+#define ATTN_MAX_TILES 4096      // tiles whose document overlap is looked up before the pass; later ones are all visited
+
+struct AttnArgs {
+    const char *q, *k, *v;                       // element pointers
+    char *out;
+    float *lse;
+    int64_t qs[3], ks[3], vs[3], os[3];          // strides: batch, head, token (elements)
+    int B, Hq, Hkv, G, Lq, Lk, D, causal, bias;  // bias: 0 none, 1 positions, 2 coordinates
+    float scale, cap;
+    const float *slope, *pos_q, *pos_k;
+    int64_t pqs, pks;
+    const int *doc_q, *doc_k;
+    int64_t dqs, dks;
+    const int *prefix;
+    int tiles;                                   // row blocks per (batch, head)
+    // backward
+    const char *dout;
+    char *dq, *dk, *dv;
+    int64_t dos[3], dqst[3], dkst[3], dvst[3];
+    float *delta, *rowscale, *dslope_part, *dslope;
+};
+
+// Blocks are dealt to the 8 XCDs in turn; giving every XCD a contiguous range of the work keeps the row blocks of one
+// head, which read the same keys and values, on one L2.
+__device__ __forceinline__ int xcd_work() { return (int)(blockIdx.x % 8) * (int)(gridDim.x / 8) + (int)(blockIdx.x / 8); }
+
+struct ScoreParams {
+    float mul, cap2, slope2;     // all in units of log2
+    int cap, bias;
+};
+__device__ __forceinline__ ScoreParams score_params(const AttnArgs &a, int h) {
+    ScoreParams p;
+    p.cap = a.cap > 0.0f;
+    p.mul = p.cap ? a.scale / a.cap : a.scale * ATTN_LOG2E;
+    p.cap2 = a.cap * ATTN_LOG2E;
+    p.bias = a.bias;
+    p.slope2 = a.bias ? a.slope[h] * ATTN_LOG2E : 0.0f;
+    return p;
+}
+// keys a query row sees: j < limit (and the document test)
+__device__ __forceinline__ int row_limit(const AttnArgs &a, int b, int i) {
+    if (i >= a.Lq) return 0;
+    if (!a.causal) return a.Lk;
+    int lim = i + a.Lk - a.Lq + 1;
+    if (a.prefix != nullptr) lim = max(lim, a.prefix[b]);
+    return max(0, min(lim, a.Lk));
+}
+// document ids with the padding of either side made unequal to everything
+__device__ __forceinline__ int doc_of_query(const AttnArgs &a, int b, int i) {
+    const int id = i < a.Lq ? a.doc_q[b * a.dqs + i] : -1;
+    return id < 0 ? -2 : id;
+}
+__device__ __forceinline__ int doc_of_key(const AttnArgs &a, int b, int j) {
+    const int id = j < a.Lk ? a.doc_k[b * a.dks + j] : -1;
+    return id < 0 ? -1 : id;
+}
+
+__device__ __forceinline__ float pair_distance(const AttnArgs &a, int b, int i, int j) {
+    if (a.bias == 1) return fabsf((float)(i + a.Lk - a.Lq - j));
+    const float *x = a.pos_q + b * a.pqs + 2 * (int64_t)i, *y = a.pos_k + b * a.pks + 2 * (int64_t)j;
+    const float dx = x[0] - y[0], dy = x[1] - y[1];
+    return __builtin_amdgcn_sqrtf(fmaf(dx, dx, dy * dy));
+}
+
+// one pair for the careful path: its score (log2 units), tanh and distance
+template <int TYPE>
+__device__ float pair_score(const AttnArgs &a, const ScoreParams &sp, int b, int i, int j, const typename Elem<TYPE>::raw *q,
+                            const typename Elem<TYPE>::raw *k, float &th, float &dist) {
+    float dot = 0.0f;
+    for (int d = 0; d < a.D; ++d) dot = fmaf(elem_to_float<TYPE>(q[d]), elem_to_float<TYPE>(k[d]), dot);
+    float s = dot * sp.mul;
+    th = 0.0f;
+    dist = 0.0f;
+    if (sp.cap) {
+        th = attn_tanh(s);
+        s = sp.cap2 * th;
+    }
+    if (sp.bias) {
+        dist = pair_distance(a, b, i, j);
+        s = fmaf(-sp.slope2, dist, s);
+    }
+    return s;
+}
+__device__ __forceinline__ bool pair_allowed(const AttnArgs &a, int b, int i, int j, int limit) {
+    if (j >= limit) return false;
+    return a.doc_q == nullptr || doc_of_query(a, b, i) == doc_of_key(a, b, j);
+}
+
+// Which 64-row tiles of the other side hold a document of this block's rows: bit set = visit; second word = every pair
+// of the tile is in one document (no test per pair).
+struct TileMap {
+    unsigned long long any[ATTN_MAX_TILES / 64], same[ATTN_MAX_TILES / 64];
+    int lo, hi, uniform;
+};
+__device__ void build_tile_map(TileMap &m, const int *own, int own_base, int own_rows, int own_n, const int *other, int other_n) {
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    if (tid == 0) {
+        m.lo = INT_MAX;
+        m.hi = -1;
+        m.uniform = 1;
+    }
+    for (int w = tid; w < ATTN_MAX_TILES / 64; w += ATTN_THREADS) m.any[w] = m.same[w] = 0;
+    __syncthreads();
+    for (int i = tid; i < own_rows; i += ATTN_THREADS) {
+        if (own_base + i >= own_n) break;
+        const int id = own[own_base + i];
+        if (id >= 0) {
+            atomicMin(&m.lo, id);
+            atomicMax(&m.hi, id);
+        } else {
+            m.uniform = 0;
+        }
+    }
+    __syncthreads();
+    const int lo = m.lo, hi = m.hi;
+    const bool one = m.uniform && lo == hi;
+    const int tiles = min(ATTN_MAX_TILES, (other_n + ATTN_ROWS - 1) / ATTN_ROWS);
+    for (int t = wave; t < tiles; t += ATTN_THREADS / 64) {
+        const int j = t * ATTN_ROWS + lane;
+        const int id = j < other_n ? other[j] : -1;
+        const unsigned long long in = __ballot(id >= 0 && id >= lo && id <= hi), eq = __ballot(id == lo);
+        if (lane == 0 && in != 0) {
+            atomicOr(&m.any[t / 64], 1ull << (t % 64));
+            if (one && eq == ~0ull) atomicOr(&m.same[t / 64], 1ull << (t % 64));
+        }
+    }
+    __syncthreads();
+}
+// first tile >= t to visit, or `end`
+__device__ __forceinline__ int next_tile(const TileMap *m, int t, int end) {
+    if (m == nullptr) return t;
+    while (t < end && t < ATTN_MAX_TILES) {
+        const unsigned long long w = m->any[t / 64] >> (t % 64);
+        if (w != 0) return min(end, t + __ffsll((long long)w) - 1);
+        t = (t / 64 + 1) * 64;
+    }
+    return min(t, end);
+}
+__device__ __forceinline__ bool tile_same(const TileMap *m, int t) {
+    return m == nullptr || (t < ATTN_MAX_TILES && ((m->same[t / 64] >> (t % 64)) & 1));
+}
+
+__device__ __forceinline__ bool finite4(const f32x4 &v) {
+    const float t = (v[0] * 0.0f + v[1] * 0.0f) + (v[2] * 0.0f + v[3] * 0.0f);
+    return t == 0.0f;
+}
+
+// --------------------------------------------------------------------------------------------------------- forward
+// One workgroup = 4 waves x NQ blocks of 16 queries of one (batch, head); keys and values pass through LDS in tiles of 64,
+// the next tile's loads in flight while the current one is computed.  Lane (g, c) holds query c of its blocks and, per
+// 16 keys, the scores against keys 4 g + r.
+template <int TYPE>
+__device__ void careful_forward_row(const AttnArgs &a, const ScoreParams &sp, int b, int h, int i, float m, float l) {
+    typedef typename Elem<TYPE>::raw raw;
+    const int lane = threadIdx.x & 63, hk = h / a.G, limit = row_limit(a, b, i);
+    const raw *q = reinterpret_cast<const raw *>(a.q) + b * a.qs[0] + h * a.qs[1] + i * a.qs[2];
+    const raw *k = reinterpret_cast<const raw *>(a.k) + b * a.ks[0] + hk * a.ks[1];
+    const raw *v = reinterpret_cast<const raw *>(a.v) + b * a.vs[0] + hk * a.vs[1];
+    float acc0 = 0.0f, acc1 = 0.0f;
+    for (int base = 0; base < limit; base += 64) {
+        const int j = base + lane;
+        const bool ok = pair_allowed(a, b, i, j, limit);
+        float p = 0.0f, th, dist;
+        if (ok) p = __builtin_amdgcn_exp2f(pair_score<TYPE>(a, sp, b, i, j, q, k + j * a.ks[2], th, dist) - m);
+        for (unsigned long long w = __ballot(ok); w != 0; w &= w - 1) {
+            const int jj = __ffsll((long long)w) - 1;
+            const float pj = __shfl(p, jj);
+            const raw *vr = v + (int64_t)(base + jj) * a.vs[2];
+            if (lane < a.D) acc0 = fmaf(pj, elem_to_float<TYPE>(vr[lane]), acc0);
+            if (lane + 64 < a.D) acc1 = fmaf(pj, elem_to_float<TYPE>(vr[lane + 64]), acc1);
+        }
+    }
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    raw *o = reinterpret_cast<raw *>(a.out) + b * a.os[0] + h * a.os[1] + i * a.os[2];
+    for (int half = 0; half < 2; ++half) {
+        const int d = lane + 64 * half;
+        const float x = (half ? acc1 : acc0) * inv;
+        if (d < a.D) {
+            if constexpr (TYPE == ATTN_F32) o[d] = x;
+            else if constexpr (TYPE == ATTN_F16) o[d] = __builtin_bit_cast(unsigned short, (_Float16)x);
+            else o[d] = __builtin_bit_cast(unsigned short, (__bf16)x);
+        }
+    }
+}
+
+template <int TYPE, int DP, int NQ>
+__global__ __launch_bounds__(ATTN_THREADS, DP <= 64 ? 2 : 1) void attn_fwd_kernel(AttnArgs a) {
+    typedef Shape<TYPE, DP> S;
+    typedef typename Elem<TYPE>::raw raw;
+    constexpr int ROWS = 64 * NQ, UNITS = (2 * S::units + ATTN_THREADS - 1) / ATTN_THREADS;
+    __shared__ __align__(16) char lds[S::row_bytes + (S::wide ? S::row_bytes : S::t_bytes)];
+    __shared__ __align__(16) float key_pos[2 * ATTN_ROWS];
+    __shared__ __align__(16) int key_doc[ATTN_ROWS];
+    __shared__ TileMap map_store;
+    raw *Kt = reinterpret_cast<raw *>(lds), *Vt = reinterpret_cast<raw *>(lds + S::row_bytes);
+
+    const int work = xcd_work();
+    if (work >= a.B * a.Hq * a.tiles) return;
+    const int bh = work / a.tiles, qt = a.tiles - 1 - work % a.tiles;        // (causal: the longest rows first)
+    const int b = bh / a.Hq, h = bh % a.Hq, hk = h / a.G;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g = lane >> 4, c = lane & 15;
+    const int row0 = qt * ROWS, wrow0 = row0 + wave * 16 * NQ;
+    const raw *q = reinterpret_cast<const raw *>(a.q) + b * a.qs[0] + h * a.qs[1];
+    const raw *k = reinterpret_cast<const raw *>(a.k) + b * a.ks[0] + hk * a.ks[1];
+    const raw *v = reinterpret_cast<const raw *>(a.v) + b * a.vs[0] + hk * a.vs[1];
+    const int *docs = a.doc_k != nullptr ? a.doc_k + b * a.dks : nullptr;
+    const ScoreParams sp = score_params(a, h);
+
+    TileMap *map = nullptr;
+    if (docs != nullptr) {
+        map = &map_store;
+        build_tile_map(map_store, a.doc_q + b * a.dqs, row0, ROWS, a.Lq, docs, a.Lk);
+    }
+    zero_padding<TYPE, DP>(Kt);
+
+    Frag<TYPE, DP> qf[NQ];
+    f32x4 o[NQ][S::dt];
+    float m[NQ], l[NQ], qx[NQ], qy[NQ];
+    int limit[NQ], doc[NQ];
+    int wave_limit = 0, wave_full = INT_MAX;          // keys some row / every row of the wave sees
+#pragma unroll
+    for (int n = 0; n < NQ; ++n) {
+        const int i = wrow0 + 16 * n + c;
+        frag_from_global<TYPE, DP>(qf[n], q + (int64_t)i * a.qs[2], i < a.Lq, a.D, g);
+        m[n] = -attn_inf();
+        l[n] = 0.0f;
+        limit[n] = row_limit(a, b, i);
+        doc[n] = map != nullptr ? doc_of_query(a, b, i) : 0;
+        qx[n] = qy[n] = 0.0f;
+        if (a.bias == 1) qx[n] = (float)(i + a.Lk - a.Lq);
+        if (a.bias == 2 && i < a.Lq) {
+            qx[n] = a.pos_q[b * a.pqs + 2 * (int64_t)i];
+            qy[n] = a.pos_q[b * a.pqs + 2 * (int64_t)i + 1];
+        }
+#pragma unroll
+        for (int d = 0; d < S::dt; ++d) o[n][d] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    }
+    if (wrow0 < a.Lq) {
+        wave_limit = row_limit(a, b, min(wrow0 + 16 * NQ, a.Lq) - 1);        // limits rise with the row
+        wave_full = row_limit(a, b, wrow0);
+    }
+    const int end = (row_limit(a, b, min(row0 + ROWS, a.Lq) - 1) + ATTN_ROWS - 1) / ATTN_ROWS;
+
+    Unit un[UNITS];
+    float stage_pos = 0.0f;
+    int stage_doc = -1;
+    auto load = [&](int tile) {
+        const int base = tile * ATTN_ROWS;
+#pragma unroll
+        for (int x = 0; x < UNITS; ++x) {
+            const int u = tid + x * ATTN_THREADS;
+            if (u < S::units) unit_load<TYPE, DP>(un[x], u, k, a.ks[2], base, a.Lk, a.D, docs);
+            else if (u < 2 * S::units) unit_load<TYPE, DP>(un[x], u - S::units, v, a.vs[2], base, a.Lk, a.D, docs);
+        }
+        if (a.bias == 2 && tid < 2 * ATTN_ROWS) stage_pos = base + tid / 2 < a.Lk ? a.pos_k[b * a.pks + 2 * (int64_t)base + tid] : 0.0f;
+        if (map != nullptr && tid < ATTN_ROWS) stage_doc = doc_of_key(a, b, base + tid);
+    };
+    int tile = next_tile(map, 0, end);
+    if (tile < end) load(tile);
+    while (tile < end) {
+        __syncthreads();
+#pragma unroll
+        for (int x = 0; x < UNITS; ++x) {
+            const int u = tid + x * ATTN_THREADS;
+            if (u < S::units) unit_write<TYPE, DP, true, false>(un[x], u, Kt, nullptr);
+            else if (u < 2 * S::units) unit_write<TYPE, DP, false, true>(un[x], u - S::units, Vt, Vt);
+        }
+        if (a.bias == 2 && tid < 2 * ATTN_ROWS) key_pos[tid] = stage_pos;
+        if (map != nullptr && tid < ATTN_ROWS) key_doc[tid] = stage_doc;
+        const int here = tile, base = here * ATTN_ROWS;
+        tile = next_tile(map, here + 1, end);
+        if (tile < end) load(tile);
+        __syncthreads();
+        if (base >= wave_limit) continue;
+        const bool by_doc = !tile_same(map, here), by_limit = base + ATTN_ROWS > wave_full;
+
+        f32x4 s[4][NQ];
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+            Frag<TYPE, DP> kf;
+            frag_from_lds<TYPE, DP>(kf, Kt, 16 * t + c, g);
+#pragma unroll
+            for (int n = 0; n < NQ; ++n) s[t][n] = dot_block<TYPE, DP>(kf, qf[n]);
+        }
+        if (sp.cap) {
+#pragma unroll
+            for (int t = 0; t < 4; ++t)
+#pragma unroll
+                for (int n = 0; n < NQ; ++n)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) s[t][n][r] = sp.cap2 * attn_tanh(s[t][n][r] * sp.mul);
+        } else {
+#pragma unroll
+            for (int t = 0; t < 4; ++t)
+#pragma unroll
+                for (int n = 0; n < NQ; ++n) s[t][n] = s[t][n] * sp.mul;
+        }
+        if (sp.bias == 1) {
+            const float k0 = (float)(base + 4 * g);
+#pragma unroll
+            for (int t = 0; t < 4; ++t)
+#pragma unroll
+                for (int n = 0; n < NQ; ++n)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) s[t][n][r] = fmaf(-sp.slope2, fabsf(qx[n] - (k0 + (float)(16 * t + r))), s[t][n][r]);
+        } else if (sp.bias == 2) {
+#pragma unroll
+            for (int t = 0; t < 4; ++t) {
+                const f32x4 p0 = *reinterpret_cast<const f32x4 *>(key_pos + 2 * (16 * t + 4 * g));
+                const f32x4 p1 = *reinterpret_cast<const f32x4 *>(key_pos + 2 * (16 * t + 4 * g) + 4);
+                const float kx[4] = {p0[0], p0[2], p1[0], p1[2]}, ky[4] = {p0[1], p0[3], p1[1], p1[3]};
+#pragma unroll
+                for (int n = 0; n < NQ; ++n)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        const float dx = qx[n] - kx[r], dy = qy[n] - ky[r];
+                        s[t][n][r] = fmaf(-sp.slope2, __builtin_amdgcn_sqrtf(fmaf(dx, dx, dy * dy)), s[t][n][r]);
+                    }
+            }
+        }
+        if (by_limit) {
+#pragma unroll
+            for (int t = 0; t < 4; ++t)
+#pragma unroll
+                for (int n = 0; n < NQ; ++n)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        s[t][n][r] = base + 16 * t + 4 * g + r < limit[n] ? s[t][n][r] : -attn_inf();
+        }
+        if (by_doc) {
+#pragma unroll
+            for (int t = 0; t < 4; ++t) {
+                const i32x4 kd = *reinterpret_cast<const i32x4 *>(key_doc + 16 * t + 4 * g);
+#pragma unroll
+                for (int n = 0; n < NQ; ++n)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) s[t][n][r] = kd[r] == doc[n] ? s[t][n][r] : -attn_inf();
+            }
+        }
+#pragma unroll
+        for (int n = 0; n < NQ; ++n) {
+            float top = s[0][n][0];
+#pragma unroll
+            for (int t = 0; t < 4; ++t)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) top = fmaxf(top, s[t][n][r]);
+            top = fmaxf(group_max(top), m[n]);
+            if (__any(top > m[n])) {
+                const float shift = top == -attn_inf() ? 0.0f : top;
+                const float f = __builtin_amdgcn_exp2f(m[n] - shift);
+                l[n] *= f;
+#pragma unroll
+                for (int d = 0; d < S::dt; ++d) o[n][d] = o[n][d] * f;
+                m[n] = top;
+            }
+            const float shift = m[n] == -attn_inf() ? 0.0f : m[n];
+#pragma unroll
+            for (int t = 0; t < 4; ++t)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    s[t][n][r] = __builtin_amdgcn_exp2f(s[t][n][r] - shift);
+                    l[n] += s[t][n][r];
+                }
+        }
+        accumulate<TYPE, DP, NQ>(o, Vt, Vt, 0, s[0], s[1], g, c);
+        accumulate<TYPE, DP, NQ>(o, Vt, Vt, 1, s[2], s[3], g, c);
+    }
+
+#pragma unroll
+    for (int n = 0; n < NQ; ++n) {
+        const int i = wrow0 + 16 * n + c;
+        const float total = group_sum(l[n]);
+        const float inv = total == 0.0f ? 0.0f : 1.0f / total;
+        const float shift = m[n] == -attn_inf() ? 0.0f : m[n];
+        bool fine = true;
+#pragma unroll
+        for (int d = 0; d < S::dt; ++d) fine = fine && finite4(o[n][d]);
+        if (i < a.Lq) {
+            raw *out = reinterpret_cast<raw *>(a.out) + b * a.os[0] + h * a.os[1] + (int64_t)i * a.os[2];
+#pragma unroll
+            for (int d = 0; d < S::dt; ++d)
+                if (16 * d + 4 * g < a.D) store4<TYPE>(out + 16 * d + 4 * g, o[n][d] * inv);
+            if (a.lse != nullptr && g == 0)
+                a.lse[((int64_t)b * a.Hq + h) * a.Lq + i] = total == 0.0f ? -attn_inf() : (shift + __builtin_amdgcn_logf(total)) * ATTN_LN2;
+        }
+        unsigned long long bad = __ballot(!fine && i < a.Lq);
+        bad = (bad | bad >> 16 | bad >> 32 | bad >> 48) & 0xffff;
+        for (; bad != 0; bad &= bad - 1) {
+            const int cc = __ffsll((long long)bad) - 1;
+            careful_forward_row<TYPE>(a, sp, b, h, wrow0 + 16 * n + cc, __shfl(shift, cc), __shfl(total, cc));
+        }
+    }
+}
+
+// -------------------------------------------------------------------------------------------- backward: query rows
+// dq of NQ x 16 query rows per wave, with delta_i = do_i . o_i on the way (kept for the kernel that owns the keys) and
+// the rows' share of dslope.  sum_j ds_ij is zero by definition; what it is with the delta at hand (o may have been
+// rounded to 16 bits) is measured and its part of the slope's gradient taken out again.
+template <int TYPE>
+__device__ void careful_dq_row(const AttnArgs &a, const ScoreParams &sp, int b, int h, int i, float lse2, float delta) {
+    typedef typename Elem<TYPE>::raw raw;
+    const int lane = threadIdx.x & 63, hk = h / a.G, limit = row_limit(a, b, i);
+    const raw *q = reinterpret_cast<const raw *>(a.q) + b * a.qs[0] + h * a.qs[1] + i * a.qs[2];
+    const raw *o = reinterpret_cast<const raw *>(a.dout) + b * a.dos[0] + h * a.dos[1] + i * a.dos[2];
+    const raw *k = reinterpret_cast<const raw *>(a.k) + b * a.ks[0] + hk * a.ks[1];
+    const raw *v = reinterpret_cast<const raw *>(a.v) + b * a.vs[0] + hk * a.vs[1];
+    float acc0 = 0.0f, acc1 = 0.0f;
+    for (int base = 0; base < limit; base += 64) {
+        const int j = base + lane;
+        const bool ok = pair_allowed(a, b, i, j, limit);
+        float ds = 0.0f, th, dist;
+        if (ok) {
+            const float p = __builtin_amdgcn_exp2f(pair_score<TYPE>(a, sp, b, i, j, q, k + j * a.ks[2], th, dist) - lse2);
+            float dp = 0.0f;
+            for (int d = 0; d < a.D; ++d) dp = fmaf(elem_to_float<TYPE>(o[d]), elem_to_float<TYPE>(v[j * a.vs[2] + d]), dp);
+            ds = p * (dp - delta);
+            if (sp.cap) ds *= fmaf(-th, th, 1.0f);
+        }
+        for (unsigned long long w = __ballot(ok); w != 0; w &= w - 1) {
+            const int jj = __ffsll((long long)w) - 1;
+            const float x = __shfl(ds, jj);
+            const raw *kr = k + (int64_t)(base + jj) * a.ks[2];
+            if (lane < a.D) acc0 = fmaf(x, elem_to_float<TYPE>(kr[lane]), acc0);
+            if (lane + 64 < a.D) acc1 = fmaf(x, elem_to_float<TYPE>(kr[lane + 64]), acc1);
+        }
+    }
+    raw *out = reinterpret_cast<raw *>(a.dq) + b * a.dqst[0] + h * a.dqst[1] + i * a.dqst[2];
+    for (int half = 0; half < 2; ++half) {
+        const int d = lane + 64 * half;
+        const float x = (half ? acc1 : acc0) * a.scale;
+        if (d < a.D) {
+            if constexpr (TYPE == ATTN_F32) out[d] = x;
+            else if constexpr (TYPE == ATTN_F16) out[d] = __builtin_bit_cast(unsigned short, (_Float16)x);
+            else out[d] = __builtin_bit_cast(unsigned short, (__bf16)x);
+        }
+    }
+}
+
+// Half precision keeps 2^-24 at the least: score gradients of rows with a small do would vanish.  They are scaled by a
+// power of two that brings the row's largest |do| to 8..16 (undone exactly in the result).
+__device__ __forceinline__ float gradient_scale(float amax) {
+    if (!(amax > 0.0f) || !(amax < 3.0e38f)) return 1.0f;
+    const int e = (int)(__float_as_uint(amax) >> 23) - 127;
+    return __uint_as_float((unsigned)(127 + max(-100, min(100, 3 - e))) << 23);
+}
+
+template <int TYPE, int DP, int NQ>
+__global__ __launch_bounds__(ATTN_THREADS, DP <= 64 ? 2 : 1) void attn_bwd_q_kernel(AttnArgs a) {
+    typedef Shape<TYPE, DP> S;
+    typedef typename Elem<TYPE>::raw raw;
+    constexpr int ROWS = 64 * NQ, UNITS = (2 * S::units + ATTN_THREADS - 1) / ATTN_THREADS;
+    __shared__ __align__(16) char lds[2 * S::row_bytes + S::t_bytes];
+    __shared__ __align__(16) float key_pos[2 * ATTN_ROWS];
+    __shared__ __align__(16) int key_doc[ATTN_ROWS];
+    __shared__ TileMap map_store;
+    __shared__ float part[4];
+    raw *Kt = reinterpret_cast<raw *>(lds), *Vt = reinterpret_cast<raw *>(lds + S::row_bytes);
+    raw *KT = reinterpret_cast<raw *>(lds + 2 * S::row_bytes);
+
+    const int work = xcd_work();
+    if (work >= a.B * a.Hq * a.tiles) return;
+    const int bh = work / a.tiles, qt = a.tiles - 1 - work % a.tiles;
+    const int b = bh / a.Hq, h = bh % a.Hq, hk = h / a.G;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g = lane >> 4, c = lane & 15;
+    const int row0 = qt * ROWS, wrow0 = row0 + wave * 16 * NQ;
+    const raw *q = reinterpret_cast<const raw *>(a.q) + b * a.qs[0] + h * a.qs[1];
+    const raw *k = reinterpret_cast<const raw *>(a.k) + b * a.ks[0] + hk * a.ks[1];
+    const raw *v = reinterpret_cast<const raw *>(a.v) + b * a.vs[0] + hk * a.vs[1];
+    const raw *go = reinterpret_cast<const raw *>(a.dout) + b * a.dos[0] + h * a.dos[1];
+    const raw *fo = reinterpret_cast<const raw *>(a.out) + b * a.os[0] + h * a.os[1];
+    const int *docs = a.doc_k != nullptr ? a.doc_k + b * a.dks : nullptr;
+    const ScoreParams sp = score_params(a, h);
+
+    TileMap *map = nullptr;
+    if (docs != nullptr) {
+        map = &map_store;
+        build_tile_map(map_store, a.doc_q + b * a.dqs, row0, ROWS, a.Lq, docs, a.Lk);
+    }
+    zero_padding<TYPE, DP>(Kt);
+    zero_padding<TYPE, DP>(Vt);
+
+    Frag<TYPE, DP> qf[NQ], of[NQ];
+    f32x4 dq[NQ][S::dt];
+    float lse2[NQ], delta[NQ], rs[NQ], qx[NQ], qy[NQ], excess[NQ], pd[NQ], dsl[NQ];
+    int limit[NQ], doc[NQ];
+    int wave_limit = 0, wave_full = INT_MAX;
+#pragma unroll
+    for (int n = 0; n < NQ; ++n) {
+        const int i = wrow0 + 16 * n + c;
+        const bool live = i < a.Lq;
+        frag_from_global<TYPE, DP>(qf[n], q + (int64_t)i * a.qs[2], live, a.D, g);
+        frag_from_global<TYPE, DP>(of[n], go + (int64_t)i * a.dos[2], live, a.D, g);
+        Frag<TYPE, DP> ff;
+        frag_from_global<TYPE, DP>(ff, fo + (int64_t)i * a.os[2], live, a.D, g);
+        float dot = 0.0f, amax = 0.0f;
+#pragma unroll
+        for (int x = 0; x < S::chunks; ++x)
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+                if constexpr (S::wide) {
+                    dot = fmaf(__uint_as_float(of[n].c[x][w]), __uint_as_float(ff.c[x][w]), dot);
+                } else {
+#pragma unroll
+                    for (int half = 0; half < 2; ++half) {
+                        const float e = elem_to_float<TYPE>((unsigned short)(of[n].c[x][w] >> (16 * half)));
+                        dot = fmaf(e, elem_to_float<TYPE>((unsigned short)(ff.c[x][w] >> (16 * half))), dot);
+                        amax = fmaxf(amax, fabsf(e));
+                    }
+                }
+            }
+        delta[n] = group_sum(dot);
+        rs[n] = TYPE == ATTN_F16 ? gradient_scale(group_max(amax)) : 1.0f;
+        const int64_t at = ((int64_t)b * a.Hq + h) * a.Lq + i;
+        const float lse = live ? a.lse[at] : -attn_inf();
+        lse2[n] = lse == -attn_inf() ? attn_inf() : lse * ATTN_LOG2E;
+        if (live && g == 0) {
+            a.delta[at] = delta[n];
+            if (TYPE == ATTN_F16) a.rowscale[at] = rs[n];
+        }
+        limit[n] = row_limit(a, b, i);
+        doc[n] = map != nullptr ? doc_of_query(a, b, i) : 0;
+        qx[n] = qy[n] = excess[n] = pd[n] = dsl[n] = 0.0f;
+        if (a.bias == 1) qx[n] = (float)(i + a.Lk - a.Lq);
+        if (a.bias == 2 && live) {
+            qx[n] = a.pos_q[b * a.pqs + 2 * (int64_t)i];
+            qy[n] = a.pos_q[b * a.pqs + 2 * (int64_t)i + 1];
+        }
+#pragma unroll
+        for (int d = 0; d < S::dt; ++d) dq[n][d] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    }
+    if (wrow0 < a.Lq) {
+        wave_limit = row_limit(a, b, min(wrow0 + 16 * NQ, a.Lq) - 1);
+        wave_full = row_limit(a, b, wrow0);
+    }
+    const int end = (row_limit(a, b, min(row0 + ROWS, a.Lq) - 1) + ATTN_ROWS - 1) / ATTN_ROWS;
+    const bool want_slope = a.dslope_part != nullptr;
+
+    Unit un[UNITS];
+    float stage_pos = 0.0f;
+    int stage_doc = -1;
+    auto load = [&](int tile) {
+        const int base = tile * ATTN_ROWS;
+#pragma unroll
+        for (int x = 0; x < UNITS; ++x) {
+            const int u = tid + x * ATTN_THREADS;
+            if (u < S::units) unit_load<TYPE, DP>(un[x], u, k, a.ks[2], base, a.Lk, a.D, docs);
+            else if (u < 2 * S::units) unit_load<TYPE, DP>(un[x], u - S::units, v, a.vs[2], base, a.Lk, a.D, docs);
+        }
+        if (a.bias == 2 && tid < 2 * ATTN_ROWS) stage_pos = base + tid / 2 < a.Lk ? a.pos_k[b * a.pks + 2 * (int64_t)base + tid] : 0.0f;
+        if (map != nullptr && tid < ATTN_ROWS) stage_doc = doc_of_key(a, b, base + tid);
+    };
+    int tile = next_tile(map, 0, end);
+    if (tile < end) load(tile);
+    while (tile < end) {
+        __syncthreads();
+#pragma unroll
+        for (int x = 0; x < UNITS; ++x) {
+            const int u = tid + x * ATTN_THREADS;
+            if (u < S::units) unit_write<TYPE, DP, true, true>(un[x], u, Kt, KT);
+            else if (u < 2 * S::units) unit_write<TYPE, DP, true, false>(un[x], u - S::units, Vt, nullptr);
+        }
+        if (a.bias == 2 && tid < 2 * ATTN_ROWS) key_pos[tid] = stage_pos;
+        if (map != nullptr && tid < ATTN_ROWS) key_doc[tid] = stage_doc;
+        const int here = tile, base = here * ATTN_ROWS;
+        tile = next_tile(map, here + 1, end);
+        if (tile < end) load(tile);
+        __syncthreads();
+        if (base >= wave_limit) continue;
+        const bool by_doc = !tile_same(map, here), by_limit = base + ATTN_ROWS > wave_full;
+
+#pragma unroll
+        for (int tp = 0; tp < 2; ++tp) {
+            f32x4 w[2][NQ];
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                const int at = 32 * tp + 16 * t;
+                f32x4 s[NQ], dp[NQ];
+                Frag<TYPE, DP> f;
+                frag_from_lds<TYPE, DP>(f, Kt, at + c, g);
+#pragma unroll
+                for (int n = 0; n < NQ; ++n) s[n] = dot_block<TYPE, DP>(f, qf[n]);
+                frag_from_lds<TYPE, DP>(f, Vt, at + c, g);
+#pragma unroll
+                for (int n = 0; n < NQ; ++n) dp[n] = dot_block<TYPE, DP>(f, of[n]);
+                f32x4 p0 = {0, 0, 0, 0}, p1 = {0, 0, 0, 0};
+                i32x4 kd = {0, 0, 0, 0};
+                if (sp.bias == 2) {
+                    p0 = *reinterpret_cast<const f32x4 *>(key_pos + 2 * (at + 4 * g));
+                    p1 = *reinterpret_cast<const f32x4 *>(key_pos + 2 * (at + 4 * g) + 4);
+                }
+                if (by_doc) kd = *reinterpret_cast<const i32x4 *>(key_doc + at + 4 * g);
+                const float kx[4] = {p0[0], p0[2], p1[0], p1[2]}, ky[4] = {p0[1], p0[3], p1[1], p1[3]};
+                const float k0 = (float)(base + at + 4 * g);
+#pragma unroll
+                for (int n = 0; n < NQ; ++n) {
+                    f32x4 x = s[n] * sp.mul, slack = {1.0f, 1.0f, 1.0f, 1.0f}, dist = {0, 0, 0, 0};
+                    if (sp.cap) {
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) {
+                            const float th = attn_tanh(x[r]);
+                            slack[r] = fmaf(-th, th, 1.0f);
+                            x[r] = sp.cap2 * th;
+                        }
+                    }
+                    if (sp.bias == 1) {
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) dist[r] = fabsf(qx[n] - (k0 + (float)r));
+                    } else if (sp.bias == 2) {
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) {
+                            const float dx = qx[n] - kx[r], dy = qy[n] - ky[r];
+                            dist[r] = __builtin_amdgcn_sqrtf(fmaf(dx, dx, dy * dy));
+                        }
+                    }
+                    if (sp.bias) {
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) x[r] = fmaf(-sp.slope2, dist[r], x[r]);
+                    }
+                    f32x4 p, ds;
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) p[r] = __builtin_amdgcn_exp2f(x[r] - lse2[n]);
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) ds[r] = p[r] * (dp[n][r] - delta[n]);
+                    if (by_limit || by_doc) {
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) {
+                            const bool ok = base + at + 4 * g + r < limit[n] && (!by_doc || kd[r] == doc[n]);
+                            p[r] = ok ? p[r] : 0.0f;
+                            ds[r] = ok ? ds[r] : 0.0f;
+                            dist[r] = ok ? dist[r] : 0.0f;
+                        }
+                    }
+                    if (want_slope) {
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) {
+                            excess[n] += ds[r];
+                            pd[n] = fmaf(p[r], dist[r], pd[n]);
+                            dsl[n] = fmaf(ds[r], dist[r], dsl[n]);
+                        }
+                    }
+                    if (TYPE == ATTN_F16) ds = ds * rs[n];
+                    w[t][n] = ds * slack;
+                }
+            }
+            accumulate<TYPE, DP, NQ>(dq, Kt, KT, tp, w[0], w[1], g, c);
+        }
+    }
+
+    float slope_sum = 0.0f;
+#pragma unroll
+    for (int n = 0; n < NQ; ++n) {
+        const int i = wrow0 + 16 * n + c;
+        const bool live = i < a.Lq;
+        bool fine = true;
+        const float undo = TYPE == ATTN_F16 ? a.scale / rs[n] : a.scale;
+#pragma unroll
+        for (int d = 0; d < S::dt; ++d) fine = fine && finite4(dq[n][d]);
+        if (live) {
+            raw *out = reinterpret_cast<raw *>(a.dq) + b * a.dqst[0] + h * a.dqst[1] + (int64_t)i * a.dqst[2];
+#pragma unroll
+            for (int d = 0; d < S::dt; ++d)
+                if (16 * d + 4 * g < a.D) store4<TYPE>(out + 16 * d + 4 * g, dq[n][d] * undo);
+        }
+        unsigned long long bad = __ballot(!fine && live);
+        bad = (bad | bad >> 16 | bad >> 32 | bad >> 48) & 0xffff;
+        for (; bad != 0; bad &= bad - 1) {
+            const int cc = __ffsll((long long)bad) - 1;
+            careful_dq_row<TYPE>(a, sp, b, h, wrow0 + 16 * n + cc, __shfl(lse2[n], cc), __shfl(delta[n], cc));
+        }
+        if (want_slope) {
+            const float e = group_sum(excess[n]), x = group_sum(pd[n]), y = group_sum(dsl[n]);
+            slope_sum += live ? fmaf(-e, x, y) : 0.0f;
+        }
+    }
+    if (want_slope) {
+#pragma unroll
+        for (int x = 1; x < 16; x <<= 1) slope_sum += __shfl_xor(slope_sum, x);
+        if (lane == 0) part[wave] = slope_sum;
+        __syncthreads();
+        if (tid == 0) a.dslope_part[(int64_t)bh * a.tiles + qt] = (part[0] + part[1]) + (part[2] + part[3]);
+    }
+}
+
+// dslope[h] = - sum over batch entries and row blocks, in a fixed order, in binary64
+__global__ __launch_bounds__(256) void attn_dslope_kernel(AttnArgs a) {
+    __shared__ double sums[256];
+    const int h = blockIdx.x, tid = threadIdx.x;
+    double s = 0.0;
+    for (int64_t x = tid; x < (int64_t)a.B * a.tiles; x += 256)
+        s += (double)a.dslope_part[((x / a.tiles) * a.Hq + h) * a.tiles + x % a.tiles];
+    sums[tid] = s;
+    __syncthreads();
+    for (int w = 128; w > 0; w >>= 1) {
+        if (tid < w) sums[tid] += sums[tid + w];
+        __syncthreads();
+    }
+    if (tid == 0) a.dslope[h] = (float)-sums[0];
+}
+
+// ----------------------------------------------------------------------------------------------- backward: key rows
+// dk and dv of NK x 16 keys per wave, over the query rows of all heads that share them.  Lane (g, c) holds key c and, per
+// 16 queries, the pairs with queries 4 g + r.
+template <int TYPE>
+__device__ void careful_dkv_row(const AttnArgs &a, int b, int hk, int j) {
+    typedef typename Elem<TYPE>::raw raw;
+    const int lane = threadIdx.x & 63;
+    const raw *k = reinterpret_cast<const raw *>(a.k) + b * a.ks[0] + hk * a.ks[1] + j * a.ks[2];
+    const raw *v = reinterpret_cast<const raw *>(a.v) + b * a.vs[0] + hk * a.vs[1] + j * a.vs[2];
+    float gk[2] = {0.0f, 0.0f}, gv[2] = {0.0f, 0.0f};
+    for (int h = hk * a.G; h < (hk + 1) * a.G; ++h) {
+        const ScoreParams sp = score_params(a, h);
+        const raw *q = reinterpret_cast<const raw *>(a.q) + b * a.qs[0] + h * a.qs[1];
+        const raw *o = reinterpret_cast<const raw *>(a.dout) + b * a.dos[0] + h * a.dos[1];
+        for (int base = 0; base < a.Lq; base += 64) {
+            const int i = base + lane;
+            const bool ok = i < a.Lq && pair_allowed(a, b, i, j, row_limit(a, b, i));
+            float p = 0.0f, ds = 0.0f, th, dist;
+            if (ok) {
+                const int64_t at = ((int64_t)b * a.Hq + h) * a.Lq + i;
+                p = __builtin_amdgcn_exp2f(pair_score<TYPE>(a, sp, b, i, j, q + i * a.qs[2], k, th, dist) - a.lse[at] * ATTN_LOG2E);
+                float dp = 0.0f;
+                for (int d = 0; d < a.D; ++d) dp = fmaf(elem_to_float<TYPE>(o[i * a.dos[2] + d]), elem_to_float<TYPE>(v[d]), dp);
+                ds = p * (dp - a.delta[at]);
+                if (sp.cap) ds *= fmaf(-th, th, 1.0f);
+            }
+            for (unsigned long long w = __ballot(ok); w != 0; w &= w - 1) {
+                const int ii = __ffsll((long long)w) - 1;
+                const float x = __shfl(ds, ii), y = __shfl(p, ii);
+                for (int half = 0; half < 2; ++half) {
+                    const int d = lane + 64 * half;
+                    if (d < a.D) {
+                        gk[half] = fmaf(x, elem_to_float<TYPE>(q[(int64_t)(base + ii) * a.qs[2] + d]), gk[half]);
+                        gv[half] = fmaf(y, elem_to_float<TYPE>(o[(int64_t)(base + ii) * a.dos[2] + d]), gv[half]);
+                    }
+                }
+            }
+        }
+    }
+    for (int which = 0; which < 2; ++which) {
+        raw *out = which ? reinterpret_cast<raw *>(a.dv) + b * a.dvst[0] + hk * a.dvst[1] + j * a.dvst[2]
+                         : reinterpret_cast<raw *>(a.dk) + b * a.dkst[0] + hk * a.dkst[1] + j * a.dkst[2];
+        for (int half = 0; half < 2; ++half) {
+            const int d = lane + 64 * half;
+            const float x = which ? gv[half] : gk[half] * a.scale;
+            if (d < a.D) {
+                if constexpr (TYPE == ATTN_F32) out[d] = x;
+                else if constexpr (TYPE == ATTN_F16) out[d] = __builtin_bit_cast(unsigned short, (_Float16)x);
+                else out[d] = __builtin_bit_cast(unsigned short, (__bf16)x);
+            }
+        }
+    }
+}
+
+#define F16_P_SCALE 1024.0f      // probabilities (<= 1) are rounded to binary16 times 2^10: those of long rows stay normal
+
+template <int TYPE, int DP, int NK>
+__global__ __launch_bounds__(ATTN_THREADS, DP <= 64 ? 2 : 1) void attn_bwd_kv_kernel(AttnArgs a) {
+    typedef Shape<TYPE, DP> S;
+    typedef typename Elem<TYPE>::raw raw;
+    constexpr int ROWS = 64 * NK, UNITS = (2 * S::units + ATTN_THREADS - 1) / ATTN_THREADS;
+    __shared__ __align__(16) char lds[2 * S::row_bytes + 2 * S::t_bytes];
+    __shared__ __align__(16) float row_lse[ATTN_ROWS], row_delta[ATTN_ROWS], row_x[ATTN_ROWS], row_y[ATTN_ROWS];
+    __shared__ __align__(16) int row_lim[ATTN_ROWS], row_doc[ATTN_ROWS];
+    __shared__ TileMap map_store;
+    __shared__ unsigned least_scale;
+    raw *Qt = reinterpret_cast<raw *>(lds), *Ot = reinterpret_cast<raw *>(lds + S::row_bytes);
+    raw *QT = reinterpret_cast<raw *>(lds + 2 * S::row_bytes), *OT = reinterpret_cast<raw *>(lds + 2 * S::row_bytes + S::t_bytes);
+
+    const int work = xcd_work();
+    if (work >= a.B * a.Hkv * a.tiles) return;
+    const int bh = work / a.tiles, kt = work % a.tiles;          // (causal: the first keys are seen by the most rows)
+    const int b = bh / a.Hkv, hk = bh % a.Hkv;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g = lane >> 4, c = lane & 15;
+    const int row0 = kt * ROWS, wrow0 = row0 + wave * 16 * NK;
+    const raw *k = reinterpret_cast<const raw *>(a.k) + b * a.ks[0] + hk * a.ks[1];
+    const raw *v = reinterpret_cast<const raw *>(a.v) + b * a.vs[0] + hk * a.vs[1];
+    const int *docs = a.doc_q != nullptr ? a.doc_q + b * a.dqs : nullptr;
+
+    TileMap *map = nullptr;
+    if (docs != nullptr) {
+        map = &map_store;
+        build_tile_map(map_store, a.doc_k + b * a.dks, row0, ROWS, a.Lk, docs, a.Lq);
+    }
+    zero_padding<TYPE, DP>(Qt);
+    zero_padding<TYPE, DP>(Ot);
+
+    Frag<TYPE, DP> kf[NK], vf[NK];
+    f32x4 dk[NK][S::dt], dv[NK][S::dt];
+    float kx[NK], ky[NK];
+    int doc[NK];
+#pragma unroll
+    for (int n = 0; n < NK; ++n) {
+        const int j = wrow0 + 16 * n + c;
+        const bool live = j < a.Lk;
+        frag_from_global<TYPE, DP>(kf[n], k + (int64_t)j * a.ks[2], live, a.D, g);
+        frag_from_global<TYPE, DP>(vf[n], v + (int64_t)j * a.vs[2], live, a.D, g);
+        doc[n] = map != nullptr ? doc_of_key(a, b, j) : 0;
+        kx[n] = ky[n] = 0.0f;
+        if (a.bias == 1) kx[n] = (float)j;
+        if (a.bias == 2 && live) {
+            kx[n] = a.pos_k[b * a.pks + 2 * (int64_t)j];
+            ky[n] = a.pos_k[b * a.pks + 2 * (int64_t)j + 1];
+        }
+#pragma unroll
+        for (int d = 0; d < S::dt; ++d) dk[n][d] = dv[n][d] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    }
+    // the first query row that sees the first key of this block / of this wave
+    int first = 0;
+    if (a.causal && (a.prefix == nullptr || row0 >= a.prefix[b])) first = max(0, row0 - (a.Lk - a.Lq));
+    const int begin = min(first, a.Lq) / ATTN_ROWS, end = (a.Lq + ATTN_ROWS - 1) / ATTN_ROWS;
+    int wave_first = 0;                              // rows before it see no key of the wave
+    if (a.causal && (a.prefix == nullptr || wrow0 >= a.prefix[b])) wave_first = max(0, wrow0 - (a.Lk - a.Lq));
+    const int wave_all = a.causal ? wrow0 + 16 * NK - 1 - (a.Lk - a.Lq) : 0;   // rows from here on see all keys of the wave
+    const bool tail = wrow0 + 16 * NK > a.Lk;
+
+    float gscale = 1.0f, undo = a.scale;
+    if constexpr (TYPE == ATTN_F16) {               // one scale for all rows: that of the largest gradient among them
+        if (tid == 0) least_scale = 0x7f000000u;
+        __syncthreads();
+        for (int64_t x = tid; x < (int64_t)a.G * a.Lq; x += ATTN_THREADS)
+            atomicMin(&least_scale, __float_as_uint(a.rowscale[((int64_t)b * a.Hq + hk * a.G) * a.Lq + x]));
+        __syncthreads();
+        gscale = __uint_as_float(least_scale);
+        undo = a.scale / gscale;
+    }
+
+    for (int h = hk * a.G; h < (hk + 1) * a.G; ++h) {
+        const raw *q = reinterpret_cast<const raw *>(a.q) + b * a.qs[0] + h * a.qs[1];
+        const raw *go = reinterpret_cast<const raw *>(a.dout) + b * a.dos[0] + h * a.dos[1];
+        const float *lse = a.lse + ((int64_t)b * a.Hq + h) * a.Lq, *del = a.delta + ((int64_t)b * a.Hq + h) * a.Lq;
+        const ScoreParams sp = score_params(a, h);
+        Unit un[UNITS];
+        float st_lse = 0.0f, st_delta = 0.0f, st_x = 0.0f, st_y = 0.0f;
+        int st_lim = 0, st_doc = -2;
+        auto load = [&](int tile) {
+            const int base = tile * ATTN_ROWS;
+#pragma unroll
+            for (int x = 0; x < UNITS; ++x) {
+                const int u = tid + x * ATTN_THREADS;
+                if (u < S::units) unit_load<TYPE, DP>(un[x], u, q, a.qs[2], base, a.Lq, a.D, docs);
+                else if (u < 2 * S::units) unit_load<TYPE, DP>(un[x], u - S::units, go, a.dos[2], base, a.Lq, a.D, docs);
+            }
+            if (tid < ATTN_ROWS) {
+                const int i = base + tid;
+                const bool live = i < a.Lq;
+                const float e = live ? lse[i] : -attn_inf();
+                st_lse = e == -attn_inf() ? attn_inf() : e * ATTN_LOG2E;
+                st_delta = live ? del[i] : 0.0f;
+                st_lim = row_limit(a, b, i);
+                if (map != nullptr) st_doc = doc_of_query(a, b, i);
+                if (a.bias == 1) st_x = (float)(i + a.Lk - a.Lq);
+                if (a.bias == 2 && live) {
+                    st_x = a.pos_q[b * a.pqs + 2 * (int64_t)i];
+                    st_y = a.pos_q[b * a.pqs + 2 * (int64_t)i + 1];
+                }
+            }
+        };
+        int tile = next_tile(map, begin, end);
+        if (tile < end) load(tile);
+        while (tile < end) {
+            __syncthreads();
+#pragma unroll
+            for (int x = 0; x < UNITS; ++x) {
+                const int u = tid + x * ATTN_THREADS;
+                if (u < S::units) unit_write<TYPE, DP, true, true>(un[x], u, Qt, QT);
+                else if (u < 2 * S::units) unit_write<TYPE, DP, true, true>(un[x], u - S::units, Ot, OT);
+            }
+            if (tid < ATTN_ROWS) {
+                row_lse[tid] = st_lse;
+                row_delta[tid] = st_delta;
+                row_lim[tid] = st_lim;
+                row_doc[tid] = st_doc;
+                row_x[tid] = st_x;
+                row_y[tid] = st_y;
+            }
+            const int here = tile, base = here * ATTN_ROWS;
+            tile = next_tile(map, here + 1, end);
+            if (tile < end) load(tile);
+            __syncthreads();
+            if (base + ATTN_ROWS <= wave_first || wrow0 >= a.Lk) continue;
+            const bool by_doc = !tile_same(map, here), by_limit = tail || base < wave_all || base + ATTN_ROWS > a.Lq;
+
+#pragma unroll
+            for (int tp = 0; tp < 2; ++tp) {
+                f32x4 wp[2][NK], ws[2][NK];
+#pragma unroll
+                for (int t = 0; t < 2; ++t) {
+                    const int at = 32 * tp + 16 * t;
+                    f32x4 s[NK], dp[NK];
+                    Frag<TYPE, DP> f;
+                    frag_from_lds<TYPE, DP>(f, Qt, at + c, g);
+#pragma unroll
+                    for (int n = 0; n < NK; ++n) s[n] = dot_block<TYPE, DP>(f, kf[n]);
+                    frag_from_lds<TYPE, DP>(f, Ot, at + c, g);
+#pragma unroll
+                    for (int n = 0; n < NK; ++n) dp[n] = dot_block<TYPE, DP>(f, vf[n]);
+                    const f32x4 e = *reinterpret_cast<const f32x4 *>(row_lse + at + 4 * g);
+                    const f32x4 dl = *reinterpret_cast<const f32x4 *>(row_delta + at + 4 * g);
+                    f32x4 qx = {0, 0, 0, 0}, qy = {0, 0, 0, 0};
+                    i32x4 lim = {0, 0, 0, 0}, qd = {0, 0, 0, 0};
+                    if (sp.bias) qx = *reinterpret_cast<const f32x4 *>(row_x + at + 4 * g);
+                    if (sp.bias == 2) qy = *reinterpret_cast<const f32x4 *>(row_y + at + 4 * g);
+                    if (by_limit || by_doc) lim = *reinterpret_cast<const i32x4 *>(row_lim + at + 4 * g);
+                    if (by_doc) qd = *reinterpret_cast<const i32x4 *>(row_doc + at + 4 * g);
+#pragma unroll
+                    for (int n = 0; n < NK; ++n) {
+                        f32x4 x = s[n] * sp.mul, slack = {1.0f, 1.0f, 1.0f, 1.0f};
+                        if (sp.cap) {
+#pragma unroll
+                            for (int r = 0; r < 4; ++r) {
+                                const float th = attn_tanh(x[r]);
+                                slack[r] = fmaf(-th, th, 1.0f);
+                                x[r] = sp.cap2 * th;
+                            }
+                        }
+                        if (sp.bias == 1) {
+#pragma unroll
+                            for (int r = 0; r < 4; ++r) x[r] = fmaf(-sp.slope2, fabsf(qx[r] - kx[n]), x[r]);
+                        } else if (sp.bias == 2) {
+#pragma unroll
+                            for (int r = 0; r < 4; ++r) {
+                                const float dx = qx[r] - kx[n], dy = qy[r] - ky[n];
+                                x[r] = fmaf(-sp.slope2, __builtin_amdgcn_sqrtf(fmaf(dx, dx, dy * dy)), x[r]);
+                            }
+                        }
+                        f32x4 p, ds;
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) p[r] = __builtin_amdgcn_exp2f(x[r] - e[r]);
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) ds[r] = p[r] * (dp[n][r] - dl[r]);
+                        if (by_limit || by_doc) {
+                            const int j = wrow0 + 16 * n + c;
+#pragma unroll
+                            for (int r = 0; r < 4; ++r) {
+                                const bool ok = j < lim[r] && (!by_doc || qd[r] == doc[n]);
+                                p[r] = ok ? p[r] : 0.0f;
+                                ds[r] = ok ? ds[r] : 0.0f;
+                            }
+                        }
+                        ds = ds * slack;
+                        if (TYPE == ATTN_F16) {
+                            p = p * F16_P_SCALE;
+                            ds = ds * gscale;
+                        }
+                        wp[t][n] = p;
+                        ws[t][n] = ds;
+                    }
+                }
+                accumulate<TYPE, DP, NK>(dv, Ot, OT, tp, wp[0], wp[1], g, c);
+                accumulate<TYPE, DP, NK>(dk, Qt, QT, tp, ws[0], ws[1], g, c);
+            }
+        }
+    }
+
+#pragma unroll
+    for (int n = 0; n < NK; ++n) {
+        const int j = wrow0 + 16 * n + c;
+        const bool live = j < a.Lk;
+        bool fine = true;
+        const float undo_v = TYPE == ATTN_F16 ? 1.0f / F16_P_SCALE : 1.0f;
+#pragma unroll
+        for (int d = 0; d < S::dt; ++d) fine = fine && finite4(dk[n][d]) && finite4(dv[n][d]);
+        if (live) {
+            raw *outk = reinterpret_cast<raw *>(a.dk) + b * a.dkst[0] + hk * a.dkst[1] + (int64_t)j * a.dkst[2];
+            raw *outv = reinterpret_cast<raw *>(a.dv) + b * a.dvst[0] + hk * a.dvst[1] + (int64_t)j * a.dvst[2];
+#pragma unroll
+            for (int d = 0; d < S::dt; ++d)
+                if (16 * d + 4 * g < a.D) {
+                    store4<TYPE>(outk + 16 * d + 4 * g, dk[n][d] * undo);
+                    store4<TYPE>(outv + 16 * d + 4 * g, dv[n][d] * undo_v);
+                }
+        }
+        unsigned long long bad = __ballot(!fine && live);
+        bad = (bad | bad >> 16 | bad >> 32 | bad >> 48) & 0xffff;
+        for (; bad != 0; bad &= bad - 1) careful_dkv_row<TYPE>(a, b, hk, wrow0 + 16 * n + __ffsll((long long)bad) - 1);
+    }
+}
+
+// ------------------------------------------------------------------------------------------------------------ launch
+bool aligned_strides(const int64_t *s, const void *p, int bytes) {
+    if ((reinterpret_cast<uintptr_t>(p) & 15) != 0) return false;
+    for (int i = 0; i < 3; ++i)
+        if ((s[i] * bytes) % 16 != 0 || s[i] < 0) return false;
+    return true;
+}
+
+int check_attention(const dgl_attention_t *p) {
+    DGL_CHECK_ARG(p != nullptr, "NULL argument");
+    DGL_CHECK_ARG(p->dtype >= DGL_DTYPE_F32 && p->dtype <= DGL_DTYPE_BF16, "unknown element type %d", p->dtype);
+    DGL_CHECK_ARG(p->B >= 1 && p->Hq >= 1 && p->Hkv >= 1 && p->Lq >= 0 && p->Lk >= 0, "B=%d Hq=%d Hkv=%d Lq=%d Lk=%d", p->B, p->Hq,
+                  p->Hkv, p->Lq, p->Lk);
+    DGL_CHECK_ARG(p->Hq % p->Hkv == 0, "%d query heads over %d key heads", p->Hq, p->Hkv);
+    DGL_CHECK_ARG(p->D >= 8 && p->D <= 128 && p->D % 8 == 0, "head size %d (a multiple of 8, at most 128)", p->D);
+    DGL_CHECK_ARG(p->Lq <= DGL_ATTENTION_MAX_LENGTH && p->Lk <= DGL_ATTENTION_MAX_LENGTH, "length above %d", DGL_ATTENTION_MAX_LENGTH);
+    DGL_CHECK_ARG(p->scale == p->scale && p->cap >= 0.0f && p->cap < 3.0e38f, "scale %g, cap %g", (double)p->scale, (double)p->cap);
+    DGL_CHECK_ARG((p->pos_q == nullptr) == (p->pos_k == nullptr), "coordinates of one side only");
+    DGL_CHECK_ARG(p->pos_q == nullptr || p->slope != nullptr, "coordinates without a slope");
+    DGL_CHECK_ARG((p->doc_q == nullptr) == (p->doc_k == nullptr), "document ids of one side only");
+    DGL_CHECK_ARG(p->prefix == nullptr || p->causal, "a prefix belongs to a causal mask");
+    DGL_CHECK_ARG((int64_t)p->B * p->Hq * (((p->Lq > p->Lk ? p->Lq : p->Lk) + 63) / 64) < (1ll << 30), "too many rows");
+    const int bytes = p->dtype == DGL_DTYPE_F32 ? 4 : 2;
+    DGL_CHECK_ARG(p->Lq == 0 || (p->q != nullptr && p->out != nullptr), "q or out is NULL");
+    DGL_CHECK_ARG(p->Lk == 0 || (p->k != nullptr && p->v != nullptr), "k or v is NULL");
+    DGL_CHECK_ARG(aligned_strides(p->q_stride, p->q, bytes) && aligned_strides(p->k_stride, p->k, bytes) &&
+                      aligned_strides(p->v_stride, p->v, bytes) && aligned_strides(p->o_stride, p->out, bytes),
+                  "q, k, v, out: 16-byte aligned pointers and strides");
+    return DGL_OK;
+}
+
+AttnArgs attention_args(const dgl_attention_t *p) {
+    AttnArgs a{};
+    a.q = (const char *)p->q; a.k = (const char *)p->k; a.v = (const char *)p->v; a.out = (char *)p->out; a.lse = p->lse;
+    for (int i = 0; i < 3; ++i) { a.qs[i] = p->q_stride[i]; a.ks[i] = p->k_stride[i]; a.vs[i] = p->v_stride[i]; a.os[i] = p->o_stride[i]; }
+    a.B = p->B; a.Hq = p->Hq; a.Hkv = p->Hkv; a.G = p->Hq / p->Hkv; a.Lq = p->Lq; a.Lk = p->Lk; a.D = p->D;
+    a.causal = p->causal != 0; a.scale = p->scale; a.cap = p->cap;
+    a.bias = p->slope == nullptr ? 0 : p->pos_q == nullptr ? 1 : 2;
+    a.slope = p->slope; a.pos_q = p->pos_q; a.pos_k = p->pos_k; a.pqs = p->pos_q_stride; a.pks = p->pos_k_stride;
+    a.doc_q = p->doc_q; a.doc_k = p->doc_k; a.dqs = p->doc_q_stride; a.dks = p->doc_k_stride; a.prefix = p->prefix;
+    return a;
+}
+
+unsigned xcd_grid(int64_t work) { return (unsigned)((work + 7) / 8 * 8); }
+int padded(int D) { return D <= 16 ? 16 : D <= 32 ? 32 : D <= 64 ? 64 : 128; }
+
+// Two blocks of 16 query rows per wave halve the LDS reads per pair; one where that would leave compute units idle
+// (fewer than two workgroups for each of the 256).
+bool two_blocks(const AttnArgs &a, int rows, int heads) { return (int64_t)a.B * heads * ((rows + 127) / 128) >= 512; }
+
+template <template <int, int, int> class Launch> int by_type(const AttnArgs &a, int dtype, int n, hipStream_t s) {
+#define ATTN_CASE(T, DPV) \
+    if (dtype == T && padded(a.D) == DPV) return n == 2 ? Launch<T, DPV, 2>::go(a, s) : Launch<T, DPV, 1>::go(a, s);
+    ATTN_CASE(ATTN_F32, 16) ATTN_CASE(ATTN_F32, 32) ATTN_CASE(ATTN_F32, 64) ATTN_CASE(ATTN_F32, 128)
+    ATTN_CASE(ATTN_F16, 16) ATTN_CASE(ATTN_F16, 32) ATTN_CASE(ATTN_F16, 64) ATTN_CASE(ATTN_F16, 128)
+    ATTN_CASE(ATTN_BF16, 16) ATTN_CASE(ATTN_BF16, 32) ATTN_CASE(ATTN_BF16, 64) ATTN_CASE(ATTN_BF16, 128)
+#undef ATTN_CASE
+    return dgl_set_error(DGL_ERR_INVALID_ARGUMENT, "unknown element type %d", dtype);
+}
+template <int T, int DP, int N> struct LaunchFwd {
+    static int go(AttnArgs a, hipStream_t s) {
+        a.tiles = (a.Lq + 64 * N - 1) / (64 * N);
+        hipLaunchKernelGGL((attn_fwd_kernel<T, DP, N>), dim3(xcd_grid((int64_t)a.B * a.Hq * a.tiles)), dim3(ATTN_THREADS), 0, s, a);
+        DGL_CHECK_LAUNCH("dgl_attention_forward");
+        return DGL_OK;
+    }
+};
+template <int T, int DP, int N> struct LaunchBwdQ {
+    static int go(AttnArgs a, hipStream_t s) {
+        a.tiles = (a.Lq + 64 * N - 1) / (64 * N);
+        hipLaunchKernelGGL((attn_bwd_q_kernel<T, DP, N>), dim3(xcd_grid((int64_t)a.B * a.Hq * a.tiles)), dim3(ATTN_THREADS), 0, s, a);
+        DGL_CHECK_LAUNCH("dgl_attention_backward (query rows)");
+        if (a.dslope != nullptr) {
+            hipLaunchKernelGGL(attn_dslope_kernel, dim3(a.Hq), dim3(256), 0, s, a);
+            DGL_CHECK_LAUNCH("dgl_attention_backward (slopes)");
+        }
+        return DGL_OK;
+    }
+};
+template <int T, int DP, int N> struct LaunchBwdKv {
+    static int go(AttnArgs a, hipStream_t s) {
+        a.tiles = (a.Lk + 64 * N - 1) / (64 * N);
+        hipLaunchKernelGGL((attn_bwd_kv_kernel<T, DP, N>), dim3(xcd_grid((int64_t)a.B * a.Hkv * a.tiles)), dim3(ATTN_THREADS), 0, s, a);
+        DGL_CHECK_LAUNCH("dgl_attention_backward (key rows)");
+        return DGL_OK;
+    }
+};
+
+}  // namespace
+
+extern "C" int dgl_attention_forward(const dgl_attention_t *p, dgl_stream_t stream) {
+    if (int e = check_attention(p)) return e;
+    if (p->Lq == 0) return DGL_OK;
+    const AttnArgs a = attention_args(p);
+    return by_type<LaunchFwd>(a, p->dtype, two_blocks(a, a.Lq, a.Hq) ? 2 : 1, (hipStream_t)stream);
+}
+
+extern "C" int64_t dgl_attention_backward_workspace_floats(const dgl_attention_t *p) {
+    if (check_attention(p) != DGL_OK) return -1;
+    const int64_t rows = (int64_t)p->B * p->Hq * p->Lq;
+    return 2 * rows + (int64_t)p->B * p->Hq * ((p->Lq + 63) / 64) + 4;
+}
+
+extern "C" int dgl_attention_backward(const dgl_attention_t *p, const dgl_attention_grad_t *g, float *ws, dgl_stream_t stream) {
+    if (int e = check_attention(p)) return e;
+    DGL_CHECK_ARG(g != nullptr && ws != nullptr, "NULL argument");
+    DGL_CHECK_ARG((p->Lq == 0 || (g->dout != nullptr && g->dq != nullptr && p->lse != nullptr)) &&
+                      (p->Lk == 0 || (g->dk != nullptr && g->dv != nullptr)), "dout, dq, dk, dv or lse is NULL");
+    DGL_CHECK_ARG(g->dslope == nullptr || p->slope != nullptr, "dslope without a slope");
+    const int bytes = p->dtype == DGL_DTYPE_F32 ? 4 : 2;
+    DGL_CHECK_ARG(aligned_strides(g->dout_stride, g->dout, bytes) && aligned_strides(g->dq_stride, g->dq, bytes) &&
+                      aligned_strides(g->dk_stride, g->dk, bytes) && aligned_strides(g->dv_stride, g->dv, bytes),
+                  "dout, dq, dk, dv: 16-byte aligned pointers and strides");
+    AttnArgs a = attention_args(p);
+    a.dout = (const char *)g->dout; a.dq = (char *)g->dq; a.dk = (char *)g->dk; a.dv = (char *)g->dv; a.dslope = g->dslope;
+    for (int i = 0; i < 3; ++i) {
+        a.dos[i] = g->dout_stride[i]; a.dqst[i] = g->dq_stride[i]; a.dkst[i] = g->dk_stride[i]; a.dvst[i] = g->dv_stride[i];
+    }
+    const int64_t rows = (int64_t)p->B * p->Hq * p->Lq;
+    a.delta = ws;
+    a.rowscale = ws + rows;
+    a.dslope_part = g->dslope != nullptr ? ws + 2 * rows : nullptr;
+    // (no rows: the slope's gradient is the empty sum, and the launcher of the query kernel would have an empty grid)
+    if (p->Lq > 0) {
+        if (int e = by_type<LaunchBwdQ>(a, p->dtype, two_blocks(a, a.Lq, a.Hq) ? 2 : 1, (hipStream_t)stream)) return e;
+    } else if (a.dslope != nullptr) {
+        a.tiles = 0;
+        hipLaunchKernelGGL(attn_dslope_kernel, dim3(a.Hq), dim3(256), 0, (hipStream_t)stream, a);
+        DGL_CHECK_LAUNCH("dgl_attention_backward (slopes)");
+    }
+    if (p->Lk > 0) return by_type<LaunchBwdKv>(a, p->dtype, two_blocks(a, a.Lk, a.Hkv) ? 2 : 1, (hipStream_t)stream);
+    return DGL_OK;
+}

@@ -359,6 +359,61 @@ DGL_API int dgl_adam_step(float *params, const float *grads, float *exp_avg, flo
                           int32_t step, float lr, float beta1, float beta2, float eps, float weight_decay,
                           float grad_scale, dgl_stream_t stream);
 
+/* ------------------------------------------------------------------ attention over nodes and sequences
+ * Multi-head attention of any length as an operator of its own (the reference's softmax(q k^T / sqrt(d)) v over the
+ * tokens of one row is TSP/TSPModel.py:420-441, which dgl_policy_forward / dgl_policy_general evaluate inside the network),
+ * extended by what attention over whole instances and over sequences needs:
+ *   s_ij = cap tanh(scale q_i.k_j / cap) - slope[h] dist(i, j)   cap = 0: no tanh; slope NULL: no bias
+ *   dist(i, j): Euclidean distance of pos_q[b][i], pos_k[b][j] (x, y), or |i + Lk - Lq - j| where pos_q = pos_k = NULL
+ *   allowed(i, j): doc_q[b][i] == doc_k[b][j] >= 0 where given (a negative id is padding: such a row is zeros, such a key
+ *     is seen by nobody), and with causal != 0 also j <= i + Lk - Lq or j < prefix[b] (prefix NULL: 0)
+ *   out_i = sum over allowed j of softmax_j(s_ij) v_j; a row without an allowed key is zeros with lse = -inf.
+ * Query head h reads key head h / (Hq / Hkv).  A masked pair contributes nothing, whatever its operands hold (NaN and
+ * infinities included).  Tensors are addressed by strides in elements {batch, head, token}, the head's D elements are
+ * consecutive; pointers and strides are multiples of 16 bytes, strides may be 0 for inputs.  D is a multiple of 8, at most
+ * 128; lengths may be 0 and are at most DGL_ATTENTION_MAX_LENGTH.  Scores, softmax and sums are binary32 for every
+ * element type; for the 16-bit types probabilities (and, backward, score gradients) are rounded to the type before they
+ * multiply v (k, q, dout). */
+#define DGL_DTYPE_F32 0
+#define DGL_DTYPE_F16 1
+#define DGL_DTYPE_BF16 2
+#define DGL_ATTENTION_MAX_LENGTH (1 << 24)
+
+typedef struct {
+    int32_t dtype;             /* DGL_DTYPE_* of q, k, v, out (and of the gradients) */
+    int32_t B, Hq, Hkv, Lq, Lk, D;
+    int32_t causal;
+    float scale, cap;
+    int64_t q_stride[3], k_stride[3], v_stride[3], o_stride[3];
+    const void *q, *k, *v;
+    void *out;
+    float *lse;                /* [B][Hq][Lq] log of the softmax's denominator; may be NULL without a backward pass */
+    const float *slope;        /* [Hq] or NULL */
+    const float *pos_q, *pos_k;             /* [B][Lq][2], [B][Lk][2] or both NULL */
+    int64_t pos_q_stride, pos_k_stride;     /* floats between batch entries */
+    const int32_t *doc_q, *doc_k;           /* [B][Lq], [B][Lk] or both NULL */
+    int64_t doc_q_stride, doc_k_stride;     /* ids between batch entries */
+    const int32_t *prefix;     /* [B] or NULL */
+} dgl_attention_t;
+
+typedef struct {
+    const void *dout;
+    void *dq, *dk, *dv;
+    int64_t dout_stride[3], dq_stride[3], dk_stride[3], dv_stride[3];
+    float *dslope;             /* [Hq] or NULL */
+} dgl_attention_grad_t;
+
+/* The operator above (beside TSP/TSPModel.py:420-441). */
+DGL_API int dgl_attention_forward(const dgl_attention_t *a, dgl_stream_t stream);
+
+/* Gradients of a forward call with the same arguments, whose out and lse are given in `a`: dq, dk, dv (written, not added
+ * to) and, where wanted, the slopes' gradient (the reference's loss.backward() through TSP/TSPModel.py:420-441).  Sums are
+ * ordered: the same call gives the same bits.  ws: dgl_attention_backward_workspace_floats(a) floats. */
+DGL_API int dgl_attention_backward(const dgl_attention_t *a, const dgl_attention_grad_t *g, float *ws, dgl_stream_t stream);
+
+/* Floats of workspace dgl_attention_backward needs for `a` (-1: invalid arguments; beside TSP/TSPModel.py:420-441). */
+DGL_API int64_t dgl_attention_backward_workspace_floats(const dgl_attention_t *a);
+
 /* ----------------------------------------------------------------- augmentation
  * mix_aug of the reference (utils/utils.py:790-878, used by reset('test') in aug_test mode,
  * TSP/TSPEnv.py:222-224, CVRP/CVRPEnv.py:462-467, and by reset('train')): instance b is copied
