@@ -71,6 +71,29 @@ class AttentionGrad(Structure):
                 ("dq_stride", c_int64 * 3), ("dk_stride", c_int64 * 3), ("dv_stride", c_int64 * 3), ("dslope", c_void_p)]
 
 
+class KVCache(Structure):
+    _fields_ = [("dtype", c_int32), ("B", c_int32), ("Hkv", c_int32), ("D", c_int32), ("page_size", c_int32),
+                ("max_pages", c_int32), ("num_pages", c_int32), ("k_stride", c_int64 * 3), ("v_stride", c_int64 * 3),
+                ("table_stride", c_int64), ("k_pages", c_void_p), ("v_pages", c_void_p), ("table", c_void_p),
+                ("lengths", c_void_p)]
+
+
+class AttentionStep(Structure):
+    _fields_ = [("cache", KVCache), ("rows_per_instance", c_int32), ("Hq", c_int32), ("scale", c_float), ("cap", c_float),
+                ("q_stride", c_int64 * 2), ("o_stride", c_int64 * 2), ("q", c_void_p), ("out", c_void_p), ("lse", c_void_p),
+                ("slope", c_void_p), ("pos_q", c_void_p), ("pos_k", c_void_p), ("pos_k_stride", c_int64),
+                ("pos_rows", c_int32), ("words", c_int32), ("blocked", c_void_p), ("blocked_stride", c_int64)]
+
+
+class Logits(Structure):
+    _fields_ = [("dtype", c_int32), ("R", c_int32), ("A", c_int32), ("period", c_int32), ("logits", c_void_p),
+                ("logits_stride", c_int64), ("blocked", c_void_p), ("blocked_stride", c_int64), ("words", c_int32),
+                ("history_cols", c_int32), ("bias", c_void_p), ("bias_stride", c_int64), ("history", c_void_p),
+                ("history_stride", c_int64), ("history_len", c_void_p), ("repetition", c_void_p), ("presence", c_void_p),
+                ("frequency", c_void_p), ("repetition_all", c_float), ("presence_all", c_float), ("frequency_all", c_float),
+                ("temperature", c_float), ("log_probs", c_void_p), ("out_stride", c_int64), ("selected", c_void_p)]
+
+
 # name -> (restype, argtypes); every symbol include/dgl_amd.h declares
 SIGNATURES = {
     "dgl_version": (c_int32, []),
@@ -119,6 +142,12 @@ SIGNATURES = {
     "dgl_attention_forward": (c_int32, [POINTER(Attention), c_void_p]),
     "dgl_attention_backward": (c_int32, [POINTER(Attention), POINTER(AttentionGrad), c_void_p, c_void_p]),
     "dgl_attention_backward_workspace_floats": (c_int64, [POINTER(Attention)]),
+    "dgl_cache_append": (c_int32, [POINTER(KVCache), c_void_p, c_void_p, POINTER(c_int64), POINTER(c_int64), c_int32, c_void_p,
+                                   c_void_p, c_void_p, c_void_p]),
+    "dgl_attention_step": (c_int32, [POINTER(AttentionStep), c_void_p, c_void_p]),
+    "dgl_attention_step_workspace_floats": (c_int64, [POINTER(AttentionStep)]),
+    "dgl_logits_process": (c_int32, [POINTER(Logits), c_void_p, c_void_p]),
+    "dgl_logits_workspace_floats": (c_int64, [POINTER(Logits)]),
     "dgl_set_sqrt_model": (c_int32, [c_int32]),
     "dgl_sqrt_apply": (c_int32, [c_void_p, c_void_p, c_int64, c_void_p]),
 }

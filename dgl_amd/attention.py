@@ -248,3 +248,161 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, scale: Optio
         if t is not None and t.requires_grad and torch.is_grad_enabled():
             raise ValueError(f"{name} requires grad: the operator is not differentiable in the coordinates")
     return _Attention.apply(q, k, v, slope, scale, cap, pos_q, pos_k, doc_q, doc_k, causal, prefix)
+
+
+class PagedCache:
+    """Keys and values of ``batch`` sequences in pages (include/dgl_amd.h, dgl_kv_cache_t): pages [num_pages, kv_heads,
+    page_size, head_dim], a table [batch, pages per sequence] and the live lengths.
+
+    Without ``num_pages`` every sequence owns the pages for ``max_tokens`` from the start; with it, sequences share a pool
+    and ``reserve`` / ``release`` move pages between them (host-side bookkeeping; the table is updated on the current
+    stream).  Appends and attention never look at the lengths on the host."""
+
+    def __init__(self, batch: int, kv_heads: int, head_dim: int, max_tokens: int, *, page_size: int = 64,
+                 num_pages: Optional[int] = None, dtype: torch.dtype = torch.float32, device="cuda"):
+        if batch < 1 or max_tokens < 1:
+            raise ValueError(f"a cache of {batch} sequences of {max_tokens} tokens")
+        per = (max_tokens + page_size - 1) // page_size
+        dev = torch.device(device)
+        if dev.type != "cuda":
+            raise ValueError(f"device {dev}: a GPU is expected")
+        if dev.index is None:
+            dev = torch.device("cuda", torch.cuda.current_device())
+        total = batch * per if num_pages is None else num_pages
+        shape = (total, kv_heads, page_size, head_dim)
+        table = torch.full((batch, per), -1, dtype=torch.int32, device=dev)
+        self._set(torch.zeros(shape, dtype=dtype, device=dev), torch.zeros(shape, dtype=dtype, device=dev), table,
+                  torch.zeros(batch, dtype=torch.int32, device=dev))
+        self._owned = [[] for _ in range(batch)]
+        self._free = list(range(total - 1, -1, -1))
+        if num_pages is None:
+            for b in range(batch):
+                self._owned[b] = [self._free.pop() for _ in range(per)]
+            table.copy_(torch.tensor(self._owned, dtype=torch.int32))
+
+    @classmethod
+    def over(cls, k_pages, v_pages, table, lengths) -> "PagedCache":
+        """A cache over tensors that exist already (their owner manages the pages)."""
+        self = cls.__new__(cls)
+        self._set(k_pages, v_pages, table, lengths)
+        self._owned = self._free = None
+        return self
+
+    def _set(self, k_pages, v_pages, table, lengths):
+        if k_pages.dim() != 4 or k_pages.shape != v_pages.shape or k_pages.dtype != v_pages.dtype:
+            raise ValueError(f"pages {tuple(k_pages.shape)} {k_pages.dtype} and {tuple(v_pages.shape)} {v_pages.dtype}: "
+                             "equal [pages, heads, page size, head size] are expected")
+        if k_pages.dtype not in _DTYPES:
+            raise ValueError(f"{k_pages.dtype}: float32, float16 or bfloat16 is expected")
+        dev = k_pages.device
+        if table.dim() != 2 or lengths.dim() != 1 or lengths.shape[0] != table.shape[0]:
+            raise ValueError(f"table {tuple(table.shape)} and lengths {tuple(lengths.shape)} do not fit")
+        if table.dtype != torch.int32 or lengths.dtype != torch.int32:
+            raise ValueError("table and lengths are int32")
+        if dev.type != "cuda" or v_pages.device != dev or table.device != dev or lengths.device != dev:
+            raise ValueError("pages, table and lengths belong on one GPU")
+        if k_pages.stride(3) != 1 or v_pages.stride(3) != 1 or table.stride(1) != 1 or lengths.stride(0) != 1:
+            raise ValueError("the head size, a row of the table and the lengths have to be consecutive")
+        self.k_pages, self.v_pages, self.table, self.lengths = k_pages, v_pages, table, lengths
+        self.device, self.dtype = dev, k_pages.dtype
+        self.page_size, self.batch = k_pages.shape[2], table.shape[0]
+        c = self.struct = _lib.KVCache()
+        c.dtype, c.B, c.Hkv, c.D = _DTYPES[self.dtype], self.batch, k_pages.shape[1], k_pages.shape[3]
+        c.page_size, c.max_pages, c.num_pages = self.page_size, table.shape[1], k_pages.shape[0]
+        c.k_stride, c.v_stride, c.table_stride = _stride3(k_pages), _stride3(v_pages), table.stride(0)
+        c.k_pages, c.v_pages, c.table, c.lengths = ptr(k_pages), ptr(v_pages), ptr(table), ptr(lengths)
+
+    # ---- pages of a pool ------------------------------------------------------------------
+    def _pool(self):
+        if self._free is None:
+            raise ValueError("the pages of this cache are managed by their owner")
+
+    def reserve(self, sequence: int, tokens: int) -> None:
+        """Give ``sequence`` the pages for ``tokens`` tokens (those it has stay)."""
+        self._pool()
+        need = (tokens + self.page_size - 1) // self.page_size
+        if need > self.table.shape[1]:
+            raise ValueError(f"{tokens} tokens: a sequence holds at most {self.table.shape[1] * self.page_size}")
+        own = self._owned[sequence]
+        if need - len(own) > len(self._free):
+            raise RuntimeError(f"{need - len(own)} pages wanted, {len(self._free)} are free")
+        if need > len(own):
+            have = len(own)
+            own.extend(self._free.pop() for _ in range(need - have))
+            self.table[sequence, have:need] = torch.tensor(own[have:need], dtype=torch.int32).to(self.device)
+
+    def release(self, sequence: int) -> None:
+        """Return the pages of ``sequence`` to the pool; it is empty afterwards."""
+        self._pool()
+        self._free.extend(reversed(self._owned[sequence]))
+        self._owned[sequence] = []
+        self.table[sequence].fill_(-1)
+        self.lengths[sequence:sequence + 1].zero_()
+
+    # ---- tokens ---------------------------------------------------------------------------
+    def append(self, k_new: torch.Tensor, v_new: torch.Tensor, *, counts: Optional[torch.Tensor] = None,
+               start: Optional[torch.Tensor] = None) -> None:
+        """Write new tokens [batch, kv heads, tokens, head size] behind each sequence (or from position ``start`` [batch]
+        on) and set the lengths to their end.  ``counts`` [batch]: only the first counts[b] of a ragged batch.  Tokens
+        beyond a sequence's pages are dropped."""
+        with torch.no_grad():
+            c = self.struct
+            want = (self.batch, c.Hkv, k_new.shape[2] if k_new.dim() == 4 else -1, c.D)
+            for name, t in (("k_new", k_new), ("v_new", v_new)):
+                if tuple(t.shape) != want or t.dtype != self.dtype or t.device != self.device:
+                    raise ValueError(f"{name} is {tuple(t.shape)} {t.dtype} on {t.device}, expected {want} {self.dtype} on {self.device}")
+            k_new, v_new = _usable(k_new), _usable(v_new)
+            counts = _side(counts, "counts", (self.batch,), torch.int32, self.device)
+            start = self.lengths if start is None else _side(start, "start", (self.batch,), torch.int32, self.device)
+            with _on(self.device):
+                check(_lib.load().dgl_cache_append(ctypes.byref(c), ptr(k_new), ptr(v_new), _stride3(k_new), _stride3(v_new), want[2],
+                                                   ptr(start), ptr(counts), ptr(self.lengths), _stream(self.device)), "dgl_cache_append")
+
+
+def attention_step(q: torch.Tensor, cache: PagedCache, *, rows_per_instance: int = 1, scale: Optional[float] = None,
+                   cap: float = 0.0, slope: Optional[torch.Tensor] = None, pos_q: Optional[torch.Tensor] = None,
+                   pos_k: Optional[torch.Tensor] = None, blocked: Optional[torch.Tensor] = None, return_lse: bool = False):
+    """Attention of one new token per row, q [R, H, D], over the cache of its instance (row r: sequence r //
+    rows_per_instance).  ``cap`` / ``slope`` as in ``attention``; coordinates ``pos_q`` [R, 2] and ``pos_k`` [batch, n, 2]
+    (n at least the live lengths), or, without them, the distance lengths[b] - 1 - j.  ``blocked`` int64 [R, words]: bit j of
+    word j // 64 set = key j is not seen, as the states' visited words.  A row that sees nothing is zeros (lse -inf)."""
+    with torch.no_grad():
+        c, dev = cache.struct, cache.device
+        if q.dim() != 3 or q.shape[0] != cache.batch * rows_per_instance or q.shape[2] != c.D or q.shape[1] % c.Hkv or q.shape[1] < 1:
+            raise ValueError(f"q has shape {tuple(q.shape)}: expected [{cache.batch} x {rows_per_instance}, a multiple of {c.Hkv}, {c.D}]")
+        if q.dtype != cache.dtype or q.device != dev:
+            raise ValueError(f"q is {q.dtype} on {q.device}, the cache {cache.dtype} on {dev}")
+        if (pos_q is None) != (pos_k is None) or (pos_q is not None and slope is None):
+            raise ValueError("coordinates are given for both sides and with a slope")
+        q = _usable(q)
+        R, H, D = q.shape
+        out = torch.empty(R, H, D, dtype=q.dtype, device=dev)
+        lse = torch.empty(R, H, dtype=torch.float32, device=dev) if return_lse else None
+        a = _lib.AttentionStep()
+        a.cache, a.rows_per_instance, a.Hq, a.cap = c, rows_per_instance, H, float(cap)
+        a.scale = D ** -0.5 if scale is None else float(scale)
+        a.q_stride, a.o_stride = (ctypes.c_int64 * 2)(*q.stride()[:2]), (ctypes.c_int64 * 2)(H * D, D)
+        a.q, a.out, a.lse = ptr(q), ptr(out), ptr(lse)
+        slope = _side(slope, "slope", (H,), torch.float32, dev)
+        a.slope = ptr(slope)
+        if pos_q is not None:
+            pos_q = _side(pos_q, "pos_q", (R, 2), torch.float32, dev)
+            if pos_q.stride(0) != 2:             # rows of one wide tensor, or one row for all
+                pos_q = pos_q.clone(memory_format=torch.contiguous_format)
+            n = pos_k.shape[1] if pos_k.dim() == 3 else -1
+            pos_k = _side(pos_k, "pos_k", (cache.batch, n, 2), torch.float32, dev)
+            if pos_k.data_ptr() % 8 or pos_k.stride(0) % 2:
+                pos_k = pos_k.clone(memory_format=torch.contiguous_format)
+            a.pos_q, a.pos_k, a.pos_k_stride, a.pos_rows = ptr(pos_q), ptr(pos_k), pos_k.stride(0), n
+        if blocked is not None:
+            if blocked.dim() != 2 or blocked.shape[0] != R or blocked.dtype != torch.int64 or blocked.device != dev:
+                raise ValueError(f"blocked is {tuple(blocked.shape)} {blocked.dtype}: int64 words [{R}, n] on {dev} are expected")
+            if blocked.shape[1] > 1 and blocked.stride(1) != 1:
+                blocked = blocked.contiguous()
+            a.blocked, a.words, a.blocked_stride = ptr(blocked), blocked.shape[1], blocked.stride(0)
+        lib = _lib.load()
+        need = lib.dgl_attention_step_workspace_floats(ctypes.byref(a))
+        with _on(dev):
+            ws = torch.empty(need, dtype=torch.float32, device=dev) if need > 0 else None
+            check(lib.dgl_attention_step(ctypes.byref(a), ptr(ws), _stream(dev)), "dgl_attention_step")
+        return (out, lse) if return_lse else out

@@ -414,6 +414,105 @@ DGL_API int dgl_attention_backward(const dgl_attention_t *a, const dgl_attention
 /* Floats of workspace dgl_attention_backward needs for `a` (-1: invalid arguments; beside TSP/TSPModel.py:420-441). */
 DGL_API int64_t dgl_attention_backward_workspace_floats(const dgl_attention_t *a);
 
+/* ------------------------------------------------------------------ paged key-value cache
+ * Keys and values of B sequences (the nodes of an instance, or the tokens decoded so far) in pages of page_size tokens: token
+ * j of sequence b lies in slot j % page_size of page table[b][j / page_size]; lengths[b] tokens are live.  The reference
+ * re-encodes its tokens at every step instead (TSP/TSPModel.py:174-231).  An entry of the table outside [0, num_pages) is
+ * an absent page: nothing is read from or written to it, its tokens are masked.  A length beyond the table's capacity counts
+ * as that capacity, a negative one as 0.  Strides in elements {page, head, slot}; the D elements of a head are consecutive;
+ * pages are 16-byte aligned in pointer and strides. */
+#define DGL_CACHE_MAX_TOKENS (1 << 30)
+
+typedef struct {
+    int32_t dtype;             /* DGL_DTYPE_* */
+    int32_t B, Hkv, D;
+    int32_t page_size;         /* a power of two, at least 16 */
+    int32_t max_pages;         /* columns of the table */
+    int32_t num_pages;         /* pages that exist */
+    int64_t k_stride[3], v_stride[3];
+    int64_t table_stride;      /* entries between the table's rows */
+    void *k_pages, *v_pages;
+    const int32_t *table;      /* [B][max_pages] */
+    const int32_t *lengths;    /* [B] */
+} dgl_kv_cache_t;
+
+/* Writes T new tokens per sequence: token t < counts[b] (NULL: T) of k_new / v_new goes to position start[b] + t (strides in
+ * elements {sequence, head, token}).  Positions outside the table's capacity and absent pages are skipped.  lengths_out
+ * (may be NULL; may be the array behind `start`) receives start[b] + counts[b], within the capacity.  Beside
+ * TSP/TSPModel.py:174-231, whose keys and values are recomputed at every step. */
+DGL_API int dgl_cache_append(const dgl_kv_cache_t *c, const void *k_new, const void *v_new, const int64_t *k_new_stride,
+                             const int64_t *v_new_stride, int32_t T, const int32_t *start, const int32_t *counts,
+                             int32_t *lengths_out, dgl_stream_t stream);
+
+/* Attention of one new token per row over its sequence: row r belongs to sequence r / rows_per_instance, all rows of a
+ * sequence share its pages.  Scores, cap and empty rows as in dgl_attention_t; the bias is -slope[h] times the distance
+ * between pos_q[r] and pos_k[b][j], or, without coordinates, lengths[b] - 1 - j.  blocked: bit j of word j / 64 of row r set
+ * = key j is not seen (the states' visited words; keys beyond the words are seen). */
+typedef struct {
+    dgl_kv_cache_t cache;
+    int32_t rows_per_instance, Hq;
+    float scale, cap;
+    int64_t q_stride[2], o_stride[2];   /* {row, head} */
+    const void *q;             /* [R][Hq][D], R = B * rows_per_instance */
+    void *out;                 /* [R][Hq][D] */
+    float *lse;                /* [R][Hq] or NULL */
+    const float *slope;        /* [Hq] or NULL */
+    const float *pos_q;        /* [R][2] or NULL */
+    const float *pos_k;        /* [B][pos_rows][2] or NULL; 8-byte aligned */
+    int64_t pos_k_stride;      /* floats between sequences */
+    int32_t pos_rows;          /* at least the live lengths */
+    int32_t words;             /* 64-bit words of a row of `blocked` */
+    const uint64_t *blocked;   /* [R][words] or NULL */
+    int64_t blocked_stride;    /* words between rows */
+} dgl_attention_step_t;
+
+/* The decoder's attention of the current node (TSP/TSPModel.py:375-441) over a cache instead of re-encoded tokens.  ws:
+ * dgl_attention_step_workspace_floats(a) floats (may be NULL where that is 0). */
+DGL_API int dgl_attention_step(const dgl_attention_step_t *a, float *ws, dgl_stream_t stream);
+
+/* Floats of workspace dgl_attention_step needs; depends on the sizes alone, not on the lengths (-1: invalid arguments;
+ * beside TSP/TSPModel.py:375-441). */
+DGL_API int64_t dgl_attention_step_workspace_floats(const dgl_attention_step_t *a);
+
+/* ------------------------------------------------------------------ logits
+ * From the logits of a decision to the log-probabilities that dgl_beam_advance takes, with the means to steer a search that
+ * the reference's masked softmax (TSP/TSPModel.py:317-337, CVRP/CVRPModel.py:480-516) does not have.  For row r, action a:
+ *   c = occurrences of a among history[r][0 .. history_len[r]);  where c > 0:
+ *     x = (x > 0 ? x / repetition : x * repetition) - presence - frequency c
+ *   x = (x + bias[a]) / temperature;  bit (a mod period) of blocked[r] set: x = -inf
+ *   log_probs[r][a] = x - log sum exp(x);  selected[r] = lowest a with the largest x (NaN is never picked)
+ * A row whose actions are all blocked is -inf throughout with selected = -1.  Arithmetic is binary32, each operation rounded
+ * once as written.  history entries outside [0, A) are ignored. */
+typedef struct {
+    int32_t dtype;             /* DGL_DTYPE_* of the logits */
+    int32_t R, A;
+    int32_t period;            /* actions a, a + period, ... share a blocked bit (CVRP's direct and via-depot moves: N + 1); divides A */
+    const void *logits;        /* [R][A] */
+    int64_t logits_stride;     /* elements between rows */
+    const uint64_t *blocked;   /* [R][words] or NULL: the states' visited words; bits beyond them are clear */
+    int64_t blocked_stride;
+    int32_t words;
+    int32_t history_cols;
+    const float *bias;         /* [A] (bias_stride 0) or [R][A], or NULL */
+    int64_t bias_stride;
+    const int32_t *history;    /* [R][history_cols] or NULL */
+    int64_t history_stride;
+    const int32_t *history_len;                       /* [R] or NULL: all columns */
+    const float *repetition, *presence, *frequency;   /* [R] each, or NULL: the values below for every row */
+    float repetition_all, presence_all, frequency_all;
+    float temperature;
+    float *log_probs;          /* [R][A] binary32, or NULL */
+    int64_t out_stride;
+    int32_t *selected;         /* [R] or NULL */
+} dgl_logits_t;
+
+/* The operator above, in front of dgl_beam_advance (utils/beamsearch.py:52-131).  ws: dgl_logits_workspace_floats floats (may
+ * be NULL where that is 0). */
+DGL_API int dgl_logits_process(const dgl_logits_t *a, float *ws, dgl_stream_t stream);
+
+/* Floats of workspace dgl_logits_process needs (-1: invalid arguments; beside utils/beamsearch.py:52-131). */
+DGL_API int64_t dgl_logits_workspace_floats(const dgl_logits_t *a);
+
 /* ----------------------------------------------------------------- augmentation
  * mix_aug of the reference (utils/utils.py:790-878, used by reset('test') in aug_test mode,
  * TSP/TSPEnv.py:222-224, CVRP/CVRPEnv.py:462-467, and by reset('train')): instance b is copied
