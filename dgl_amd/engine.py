@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import ctypes
 import functools
+import math
 import os
 from typing import Dict, Optional
 
@@ -149,6 +150,30 @@ def forward_range_guarded(engine, policy: "PackedPolicy") -> None:
             engine.forward(policy)
         finally:
             engine.arithmetic = _lib.ARITH_SPLIT_F16
+
+
+def controlled_log_probs(engine, controls):
+    """Dense log-probabilities [R, A] of the last forward() under a search's controls (dgl_amd/logits.py), and the greedy
+    pick per row.  Only actions the policy itself offers can be taken: non-candidates (1e-20 in the dense tensor) and
+    infeasible moves (the floor, 1e-7) stay out whatever the controls add.  A row whose controls leave nothing keeps the
+    policy's own probabilities.  Values below log 1e-20 are that, as in the dense tensor of the reference
+    (TSP/TSPModel.py:328-337), so that a beam wider than its candidates behaves as without controls."""
+    from .logits import process_logits
+    dense = engine.dense_probs()
+    lp = torch.where(dense > 1.0000001e-7, dense.log(), float("-inf"))
+    out, sel = process_logits(lp, blocked=controls.blocked, bias=controls.bias, temperature=controls.temperature,
+                              history=controls.history, history_len=controls.history_len, repetition=controls.repetition,
+                              presence=controls.presence, frequency=controls.frequency)
+    none = sel < 0
+    out = torch.where(none[:, None], lp, out).clamp_min_(math.log(1e-20))
+    return out, torch.where(none, engine.selected, sel)
+
+
+def dense_beam_advance(engine, controls, scores, beam, step, prev_k, action, actions):
+    """Beam expansion under controls: the dense form of the reference's Beamsearch.advance (utils/beamsearch.py:52-131)."""
+    lp, _ = controlled_log_probs(engine, controls)
+    check(engine.lib.dgl_beam_advance(ptr(lp), ptr(scores), engine.R // beam, beam, actions, step, ptr(prev_k), ptr(action),
+                                      stream_ptr()), "dgl_beam_advance")
 
 
 class TspEngine:
@@ -313,11 +338,17 @@ class TspEngine:
 
     @on_own_device
     @range_guarded
-    def greedy_rollout(self, policy: PackedPolicy, start: torch.Tensor) -> torch.Tensor:
+    def greedy_rollout(self, policy: PackedPolicy, start: torch.Tensor, controls=None) -> torch.Tensor:
         """Whole greedy decode (beam 1): N-1 policy decisions, everything stays on the device.  One launch for the
-        whole loop (dgl_tsp_greedy_decode) where that kernel applies, otherwise two launches per decision."""
+        whole loop (dgl_tsp_greedy_decode) where that kernel applies, otherwise two launches per decision.
+        ``controls`` (dgl_amd.logits.LogitControls) steer every decision."""
         self.reset()
         self.step(start)
+        if controls is not None:
+            while self.t < self.N:
+                self.forward(policy, want_logits=False)
+                self.step(controlled_log_probs(self, controls)[1])
+            return self.tour_length()
         if self.t < self.N and self.fused_decode_available():
             io = self.policy_io(want_logits=False, want_prob=False)
             check(self.lib.dgl_tsp_greedy_decode(ctypes.byref(self.state["struct"]), ptr(policy.packed), ctypes.byref(io),
@@ -337,6 +368,22 @@ class TspEngine:
         check(self.lib.dgl_beam_advance_compact(ctypes.byref(io), ptr(self.prob), ptr(scores), self.R // beam, beam,
                                                 self.N, step, ptr(prev_k), ptr(action), stream_ptr()),
               "dgl_beam_advance_compact")
+
+    @on_own_device
+    def attend(self, q: torch.Tensor, cache, *, scale=None, cap: float = 0.0, slope=None, return_lse: bool = False):
+        """Attention of every row's current node, q [R, H, D], over its instance's unvisited nodes: ``cache``
+        (dgl_amd.attention.PagedCache) holds the instances' node keys and values in node order, the visited words of the
+        state block nodes, and with ``slope`` scores fall with the distance between coordinates (TSP/TSPModel.py:375-441
+        attends over the re-encoded neighbourhood instead)."""
+        from .attention import attention_step
+        pos_q = None
+        if slope is not None:
+            if self.t < 1:
+                raise ValueError("no current node before the first step")
+            cur = self.state["tour"][:, self.t - 1].long()
+            pos_q = self.xy[torch.arange(self.R, device=self.device) // self.rpi, cur]
+        return attention_step(q, cache, rows_per_instance=self.rpi, scale=scale, cap=cap, slope=slope, pos_q=pos_q,
+                              pos_k=self.xy if slope is not None else None, blocked=self.state["visited"], return_lse=return_lse)
 
     @on_own_device
     def step_beam(self, prev_k: torch.Tensor, selected: torch.Tensor, beam: int) -> None:
@@ -365,10 +412,11 @@ class TspEngine:
 
     @on_own_device
     @range_guarded
-    def beam_rollout(self, policy: PackedPolicy, start: torch.Tensor, beam: int) -> torch.Tensor:
+    def beam_rollout(self, policy: PackedPolicy, start: torch.Tensor, beam: int, controls=None) -> torch.Tensor:
         """Beam-search decode (TSP/TSPTester.py:145-199) on the compact state: per step the policy, the beam
         expansion over beam*k candidates and one pass over the state that follows the back-pointers while it
-        updates; the tours are rebuilt from the back-pointer history at the end.  Nothing returns to the host."""
+        updates; the tours are rebuilt from the back-pointer history at the end.  Nothing returns to the host.
+        ``controls`` (dgl_amd.logits.LogitControls) steer every expansion, over dense log-probabilities."""
         assert self.rpi % beam == 0 and len(self.bufs) == 2
         G = self.R // beam
         dev = self.device
@@ -379,8 +427,11 @@ class TspEngine:
         self.step(start)
         step = 1
         while self.t < self.N:
-            self.forward(policy, want_logits=False, want_selected=False)
-            self.beam_advance(scores, beam, step, prev_k, action)
+            self.forward(policy, want_logits=False, want_selected=controls is not None)
+            if controls is None:
+                self.beam_advance(scores, beam, step, prev_k, action)
+            else:
+                dense_beam_advance(self, controls, scores, beam, step, prev_k, action, self.N)
             self.step_beam(prev_k.view(-1), action.view(-1), beam)
             step += 1
         if self.N >= 2:
@@ -560,9 +611,13 @@ class CvrpEngine:
 
     @on_own_device
     @range_guarded
-    def greedy_rollout(self, policy: PackedPolicy, start_action: torch.Tensor) -> torch.Tensor:
+    def greedy_rollout(self, policy: PackedPolicy, start_action: torch.Tensor, controls=None) -> torch.Tensor:
+        """``controls`` (dgl_amd.logits.LogitControls) steer every decision."""
         self.reset()
         self.step(start_action)
+        while controls is not None and self.t < self.N:
+            self.forward(policy, want_logits=False)
+            self.step(controlled_log_probs(self, controls)[1])
         while self.t < self.N:
             self.forward(policy, want_logits=False, want_prob=False)
             self.step(self.selected)
@@ -574,6 +629,20 @@ class CvrpEngine:
         check(self.lib.dgl_beam_advance_compact(ctypes.byref(io), ptr(self.prob), ptr(scores), self.R // beam, beam,
                                                 2 * (self.N + 1), step, ptr(prev_k), ptr(action), stream_ptr()),
               "dgl_beam_advance_compact")
+
+    @on_own_device
+    def attend(self, q: torch.Tensor, cache, *, scale=None, cap: float = 0.0, slope=None, return_lse: bool = False):
+        """As TspEngine.attend, over the N + 1 nodes (depot first) of ``cache``; the depot is visible as the state's visited
+        words have it."""
+        from .attention import attention_step
+        pos_q = None
+        if slope is not None:
+            if self.t < 1:
+                raise ValueError("no current node before the first step")
+            cur = self.state["nodes"][:, self.t - 1].long()
+            pos_q = self.xy[torch.arange(self.R, device=self.device) // self.rpi, cur]
+        return attention_step(q, cache, rows_per_instance=self.rpi, scale=scale, cap=cap, slope=slope, pos_q=pos_q,
+                              pos_k=self.xy if slope is not None else None, blocked=self.state["visited"], return_lse=return_lse)
 
     @on_own_device
     def step_beam(self, prev_k: torch.Tensor, action: torch.Tensor, beam: int) -> None:
@@ -603,9 +672,10 @@ class CvrpEngine:
 
     @on_own_device
     @range_guarded
-    def beam_rollout(self, policy: PackedPolicy, start_action: torch.Tensor, beam: int) -> torch.Tensor:
+    def beam_rollout(self, policy: PackedPolicy, start_action: torch.Tensor, beam: int, controls=None) -> torch.Tensor:
         """Beam-search decode (CVRP/CVRPTester.py:147-227) on the compact state; the step follows the
-        back-pointers while it updates, nodes and flags are rebuilt from the history at the end."""
+        back-pointers while it updates, nodes and flags are rebuilt from the history at the end.  ``controls``
+        (dgl_amd.logits.LogitControls) steer every expansion, over dense log-probabilities."""
         assert self.rpi % beam == 0 and len(self.bufs) == 2
         G = self.R // beam
         dev = self.device
@@ -616,8 +686,11 @@ class CvrpEngine:
         self.step(start_action)
         step = 1
         while self.t < self.N:
-            self.forward(policy, want_logits=False, want_selected=False)
-            self.beam_advance(scores, beam, step, prev_k, action)
+            self.forward(policy, want_logits=False, want_selected=controls is not None)
+            if controls is None:
+                self.beam_advance(scores, beam, step, prev_k, action)
+            else:
+                dense_beam_advance(self, controls, scores, beam, step, prev_k, action, 2 * (self.N + 1))
             self.step_beam(prev_k.view(-1), action.view(-1), beam)
             step += 1
         if self.N >= 2:

@@ -154,10 +154,11 @@ class TSPTester(_TesterBase):
         sel = idx.repeat(env.batch_size).repeat_interleave(env.beam_size).to(device=self.device, dtype=torch.int32)
         eng.set_knn(self.tester_params["knn"])
         policy = model.packed(self.device)
+        controls = self.tester_params.get("logit_controls")
         if beam_size == 1:
-            length = eng.greedy_rollout(policy, sel)
+            length = eng.greedy_rollout(policy, sel, controls=controls)
         else:
-            length = eng.beam_rollout(policy, sel, beam_size)
+            length = eng.beam_rollout(policy, sel, beam_size, controls=controls)
         env.selected_count = eng.t
         if getattr(env, "_orig_xy", None) is not None:             # aug_test: lengths on the original coordinates
             length = env._get_travel_distance()
@@ -179,6 +180,8 @@ class TSPTester(_TesterBase):
             self.env.load_problems(episode, nb, problem_size, beam_size)
             self.env.start_idx, self.env.step_size = 0, nb
             if tp.get("reference_protocol"):
+                if tp.get("logit_controls") is not None:
+                    raise ValueError("logit_controls steer the device-resident rollout, not the reference's protocol")
                 self.beamsearch_tour_nodes_shortest(beam_size, nb, problem_size, start=start)
                 shortest, _ = self._summarise(self.last_lengths, beam_size)
             else:
@@ -242,7 +245,9 @@ class CVRPTester(_TesterBase):
         sel = sel + 2 + env.problem_size
         eng.set_knn(self.tester_params["knn"], self.tester_params["depot_knn"])
         policy = model.packed(self.device)
-        length = eng.greedy_rollout(policy, sel) if beam_size == 1 else eng.beam_rollout(policy, sel, beam_size)
+        controls = self.tester_params.get("logit_controls")
+        length = (eng.greedy_rollout(policy, sel, controls=controls) if beam_size == 1 else
+                  eng.beam_rollout(policy, sel, beam_size, controls=controls))
         env.selected_count = eng.t
         if getattr(env, "_orig_xy", None) is not None:             # aug_test: lengths on the original coordinates
             length = env.cal_length()
@@ -266,6 +271,8 @@ class CVRPTester(_TesterBase):
             self.env.load_problems(episode, nb, problem_size)
             self.env.start_idx, self.env.step_size = 0, nb
             if tp.get("reference_protocol"):
+                if tp.get("logit_controls") is not None:
+                    raise ValueError("logit_controls steer the device-resident rollout, not the reference's protocol")
                 self.beamsearch_tour_nodes_shortest(beam_size, nb, problem_size + 1, start=start)
                 shortest, _ = self._summarise(self.last_lengths, beam_size)
             else:
