@@ -139,7 +139,8 @@ SIGNATURES = {
                                    c_void_p]),
     "dgl_beam_advance_compact": (c_int32, [POINTER(PolicyIO), c_void_p, c_void_p, c_int32, c_int32, c_int32,
                                            c_int32, c_void_p, c_void_p, c_void_p]),
-    "dgl_attention_forward": (c_int32, [POINTER(Attention), c_void_p]),
+    "dgl_attention_forward": (c_int32, [POINTER(Attention), c_void_p, c_void_p]),
+    "dgl_attention_forward_workspace_floats": (c_int64, [POINTER(Attention)]),
     "dgl_attention_backward": (c_int32, [POINTER(Attention), POINTER(AttentionGrad), c_void_p, c_void_p]),
     "dgl_attention_backward_workspace_floats": (c_int64, [POINTER(Attention)]),
     "dgl_cache_append": (c_int32, [POINTER(KVCache), c_void_p, c_void_p, POINTER(c_int64), POINTER(c_int64), c_int32, c_void_p,

@@ -46,7 +46,8 @@ def _usable(t: torch.Tensor) -> torch.Tensor:
     """The tensor itself where the kernels can address it, else a contiguous copy."""
     vec = 16 // t.element_size()
     st = t.stride()
-    if (st[-1] == 1 or t.shape[-1] <= 1) and t.data_ptr() % 16 == 0 and all(x % vec == 0 for x in st[:-1]):
+    if (st[-1] == 1 and t.data_ptr() % 16 == 0 and all(x % vec == 0 for x in st[:-1]) and
+            (len(st) != 4 or st[2] * t.element_size() < 1 << 26)):
         return t
     return t.clone(memory_format=torch.contiguous_format)
 
@@ -152,8 +153,11 @@ def _forward(call: _Call, want_lse: bool):
     lse = torch.empty(q.shape[:3], dtype=torch.float32, device=q.device) if want_lse else None
     call.set_out(out, lse)
     if out.numel():
+        lib = _lib.load()
+        need = lib.dgl_attention_forward_workspace_floats(ctypes.byref(call.a))
         with _on(q.device):
-            check(_lib.load().dgl_attention_forward(ctypes.byref(call.a), _stream(q.device)), "dgl_attention_forward")
+            ws = torch.empty(need, dtype=torch.float32, device=q.device) if need > 0 else None
+            check(lib.dgl_attention_forward(ctypes.byref(call.a), ptr(ws), _stream(q.device)), "dgl_attention_forward")
     return out, lse
 
 

@@ -37,30 +37,20 @@ struct AttnArgs {
     int64_t dqs, dks;
     const int *prefix;
     int tiles;                                   // row blocks per (batch, head)
+    int splits;                                  // forward: ranges of keys per row block; backward: ranges of rows per key block
+    float *part;                                 // results of the ranges
     // backward
     const char *dout;
     char *dq, *dk, *dv;
     int64_t dos[3], dqst[3], dkst[3], dvst[3];
     float *delta, *rowscale, *dslope_part, *dslope;
+    int head_parts;                              // key kernel: parts of the heads that share a key head
 };
 
 // Blocks are dealt to the 8 XCDs in turn; giving every XCD a contiguous range of the work keeps the row blocks of one
 // head, which read the same keys and values, on one L2.
 __device__ __forceinline__ int xcd_work() { return (int)(blockIdx.x % 8) * (int)(gridDim.x / 8) + (int)(blockIdx.x / 8); }
 
-struct ScoreParams {
-    float mul, cap2, slope2;     // all in units of log2
-    int cap, bias;
-};
-__device__ __forceinline__ ScoreParams score_params(const AttnArgs &a, int h) {
-    ScoreParams p;
-    p.cap = a.cap > 0.0f;
-    p.mul = p.cap ? a.scale / a.cap : a.scale * ATTN_LOG2E;
-    p.cap2 = a.cap * ATTN_LOG2E;
-    p.bias = a.bias;
-    p.slope2 = a.bias ? a.slope[h] * ATTN_LOG2E : 0.0f;
-    return p;
-}
 // keys a query row sees: j < limit (and the document test)
 __device__ __forceinline__ int row_limit(const AttnArgs &a, int b, int i) {
     if (i >= a.Lq) return 0;
@@ -86,24 +76,14 @@ __device__ __forceinline__ float pair_distance(const AttnArgs &a, int b, int i, 
     return __builtin_amdgcn_sqrtf(fmaf(dx, dx, dy * dy));
 }
 
-// one pair for the careful path: its score (log2 units), tanh and distance
+// one pair for the careful path: its score (log2 units) and tanh
 template <int TYPE>
 __device__ float pair_score(const AttnArgs &a, const ScoreParams &sp, int b, int i, int j, const typename Elem<TYPE>::raw *q,
-                            const typename Elem<TYPE>::raw *k, float &th, float &dist) {
+                            const typename Elem<TYPE>::raw *k, float &th) {
     float dot = 0.0f;
     for (int d = 0; d < a.D; ++d) dot = fmaf(elem_to_float<TYPE>(q[d]), elem_to_float<TYPE>(k[d]), dot);
-    float s = dot * sp.mul;
-    th = 0.0f;
-    dist = 0.0f;
-    if (sp.cap) {
-        th = attn_tanh(s);
-        s = sp.cap2 * th;
-    }
-    if (sp.bias) {
-        dist = pair_distance(a, b, i, j);
-        s = fmaf(-sp.slope2, dist, s);
-    }
-    return s;
+    const float s = score_of(sp, dot, th);
+    return sp.bias ? fmaf(-sp.slope2, pair_distance(a, b, i, j), s) : s;
 }
 __device__ __forceinline__ bool pair_allowed(const AttnArgs &a, int b, int i, int j, int limit) {
     if (j >= limit) return false;
@@ -173,6 +153,11 @@ __device__ __forceinline__ bool finite4(const f32x4 &v) {
 // One workgroup = 4 waves x NQ blocks of 16 queries of one (batch, head); keys and values pass through LDS in tiles of 64,
 // the next tile's loads in flight while the current one is computed.  Lane (g, c) holds query c of its blocks and, per
 // 16 keys, the scores against keys 4 g + r.
+template <int TYPE> __device__ __forceinline__ void store_wide(typename Elem<TYPE>::raw *o, int d, float x) {
+    if constexpr (TYPE == ATTN_F32) o[d] = x;
+    else if constexpr (TYPE == ATTN_F16) o[d] = __builtin_bit_cast(unsigned short, (_Float16)x);
+    else o[d] = __builtin_bit_cast(unsigned short, (__bf16)x);
+}
 template <int TYPE>
 __device__ void careful_forward_row(const AttnArgs &a, const ScoreParams &sp, int b, int h, int i, float m, float l) {
     typedef typename Elem<TYPE>::raw raw;
@@ -184,8 +169,8 @@ __device__ void careful_forward_row(const AttnArgs &a, const ScoreParams &sp, in
     for (int base = 0; base < limit; base += 64) {
         const int j = base + lane;
         const bool ok = pair_allowed(a, b, i, j, limit);
-        float p = 0.0f, th, dist;
-        if (ok) p = __builtin_amdgcn_exp2f(pair_score<TYPE>(a, sp, b, i, j, q, k + j * a.ks[2], th, dist) - m);
+        float p = 0.0f, th;
+        if (ok) p = __builtin_amdgcn_exp2f(pair_score<TYPE>(a, sp, b, i, j, q, k + j * a.ks[2], th) - m);
         for (unsigned long long w = __ballot(ok); w != 0; w &= w - 1) {
             const int jj = __ffsll((long long)w) - 1;
             const float pj = __shfl(p, jj);
@@ -196,39 +181,35 @@ __device__ void careful_forward_row(const AttnArgs &a, const ScoreParams &sp, in
     }
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
     raw *o = reinterpret_cast<raw *>(a.out) + b * a.os[0] + h * a.os[1] + i * a.os[2];
-    for (int half = 0; half < 2; ++half) {
-        const int d = lane + 64 * half;
-        const float x = (half ? acc1 : acc0) * inv;
-        if (d < a.D) {
-            if constexpr (TYPE == ATTN_F32) o[d] = x;
-            else if constexpr (TYPE == ATTN_F16) o[d] = __builtin_bit_cast(unsigned short, (_Float16)x);
-            else o[d] = __builtin_bit_cast(unsigned short, (__bf16)x);
-        }
-    }
+    if (lane < a.D) store_wide<TYPE>(o, lane, acc0 * inv);
+    if (lane + 64 < a.D) store_wide<TYPE>(o, lane + 64, acc1 * inv);
 }
 
 template <int TYPE, int DP, int NQ>
-__global__ __launch_bounds__(ATTN_THREADS, DP <= 64 ? 2 : 1) void attn_fwd_kernel(AttnArgs a) {
+__global__ __launch_bounds__(ATTN_THREADS, TYPE == ATTN_F32 && DP == 128 ? 1 : 2) void attn_fwd_kernel(AttnArgs a) {
     typedef Shape<TYPE, DP> S;
     typedef typename Elem<TYPE>::raw raw;
-    constexpr int ROWS = 64 * NQ, UNITS = (2 * S::units + ATTN_THREADS - 1) / ATTN_THREADS;
+    // KB: blocks of 16 keys whose scores are held at once (two for wide heads: 256 registers at two waves per SIMD)
+    constexpr int ROWS = 64 * NQ, UNITS = (2 * S::units + ATTN_THREADS - 1) / ATTN_THREADS, KB = DP == 128 ? 2 : 4;
     __shared__ __align__(16) char lds[S::row_bytes + (S::wide ? S::row_bytes : S::t_bytes)];
     __shared__ __align__(16) float key_pos[2 * ATTN_ROWS];
     __shared__ __align__(16) int key_doc[ATTN_ROWS];
     __shared__ TileMap map_store;
     raw *Kt = reinterpret_cast<raw *>(lds), *Vt = reinterpret_cast<raw *>(lds + S::row_bytes);
 
-    const int work = xcd_work();
-    if (work >= a.B * a.Hq * a.tiles) return;
+    int work = xcd_work();
+    if (work >= a.B * a.Hq * a.tiles * a.splits) return;
+    const int split = work % a.splits;
+    work /= a.splits;
     const int bh = work / a.tiles, qt = a.tiles - 1 - work % a.tiles;        // (causal: the longest rows first)
     const int b = bh / a.Hq, h = bh % a.Hq, hk = h / a.G;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g = lane >> 4, c = lane & 15;
     const int row0 = qt * ROWS, wrow0 = row0 + wave * 16 * NQ;
     const raw *q = reinterpret_cast<const raw *>(a.q) + b * a.qs[0] + h * a.qs[1];
-    const raw *k = reinterpret_cast<const raw *>(a.k) + b * a.ks[0] + hk * a.ks[1];
-    const raw *v = reinterpret_cast<const raw *>(a.v) + b * a.vs[0] + hk * a.vs[1];
+    const char *k = a.k + (b * a.ks[0] + hk * a.ks[1]) * Elem<TYPE>::bytes;
+    const char *v = a.v + (b * a.vs[0] + hk * a.vs[1]) * Elem<TYPE>::bytes;
     const int *docs = a.doc_k != nullptr ? a.doc_k + b * a.dks : nullptr;
-    const ScoreParams sp = score_params(a, h);
+    const ScoreParams sp = score_params(a.scale, a.cap, a.bias, a.slope, h);
 
     TileMap *map = nullptr;
     if (docs != nullptr) {
@@ -263,29 +244,40 @@ __global__ __launch_bounds__(ATTN_THREADS, DP <= 64 ? 2 : 1) void attn_fwd_kerne
         wave_limit = row_limit(a, b, min(wrow0 + 16 * NQ, a.Lq) - 1);        // limits rise with the row
         wave_full = row_limit(a, b, wrow0);
     }
-    const int end = (row_limit(a, b, min(row0 + ROWS, a.Lq) - 1) + ATTN_ROWS - 1) / ATTN_ROWS;
+    const int tiles = (row_limit(a, b, min(row0 + ROWS, a.Lq) - 1) + ATTN_ROWS - 1) / ATTN_ROWS;
+    const int per = (tiles + a.splits - 1) / a.splits, end = min(tiles, (split + 1) * per);
 
+    UnitPlan plan[UNITS];
+#pragma unroll
+    for (int x = 0; x < UNITS; ++x) {
+        const int u = tid + x * ATTN_THREADS;
+        plan[x] = u < S::units ? unit_plan<TYPE, DP>(u, a.ks[2], a.D) : unit_plan<TYPE, DP>(u - S::units, a.vs[2], a.D);
+    }
     Unit un[UNITS];
+    UnitIds ids[UNITS];
     float stage_pos = 0.0f;
     int stage_doc = -1;
     auto load = [&](int tile) {
-        const int base = tile * ATTN_ROWS;
+        const int base = tile * ATTN_ROWS, left = a.Lk - base;
+        const char *kt = k + base * a.ks[2] * Elem<TYPE>::bytes, *vt = v + base * a.vs[2] * Elem<TYPE>::bytes;
 #pragma unroll
         for (int x = 0; x < UNITS; ++x) {
             const int u = tid + x * ATTN_THREADS;
-            if (u < S::units) unit_load<TYPE, DP>(un[x], u, k, a.ks[2], base, a.Lk, a.D, docs);
-            else if (u < 2 * S::units) unit_load<TYPE, DP>(un[x], u - S::units, v, a.vs[2], base, a.Lk, a.D, docs);
+            if (u < S::units) unit_load(un[x], plan[x], kt, left);
+            else if (u < 2 * S::units) unit_load(un[x], plan[x], vt, left);
+            if (map != nullptr && u < 2 * S::units) unit_load_ids(ids[x], plan[x], docs + base, left);
         }
-        if (a.bias == 2 && tid < 2 * ATTN_ROWS) stage_pos = base + tid / 2 < a.Lk ? a.pos_k[b * a.pks + 2 * (int64_t)base + tid] : 0.0f;
+        if (a.bias == 2 && tid < 2 * ATTN_ROWS) stage_pos = tid < 2 * left ? a.pos_k[b * a.pks + 2 * (int64_t)base + tid] : 0.0f;
         if (map != nullptr && tid < ATTN_ROWS) stage_doc = doc_of_key(a, b, base + tid);
     };
-    int tile = next_tile(map, 0, end);
+    int tile = next_tile(map, split * per, end);
     if (tile < end) load(tile);
     while (tile < end) {
         __syncthreads();
 #pragma unroll
         for (int x = 0; x < UNITS; ++x) {
             const int u = tid + x * ATTN_THREADS;
+            if (map != nullptr && u < 2 * S::units) unit_skip(un[x], ids[x]);
             if (u < S::units) unit_write<TYPE, DP, true, false>(un[x], u, Kt, nullptr);
             else if (u < 2 * S::units) unit_write<TYPE, DP, false, true>(un[x], u - S::units, Vt, Vt);
         }
@@ -298,104 +290,125 @@ __global__ __launch_bounds__(ATTN_THREADS, DP <= 64 ? 2 : 1) void attn_fwd_kerne
         if (base >= wave_limit) continue;
         const bool by_doc = !tile_same(map, here), by_limit = base + ATTN_ROWS > wave_full;
 
-        f32x4 s[4][NQ];
 #pragma unroll
-        for (int t = 0; t < 4; ++t) {
-            Frag<TYPE, DP> kf;
-            frag_from_lds<TYPE, DP>(kf, Kt, 16 * t + c, g);
+        for (int kb = 0; kb < 4; kb += KB) {
+            f32x4 s[KB][NQ];
 #pragma unroll
-            for (int n = 0; n < NQ; ++n) s[t][n] = dot_block<TYPE, DP>(kf, qf[n]);
-        }
-        if (sp.cap) {
+            for (int t = 0; t < KB; ++t) {
+                Frag<TYPE, DP> kf;
+                frag_from_lds<TYPE, DP>(kf, Kt, 16 * (kb + t) + c, g);
 #pragma unroll
-            for (int t = 0; t < 4; ++t)
+                for (int n = 0; n < NQ; ++n) s[t][n] = dot_block<TYPE, DP>(kf, qf[n]);
+            }
+            if (sp.cap == CAP_NONE) {
 #pragma unroll
-                for (int n = 0; n < NQ; ++n)
+                for (int t = 0; t < KB; ++t)
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) s[t][n][r] = sp.cap2 * attn_tanh(s[t][n][r] * sp.mul);
-        } else {
+                    for (int n = 0; n < NQ; ++n) s[t][n] = s[t][n] * sp.mul;
+            } else if (sp.cap == CAP_FAST) {
 #pragma unroll
-            for (int t = 0; t < 4; ++t)
+                for (int t = 0; t < KB; ++t)
 #pragma unroll
-                for (int n = 0; n < NQ; ++n) s[t][n] = s[t][n] * sp.mul;
-        }
-        if (sp.bias == 1) {
-            const float k0 = (float)(base + 4 * g);
+                    for (int n = 0; n < NQ; ++n)
 #pragma unroll
-            for (int t = 0; t < 4; ++t)
+                        for (int r = 0; r < 4; ++r) s[t][n][r] = fmaf(-2.0f * sp.cap2, cap_r(s[t][n][r] * sp.mul2), sp.cap2);
+            } else {
 #pragma unroll
-                for (int n = 0; n < NQ; ++n)
+                for (int t = 0; t < KB; ++t)
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) s[t][n][r] = fmaf(-sp.slope2, fabsf(qx[n] - (k0 + (float)(16 * t + r))), s[t][n][r]);
-        } else if (sp.bias == 2) {
+                    for (int n = 0; n < NQ; ++n)
 #pragma unroll
-            for (int t = 0; t < 4; ++t) {
-                const f32x4 p0 = *reinterpret_cast<const f32x4 *>(key_pos + 2 * (16 * t + 4 * g));
-                const f32x4 p1 = *reinterpret_cast<const f32x4 *>(key_pos + 2 * (16 * t + 4 * g) + 4);
-                const float kx[4] = {p0[0], p0[2], p1[0], p1[2]}, ky[4] = {p0[1], p0[3], p1[1], p1[3]};
+                        for (int r = 0; r < 4; ++r) s[t][n][r] = sp.cap2 * attn_tanh(s[t][n][r] * sp.mul);
+            }
+            if (sp.bias == 1) {
+                const float k0 = (float)(base + 16 * kb + 4 * g);
 #pragma unroll
-                for (int n = 0; n < NQ; ++n)
+                for (int t = 0; t < KB; ++t)
+#pragma unroll
+                    for (int n = 0; n < NQ; ++n)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) s[t][n][r] = fmaf(-sp.slope2, fabsf((qx[n] - k0) - (float)(16 * t + r)), s[t][n][r]);
+            } else if (sp.bias == 2) {
+#pragma unroll
+                for (int t = 0; t < KB; ++t) {
+                    const float *at = key_pos + 2 * (16 * (kb + t) + 4 * g);
+                    const f32x4 p0 = *reinterpret_cast<const f32x4 *>(at), p1 = *reinterpret_cast<const f32x4 *>(at + 4);
+                    const float kx[4] = {p0[0], p0[2], p1[0], p1[2]}, ky[4] = {p0[1], p0[3], p1[1], p1[3]};
+#pragma unroll
+                    for (int n = 0; n < NQ; ++n)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) {
+                            const float dx = qx[n] - kx[r], dy = qy[n] - ky[r];
+                            s[t][n][r] = fmaf(-sp.slope2, __builtin_amdgcn_sqrtf(fmaf(dx, dx, dy * dy)), s[t][n][r]);
+                        }
+                }
+            }
+            if (by_limit) {
+#pragma unroll
+                for (int n = 0; n < NQ; ++n) {
+                    const int left = limit[n] - (base + 16 * kb + 4 * g);
+#pragma unroll
+                    for (int t = 0; t < KB; ++t)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) s[t][n][r] = 16 * t + r < left ? s[t][n][r] : -attn_inf();
+                }
+            }
+            if (by_doc) {
+#pragma unroll
+                for (int t = 0; t < KB; ++t) {
+                    const i32x4 kd = *reinterpret_cast<const i32x4 *>(key_doc + 16 * (kb + t) + 4 * g);
+#pragma unroll
+                    for (int n = 0; n < NQ; ++n)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) s[t][n][r] = kd[r] == doc[n] ? s[t][n][r] : -attn_inf();
+                }
+            }
+#pragma unroll
+            for (int n = 0; n < NQ; ++n) {
+                float top = s[0][n][0];
+#pragma unroll
+                for (int t = 0; t < KB; ++t)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) top = fast_max(top, s[t][n][r]);
+                top = fast_max(group_max(top), m[n]);
+                if (__any(top > m[n])) {
+                    const float shift = top == -attn_inf() ? 0.0f : top;
+                    const float f = __builtin_amdgcn_exp2f(m[n] - shift);
+                    l[n] *= f;
+#pragma unroll
+                    for (int d = 0; d < S::dt; ++d) o[n][d] = o[n][d] * f;
+                    m[n] = top;
+                }
+                const float shift = m[n] == -attn_inf() ? 0.0f : m[n];
+#pragma unroll
+                for (int t = 0; t < KB; ++t)
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
-                        const float dx = qx[n] - kx[r], dy = qy[n] - ky[r];
-                        s[t][n][r] = fmaf(-sp.slope2, __builtin_amdgcn_sqrtf(fmaf(dx, dx, dy * dy)), s[t][n][r]);
+                        s[t][n][r] = __builtin_amdgcn_exp2f(s[t][n][r] - shift);
+                        l[n] += s[t][n][r];
                     }
             }
+#pragma unroll
+            for (int t = 0; t < KB; t += 2) accumulate<TYPE, DP, NQ>(o, Vt, Vt, (kb + t) / 2, s[t], s[t + 1], g, c);
         }
-        if (by_limit) {
-#pragma unroll
-            for (int t = 0; t < 4; ++t)
-#pragma unroll
-                for (int n = 0; n < NQ; ++n)
-#pragma unroll
-                    for (int r = 0; r < 4; ++r)
-                        s[t][n][r] = base + 16 * t + 4 * g + r < limit[n] ? s[t][n][r] : -attn_inf();
-        }
-        if (by_doc) {
-#pragma unroll
-            for (int t = 0; t < 4; ++t) {
-                const i32x4 kd = *reinterpret_cast<const i32x4 *>(key_doc + 16 * t + 4 * g);
-#pragma unroll
-                for (int n = 0; n < NQ; ++n)
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) s[t][n][r] = kd[r] == doc[n] ? s[t][n][r] : -attn_inf();
-            }
-        }
-#pragma unroll
-        for (int n = 0; n < NQ; ++n) {
-            float top = s[0][n][0];
-#pragma unroll
-            for (int t = 0; t < 4; ++t)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) top = fmaxf(top, s[t][n][r]);
-            top = fmaxf(group_max(top), m[n]);
-            if (__any(top > m[n])) {
-                const float shift = top == -attn_inf() ? 0.0f : top;
-                const float f = __builtin_amdgcn_exp2f(m[n] - shift);
-                l[n] *= f;
-#pragma unroll
-                for (int d = 0; d < S::dt; ++d) o[n][d] = o[n][d] * f;
-                m[n] = top;
-            }
-            const float shift = m[n] == -attn_inf() ? 0.0f : m[n];
-#pragma unroll
-            for (int t = 0; t < 4; ++t)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    s[t][n][r] = __builtin_amdgcn_exp2f(s[t][n][r] - shift);
-                    l[n] += s[t][n][r];
-                }
-        }
-        accumulate<TYPE, DP, NQ>(o, Vt, Vt, 0, s[0], s[1], g, c);
-        accumulate<TYPE, DP, NQ>(o, Vt, Vt, 1, s[2], s[3], g, c);
     }
 
 #pragma unroll
     for (int n = 0; n < NQ; ++n) {
         const int i = wrow0 + 16 * n + c;
         const float total = group_sum(l[n]);
-        const float inv = total == 0.0f ? 0.0f : 1.0f / total;
         const float shift = m[n] == -attn_inf() ? 0.0f : m[n];
+        if (a.splits > 1) {
+            if (i < a.Lq) {
+                float *to = a.part + (((int64_t)bh * a.splits + split) * a.Lq + i) * (a.D + 4);
+#pragma unroll
+                for (int d = 0; d < S::dt; ++d)
+                    if (16 * d + 4 * g < a.D) *reinterpret_cast<f32x4 *>(to + 16 * d + 4 * g) = o[n][d];
+                if (g == 0) *reinterpret_cast<f32x2 *>(to + a.D) = f32x2{m[n], total};
+            }
+            continue;
+        }
+        const float inv = total == 0.0f ? 0.0f : 1.0f / total;
         bool fine = true;
 #pragma unroll
         for (int d = 0; d < S::dt; ++d) fine = fine && finite4(o[n][d]);
@@ -416,10 +429,95 @@ __global__ __launch_bounds__(ATTN_THREADS, DP <= 64 ? 2 : 1) void attn_fwd_kerne
     }
 }
 
-// -------------------------------------------------------------------------------------------- backward: query rows
-// dq of NQ x 16 query rows per wave, with delta_i = do_i . o_i on the way (kept for the kernel that owns the keys) and
-// the rows' share of dslope.  sum_j ds_ij is zero by definition; what it is with the delta at hand (o may have been
-// rounded to 16 bits) is measured and its part of the slope's gradient taken out again.
+// Joins the ranges of keys: one wave per row, lanes over the head size, in the order of the ranges.
+template <int TYPE> __global__ __launch_bounds__(ATTN_THREADS) void attn_fwd_join_kernel(AttnArgs a) {
+    typedef typename Elem<TYPE>::raw raw;
+    const int lane = threadIdx.x & 63;
+    const int64_t row = (int64_t)blockIdx.x * (ATTN_THREADS / 64) + (threadIdx.x >> 6);
+    if (row >= (int64_t)a.B * a.Hq * a.Lq) return;
+    const int64_t bh = row / a.Lq;
+    const int i = (int)(row % a.Lq), b = (int)(bh / a.Hq), h = (int)(bh % a.Hq);
+    const float *from = a.part + (bh * a.splits * a.Lq + i) * (a.D + 4);
+    const int64_t stride = (int64_t)a.Lq * (a.D + 4);
+    float top = -attn_inf();
+    for (int s = 0; s < a.splits; ++s) top = fmaxf(top, from[s * stride + a.D]);
+    const float shift = top == -attn_inf() ? 0.0f : top;
+    float total = 0.0f, acc0 = 0.0f, acc1 = 0.0f;
+    for (int s = 0; s < a.splits; ++s) {
+        const float *x = from + s * stride;
+        const float f = __builtin_amdgcn_exp2f(x[a.D] - shift);
+        total = fmaf(x[a.D + 1], f, total);
+        if (lane < a.D) acc0 = fmaf(x[lane], f, acc0);
+        if (lane + 64 < a.D) acc1 = fmaf(x[lane + 64], f, acc1);
+    }
+    const float inv = total == 0.0f ? 0.0f : 1.0f / total;
+    raw *o = reinterpret_cast<raw *>(a.out) + b * a.os[0] + h * a.os[1] + i * a.os[2];
+    if (lane < a.D) store_wide<TYPE>(o, lane, acc0 * inv);
+    if (lane + 64 < a.D) store_wide<TYPE>(o, lane + 64, acc1 * inv);
+    if (a.lse != nullptr && lane == 0) a.lse[row] = total == 0.0f ? -attn_inf() : (shift + __builtin_amdgcn_logf(total)) * ATTN_LN2;
+    if (__any((acc0 + acc1) * 0.0f != 0.0f))
+        careful_forward_row<TYPE>(a, score_params(a.scale, a.cap, a.bias, a.slope, h), b, h, i, shift, total);
+}
+
+// ---------------------------------------------------------------------------------------------------------- backward
+// Probabilities and score gradients of four pairs from their dot products: s = q.k, dp = do.v - delta (the subtraction is
+// the matrix instruction's initial accumulator), e = lse in units of log2 (infinite for rows without a key).  du comes
+// without the factor scale, and without the 4 of 1 - tanh^2 = 4 (r - r^2) where scores are capped (undo_factor).
+struct PairGrad {
+    f32x4 p, ds, du;
+};
+__device__ __forceinline__ PairGrad pair_grad(const ScoreParams &sp, f32x4 s, f32x4 dp, f32x4 e, f32x4 dist, bool masked, const bool (&ok)[4]) {
+    PairGrad w;
+    f32x4 x, slack = {1.0f, 1.0f, 1.0f, 1.0f};
+    if (sp.cap == CAP_NONE) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) x[r] = fmaf(s[r], sp.mul, -e[r]);
+    } else if (sp.cap == CAP_FAST) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const float y = cap_r(s[r] * sp.mul2);
+            x[r] = fmaf(-2.0f * sp.cap2, y, sp.cap2 - e[r]);
+            slack[r] = fmaf(-y, y, y);
+        }
+    } else {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const float th = attn_tanh(s[r] * sp.mul);
+            x[r] = fmaf(sp.cap2, th, -e[r]);
+            slack[r] = 0.25f * fmaf(-th, th, 1.0f);
+        }
+    }
+    if (sp.bias) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) x[r] = fmaf(-sp.slope2, dist[r], x[r]);
+    }
+#pragma unroll
+    for (int r = 0; r < 4; ++r) w.p[r] = __builtin_amdgcn_exp2f(x[r]);
+#pragma unroll
+    for (int r = 0; r < 4; ++r) w.ds[r] = w.p[r] * dp[r];
+    if (masked) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            w.p[r] = ok[r] ? w.p[r] : 0.0f;
+            w.ds[r] = ok[r] ? w.ds[r] : 0.0f;
+        }
+    }
+    w.du = sp.cap ? w.ds * slack : w.ds;
+    return w;
+}
+__device__ __forceinline__ float undo_factor(const AttnArgs &a) { return a.cap > 0.0f ? 4.0f * a.scale : a.scale; }
+
+// Half precision keeps 2^-24 at the least: score gradients of rows with a small do would vanish.  They are scaled by a
+// power of two that brings the row's largest |do| to 8..16 (undone exactly in the result).
+__device__ __forceinline__ int gradient_exponent(float amax) {
+    if (!(amax > 0.0f) || !(amax < 3.0e38f)) return 0;
+    return max(-100, min(100, 3 - ((int)(__float_as_uint(amax) >> 23) - 127)));
+}
+__device__ __forceinline__ float exp2_of(int e) { return __uint_as_float((unsigned)(127 + e) << 23); }
+
+// ---- query rows: dq of NQ x 16 rows per wave, with delta_i = do_i . o_i on the way (kept for the kernel that owns the
+// keys) and the rows' share of dslope.  sum_j ds_ij is zero by definition; what it is with the delta at hand (o may have
+// been rounded to 16 bits) is measured and its part of the slope's gradient taken out again.
 template <int TYPE>
 __device__ void careful_dq_row(const AttnArgs &a, const ScoreParams &sp, int b, int h, int i, float lse2, float delta) {
     typedef typename Elem<TYPE>::raw raw;
@@ -432,13 +530,12 @@ __device__ void careful_dq_row(const AttnArgs &a, const ScoreParams &sp, int b, 
     for (int base = 0; base < limit; base += 64) {
         const int j = base + lane;
         const bool ok = pair_allowed(a, b, i, j, limit);
-        float ds = 0.0f, th, dist;
+        float ds = 0.0f, th;
         if (ok) {
-            const float p = __builtin_amdgcn_exp2f(pair_score<TYPE>(a, sp, b, i, j, q, k + j * a.ks[2], th, dist) - lse2);
+            const float p = __builtin_amdgcn_exp2f(pair_score<TYPE>(a, sp, b, i, j, q, k + j * a.ks[2], th) - lse2);
             float dp = 0.0f;
             for (int d = 0; d < a.D; ++d) dp = fmaf(elem_to_float<TYPE>(o[d]), elem_to_float<TYPE>(v[j * a.vs[2] + d]), dp);
-            ds = p * (dp - delta);
-            if (sp.cap) ds *= fmaf(-th, th, 1.0f);
+            ds = p * (dp - delta) * fmaf(-th, th, 1.0f);
         }
         for (unsigned long long w = __ballot(ok); w != 0; w &= w - 1) {
             const int jj = __ffsll((long long)w) - 1;
@@ -449,23 +546,8 @@ __device__ void careful_dq_row(const AttnArgs &a, const ScoreParams &sp, int b, 
         }
     }
     raw *out = reinterpret_cast<raw *>(a.dq) + b * a.dqst[0] + h * a.dqst[1] + i * a.dqst[2];
-    for (int half = 0; half < 2; ++half) {
-        const int d = lane + 64 * half;
-        const float x = (half ? acc1 : acc0) * a.scale;
-        if (d < a.D) {
-            if constexpr (TYPE == ATTN_F32) out[d] = x;
-            else if constexpr (TYPE == ATTN_F16) out[d] = __builtin_bit_cast(unsigned short, (_Float16)x);
-            else out[d] = __builtin_bit_cast(unsigned short, (__bf16)x);
-        }
-    }
-}
-
-// Half precision keeps 2^-24 at the least: score gradients of rows with a small do would vanish.  They are scaled by a
-// power of two that brings the row's largest |do| to 8..16 (undone exactly in the result).
-__device__ __forceinline__ float gradient_scale(float amax) {
-    if (!(amax > 0.0f) || !(amax < 3.0e38f)) return 1.0f;
-    const int e = (int)(__float_as_uint(amax) >> 23) - 127;
-    return __uint_as_float((unsigned)(127 + max(-100, min(100, 3 - e))) << 23);
+    if (lane < a.D) store_wide<TYPE>(out, lane, acc0 * a.scale);
+    if (lane + 64 < a.D) store_wide<TYPE>(out, lane + 64, acc1 * a.scale);
 }
 
 template <int TYPE, int DP, int NQ>
@@ -488,12 +570,12 @@ __global__ __launch_bounds__(ATTN_THREADS, DP <= 64 ? 2 : 1) void attn_bwd_q_ker
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g = lane >> 4, c = lane & 15;
     const int row0 = qt * ROWS, wrow0 = row0 + wave * 16 * NQ;
     const raw *q = reinterpret_cast<const raw *>(a.q) + b * a.qs[0] + h * a.qs[1];
-    const raw *k = reinterpret_cast<const raw *>(a.k) + b * a.ks[0] + hk * a.ks[1];
-    const raw *v = reinterpret_cast<const raw *>(a.v) + b * a.vs[0] + hk * a.vs[1];
+    const char *k = a.k + (b * a.ks[0] + hk * a.ks[1]) * Elem<TYPE>::bytes;
+    const char *v = a.v + (b * a.vs[0] + hk * a.vs[1]) * Elem<TYPE>::bytes;
     const raw *go = reinterpret_cast<const raw *>(a.dout) + b * a.dos[0] + h * a.dos[1];
     const raw *fo = reinterpret_cast<const raw *>(a.out) + b * a.os[0] + h * a.os[1];
     const int *docs = a.doc_k != nullptr ? a.doc_k + b * a.dks : nullptr;
-    const ScoreParams sp = score_params(a, h);
+    const ScoreParams sp = score_params(a.scale, a.cap, a.bias, a.slope, h);
 
     TileMap *map = nullptr;
     if (docs != nullptr) {
@@ -533,10 +615,15 @@ __global__ __launch_bounds__(ATTN_THREADS, DP <= 64 ? 2 : 1) void attn_bwd_q_ker
                 }
             }
         delta[n] = group_sum(dot);
-        rs[n] = TYPE == ATTN_F16 ? gradient_scale(group_max(amax)) : 1.0f;
         const int64_t at = ((int64_t)b * a.Hq + h) * a.Lq + i;
         const float lse = live ? a.lse[at] : -attn_inf();
         lse2[n] = lse == -attn_inf() ? attn_inf() : lse * ATTN_LOG2E;
+        rs[n] = 1.0f;
+        if constexpr (TYPE == ATTN_F16) {          // probabilities carry the row's scale through their exponent
+            const int e = gradient_exponent(group_max(amax));
+            rs[n] = exp2_of(e);
+            lse2[n] -= (float)e;
+        }
         if (live && g == 0) {
             a.delta[at] = delta[n];
             if (TYPE == ATTN_F16) a.rowscale[at] = rs[n];
@@ -559,18 +646,27 @@ __global__ __launch_bounds__(ATTN_THREADS, DP <= 64 ? 2 : 1) void attn_bwd_q_ker
     const int end = (row_limit(a, b, min(row0 + ROWS, a.Lq) - 1) + ATTN_ROWS - 1) / ATTN_ROWS;
     const bool want_slope = a.dslope_part != nullptr;
 
+    UnitPlan plan[UNITS];
+#pragma unroll
+    for (int x = 0; x < UNITS; ++x) {
+        const int u = tid + x * ATTN_THREADS;
+        plan[x] = u < S::units ? unit_plan<TYPE, DP>(u, a.ks[2], a.D) : unit_plan<TYPE, DP>(u - S::units, a.vs[2], a.D);
+    }
     Unit un[UNITS];
+    UnitIds ids[UNITS];
     float stage_pos = 0.0f;
     int stage_doc = -1;
     auto load = [&](int tile) {
-        const int base = tile * ATTN_ROWS;
+        const int base = tile * ATTN_ROWS, left = a.Lk - base;
+        const char *kt = k + base * a.ks[2] * Elem<TYPE>::bytes, *vt = v + base * a.vs[2] * Elem<TYPE>::bytes;
 #pragma unroll
         for (int x = 0; x < UNITS; ++x) {
             const int u = tid + x * ATTN_THREADS;
-            if (u < S::units) unit_load<TYPE, DP>(un[x], u, k, a.ks[2], base, a.Lk, a.D, docs);
-            else if (u < 2 * S::units) unit_load<TYPE, DP>(un[x], u - S::units, v, a.vs[2], base, a.Lk, a.D, docs);
+            if (u < S::units) unit_load(un[x], plan[x], kt, left);
+            else if (u < 2 * S::units) unit_load(un[x], plan[x], vt, left);
+            if (map != nullptr && u < 2 * S::units) unit_load_ids(ids[x], plan[x], docs + base, left);
         }
-        if (a.bias == 2 && tid < 2 * ATTN_ROWS) stage_pos = base + tid / 2 < a.Lk ? a.pos_k[b * a.pks + 2 * (int64_t)base + tid] : 0.0f;
+        if (a.bias == 2 && tid < 2 * ATTN_ROWS) stage_pos = tid < 2 * left ? a.pos_k[b * a.pks + 2 * (int64_t)base + tid] : 0.0f;
         if (map != nullptr && tid < ATTN_ROWS) stage_doc = doc_of_key(a, b, base + tid);
     };
     int tile = next_tile(map, 0, end);
@@ -580,6 +676,7 @@ __global__ __launch_bounds__(ATTN_THREADS, DP <= 64 ? 2 : 1) void attn_bwd_q_ker
 #pragma unroll
         for (int x = 0; x < UNITS; ++x) {
             const int u = tid + x * ATTN_THREADS;
+            if (map != nullptr && u < 2 * S::units) unit_skip(un[x], ids[x]);
             if (u < S::units) unit_write<TYPE, DP, true, true>(un[x], u, Kt, KT);
             else if (u < 2 * S::units) unit_write<TYPE, DP, true, false>(un[x], u - S::units, Vt, nullptr);
         }
@@ -590,7 +687,7 @@ __global__ __launch_bounds__(ATTN_THREADS, DP <= 64 ? 2 : 1) void attn_bwd_q_ker
         if (tile < end) load(tile);
         __syncthreads();
         if (base >= wave_limit) continue;
-        const bool by_doc = !tile_same(map, here), by_limit = base + ATTN_ROWS > wave_full;
+        const bool by_doc = !tile_same(map, here), masked = by_doc || base + ATTN_ROWS > wave_full;
 
 #pragma unroll
         for (int tp = 0; tp < 2; ++tp) {
@@ -605,7 +702,7 @@ __global__ __launch_bounds__(ATTN_THREADS, DP <= 64 ? 2 : 1) void attn_bwd_q_ker
                 for (int n = 0; n < NQ; ++n) s[n] = dot_block<TYPE, DP>(f, qf[n]);
                 frag_from_lds<TYPE, DP>(f, Vt, at + c, g);
 #pragma unroll
-                for (int n = 0; n < NQ; ++n) dp[n] = dot_block<TYPE, DP>(f, of[n]);
+                for (int n = 0; n < NQ; ++n) dp[n] = dot_block<TYPE, DP>(f, of[n], f32x4{-delta[n], -delta[n], -delta[n], -delta[n]});
                 f32x4 p0 = {0, 0, 0, 0}, p1 = {0, 0, 0, 0};
                 i32x4 kd = {0, 0, 0, 0};
                 if (sp.bias == 2) {
@@ -614,21 +711,13 @@ __global__ __launch_bounds__(ATTN_THREADS, DP <= 64 ? 2 : 1) void attn_bwd_q_ker
                 }
                 if (by_doc) kd = *reinterpret_cast<const i32x4 *>(key_doc + at + 4 * g);
                 const float kx[4] = {p0[0], p0[2], p1[0], p1[2]}, ky[4] = {p0[1], p0[3], p1[1], p1[3]};
-                const float k0 = (float)(base + at + 4 * g);
 #pragma unroll
                 for (int n = 0; n < NQ; ++n) {
-                    f32x4 x = s[n] * sp.mul, slack = {1.0f, 1.0f, 1.0f, 1.0f}, dist = {0, 0, 0, 0};
-                    if (sp.cap) {
-#pragma unroll
-                        for (int r = 0; r < 4; ++r) {
-                            const float th = attn_tanh(x[r]);
-                            slack[r] = fmaf(-th, th, 1.0f);
-                            x[r] = sp.cap2 * th;
-                        }
-                    }
+                    f32x4 dist = {0, 0, 0, 0};
                     if (sp.bias == 1) {
+                        const float d0 = qx[n] - (float)(base + at + 4 * g);
 #pragma unroll
-                        for (int r = 0; r < 4; ++r) dist[r] = fabsf(qx[n] - (k0 + (float)r));
+                        for (int r = 0; r < 4; ++r) dist[r] = fabsf(d0 - (float)r);
                     } else if (sp.bias == 2) {
 #pragma unroll
                         for (int r = 0; r < 4; ++r) {
@@ -636,34 +725,24 @@ __global__ __launch_bounds__(ATTN_THREADS, DP <= 64 ? 2 : 1) void attn_bwd_q_ker
                             dist[r] = __builtin_amdgcn_sqrtf(fmaf(dx, dx, dy * dy));
                         }
                     }
-                    if (sp.bias) {
+                    bool ok[4] = {true, true, true, true};
+                    if (masked) {
+                        const int left = limit[n] - (base + at + 4 * g);
 #pragma unroll
-                        for (int r = 0; r < 4; ++r) x[r] = fmaf(-sp.slope2, dist[r], x[r]);
+                        for (int r = 0; r < 4; ++r) ok[r] = r < left && (!by_doc || kd[r] == doc[n]);
                     }
-                    f32x4 p, ds;
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) p[r] = __builtin_amdgcn_exp2f(x[r] - lse2[n]);
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) ds[r] = p[r] * (dp[n][r] - delta[n]);
-                    if (by_limit || by_doc) {
-#pragma unroll
-                        for (int r = 0; r < 4; ++r) {
-                            const bool ok = base + at + 4 * g + r < limit[n] && (!by_doc || kd[r] == doc[n]);
-                            p[r] = ok ? p[r] : 0.0f;
-                            ds[r] = ok ? ds[r] : 0.0f;
-                            dist[r] = ok ? dist[r] : 0.0f;
-                        }
-                    }
+                    const PairGrad pg = pair_grad(sp, s[n], dp[n], f32x4{lse2[n], lse2[n], lse2[n], lse2[n]}, dist, masked, ok);
                     if (want_slope) {
 #pragma unroll
                         for (int r = 0; r < 4; ++r) {
-                            excess[n] += ds[r];
-                            pd[n] = fmaf(p[r], dist[r], pd[n]);
-                            dsl[n] = fmaf(ds[r], dist[r], dsl[n]);
+                            // (coordinates of a masked key may be NaN as well)
+                            const float x = masked && !ok[r] ? 0.0f : dist[r];
+                            excess[n] += pg.ds[r];
+                            pd[n] = fmaf(pg.p[r], x, pd[n]);
+                            dsl[n] = fmaf(pg.ds[r], x, dsl[n]);
                         }
                     }
-                    if (TYPE == ATTN_F16) ds = ds * rs[n];
-                    w[t][n] = ds * slack;
+                    w[t][n] = pg.du;
                 }
             }
             accumulate<TYPE, DP, NQ>(dq, Kt, KT, tp, w[0], w[1], g, c);
@@ -676,7 +755,7 @@ __global__ __launch_bounds__(ATTN_THREADS, DP <= 64 ? 2 : 1) void attn_bwd_q_ker
         const int i = wrow0 + 16 * n + c;
         const bool live = i < a.Lq;
         bool fine = true;
-        const float undo = TYPE == ATTN_F16 ? a.scale / rs[n] : a.scale;
+        const float inv_rs = 1.0f / rs[n], undo = undo_factor(a) * inv_rs;
 #pragma unroll
         for (int d = 0; d < S::dt; ++d) fine = fine && finite4(dq[n][d]);
         if (live) {
@@ -689,10 +768,11 @@ __global__ __launch_bounds__(ATTN_THREADS, DP <= 64 ? 2 : 1) void attn_bwd_q_ker
         bad = (bad | bad >> 16 | bad >> 32 | bad >> 48) & 0xffff;
         for (; bad != 0; bad &= bad - 1) {
             const int cc = __ffsll((long long)bad) - 1;
-            careful_dq_row<TYPE>(a, sp, b, h, wrow0 + 16 * n + cc, __shfl(lse2[n], cc), __shfl(delta[n], cc));
+            const int64_t at = ((int64_t)b * a.Hq + h) * a.Lq + wrow0 + 16 * n + cc;
+            careful_dq_row<TYPE>(a, sp, b, h, wrow0 + 16 * n + cc, a.lse[at] * ATTN_LOG2E, __shfl(delta[n], cc));
         }
         if (want_slope) {
-            const float e = group_sum(excess[n]), x = group_sum(pd[n]), y = group_sum(dsl[n]);
+            const float e = group_sum(excess[n]) * inv_rs, x = group_sum(pd[n]) * inv_rs, y = group_sum(dsl[n]) * inv_rs;
             slope_sum += live ? fmaf(-e, x, y) : 0.0f;
         }
     }
@@ -721,61 +801,59 @@ __global__ __launch_bounds__(256) void attn_dslope_kernel(AttnArgs a) {
     if (tid == 0) a.dslope[h] = (float)-sums[0];
 }
 
-// ----------------------------------------------------------------------------------------------- backward: key rows
-// dk and dv of NK x 16 keys per wave, over the query rows of all heads that share them.  Lane (g, c) holds key c and, per
-// 16 queries, the pairs with queries 4 g + r.
+// ---- key rows: dk and dv of NK x 16 keys per wave, over the query rows of the heads that share them.  Lane (g, c) holds key
+// c and, per 16 queries, the pairs with queries 4 g + r.  Where key blocks alone do not fill the chip, the heads of a group
+// and the query rows are dealt to several workgroups (head_parts x splits), whose binary32 sums a second kernel adds.
 template <int TYPE>
 __device__ void careful_dkv_row(const AttnArgs &a, int b, int hk, int j) {
     typedef typename Elem<TYPE>::raw raw;
     const int lane = threadIdx.x & 63;
     const raw *k = reinterpret_cast<const raw *>(a.k) + b * a.ks[0] + hk * a.ks[1] + j * a.ks[2];
     const raw *v = reinterpret_cast<const raw *>(a.v) + b * a.vs[0] + hk * a.vs[1] + j * a.vs[2];
-    float gk[2] = {0.0f, 0.0f}, gv[2] = {0.0f, 0.0f};
+    float gk0 = 0.0f, gk1 = 0.0f, gv0 = 0.0f, gv1 = 0.0f;
     for (int h = hk * a.G; h < (hk + 1) * a.G; ++h) {
-        const ScoreParams sp = score_params(a, h);
+        const ScoreParams sp = score_params(a.scale, a.cap, a.bias, a.slope, h);
         const raw *q = reinterpret_cast<const raw *>(a.q) + b * a.qs[0] + h * a.qs[1];
         const raw *o = reinterpret_cast<const raw *>(a.dout) + b * a.dos[0] + h * a.dos[1];
         for (int base = 0; base < a.Lq; base += 64) {
             const int i = base + lane;
             const bool ok = i < a.Lq && pair_allowed(a, b, i, j, row_limit(a, b, i));
-            float p = 0.0f, ds = 0.0f, th, dist;
+            float p = 0.0f, ds = 0.0f, th;
             if (ok) {
                 const int64_t at = ((int64_t)b * a.Hq + h) * a.Lq + i;
-                p = __builtin_amdgcn_exp2f(pair_score<TYPE>(a, sp, b, i, j, q + i * a.qs[2], k, th, dist) - a.lse[at] * ATTN_LOG2E);
+                p = __builtin_amdgcn_exp2f(pair_score<TYPE>(a, sp, b, i, j, q + i * a.qs[2], k, th) - a.lse[at] * ATTN_LOG2E);
                 float dp = 0.0f;
                 for (int d = 0; d < a.D; ++d) dp = fmaf(elem_to_float<TYPE>(o[i * a.dos[2] + d]), elem_to_float<TYPE>(v[d]), dp);
-                ds = p * (dp - a.delta[at]);
-                if (sp.cap) ds *= fmaf(-th, th, 1.0f);
+                ds = p * (dp - a.delta[at]) * fmaf(-th, th, 1.0f);
             }
             for (unsigned long long w = __ballot(ok); w != 0; w &= w - 1) {
                 const int ii = __ffsll((long long)w) - 1;
                 const float x = __shfl(ds, ii), y = __shfl(p, ii);
-                for (int half = 0; half < 2; ++half) {
-                    const int d = lane + 64 * half;
-                    if (d < a.D) {
-                        gk[half] = fmaf(x, elem_to_float<TYPE>(q[(int64_t)(base + ii) * a.qs[2] + d]), gk[half]);
-                        gv[half] = fmaf(y, elem_to_float<TYPE>(o[(int64_t)(base + ii) * a.dos[2] + d]), gv[half]);
-                    }
+                const raw *qr = q + (int64_t)(base + ii) * a.qs[2], *orow = o + (int64_t)(base + ii) * a.dos[2];
+                if (lane < a.D) {
+                    gk0 = fmaf(x, elem_to_float<TYPE>(qr[lane]), gk0);
+                    gv0 = fmaf(y, elem_to_float<TYPE>(orow[lane]), gv0);
+                }
+                if (lane + 64 < a.D) {
+                    gk1 = fmaf(x, elem_to_float<TYPE>(qr[lane + 64]), gk1);
+                    gv1 = fmaf(y, elem_to_float<TYPE>(orow[lane + 64]), gv1);
                 }
             }
         }
     }
-    for (int which = 0; which < 2; ++which) {
-        raw *out = which ? reinterpret_cast<raw *>(a.dv) + b * a.dvst[0] + hk * a.dvst[1] + j * a.dvst[2]
-                         : reinterpret_cast<raw *>(a.dk) + b * a.dkst[0] + hk * a.dkst[1] + j * a.dkst[2];
-        for (int half = 0; half < 2; ++half) {
-            const int d = lane + 64 * half;
-            const float x = which ? gv[half] : gk[half] * a.scale;
-            if (d < a.D) {
-                if constexpr (TYPE == ATTN_F32) out[d] = x;
-                else if constexpr (TYPE == ATTN_F16) out[d] = __builtin_bit_cast(unsigned short, (_Float16)x);
-                else out[d] = __builtin_bit_cast(unsigned short, (__bf16)x);
-            }
-        }
+    raw *outk = reinterpret_cast<raw *>(a.dk) + b * a.dkst[0] + hk * a.dkst[1] + j * a.dkst[2];
+    raw *outv = reinterpret_cast<raw *>(a.dv) + b * a.dvst[0] + hk * a.dvst[1] + j * a.dvst[2];
+    if (lane < a.D) {
+        store_wide<TYPE>(outk, lane, gk0 * a.scale);
+        store_wide<TYPE>(outv, lane, gv0);
+    }
+    if (lane + 64 < a.D) {
+        store_wide<TYPE>(outk, lane + 64, gk1 * a.scale);
+        store_wide<TYPE>(outv, lane + 64, gv1);
     }
 }
 
-#define F16_P_SCALE 1024.0f      // probabilities (<= 1) are rounded to binary16 times 2^10: those of long rows stay normal
+#define F16_P_EXPONENT 10        // probabilities (<= 1) are rounded to binary16 times 2^10: those of long rows stay normal
 
 template <int TYPE, int DP, int NK>
 __global__ __launch_bounds__(ATTN_THREADS, DP <= 64 ? 2 : 1) void attn_bwd_kv_kernel(AttnArgs a) {
@@ -790,10 +868,15 @@ __global__ __launch_bounds__(ATTN_THREADS, DP <= 64 ? 2 : 1) void attn_bwd_kv_ke
     raw *Qt = reinterpret_cast<raw *>(lds), *Ot = reinterpret_cast<raw *>(lds + S::row_bytes);
     raw *QT = reinterpret_cast<raw *>(lds + 2 * S::row_bytes), *OT = reinterpret_cast<raw *>(lds + 2 * S::row_bytes + S::t_bytes);
 
-    const int work = xcd_work();
-    if (work >= a.B * a.Hkv * a.tiles) return;
+    const int parts = a.head_parts * a.splits;
+    int work = xcd_work();
+    if (work >= a.B * a.Hkv * a.tiles * parts) return;
+    const int part = work % parts;
+    work /= parts;
     const int bh = work / a.tiles, kt = work % a.tiles;          // (causal: the first keys are seen by the most rows)
     const int b = bh / a.Hkv, hk = bh % a.Hkv;
+    const int hper = (a.G + a.head_parts - 1) / a.head_parts, h0 = hk * a.G + part / a.splits * hper;
+    const int h1 = min(h0 + hper, (hk + 1) * a.G), split = part % a.splits;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g = lane >> 4, c = lane & 15;
     const int row0 = kt * ROWS, wrow0 = row0 + wave * 16 * NK;
     const raw *k = reinterpret_cast<const raw *>(a.k) + b * a.ks[0] + hk * a.ks[1];
@@ -831,45 +914,61 @@ __global__ __launch_bounds__(ATTN_THREADS, DP <= 64 ? 2 : 1) void attn_bwd_kv_ke
     // the first query row that sees the first key of this block / of this wave
     int first = 0;
     if (a.causal && (a.prefix == nullptr || row0 >= a.prefix[b])) first = max(0, row0 - (a.Lk - a.Lq));
-    const int begin = min(first, a.Lq) / ATTN_ROWS, end = (a.Lq + ATTN_ROWS - 1) / ATTN_ROWS;
+    const int all_begin = min(first, a.Lq) / ATTN_ROWS, all_end = (a.Lq + ATTN_ROWS - 1) / ATTN_ROWS;
+    const int per = (all_end - all_begin + a.splits - 1) / a.splits;
+    const int begin = all_begin + split * per, end = min(all_end, begin + per);
     int wave_first = 0;                              // rows before it see no key of the wave
     if (a.causal && (a.prefix == nullptr || wrow0 >= a.prefix[b])) wave_first = max(0, wrow0 - (a.Lk - a.Lq));
     const int wave_all = a.causal ? wrow0 + 16 * NK - 1 - (a.Lk - a.Lq) : 0;   // rows from here on see all keys of the wave
     const bool tail = wrow0 + 16 * NK > a.Lk;
 
-    float gscale = 1.0f, undo = a.scale;
+    float gscale = 1.0f;
     if constexpr (TYPE == ATTN_F16) {               // one scale for all rows: that of the largest gradient among them
+        unsigned least = 0x7f000000u;
+        for (int h = h0; h < h1; ++h)
+            for (int x = tid; x < a.Lq; x += ATTN_THREADS) least = min(least, __float_as_uint(a.rowscale[((int64_t)b * a.Hq + h) * a.Lq + x]));
+#pragma unroll
+        for (int x = 1; x < 64; x <<= 1) least = min(least, (unsigned)__shfl_xor((int)least, x));
         if (tid == 0) least_scale = 0x7f000000u;
         __syncthreads();
-        for (int64_t x = tid; x < (int64_t)a.G * a.Lq; x += ATTN_THREADS)
-            atomicMin(&least_scale, __float_as_uint(a.rowscale[((int64_t)b * a.Hq + hk * a.G) * a.Lq + x]));
+        if (lane == 0) atomicMin(&least_scale, least);
         __syncthreads();
         gscale = __uint_as_float(least_scale);
-        undo = a.scale / gscale;
     }
+    const float gmul = TYPE == ATTN_F16 ? gscale * exp2_of(-F16_P_EXPONENT) : 1.0f;
 
-    for (int h = hk * a.G; h < (hk + 1) * a.G; ++h) {
-        const raw *q = reinterpret_cast<const raw *>(a.q) + b * a.qs[0] + h * a.qs[1];
-        const raw *go = reinterpret_cast<const raw *>(a.dout) + b * a.dos[0] + h * a.dos[1];
+    UnitPlan plan[UNITS];
+#pragma unroll
+    for (int x = 0; x < UNITS; ++x) {
+        const int u = tid + x * ATTN_THREADS;
+        plan[x] = u < S::units ? unit_plan<TYPE, DP>(u, a.qs[2], a.D) : unit_plan<TYPE, DP>(u - S::units, a.dos[2], a.D);
+    }
+    for (int h = h0; h < h1; ++h) {
+        const char *q = a.q + (b * a.qs[0] + h * a.qs[1]) * Elem<TYPE>::bytes;
+        const char *go = a.dout + (b * a.dos[0] + h * a.dos[1]) * Elem<TYPE>::bytes;
         const float *lse = a.lse + ((int64_t)b * a.Hq + h) * a.Lq, *del = a.delta + ((int64_t)b * a.Hq + h) * a.Lq;
-        const ScoreParams sp = score_params(a, h);
+        const ScoreParams sp = score_params(a.scale, a.cap, a.bias, a.slope, h);
         Unit un[UNITS];
+        UnitIds ids[UNITS];
         float st_lse = 0.0f, st_delta = 0.0f, st_x = 0.0f, st_y = 0.0f;
         int st_lim = 0, st_doc = -2;
         auto load = [&](int tile) {
-            const int base = tile * ATTN_ROWS;
+            const int base = tile * ATTN_ROWS, left = a.Lq - base;
+            const char *qt = q + base * a.qs[2] * Elem<TYPE>::bytes, *ot = go + base * a.dos[2] * Elem<TYPE>::bytes;
 #pragma unroll
             for (int x = 0; x < UNITS; ++x) {
                 const int u = tid + x * ATTN_THREADS;
-                if (u < S::units) unit_load<TYPE, DP>(un[x], u, q, a.qs[2], base, a.Lq, a.D, docs);
-                else if (u < 2 * S::units) unit_load<TYPE, DP>(un[x], u - S::units, go, a.dos[2], base, a.Lq, a.D, docs);
+                if (u < S::units) unit_load(un[x], plan[x], qt, left);
+                else if (u < 2 * S::units) unit_load(un[x], plan[x], ot, left);
+                if (map != nullptr && u < 2 * S::units) unit_load_ids(ids[x], plan[x], docs + base, left);
             }
             if (tid < ATTN_ROWS) {
                 const int i = base + tid;
                 const bool live = i < a.Lq;
                 const float e = live ? lse[i] : -attn_inf();
                 st_lse = e == -attn_inf() ? attn_inf() : e * ATTN_LOG2E;
-                st_delta = live ? del[i] : 0.0f;
+                if (TYPE == ATTN_F16) st_lse -= (float)F16_P_EXPONENT;
+                st_delta = live ? -del[i] : 0.0f;
                 st_lim = row_limit(a, b, i);
                 if (map != nullptr) st_doc = doc_of_query(a, b, i);
                 if (a.bias == 1) st_x = (float)(i + a.Lk - a.Lq);
@@ -886,6 +985,7 @@ __global__ __launch_bounds__(ATTN_THREADS, DP <= 64 ? 2 : 1) void attn_bwd_kv_ke
 #pragma unroll
             for (int x = 0; x < UNITS; ++x) {
                 const int u = tid + x * ATTN_THREADS;
+                if (map != nullptr && u < 2 * S::units) unit_skip(un[x], ids[x]);
                 if (u < S::units) unit_write<TYPE, DP, true, true>(un[x], u, Qt, QT);
                 else if (u < 2 * S::units) unit_write<TYPE, DP, true, true>(un[x], u - S::units, Ot, OT);
             }
@@ -902,7 +1002,7 @@ __global__ __launch_bounds__(ATTN_THREADS, DP <= 64 ? 2 : 1) void attn_bwd_kv_ke
             if (tile < end) load(tile);
             __syncthreads();
             if (base + ATTN_ROWS <= wave_first || wrow0 >= a.Lk) continue;
-            const bool by_doc = !tile_same(map, here), by_limit = tail || base < wave_all || base + ATTN_ROWS > a.Lq;
+            const bool by_doc = !tile_same(map, here), masked = by_doc || tail || base < wave_all || base + ATTN_ROWS > a.Lq;
 
 #pragma unroll
             for (int tp = 0; tp < 2; ++tp) {
@@ -915,59 +1015,39 @@ __global__ __launch_bounds__(ATTN_THREADS, DP <= 64 ? 2 : 1) void attn_bwd_kv_ke
                     frag_from_lds<TYPE, DP>(f, Qt, at + c, g);
 #pragma unroll
                     for (int n = 0; n < NK; ++n) s[n] = dot_block<TYPE, DP>(f, kf[n]);
+                    const f32x4 minus_delta = *reinterpret_cast<const f32x4 *>(row_delta + at + 4 * g);
                     frag_from_lds<TYPE, DP>(f, Ot, at + c, g);
 #pragma unroll
-                    for (int n = 0; n < NK; ++n) dp[n] = dot_block<TYPE, DP>(f, vf[n]);
+                    for (int n = 0; n < NK; ++n) dp[n] = dot_block<TYPE, DP>(f, vf[n], minus_delta);
                     const f32x4 e = *reinterpret_cast<const f32x4 *>(row_lse + at + 4 * g);
-                    const f32x4 dl = *reinterpret_cast<const f32x4 *>(row_delta + at + 4 * g);
                     f32x4 qx = {0, 0, 0, 0}, qy = {0, 0, 0, 0};
                     i32x4 lim = {0, 0, 0, 0}, qd = {0, 0, 0, 0};
                     if (sp.bias) qx = *reinterpret_cast<const f32x4 *>(row_x + at + 4 * g);
                     if (sp.bias == 2) qy = *reinterpret_cast<const f32x4 *>(row_y + at + 4 * g);
-                    if (by_limit || by_doc) lim = *reinterpret_cast<const i32x4 *>(row_lim + at + 4 * g);
+                    if (masked) lim = *reinterpret_cast<const i32x4 *>(row_lim + at + 4 * g);
                     if (by_doc) qd = *reinterpret_cast<const i32x4 *>(row_doc + at + 4 * g);
 #pragma unroll
                     for (int n = 0; n < NK; ++n) {
-                        f32x4 x = s[n] * sp.mul, slack = {1.0f, 1.0f, 1.0f, 1.0f};
-                        if (sp.cap) {
-#pragma unroll
-                            for (int r = 0; r < 4; ++r) {
-                                const float th = attn_tanh(x[r]);
-                                slack[r] = fmaf(-th, th, 1.0f);
-                                x[r] = sp.cap2 * th;
-                            }
-                        }
+                        f32x4 dist = {0, 0, 0, 0};
                         if (sp.bias == 1) {
 #pragma unroll
-                            for (int r = 0; r < 4; ++r) x[r] = fmaf(-sp.slope2, fabsf(qx[r] - kx[n]), x[r]);
+                            for (int r = 0; r < 4; ++r) dist[r] = fabsf(qx[r] - kx[n]);
                         } else if (sp.bias == 2) {
 #pragma unroll
                             for (int r = 0; r < 4; ++r) {
                                 const float dx = qx[r] - kx[n], dy = qy[r] - ky[n];
-                                x[r] = fmaf(-sp.slope2, __builtin_amdgcn_sqrtf(fmaf(dx, dx, dy * dy)), x[r]);
+                                dist[r] = __builtin_amdgcn_sqrtf(fmaf(dx, dx, dy * dy));
                             }
                         }
-                        f32x4 p, ds;
-#pragma unroll
-                        for (int r = 0; r < 4; ++r) p[r] = __builtin_amdgcn_exp2f(x[r] - e[r]);
-#pragma unroll
-                        for (int r = 0; r < 4; ++r) ds[r] = p[r] * (dp[n][r] - dl[r]);
-                        if (by_limit || by_doc) {
+                        bool ok[4] = {true, true, true, true};
+                        if (masked) {
                             const int j = wrow0 + 16 * n + c;
 #pragma unroll
-                            for (int r = 0; r < 4; ++r) {
-                                const bool ok = j < lim[r] && (!by_doc || qd[r] == doc[n]);
-                                p[r] = ok ? p[r] : 0.0f;
-                                ds[r] = ok ? ds[r] : 0.0f;
-                            }
+                            for (int r = 0; r < 4; ++r) ok[r] = j < lim[r] && (!by_doc || qd[r] == doc[n]);
                         }
-                        ds = ds * slack;
-                        if (TYPE == ATTN_F16) {
-                            p = p * F16_P_SCALE;
-                            ds = ds * gscale;
-                        }
-                        wp[t][n] = p;
-                        ws[t][n] = ds;
+                        const PairGrad pg = pair_grad(sp, s[n], dp[n], e, dist, masked, ok);
+                        wp[t][n] = pg.p;
+                        ws[t][n] = TYPE == ATTN_F16 ? pg.du * gmul : pg.du;
                     }
                 }
                 accumulate<TYPE, DP, NK>(dv, Ot, OT, tp, wp[0], wp[1], g, c);
@@ -976,12 +1056,24 @@ __global__ __launch_bounds__(ATTN_THREADS, DP <= 64 ? 2 : 1) void attn_bwd_kv_ke
         }
     }
 
+    const float undo = undo_factor(a) / gscale, undo_v = TYPE == ATTN_F16 ? exp2_of(-F16_P_EXPONENT) : 1.0f;
 #pragma unroll
     for (int n = 0; n < NK; ++n) {
         const int j = wrow0 + 16 * n + c;
         const bool live = j < a.Lk;
+        if (parts > 1) {
+            if (live) {
+                float *to = a.part + (((int64_t)part * a.B * a.Hkv + bh) * a.Lk + j) * 2 * a.D;
+#pragma unroll
+                for (int d = 0; d < S::dt; ++d)
+                    if (16 * d + 4 * g < a.D) {
+                        *reinterpret_cast<f32x4 *>(to + 16 * d + 4 * g) = dk[n][d] * undo;
+                        *reinterpret_cast<f32x4 *>(to + a.D + 16 * d + 4 * g) = dv[n][d] * undo_v;
+                    }
+            }
+            continue;
+        }
         bool fine = true;
-        const float undo_v = TYPE == ATTN_F16 ? 1.0f / F16_P_SCALE : 1.0f;
 #pragma unroll
         for (int d = 0; d < S::dt; ++d) fine = fine && finite4(dk[n][d]) && finite4(dv[n][d]);
         if (live) {
@@ -1000,12 +1092,38 @@ __global__ __launch_bounds__(ATTN_THREADS, DP <= 64 ? 2 : 1) void attn_bwd_kv_ke
     }
 }
 
+// Adds the parts of dk and dv, in order: one wave per key row.
+template <int TYPE> __global__ __launch_bounds__(ATTN_THREADS) void attn_bwd_kv_join_kernel(AttnArgs a) {
+    typedef typename Elem<TYPE>::raw raw;
+    const int lane = threadIdx.x & 63;
+    const int64_t row = (int64_t)blockIdx.x * (ATTN_THREADS / 64) + (threadIdx.x >> 6), rows = (int64_t)a.B * a.Hkv * a.Lk;
+    if (row >= rows) return;
+    const int64_t bh = row / a.Lk;
+    const int j = (int)(row % a.Lk), b = (int)(bh / a.Hkv), hk = (int)(bh % a.Hkv), parts = a.head_parts * a.splits;
+    float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};                  // dk, dv together are 2 D <= 256 values
+    for (int p = 0; p < parts; ++p) {
+        const float *from = a.part + (p * rows + row) * 2 * a.D;
+#pragma unroll
+        for (int x = 0; x < 4; ++x)
+            if (lane + 64 * x < 2 * a.D) sum[x] += from[lane + 64 * x];
+    }
+    raw *outk = reinterpret_cast<raw *>(a.dk) + b * a.dkst[0] + hk * a.dkst[1] + j * a.dkst[2];
+    raw *outv = reinterpret_cast<raw *>(a.dv) + b * a.dvst[0] + hk * a.dvst[1] + j * a.dvst[2];
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+        const int d = lane + 64 * x;
+        if (d < a.D) store_wide<TYPE>(outk, d, sum[x]);
+        else if (d < 2 * a.D) store_wide<TYPE>(outv, d - a.D, sum[x]);
+    }
+    if (__any((sum[0] + sum[1] + sum[2] + sum[3]) * 0.0f != 0.0f)) careful_dkv_row<TYPE>(a, b, hk, j);
+}
+
 // ------------------------------------------------------------------------------------------------------------ launch
 bool aligned_strides(const int64_t *s, const void *p, int bytes) {
     if ((reinterpret_cast<uintptr_t>(p) & 15) != 0) return false;
     for (int i = 0; i < 3; ++i)
         if ((s[i] * bytes) % 16 != 0 || s[i] < 0) return false;
-    return true;
+    return s[2] * bytes < (1 << 26);             // a tile's rows are addressed by 32-bit offsets
 }
 
 int check_attention(const dgl_attention_t *p) {
@@ -1027,7 +1145,7 @@ int check_attention(const dgl_attention_t *p) {
     DGL_CHECK_ARG(p->Lk == 0 || (p->k != nullptr && p->v != nullptr), "k or v is NULL");
     DGL_CHECK_ARG(aligned_strides(p->q_stride, p->q, bytes) && aligned_strides(p->k_stride, p->k, bytes) &&
                       aligned_strides(p->v_stride, p->v, bytes) && aligned_strides(p->o_stride, p->out, bytes),
-                  "q, k, v, out: 16-byte aligned pointers and strides");
+                  "q, k, v, out: 16-byte aligned pointers and strides, tokens less than 64 MiB apart");
     return DGL_OK;
 }
 
@@ -1046,13 +1164,56 @@ AttnArgs attention_args(const dgl_attention_t *p) {
 unsigned xcd_grid(int64_t work) { return (unsigned)((work + 7) / 8 * 8); }
 int padded(int D) { return D <= 16 ? 16 : D <= 32 ? 32 : D <= 64 ? 64 : 128; }
 
-// Two blocks of 16 query rows per wave halve the LDS reads per pair; one where that would leave compute units idle
-// (fewer than two workgroups for each of the 256).
-bool two_blocks(const AttnArgs &a, int rows, int heads) { return (int64_t)a.B * heads * ((rows + 127) / 128) >= 512; }
+// Two blocks of 16 rows per wave halve the LDS reads per pair.  Two where the operands and sums of both fit the 256 registers
+// of two waves per SIMD, and one where two would leave compute units idle (fewer than two workgroups for each of the 256).
+enum { KERNEL_FWD, KERNEL_BWD_Q, KERNEL_BWD_KV };
+constexpr bool two_fit(int kernel, int type, int DP) {
+    return kernel == KERNEL_FWD ? !(type == ATTN_F32 && DP == 128) : kernel == KERNEL_BWD_Q ? DP <= (type == ATTN_F32 ? 32 : 64) : DP <= 32;
+}
+bool two_blocks(int kernel, int dtype, const AttnArgs &a, int rows, int heads) {
+    return two_fit(kernel, dtype, padded(a.D)) && (int64_t)a.B * heads * ((rows + 127) / 128) >= 512;
+}
+
+// A long side is cut into ranges where the blocks of the other side are too few for the chip (512 workgroups wanted), as
+// long as a range keeps eight tiles: below that the second launch costs more than the idle units.
+int ranges(int64_t blocks, int length) {
+    const int64_t want = blocks >= 512 ? 1 : (512 + blocks - 1) / blocks, most = (length + 511) / 512;
+    return (int)(want < most ? want : most < 1 ? 1 : most);
+}
+void plan_forward(AttnArgs &a, int dtype, int &n) {
+    n = two_blocks(KERNEL_FWD, dtype, a, a.Lq, a.Hq) ? 2 : 1;
+    a.tiles = (a.Lq + 64 * n - 1) / (64 * n);
+    a.splits = a.tiles > 0 ? ranges((int64_t)a.B * a.Hq * a.tiles, a.Lk) : 1;
+}
+void plan_keys(AttnArgs &a, int dtype, int &n) {
+    n = two_blocks(KERNEL_BWD_KV, dtype, a, a.Lk, a.Hkv) ? 2 : 1;
+    a.tiles = (a.Lk + 64 * n - 1) / (64 * n);
+    const int64_t blocks = (int64_t)a.B * a.Hkv * (a.tiles > 0 ? a.tiles : 1);
+    const int64_t want = blocks >= 768 ? 1 : (768 + blocks - 1) / blocks;       // (two or three workgroups fit a unit)
+    a.head_parts = (int)(want < a.G ? want : a.G);
+    a.head_parts = (a.G + (a.G + a.head_parts - 1) / a.head_parts - 1) / ((a.G + a.head_parts - 1) / a.head_parts);   // no empty part
+    a.splits = ranges(blocks * a.head_parts, a.Lq);
+}
+int64_t forward_floats(AttnArgs a, int dtype) {
+    int n;
+    plan_forward(a, dtype, n);
+    return a.splits > 1 ? (int64_t)a.B * a.Hq * a.splits * a.Lq * (a.D + 4) : 0;
+}
+int64_t keys_floats(AttnArgs a, int dtype) {
+    int n;
+    plan_keys(a, dtype, n);
+    const int64_t parts = (int64_t)a.head_parts * a.splits;
+    return parts > 1 ? parts * a.B * a.Hkv * a.Lk * 2 * a.D : 0;
+}
 
 template <template <int, int, int> class Launch> int by_type(const AttnArgs &a, int dtype, int n, hipStream_t s) {
 #define ATTN_CASE(T, DPV) \
-    if (dtype == T && padded(a.D) == DPV) return n == 2 ? Launch<T, DPV, 2>::go(a, s) : Launch<T, DPV, 1>::go(a, s);
+    if (dtype == T && padded(a.D) == DPV) { \
+        if constexpr (two_fit(Launch<T, DPV, 1>::kernel, T, DPV)) { \
+            if (n == 2) return Launch<T, DPV, 2>::go(a, s); \
+        } \
+        return Launch<T, DPV, 1>::go(a, s); \
+    }
     ATTN_CASE(ATTN_F32, 16) ATTN_CASE(ATTN_F32, 32) ATTN_CASE(ATTN_F32, 64) ATTN_CASE(ATTN_F32, 128)
     ATTN_CASE(ATTN_F16, 16) ATTN_CASE(ATTN_F16, 32) ATTN_CASE(ATTN_F16, 64) ATTN_CASE(ATTN_F16, 128)
     ATTN_CASE(ATTN_BF16, 16) ATTN_CASE(ATTN_BF16, 32) ATTN_CASE(ATTN_BF16, 64) ATTN_CASE(ATTN_BF16, 128)
@@ -1060,76 +1221,100 @@ template <template <int, int, int> class Launch> int by_type(const AttnArgs &a, 
     return dgl_set_error(DGL_ERR_INVALID_ARGUMENT, "unknown element type %d", dtype);
 }
 template <int T, int DP, int N> struct LaunchFwd {
-    static int go(AttnArgs a, hipStream_t s) {
-        a.tiles = (a.Lq + 64 * N - 1) / (64 * N);
-        hipLaunchKernelGGL((attn_fwd_kernel<T, DP, N>), dim3(xcd_grid((int64_t)a.B * a.Hq * a.tiles)), dim3(ATTN_THREADS), 0, s, a);
+    static constexpr int kernel = KERNEL_FWD;
+    static int go(const AttnArgs &a, hipStream_t s) {
+        hipLaunchKernelGGL((attn_fwd_kernel<T, DP, N>), dim3(xcd_grid((int64_t)a.B * a.Hq * a.tiles * a.splits)), dim3(ATTN_THREADS), 0, s, a);
         DGL_CHECK_LAUNCH("dgl_attention_forward");
-        return DGL_OK;
-    }
-};
-template <int T, int DP, int N> struct LaunchBwdQ {
-    static int go(AttnArgs a, hipStream_t s) {
-        a.tiles = (a.Lq + 64 * N - 1) / (64 * N);
-        hipLaunchKernelGGL((attn_bwd_q_kernel<T, DP, N>), dim3(xcd_grid((int64_t)a.B * a.Hq * a.tiles)), dim3(ATTN_THREADS), 0, s, a);
-        DGL_CHECK_LAUNCH("dgl_attention_backward (query rows)");
-        if (a.dslope != nullptr) {
-            hipLaunchKernelGGL(attn_dslope_kernel, dim3(a.Hq), dim3(256), 0, s, a);
-            DGL_CHECK_LAUNCH("dgl_attention_backward (slopes)");
+        if (a.splits > 1) {
+            const int64_t rows = (int64_t)a.B * a.Hq * a.Lq;
+            hipLaunchKernelGGL((attn_fwd_join_kernel<T>), dim3((unsigned)((rows + 3) / 4)), dim3(ATTN_THREADS), 0, s, a);
+            DGL_CHECK_LAUNCH("dgl_attention_forward (join)");
         }
         return DGL_OK;
     }
 };
+template <int T, int DP, int N> struct LaunchBwdQ {
+    static constexpr int kernel = KERNEL_BWD_Q;
+    static int go(const AttnArgs &a, hipStream_t s) {
+        hipLaunchKernelGGL((attn_bwd_q_kernel<T, DP, N>), dim3(xcd_grid((int64_t)a.B * a.Hq * a.tiles)), dim3(ATTN_THREADS), 0, s, a);
+        DGL_CHECK_LAUNCH("dgl_attention_backward (query rows)");
+        return DGL_OK;
+    }
+};
 template <int T, int DP, int N> struct LaunchBwdKv {
-    static int go(AttnArgs a, hipStream_t s) {
-        a.tiles = (a.Lk + 64 * N - 1) / (64 * N);
-        hipLaunchKernelGGL((attn_bwd_kv_kernel<T, DP, N>), dim3(xcd_grid((int64_t)a.B * a.Hkv * a.tiles)), dim3(ATTN_THREADS), 0, s, a);
+    static constexpr int kernel = KERNEL_BWD_KV;
+    static int go(const AttnArgs &a, hipStream_t s) {
+        const int64_t blocks = (int64_t)a.B * a.Hkv * a.tiles * a.head_parts * a.splits;
+        hipLaunchKernelGGL((attn_bwd_kv_kernel<T, DP, N>), dim3(xcd_grid(blocks)), dim3(ATTN_THREADS), 0, s, a);
         DGL_CHECK_LAUNCH("dgl_attention_backward (key rows)");
+        if (a.head_parts * a.splits > 1) {
+            const int64_t rows = (int64_t)a.B * a.Hkv * a.Lk;
+            hipLaunchKernelGGL((attn_bwd_kv_join_kernel<T>), dim3((unsigned)((rows + 3) / 4)), dim3(ATTN_THREADS), 0, s, a);
+            DGL_CHECK_LAUNCH("dgl_attention_backward (join)");
+        }
         return DGL_OK;
     }
 };
 
 }  // namespace
 
-extern "C" int dgl_attention_forward(const dgl_attention_t *p, dgl_stream_t stream) {
+extern "C" int64_t dgl_attention_forward_workspace_floats(const dgl_attention_t *p) {
+    return check_attention(p) != DGL_OK ? -1 : forward_floats(attention_args(p), p->dtype);
+}
+
+extern "C" int dgl_attention_forward(const dgl_attention_t *p, float *ws, dgl_stream_t stream) {
     if (int e = check_attention(p)) return e;
     if (p->Lq == 0) return DGL_OK;
-    const AttnArgs a = attention_args(p);
-    return by_type<LaunchFwd>(a, p->dtype, two_blocks(a, a.Lq, a.Hq) ? 2 : 1, (hipStream_t)stream);
+    AttnArgs a = attention_args(p);
+    int n;
+    plan_forward(a, p->dtype, n);
+    DGL_CHECK_ARG(a.splits == 1 || (ws != nullptr && (reinterpret_cast<uintptr_t>(ws) & 15) == 0), "a 16-byte aligned workspace is needed");
+    a.part = ws;
+    return by_type<LaunchFwd>(a, p->dtype, n, (hipStream_t)stream);
 }
+
+// Workspace of the backward pass: delta and (half precision) the row scales, the slopes' partial sums, the parts of dk / dv
+int64_t backward_rows(const dgl_attention_t *p) { return ((int64_t)p->B * p->Hq * p->Lq + 3) / 4 * 4; }
+int64_t backward_slopes(const dgl_attention_t *p) { return ((int64_t)p->B * p->Hq * ((p->Lq + 63) / 64) + 3) / 4 * 4; }
 
 extern "C" int64_t dgl_attention_backward_workspace_floats(const dgl_attention_t *p) {
     if (check_attention(p) != DGL_OK) return -1;
-    const int64_t rows = (int64_t)p->B * p->Hq * p->Lq;
-    return 2 * rows + (int64_t)p->B * p->Hq * ((p->Lq + 63) / 64) + 4;
+    return 2 * backward_rows(p) + backward_slopes(p) + keys_floats(attention_args(p), p->dtype) + 4;
 }
 
 extern "C" int dgl_attention_backward(const dgl_attention_t *p, const dgl_attention_grad_t *g, float *ws, dgl_stream_t stream) {
     if (int e = check_attention(p)) return e;
-    DGL_CHECK_ARG(g != nullptr && ws != nullptr, "NULL argument");
+    DGL_CHECK_ARG(g != nullptr && ws != nullptr && (reinterpret_cast<uintptr_t>(ws) & 15) == 0, "NULL argument or misaligned workspace");
     DGL_CHECK_ARG((p->Lq == 0 || (g->dout != nullptr && g->dq != nullptr && p->lse != nullptr)) &&
                       (p->Lk == 0 || (g->dk != nullptr && g->dv != nullptr)), "dout, dq, dk, dv or lse is NULL");
     DGL_CHECK_ARG(g->dslope == nullptr || p->slope != nullptr, "dslope without a slope");
     const int bytes = p->dtype == DGL_DTYPE_F32 ? 4 : 2;
     DGL_CHECK_ARG(aligned_strides(g->dout_stride, g->dout, bytes) && aligned_strides(g->dq_stride, g->dq, bytes) &&
                       aligned_strides(g->dk_stride, g->dk, bytes) && aligned_strides(g->dv_stride, g->dv, bytes),
-                  "dout, dq, dk, dv: 16-byte aligned pointers and strides");
+                  "dout, dq, dk, dv: 16-byte aligned pointers and strides, tokens less than 64 MiB apart");
     AttnArgs a = attention_args(p);
     a.dout = (const char *)g->dout; a.dq = (char *)g->dq; a.dk = (char *)g->dk; a.dv = (char *)g->dv; a.dslope = g->dslope;
     for (int i = 0; i < 3; ++i) {
         a.dos[i] = g->dout_stride[i]; a.dqst[i] = g->dq_stride[i]; a.dkst[i] = g->dk_stride[i]; a.dvst[i] = g->dv_stride[i];
     }
-    const int64_t rows = (int64_t)p->B * p->Hq * p->Lq;
     a.delta = ws;
-    a.rowscale = ws + rows;
-    a.dslope_part = g->dslope != nullptr ? ws + 2 * rows : nullptr;
-    // (no rows: the slope's gradient is the empty sum, and the launcher of the query kernel would have an empty grid)
+    a.rowscale = ws + backward_rows(p);
+    a.dslope_part = g->dslope != nullptr ? ws + 2 * backward_rows(p) : nullptr;
+    a.part = ws + 2 * backward_rows(p) + backward_slopes(p);
+    hipStream_t s = (hipStream_t)stream;
     if (p->Lq > 0) {
-        if (int e = by_type<LaunchBwdQ>(a, p->dtype, two_blocks(a, a.Lq, a.Hq) ? 2 : 1, (hipStream_t)stream)) return e;
-    } else if (a.dslope != nullptr) {
-        a.tiles = 0;
-        hipLaunchKernelGGL(attn_dslope_kernel, dim3(a.Hq), dim3(256), 0, (hipStream_t)stream, a);
+        const int n = two_blocks(KERNEL_BWD_Q, p->dtype, a, a.Lq, a.Hq) ? 2 : 1;
+        a.tiles = (a.Lq + 64 * n - 1) / (64 * n);
+        if (int e = by_type<LaunchBwdQ>(a, p->dtype, n, s)) return e;
+    }
+    if (a.dslope != nullptr) {                       // (without rows: the empty sum)
+        hipLaunchKernelGGL(attn_dslope_kernel, dim3(a.Hq), dim3(256), 0, s, a);
         DGL_CHECK_LAUNCH("dgl_attention_backward (slopes)");
     }
-    if (p->Lk > 0) return by_type<LaunchBwdKv>(a, p->dtype, two_blocks(a, a.Lk, a.Hkv) ? 2 : 1, (hipStream_t)stream);
+    if (p->Lk > 0) {
+        int n;
+        plan_keys(a, p->dtype, n);
+        return by_type<LaunchBwdKv>(a, p->dtype, n, s);
+    }
     return DGL_OK;
 }

@@ -43,24 +43,12 @@ __device__ __forceinline__ int live_length(const StepArgs &a, int b) {
     return max(0, min(a.lengths[b], a.max_pages << a.shift));
 }
 
-struct StepScore {
-    float mul, cap2;
-    int cap;
-};
-__device__ __forceinline__ StepScore step_score(const StepArgs &a) {
-    StepScore s;
-    s.cap = a.cap > 0.0f;
-    s.mul = s.cap ? a.scale / a.cap : a.scale * ATTN_LOG2E;
-    s.cap2 = a.cap * ATTN_LOG2E;
-    return s;
-}
-
 // one (row, head) key by key: the wave's lanes hold keys for the scores and dimensions for the sum
 template <int TYPE> __device__ void careful_step_row(const StepArgs &a, int b, int hk, int m, float top, float total) {
     typedef typename Elem<TYPE>::raw raw;
     const int lane = threadIdx.x & 63, p = m / a.G, h = hk * a.G + m % a.G, n = live_length(a, b);
     const int64_t row = (int64_t)b * a.P + p;
-    const StepScore sp = step_score(a);
+    const ScoreParams sp = score_params(a.scale, a.cap, 0, nullptr, 0);
     const raw *q = reinterpret_cast<const raw *>(a.q) + row * a.qs[0] + h * a.qs[1];
     float acc0 = 0.0f, acc1 = 0.0f;
     for (int base = 0; base < n; base += 64) {
@@ -73,8 +61,7 @@ template <int TYPE> __device__ void careful_step_row(const StepArgs &a, int b, i
             const raw *k = reinterpret_cast<const raw *>(a.k) + page * a.ks[0] + hk * a.ks[1] + (j & ((1 << a.shift) - 1)) * a.ks[2];
             float dot = 0.0f;
             for (int d = 0; d < a.D; ++d) dot = fmaf(elem_to_float<TYPE>(q[d]), elem_to_float<TYPE>(k[d]), dot);
-            float s = dot * sp.mul;
-            if (sp.cap) s = sp.cap2 * attn_tanh(s);
+            float th, s = score_of(sp, dot, th);
             if (a.bias == 1) s = fmaf(-a.slope[h] * ATTN_LOG2E, (float)(n - 1 - j), s);
             if (a.bias == 2) {
                 const int at = min(j, a.pos_rows - 1);
@@ -224,7 +211,7 @@ __global__ __launch_bounds__(64 * STEP_WAVES) void attn_step_kernel(StepArgs a) 
     const int n_keys = live_length(a, b);
     const int tiles = (n_keys + STEP_TILE - 1) / STEP_TILE, per = (tiles + a.splits - 1) / a.splits;
     const int end = min(tiles, (split + 1) * per);
-    const StepScore sp = step_score(a);
+    const ScoreParams sp = score_params(a.scale, a.cap, 0, nullptr, 0);
 
     Frag<TYPE, DP> qf[NQ];
     f32x4 o[NQ][S::dt];
@@ -259,17 +246,25 @@ __global__ __launch_bounds__(64 * STEP_WAVES) void attn_step_kernel(StepArgs a) 
         for (int x = 0; x < 2; ++x)
 #pragma unroll
             for (int n = 0; n < NQ; ++n) s[x][n] = dot_block<TYPE, DP>(t.k[x], qf[n]);
+        if (sp.cap == CAP_NONE) {
 #pragma unroll
-        for (int x = 0; x < 2; ++x)
+            for (int x = 0; x < 2; ++x)
 #pragma unroll
-            for (int n = 0; n < NQ; ++n) s[x][n] = s[x][n] * sp.mul;
-        if (sp.cap) {
+                for (int n = 0; n < NQ; ++n) s[x][n] = s[x][n] * sp.mul;
+        } else if (sp.cap == CAP_FAST) {
 #pragma unroll
             for (int x = 0; x < 2; ++x)
 #pragma unroll
                 for (int n = 0; n < NQ; ++n)
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) s[x][n][r] = sp.cap2 * attn_tanh(s[x][n][r]);
+                    for (int r = 0; r < 4; ++r) s[x][n][r] = fmaf(-2.0f * sp.cap2, cap_r(s[x][n][r] * sp.mul2), sp.cap2);
+        } else {
+#pragma unroll
+            for (int x = 0; x < 2; ++x)
+#pragma unroll
+                for (int n = 0; n < NQ; ++n)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) s[x][n][r] = sp.cap2 * attn_tanh(s[x][n][r] * sp.mul);
         }
         if (a.bias == 1) {
             const float k0 = (float)(base + 4 * g);
@@ -312,9 +307,9 @@ __global__ __launch_bounds__(64 * STEP_WAVES) void attn_step_kernel(StepArgs a) 
         }
 #pragma unroll
         for (int n = 0; n < NQ; ++n) {
-            float top = fmaxf(fmaxf(fmaxf(s[0][n][0], s[0][n][1]), fmaxf(s[0][n][2], s[0][n][3])),
-                              fmaxf(fmaxf(s[1][n][0], s[1][n][1]), fmaxf(s[1][n][2], s[1][n][3])));
-            top = fmaxf(group_max(top), m[n]);
+            float top = fast_max(fast_max(fast_max(s[0][n][0], s[0][n][1]), fast_max(s[0][n][2], s[0][n][3])),
+                                 fast_max(fast_max(s[1][n][0], s[1][n][1]), fast_max(s[1][n][2], s[1][n][3])));
+            top = fast_max(group_max(top), m[n]);
             const float shift = top == -attn_inf() ? 0.0f : top;
             if (__any(top > m[n])) {
                 const float f = __builtin_amdgcn_exp2f(m[n] - shift);

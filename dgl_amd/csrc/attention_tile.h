@@ -39,6 +39,10 @@ __device__ __forceinline__ float group_sum(float x) {
     return __uint_as_float(s[0]) + __uint_as_float(s[1]);
 }
 
+// Maximum as a median with infinity: one instruction, where fmaxf first quiets operands it cannot prove to be no signalling
+// NaN.  (A NaN score makes its row NaN through the sum, whatever the maximum is.)
+__device__ __forceinline__ float fast_max(float a, float b) { return __builtin_amdgcn_fmed3f(a, b, __builtin_inff()); }
+
 // tanh to about 4 ulp: 1 - 2 / (e^{2y} + 1) away from zero, its odd series (to y^11) near it, where the difference would cancel
 __device__ __forceinline__ float attn_tanh(float y) {
     const float e = __builtin_amdgcn_exp2f(y * (2.0f * ATTN_LOG2E));
@@ -50,6 +54,35 @@ __device__ __forceinline__ float attn_tanh(float y) {
     p = fmaf(z, p, -3.3333334e-1f);
     const float near = fmaf(y * z, p, y);
     return z < 0.16f ? near : far;
+}
+// A capped score cap tanh(x / cap) is cap - 2 cap r with r = 1 / (e^{2x/cap} + 1): off by about cap 2^-24 absolutely, no
+// more than a binary32 score of that size is anyhow, in 11 issue slots instead of 23.  Above CAP_PRECISE the relative error
+// of small scores would count (4e-6 at 64): there tanh is taken to a few ulp.  In both, 1 - tanh^2 = 4 (r - r^2).
+#define CAP_PRECISE 64.0f
+enum { CAP_NONE = 0, CAP_FAST = 1, CAP_EXACT = 2 };
+__device__ __forceinline__ float cap_r(float y2) { return __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(y2) + 1.0f); }
+
+// the scalar part of a score, in units of log2
+struct ScoreParams {
+    float mul, mul2, cap2, slope2;     // factor of the dot product; 2 log2(e) scale / cap; cap log2(e); slope log2(e)
+    int cap, bias;
+};
+__device__ __forceinline__ ScoreParams score_params(float scale, float cap, int bias, const float *slope, int h) {
+    ScoreParams p;
+    p.cap = cap > 0.0f ? (cap <= CAP_PRECISE ? CAP_FAST : CAP_EXACT) : CAP_NONE;
+    p.mul = p.cap ? scale / cap : scale * ATTN_LOG2E;
+    p.mul2 = p.mul * (2.0f * ATTN_LOG2E);
+    p.cap2 = cap * ATTN_LOG2E;
+    p.bias = bias;
+    p.slope2 = bias ? slope[h] * ATTN_LOG2E : 0.0f;
+    return p;
+}
+// without the bias, for a single dot product (th: its tanh, 0 without a cap)
+__device__ __forceinline__ float score_of(const ScoreParams &p, float dot, float &th) {
+    th = 0.0f;
+    if (p.cap == CAP_NONE) return dot * p.mul;
+    th = p.cap == CAP_FAST ? fmaf(-2.0f, cap_r(dot * p.mul2), 1.0f) : attn_tanh(dot * p.mul);
+    return p.cap2 * th;
 }
 
 // ---- element types -----------------------------------------------------------------------------------------------
@@ -63,8 +96,11 @@ template <> struct Elem<ATTN_F32> { typedef float raw; static constexpr int byte
 
 template <int TYPE> __device__ __forceinline__ float elem_to_float(typename Elem<TYPE>::raw x) {
     if constexpr (TYPE == ATTN_F32) return x;
-    else if constexpr (TYPE == ATTN_F16) return (float)__builtin_bit_cast(_Float16, x);
-    else return __uint_as_float((unsigned)x << 16);
+    else if constexpr (TYPE == ATTN_F16) {
+        float f = (float)__builtin_bit_cast(_Float16, x);
+        asm("" : "+v"(f));     // keeps the conversion apart: mixed-precision FMAs stay the sign of split_f16.h's assembly
+        return f;
+    } else return __uint_as_float((unsigned)x << 16);
 }
 
 // four consecutive elements stored with one access (8 or 16 bytes)
@@ -128,8 +164,8 @@ template <int TYPE> __device__ __forceinline__ f32x4 mfma16(u32x4 a, u32x4 b, f3
 }
 
 // acc[row 4g+r][column c] += (tile rows 16 t ..) . (block whose operand registers are b)
-template <int TYPE, int DP> __device__ __forceinline__ f32x4 dot_block(const Frag<TYPE, DP> &a, const Frag<TYPE, DP> &b) {
-    f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
+template <int TYPE, int DP>
+__device__ __forceinline__ f32x4 dot_block(const Frag<TYPE, DP> &a, const Frag<TYPE, DP> &b, f32x4 acc = f32x4{0.0f, 0.0f, 0.0f, 0.0f}) {
 #pragma unroll
     for (int k = 0; k < Shape<TYPE, DP>::chunks; ++k) acc = mfma16<TYPE>(a.c[k], b.c[k], acc);
     return acc;
@@ -197,21 +233,47 @@ template <int TYPE, int DP> __device__ __forceinline__ void unit_place(int u, in
     }
 }
 
-// rows base + 0..63 of a [rows][D] matrix with `stride` elements between rows; rows at or beyond `rows`, and rows whose
-// entry of `skip` is negative, are zero
-template <int TYPE, int DP>
-__device__ __forceinline__ void unit_load(Unit &un, int u, const typename Elem<TYPE>::raw *src, int64_t stride, int base, int rows,
-                                          int D, const int *skip) {
-    int grp, piece;
-    unit_place<TYPE, DP>(u, grp, piece);
-    const int d = piece * Shape<TYPE, DP>::vec;
+// What a thread knows about its unit of every tile: byte offsets of the four rows from the tile's first (below 2^32 by the
+// launcher's check, so that a load is a scalar address plus a 32-bit offset)
+struct UnitPlan {
+    unsigned off, row_bytes;
+    int grp;
+    bool in;                                   // the piece lies within the head size
+};
+template <int TYPE, int DP> __device__ __forceinline__ UnitPlan unit_plan(int u, int64_t stride, int D) {
+    UnitPlan p;
+    int piece;
+    unit_place<TYPE, DP>(u, p.grp, piece);
+    p.row_bytes = (unsigned)(stride * Elem<TYPE>::bytes);
+    p.off = 4u * (unsigned)p.grp * p.row_bytes + 16u * (unsigned)piece;
+    p.in = piece * Shape<TYPE, DP>::vec < D;
+    return p;
+}
+// the rows of a tile that starts at `tile` with `rows` rows left; rows beyond are zero
+__device__ __forceinline__ void unit_load(Unit &un, const UnitPlan &p, const char *tile, int rows) {
+    if (rows >= ATTN_ROWS) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int row = base + 4 * grp + i;
-        bool live = row < rows && d < D;
-        if (live && skip != nullptr) live = skip[row] >= 0;
-        un.r[i] = live ? *reinterpret_cast<const u32x4 *>(src + (int64_t)row * stride + d) : u32x4{0, 0, 0, 0};
+        for (int i = 0; i < 4; ++i) un.r[i] = p.in ? *reinterpret_cast<const u32x4 *>(tile + (p.off + i * p.row_bytes)) : u32x4{0, 0, 0, 0};
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            un.r[i] = p.in && 4 * p.grp + i < rows ? *reinterpret_cast<const u32x4 *>(tile + (p.off + i * p.row_bytes)) : u32x4{0, 0, 0, 0};
     }
+}
+// rows of padding (document id < 0) may hold anything: they are staged as zeros, so that a NaN among them does not send the
+// whole tile down the careful path
+struct UnitIds {
+    int id[4];
+};
+__device__ __forceinline__ void unit_load_ids(UnitIds &ids, const UnitPlan &p, const int *tile, int rows) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) ids.id[i] = 4 * p.grp + i < rows ? tile[4 * p.grp + i] : -1;
+}
+__device__ __forceinline__ void unit_skip(Unit &un, const UnitIds &ids) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int w = 0; w < 4; ++w) un.r[i][w] = ids.id[i] >= 0 ? un.r[i][w] : 0u;
 }
 
 template <int TYPE, int DP, bool ROWMAJOR, bool TRANSPOSED>

@@ -370,8 +370,8 @@ DGL_API int dgl_adam_step(float *params, const float *grads, float *exp_avg, flo
  *   out_i = sum over allowed j of softmax_j(s_ij) v_j; a row without an allowed key is zeros with lse = -inf.
  * Query head h reads key head h / (Hq / Hkv).  A masked pair contributes nothing, whatever its operands hold (NaN and
  * infinities included).  Tensors are addressed by strides in elements {batch, head, token}, the head's D elements are
- * consecutive; pointers and strides are multiples of 16 bytes, strides may be 0 for inputs.  D is a multiple of 8, at most
- * 128; lengths may be 0 and are at most DGL_ATTENTION_MAX_LENGTH.  Scores, softmax and sums are binary32 for every
+ * consecutive; pointers and strides are multiples of 16 bytes, tokens less than 64 MiB apart, strides may be 0 for inputs.
+ * D is a multiple of 8, at most 128; lengths may be 0 and are at most DGL_ATTENTION_MAX_LENGTH.  Scores, softmax and sums are binary32 for every
  * element type; for the 16-bit types probabilities (and, backward, score gradients) are rounded to the type before they
  * multiply v (k, q, dout). */
 #define DGL_DTYPE_F32 0
@@ -403,12 +403,17 @@ typedef struct {
     float *dslope;             /* [Hq] or NULL */
 } dgl_attention_grad_t;
 
-/* The operator above (beside TSP/TSPModel.py:420-441). */
-DGL_API int dgl_attention_forward(const dgl_attention_t *a, dgl_stream_t stream);
+/* The operator above (beside TSP/TSPModel.py:420-441).  ws: dgl_attention_forward_workspace_floats(a) floats, 16-byte aligned
+ * (may be NULL where that is 0). */
+DGL_API int dgl_attention_forward(const dgl_attention_t *a, float *ws, dgl_stream_t stream);
+
+/* Floats of workspace dgl_attention_forward needs for `a`: few query rows against many keys are cut into ranges of keys (-1:
+ * invalid arguments; beside TSP/TSPModel.py:420-441). */
+DGL_API int64_t dgl_attention_forward_workspace_floats(const dgl_attention_t *a);
 
 /* Gradients of a forward call with the same arguments, whose out and lse are given in `a`: dq, dk, dv (written, not added
  * to) and, where wanted, the slopes' gradient (the reference's loss.backward() through TSP/TSPModel.py:420-441).  Sums are
- * ordered: the same call gives the same bits.  ws: dgl_attention_backward_workspace_floats(a) floats. */
+ * ordered: the same call gives the same bits.  ws: dgl_attention_backward_workspace_floats(a) floats, 16-byte aligned. */
 DGL_API int dgl_attention_backward(const dgl_attention_t *a, const dgl_attention_grad_t *g, float *ws, dgl_stream_t stream);
 
 /* Floats of workspace dgl_attention_backward needs for `a` (-1: invalid arguments; beside TSP/TSPModel.py:420-441). */

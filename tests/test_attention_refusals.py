@@ -32,15 +32,26 @@ def struct(**kw):
 def test_forward_refuses(kw, word):
     lib = _lib.load()
     a = struct(**kw)
-    assert lib.dgl_attention_forward(ctypes.byref(a), None) == -1
+    assert lib.dgl_attention_forward(ctypes.byref(a), None, None) == -1
     assert word in lib.dgl_last_error_string()
     assert lib.dgl_attention_backward_workspace_floats(ctypes.byref(a)) == -1
+    assert lib.dgl_attention_forward_workspace_floats(ctypes.byref(a)) == -1
+
+
+def test_few_rows_against_many_keys_need_a_workspace():
+    lib = _lib.load()
+    a = struct(Lk=20000)
+    assert lib.dgl_attention_forward_workspace_floats(ctypes.byref(a)) > 0
+    assert lib.dgl_attention_forward(ctypes.byref(a), None, None) == -1 and b"workspace" in lib.dgl_last_error_string()
+    assert lib.dgl_attention_forward(ctypes.byref(a), FAKE + 4, None) == -1
+    a = struct(k_stride=(ctypes.c_int64 * 3)(1 << 30, 1 << 29, 1 << 24))
+    assert lib.dgl_attention_forward(ctypes.byref(a), None, None) == -1 and b"64 MiB" in lib.dgl_last_error_string()
 
 
 def test_backward_refuses():
     lib = _lib.load()
     a, g = struct(), _lib.AttentionGrad()
-    assert lib.dgl_attention_forward(None, None) == -1
+    assert lib.dgl_attention_forward(None, None, None) == -1
     assert lib.dgl_attention_backward(ctypes.byref(a), None, FAKE, None) == -1
     assert lib.dgl_attention_backward(ctypes.byref(a), ctypes.byref(g), FAKE, None) == -1
     g.dout = g.dq = g.dk = g.dv = FAKE

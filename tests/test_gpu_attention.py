@@ -107,6 +107,19 @@ def test_two_blocks_wide_heads(device, dtype, D):
     check_all(t, kw)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("H,K,L,M,D", [(2, 1, 5, 3000, 16), (8, 2, 600, 1100, 64), (4, 1, 1500, 130, 32), (8, 1, 1200, 1200, 128)])
+def test_long_sides_are_split_and_joined(device, dtype, causal, H, K, L, M, D):
+    """Few rows against many keys (forward), few keys or many shared heads against many rows (backward)."""
+    t, kw = inputs(1, H, K, L, M, D, TYPES[dtype], L, bias="coords")
+    kw["doc_q"] = torch.zeros(1, L, dtype=torch.int32, device=device)
+    kw["doc_k"] = torch.zeros(1, M, dtype=torch.int32, device=device)
+    kw["doc_k"][0, 100:120] = -1
+    t["v"][:, :, 100:120] = math.nan
+    check_all(t, kw, cap=8.0, causal=causal)
+
+
 def test_scores_of_large_magnitude_and_flat_caps(device):
     t, kw = inputs(1, 2, 2, 80, 80, 16, torch.float32, 4)
     check_all({**t, "q": t["q"] * 30}, kw)                       # nearly one-hot rows
