@@ -460,50 +460,77 @@ template <int TYPE> __global__ __launch_bounds__(ATTN_THREADS) void attn_fwd_joi
 }
 
 // ---------------------------------------------------------------------------------------------------------- backward
-// Probabilities and score gradients of four pairs from their dot products: s = q.k, dp = do.v - delta (the subtraction is
-// the matrix instruction's initial accumulator), e = lse in units of log2 (infinite for rows without a key).  du comes
-// without the factor scale, and without the 4 of 1 - tanh^2 = 4 (r - r^2) where scores are capped (undo_factor).
-struct PairGrad {
-    f32x4 p, ds, du;
-};
-__device__ __forceinline__ PairGrad pair_grad(const ScoreParams &sp, f32x4 s, f32x4 dp, f32x4 e, f32x4 dist, bool masked, const bool (&ok)[4]) {
-    PairGrad w;
-    f32x4 x, slack = {1.0f, 1.0f, 1.0f, 1.0f};
+// The scalar part of the backward pass on the pairs of 2 x N blocks of 16 x 16, phase by phase: each phase is one uniform
+// branch around 8 N independent chains a lane (a branch per block left too few to hide the latency of exp and rcp).
+//   in   s = q.k,  dp = do.v - delta (the subtraction is the matrix instruction's initial accumulator), e = lse in units of
+//        log2 (infinite for rows without a key), dist
+//   out  s = p,  dp = ds = p (dp - delta)
+// slack is 1 - tanh^2 = 4 (r - r^2) without its 4 (undo_factor), and undefined without a cap.
+template <int N>
+__device__ __forceinline__ void pair_probability(const ScoreParams &sp, f32x4 (&s)[2][N], f32x4 (&dp)[2][N], f32x4 (&slack)[2][N],
+                                                 const f32x4 (&dist)[2][N], const f32x4 (&e)[2][N]) {
     if (sp.cap == CAP_NONE) {
 #pragma unroll
-        for (int r = 0; r < 4; ++r) x[r] = fmaf(s[r], sp.mul, -e[r]);
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int n = 0; n < N; ++n) {
+                f32x4 x = s[t][n];
+#pragma unroll
+                for (int r = 0; r < 4; ++r) x[r] = fmaf(x[r], sp.mul, -e[t][n][r]);
+                s[t][n] = x;
+            }
     } else if (sp.cap == CAP_FAST) {
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            const float y = cap_r(s[r] * sp.mul2);
-            x[r] = fmaf(-2.0f * sp.cap2, y, sp.cap2 - e[r]);
-            slack[r] = fmaf(-y, y, y);
-        }
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int n = 0; n < N; ++n) {
+                f32x4 x = s[t][n], k = x;
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const float y = cap_r(x[r] * sp.mul2);
+                    x[r] = fmaf(-2.0f * sp.cap2, y, sp.cap2 - e[t][n][r]);
+                    k[r] = fmaf(-y, y, y);
+                }
+                s[t][n] = x;
+                slack[t][n] = k;
+            }
     } else {
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            const float th = attn_tanh(s[r] * sp.mul);
-            x[r] = fmaf(sp.cap2, th, -e[r]);
-            slack[r] = 0.25f * fmaf(-th, th, 1.0f);
-        }
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int n = 0; n < N; ++n) {
+                f32x4 x = s[t][n], k = x;
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const float th = attn_tanh(x[r] * sp.mul);
+                    x[r] = fmaf(sp.cap2, th, -e[t][n][r]);
+                    k[r] = 0.25f * fmaf(-th, th, 1.0f);
+                }
+                s[t][n] = x;
+                slack[t][n] = k;
+            }
     }
     if (sp.bias) {
 #pragma unroll
-        for (int r = 0; r < 4; ++r) x[r] = fmaf(-sp.slope2, dist[r], x[r]);
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int n = 0; n < N; ++n) {
+                f32x4 x = s[t][n];
+#pragma unroll
+                for (int r = 0; r < 4; ++r) x[r] = fmaf(-sp.slope2, dist[t][n][r], x[r]);
+                s[t][n] = x;
+            }
     }
 #pragma unroll
-    for (int r = 0; r < 4; ++r) w.p[r] = __builtin_amdgcn_exp2f(x[r]);
+    for (int t = 0; t < 2; ++t)
 #pragma unroll
-    for (int r = 0; r < 4; ++r) w.ds[r] = w.p[r] * dp[r];
-    if (masked) {
+        for (int n = 0; n < N; ++n) {
+            f32x4 x = s[t][n];
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            w.p[r] = ok[r] ? w.p[r] : 0.0f;
-            w.ds[r] = ok[r] ? w.ds[r] : 0.0f;
+            for (int r = 0; r < 4; ++r) x[r] = __builtin_amdgcn_exp2f(x[r]);
+            s[t][n] = x;
+            dp[t][n] = x * dp[t][n];
         }
-    }
-    w.du = sp.cap ? w.ds * slack : w.ds;
-    return w;
 }
 __device__ __forceinline__ float undo_factor(const AttnArgs &a) { return a.cap > 0.0f ? 4.0f * a.scale : a.scale; }
 
@@ -691,61 +718,85 @@ __global__ __launch_bounds__(ATTN_THREADS, DP <= 64 ? 2 : 1) void attn_bwd_q_ker
 
 #pragma unroll
         for (int tp = 0; tp < 2; ++tp) {
-            f32x4 w[2][NQ];
+            f32x4 s[2][NQ], dp[2][NQ], slack[2][NQ] = {}, dist[2][NQ] = {};
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
-                const int at = 32 * tp + 16 * t;
-                f32x4 s[NQ], dp[NQ];
                 Frag<TYPE, DP> f;
-                frag_from_lds<TYPE, DP>(f, Kt, at + c, g);
+                frag_from_lds<TYPE, DP>(f, Kt, 32 * tp + 16 * t + c, g);
 #pragma unroll
-                for (int n = 0; n < NQ; ++n) s[n] = dot_block<TYPE, DP>(f, qf[n]);
-                frag_from_lds<TYPE, DP>(f, Vt, at + c, g);
+                for (int n = 0; n < NQ; ++n) s[t][n] = dot_block<TYPE, DP>(f, qf[n]);
+                frag_from_lds<TYPE, DP>(f, Vt, 32 * tp + 16 * t + c, g);
 #pragma unroll
-                for (int n = 0; n < NQ; ++n) dp[n] = dot_block<TYPE, DP>(f, of[n], f32x4{-delta[n], -delta[n], -delta[n], -delta[n]});
-                f32x4 p0 = {0, 0, 0, 0}, p1 = {0, 0, 0, 0};
-                i32x4 kd = {0, 0, 0, 0};
-                if (sp.bias == 2) {
-                    p0 = *reinterpret_cast<const f32x4 *>(key_pos + 2 * (at + 4 * g));
-                    p1 = *reinterpret_cast<const f32x4 *>(key_pos + 2 * (at + 4 * g) + 4);
-                }
-                if (by_doc) kd = *reinterpret_cast<const i32x4 *>(key_doc + at + 4 * g);
-                const float kx[4] = {p0[0], p0[2], p1[0], p1[2]}, ky[4] = {p0[1], p0[3], p1[1], p1[3]};
+                for (int n = 0; n < NQ; ++n) dp[t][n] = dot_block<TYPE, DP>(f, of[n], f32x4{-delta[n], -delta[n], -delta[n], -delta[n]});
+            }
+            if (sp.bias == 1) {
+                const float k0 = (float)(base + 32 * tp + 4 * g);
 #pragma unroll
-                for (int n = 0; n < NQ; ++n) {
-                    f32x4 dist = {0, 0, 0, 0};
-                    if (sp.bias == 1) {
-                        const float d0 = qx[n] - (float)(base + at + 4 * g);
+                for (int t = 0; t < 2; ++t)
 #pragma unroll
-                        for (int r = 0; r < 4; ++r) dist[r] = fabsf(d0 - (float)r);
-                    } else if (sp.bias == 2) {
+                    for (int n = 0; n < NQ; ++n)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) dist[t][n][r] = fabsf((qx[n] - k0) - (float)(16 * t + r));
+            } else if (sp.bias == 2) {
+#pragma unroll
+                for (int t = 0; t < 2; ++t) {
+                    const float *at = key_pos + 2 * (32 * tp + 16 * t + 4 * g);
+                    const f32x4 p0 = *reinterpret_cast<const f32x4 *>(at), p1 = *reinterpret_cast<const f32x4 *>(at + 4);
+                    const float kx[4] = {p0[0], p0[2], p1[0], p1[2]}, ky[4] = {p0[1], p0[3], p1[1], p1[3]};
+#pragma unroll
+                    for (int n = 0; n < NQ; ++n)
 #pragma unroll
                         for (int r = 0; r < 4; ++r) {
                             const float dx = qx[n] - kx[r], dy = qy[n] - ky[r];
-                            dist[r] = __builtin_amdgcn_sqrtf(fmaf(dx, dx, dy * dy));
+                            dist[t][n][r] = __builtin_amdgcn_sqrtf(fmaf(dx, dx, dy * dy));
                         }
-                    }
-                    bool ok[4] = {true, true, true, true};
-                    if (masked) {
-                        const int left = limit[n] - (base + at + 4 * g);
-#pragma unroll
-                        for (int r = 0; r < 4; ++r) ok[r] = r < left && (!by_doc || kd[r] == doc[n]);
-                    }
-                    const PairGrad pg = pair_grad(sp, s[n], dp[n], f32x4{lse2[n], lse2[n], lse2[n], lse2[n]}, dist, masked, ok);
-                    if (want_slope) {
-#pragma unroll
-                        for (int r = 0; r < 4; ++r) {
-                            // (coordinates of a masked key may be NaN as well)
-                            const float x = masked && !ok[r] ? 0.0f : dist[r];
-                            excess[n] += pg.ds[r];
-                            pd[n] = fmaf(pg.p[r], x, pd[n]);
-                            dsl[n] = fmaf(pg.ds[r], x, dsl[n]);
-                        }
-                    }
-                    w[t][n] = pg.du;
                 }
             }
-            accumulate<TYPE, DP, NQ>(dq, Kt, KT, tp, w[0], w[1], g, c);
+            f32x4 e[2][NQ];
+#pragma unroll
+            for (int n = 0; n < NQ; ++n) e[0][n] = e[1][n] = f32x4{lse2[n], lse2[n], lse2[n], lse2[n]};
+            pair_probability<NQ>(sp, s, dp, slack, dist, e);
+            if (masked) {
+#pragma unroll
+                for (int t = 0; t < 2; ++t) {
+                    i32x4 kd = {0, 0, 0, 0};
+                    if (by_doc) kd = *reinterpret_cast<const i32x4 *>(key_doc + 32 * tp + 16 * t + 4 * g);
+#pragma unroll
+                    for (int n = 0; n < NQ; ++n) {
+                        const int left = limit[n] - (base + 32 * tp + 4 * g), own = by_doc ? doc[n] : 0;
+                        f32x4 p = s[t][n], ds = dp[t][n], away = dist[t][n];
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) {
+                            const bool ok = (16 * t + r < left) & (kd[r] == own);
+                            p[r] = ok ? p[r] : 0.0f;
+                            ds[r] = ok ? ds[r] : 0.0f;
+                            away[r] = ok ? away[r] : 0.0f;                   // (a masked key's coordinates may be NaN)
+                        }
+                        s[t][n] = p;
+                        dp[t][n] = ds;
+                        dist[t][n] = away;
+                    }
+                }
+            }
+            if (want_slope) {
+#pragma unroll
+                for (int t = 0; t < 2; ++t)
+#pragma unroll
+                    for (int n = 0; n < NQ; ++n)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) {
+                            excess[n] += dp[t][n][r];
+                            pd[n] = fmaf(s[t][n][r], dist[t][n][r], pd[n]);
+                            dsl[n] = fmaf(dp[t][n][r], dist[t][n][r], dsl[n]);
+                        }
+            }
+            if (sp.cap) {
+#pragma unroll
+                for (int t = 0; t < 2; ++t)
+#pragma unroll
+                    for (int n = 0; n < NQ; ++n) dp[t][n] = dp[t][n] * slack[t][n];
+            }
+            accumulate<TYPE, DP, NQ>(dq, Kt, KT, tp, dp[0], dp[1], g, c);
         }
     }
 
@@ -1006,52 +1057,79 @@ __global__ __launch_bounds__(ATTN_THREADS, DP <= 64 ? 2 : 1) void attn_bwd_kv_ke
 
 #pragma unroll
             for (int tp = 0; tp < 2; ++tp) {
-                f32x4 wp[2][NK], ws[2][NK];
+                f32x4 s[2][NK], dp[2][NK], slack[2][NK] = {}, dist[2][NK] = {}, e[2][NK];
 #pragma unroll
                 for (int t = 0; t < 2; ++t) {
                     const int at = 32 * tp + 16 * t;
-                    f32x4 s[NK], dp[NK];
                     Frag<TYPE, DP> f;
                     frag_from_lds<TYPE, DP>(f, Qt, at + c, g);
 #pragma unroll
-                    for (int n = 0; n < NK; ++n) s[n] = dot_block<TYPE, DP>(f, kf[n]);
+                    for (int n = 0; n < NK; ++n) s[t][n] = dot_block<TYPE, DP>(f, kf[n]);
                     const f32x4 minus_delta = *reinterpret_cast<const f32x4 *>(row_delta + at + 4 * g);
                     frag_from_lds<TYPE, DP>(f, Ot, at + c, g);
 #pragma unroll
-                    for (int n = 0; n < NK; ++n) dp[n] = dot_block<TYPE, DP>(f, vf[n], minus_delta);
-                    const f32x4 e = *reinterpret_cast<const f32x4 *>(row_lse + at + 4 * g);
-                    f32x4 qx = {0, 0, 0, 0}, qy = {0, 0, 0, 0};
-                    i32x4 lim = {0, 0, 0, 0}, qd = {0, 0, 0, 0};
-                    if (sp.bias) qx = *reinterpret_cast<const f32x4 *>(row_x + at + 4 * g);
-                    if (sp.bias == 2) qy = *reinterpret_cast<const f32x4 *>(row_y + at + 4 * g);
-                    if (masked) lim = *reinterpret_cast<const i32x4 *>(row_lim + at + 4 * g);
-                    if (by_doc) qd = *reinterpret_cast<const i32x4 *>(row_doc + at + 4 * g);
+                    for (int n = 0; n < NK; ++n) dp[t][n] = dot_block<TYPE, DP>(f, vf[n], minus_delta);
+                    const f32x4 lse2 = *reinterpret_cast<const f32x4 *>(row_lse + at + 4 * g);
 #pragma unroll
-                    for (int n = 0; n < NK; ++n) {
-                        f32x4 dist = {0, 0, 0, 0};
+                    for (int n = 0; n < NK; ++n) e[t][n] = lse2;
+                }
+                if (sp.bias) {
+#pragma unroll
+                    for (int t = 0; t < 2; ++t) {
+                        const f32x4 qx = *reinterpret_cast<const f32x4 *>(row_x + 32 * tp + 16 * t + 4 * g);
                         if (sp.bias == 1) {
 #pragma unroll
-                            for (int r = 0; r < 4; ++r) dist[r] = fabsf(qx[r] - kx[n]);
-                        } else if (sp.bias == 2) {
+                            for (int n = 0; n < NK; ++n)
 #pragma unroll
-                            for (int r = 0; r < 4; ++r) {
-                                const float dx = qx[r] - kx[n], dy = qy[r] - ky[n];
-                                dist[r] = __builtin_amdgcn_sqrtf(fmaf(dx, dx, dy * dy));
-                            }
-                        }
-                        bool ok[4] = {true, true, true, true};
-                        if (masked) {
-                            const int j = wrow0 + 16 * n + c;
+                                for (int r = 0; r < 4; ++r) dist[t][n][r] = fabsf(qx[r] - kx[n]);
+                        } else {
+                            const f32x4 qy = *reinterpret_cast<const f32x4 *>(row_y + 32 * tp + 16 * t + 4 * g);
 #pragma unroll
-                            for (int r = 0; r < 4; ++r) ok[r] = j < lim[r] && (!by_doc || qd[r] == doc[n]);
+                            for (int n = 0; n < NK; ++n)
+#pragma unroll
+                                for (int r = 0; r < 4; ++r) {
+                                    const float dx = qx[r] - kx[n], dy = qy[r] - ky[n];
+                                    dist[t][n][r] = __builtin_amdgcn_sqrtf(fmaf(dx, dx, dy * dy));
+                                }
                         }
-                        const PairGrad pg = pair_grad(sp, s[n], dp[n], e, dist, masked, ok);
-                        wp[t][n] = pg.p;
-                        ws[t][n] = TYPE == ATTN_F16 ? pg.du * gmul : pg.du;
                     }
                 }
-                accumulate<TYPE, DP, NK>(dv, Ot, OT, tp, wp[0], wp[1], g, c);
-                accumulate<TYPE, DP, NK>(dk, Qt, QT, tp, ws[0], ws[1], g, c);
+                pair_probability<NK>(sp, s, dp, slack, dist, e);
+                if (masked) {
+#pragma unroll
+                    for (int t = 0; t < 2; ++t) {
+                        const i32x4 lim = *reinterpret_cast<const i32x4 *>(row_lim + 32 * tp + 16 * t + 4 * g);
+                        i32x4 qd = {0, 0, 0, 0};
+                        if (by_doc) qd = *reinterpret_cast<const i32x4 *>(row_doc + 32 * tp + 16 * t + 4 * g);
+#pragma unroll
+                        for (int n = 0; n < NK; ++n) {
+                            const int j = wrow0 + 16 * n + c, own = by_doc ? doc[n] : 0;
+                            f32x4 p = s[t][n], ds = dp[t][n];
+#pragma unroll
+                            for (int r = 0; r < 4; ++r) {
+                                const bool ok = (j < lim[r]) & (qd[r] == own);
+                                p[r] = ok ? p[r] : 0.0f;
+                                ds[r] = ok ? ds[r] : 0.0f;
+                            }
+                            s[t][n] = p;
+                            dp[t][n] = ds;
+                        }
+                    }
+                }
+                accumulate<TYPE, DP, NK>(dv, Ot, OT, tp, s[0], s[1], g, c);
+                if (sp.cap) {
+#pragma unroll
+                    for (int t = 0; t < 2; ++t)
+#pragma unroll
+                        for (int n = 0; n < NK; ++n) dp[t][n] = dp[t][n] * slack[t][n];
+                }
+                if (TYPE == ATTN_F16) {
+#pragma unroll
+                    for (int t = 0; t < 2; ++t)
+#pragma unroll
+                        for (int n = 0; n < NK; ++n) dp[t][n] = dp[t][n] * gmul;
+                }
+                accumulate<TYPE, DP, NK>(dk, Qt, QT, tp, dp[0], dp[1], g, c);
             }
         }
     }
@@ -1168,7 +1246,7 @@ int padded(int D) { return D <= 16 ? 16 : D <= 32 ? 32 : D <= 64 ? 64 : 128; }
 // of two waves per SIMD, and one where two would leave compute units idle (fewer than two workgroups for each of the 256).
 enum { KERNEL_FWD, KERNEL_BWD_Q, KERNEL_BWD_KV };
 constexpr bool two_fit(int kernel, int type, int DP) {
-    return kernel == KERNEL_FWD ? !(type == ATTN_F32 && DP == 128) : kernel == KERNEL_BWD_Q ? DP <= (type == ATTN_F32 ? 32 : 64) : DP <= 32;
+    return kernel == KERNEL_FWD ? !(type == ATTN_F32 && DP == 128) : DP <= (type == ATTN_F32 ? 32 : 64);
 }
 bool two_blocks(int kernel, int dtype, const AttnArgs &a, int rows, int heads) {
     return two_fit(kernel, dtype, padded(a.D)) && (int64_t)a.B * heads * ((rows + 127) / 128) >= 512;
@@ -1186,12 +1264,14 @@ void plan_forward(AttnArgs &a, int dtype, int &n) {
     a.splits = a.tiles > 0 ? ranges((int64_t)a.B * a.Hq * a.tiles, a.Lk) : 1;
 }
 void plan_keys(AttnArgs &a, int dtype, int &n) {
-    n = two_blocks(KERNEL_BWD_KV, dtype, a, a.Lk, a.Hkv) ? 2 : 1;
+    // (the heads of a group and ranges of 512 query rows can be dealt out as well, so two blocks of keys fill the chip earlier)
+    const int64_t pairs = (int64_t)a.B * a.Hq * ((a.Lk + 127) / 128) * ((a.Lq + 511) / 512);
+    n = two_fit(KERNEL_BWD_KV, dtype, padded(a.D)) && pairs >= 512 ? 2 : 1;
     a.tiles = (a.Lk + 64 * n - 1) / (64 * n);
     const int64_t blocks = (int64_t)a.B * a.Hkv * (a.tiles > 0 ? a.tiles : 1);
     const int64_t want = blocks >= 768 ? 1 : (768 + blocks - 1) / blocks;       // (two or three workgroups fit a unit)
-    a.head_parts = (int)(want < a.G ? want : a.G);
-    a.head_parts = (a.G + (a.G + a.head_parts - 1) / a.head_parts - 1) / ((a.G + a.head_parts - 1) / a.head_parts);   // no empty part
+    const int heads = (int)((a.G + (want < a.G ? want : a.G) - 1) / (want < a.G ? want : a.G));
+    a.head_parts = (a.G + heads - 1) / heads;
     a.splits = ranges(blocks * a.head_parts, a.Lq);
 }
 int64_t forward_floats(AttnArgs a, int dtype) {
