@@ -12,6 +12,7 @@ are copied), float32, float16 or bfloat16.  The computation runs in libdgl_amd o
 from __future__ import annotations
 
 import ctypes
+import struct
 from typing import Optional, Tuple
 
 import torch
@@ -20,40 +21,41 @@ from . import _lib
 from ._lib import check, ptr
 
 _DTYPES = {torch.float32: _lib.DTYPE_F32, torch.float16: _lib.DTYPE_F16, torch.bfloat16: _lib.DTYPE_BF16}
+_VEC = {torch.float32: 4, torch.float16: 8, torch.bfloat16: 8}      # elements of 16 bytes
+
+# A call of a few microseconds on the device is lost in a host path that sets ctypes fields one by one: the ABI structs are
+# packed in one go (the formats restate include/dgl_amd.h; a wrong size fails here, at import).
+_PACK_ATTENTION = struct.Struct("@8i2f12q5P3P2q2P2qP")
+_PACK_GRAD = struct.Struct("@4P12qP")
+_PACK_STEP = struct.Struct("@2i2f4q6Pq2iPq")
+_STEP_AT = _lib.AttentionStep.rows_per_instance.offset
+assert _PACK_ATTENTION.size == ctypes.sizeof(_lib.Attention) and _PACK_GRAD.size == ctypes.sizeof(_lib.AttentionGrad)
+assert _STEP_AT == ctypes.sizeof(_lib.KVCache) and _STEP_AT + _PACK_STEP.size == ctypes.sizeof(_lib.AttentionStep)
+_raw_stream = torch._C._cuda_getCurrentRawStream
 
 
-def _stream(device) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
-
-
-class _on:
-    """Make a tensor's device current for a launch (nothing to do where it already is)."""
-
-    def __init__(self, device):
-        self.device, self.guard = device, None
-
-    def __enter__(self):
-        if self.device.index != torch.cuda.current_device():
-            self.guard = torch.cuda.device(self.device)
-            self.guard.__enter__()
-
-    def __exit__(self, *exc):
-        if self.guard is not None:
-            self.guard.__exit__(*exc)
+def _launch(device, function, *args, what: str) -> None:
+    """An entry point on the device's current stream, with that device current."""
+    index = device.index
+    if index == torch.cuda.current_device():
+        code = function(*args, _raw_stream(index))
+    else:
+        with torch.cuda.device(index):
+            code = function(*args, _raw_stream(index))
+    if code:
+        check(code, what)
 
 
 def _usable(t: torch.Tensor) -> torch.Tensor:
     """The tensor itself where the kernels can address it, else a contiguous copy."""
-    vec = 16 // t.element_size()
-    st = t.stride()
-    if (st[-1] == 1 and t.data_ptr() % 16 == 0 and all(x % vec == 0 for x in st[:-1]) and
-            (len(st) != 4 or st[2] * t.element_size() < 1 << 26)):
-        return t
+    vec, st = _VEC[t.dtype], t.stride()
+    if st[-1] == 1 and t.data_ptr() % 16 == 0:
+        if len(st) == 4:
+            if not (st[0] % vec or st[1] % vec or st[2] % vec) and st[2] < (1 << 24):
+                return t
+        elif not any(x % vec for x in st[:-1]):
+            return t
     return t.clone(memory_format=torch.contiguous_format)
-
-
-def _stride3(t: torch.Tensor):
-    return (ctypes.c_int64 * 3)(*t.stride()[:3])
 
 
 def _check_qkv(q, k, v):
@@ -78,30 +80,31 @@ def _side(t: Optional[torch.Tensor], name, shape, dtype, device) -> Optional[tor
     if t is None:
         return None
     if t.device != device:
-        raise ValueError(f"{name} is on {t.device}, q on {device}")
-    if tuple(t.shape) != shape:
-        raise ValueError(f"{name} has shape {tuple(t.shape)}, expected {shape}")
+        raise ValueError(f"{name} is on {t.device}, expected {device}")
+    if t.shape != shape:
+        raise ValueError(f"{name} has shape {tuple(t.shape)}, expected {tuple(shape)}")
     if t.dtype != dtype:
         if dtype == torch.int32 and t.is_floating_point() or dtype == torch.float32 and not t.is_floating_point():
             raise ValueError(f"{name} is {t.dtype}, expected {dtype}")
         t = t.to(dtype)
-    inner, want = t.stride()[1:], []
+    if t.is_contiguous():
+        return t
     n = 1
-    for s in reversed(shape[1:]):
-        want.insert(0, n)
-        n *= s
-    if any(a != b and s > 1 for a, b, s in zip(inner, want, shape[1:])) or (t.dim() == 1 and shape[0] > 1 and t.stride(0) != 1):
-        t = t.contiguous()
-    return t
+    for size, stride in zip(reversed(shape[1:]), reversed(t.stride()[1:])):
+        if size > 1 and stride != n:
+            return t.contiguous()
+        n *= size
+    return t.contiguous() if len(shape) == 1 else t
 
 
 class _Call:
-    """Arguments of one operator call: the ABI struct and the tensors it points to."""
+    """Arguments of one operator call: the tensors the kernels can address, and the ABI struct over them."""
+    __slots__ = ("q", "k", "v", "slope", "pos_q", "pos_k", "doc_q", "doc_k", "prefix", "head", "tail", "a", "out", "lse")
 
     def __init__(self, q, k, v, scale, cap, slope, pos_q, pos_k, doc_q, doc_k, causal, prefix):
         _check_qkv(q, k, v)
         B, H, L, D = q.shape
-        M = k.shape[2]
+        _, K, M, _ = k.shape
         dev = q.device
         cap = float(cap)
         if not 0.0 <= cap < float("inf"):
@@ -112,6 +115,8 @@ class _Call:
             raise ValueError("coordinates without a slope")
         if prefix is not None and not causal:
             raise ValueError("a prefix belongs to a causal mask")
+        if max(L, M) > _lib.ATTENTION_MAX_LENGTH or B * H * (max(L, M) + 63) // 64 >= 1 << 30:
+            raise ValueError(f"q {tuple(q.shape)}, k {tuple(k.shape)}: too long")
         self.q, self.k, self.v = _usable(q), _usable(k), _usable(v)
         self.slope = _side(slope, "slope", (H,), torch.float32, dev)
         self.pos_q = _side(pos_q, "pos_q", (B, L, 2), torch.float32, dev)
@@ -119,23 +124,18 @@ class _Call:
         self.doc_q = _side(doc_q, "doc_q", (B, L), torch.int32, dev)
         self.doc_k = _side(doc_k, "doc_k", (B, M), torch.int32, dev)
         self.prefix = _side(prefix, "prefix", (B,), torch.int32, dev)
-        a = self.a = _lib.Attention()
-        a.dtype, a.B, a.Hq, a.Hkv, a.Lq, a.Lk, a.D = _DTYPES[q.dtype], B, H, k.shape[1], L, M, D
-        a.causal, a.cap = int(bool(causal)), cap
-        a.scale = D ** -0.5 if scale is None else float(scale)
-        a.q_stride, a.k_stride, a.v_stride = _stride3(self.q), _stride3(self.k), _stride3(self.v)
-        a.q, a.k, a.v = ptr(self.q), ptr(self.k), ptr(self.v)
-        a.slope, a.prefix = ptr(self.slope), ptr(self.prefix)
-        if pos_q is not None:
-            a.pos_q, a.pos_k = ptr(self.pos_q), ptr(self.pos_k)
-            a.pos_q_stride, a.pos_k_stride = self.pos_q.stride(0), self.pos_k.stride(0)
-        if doc_q is not None:
-            a.doc_q, a.doc_k = ptr(self.doc_q), ptr(self.doc_k)
-            a.doc_q_stride, a.doc_k_stride = self.doc_q.stride(0), self.doc_k.stride(0)
+        self.head = (_DTYPES[q.dtype], B, H, K, L, M, D, 1 if causal else 0, D ** -0.5 if scale is None else float(scale), cap,
+                     *self.q.stride()[:3], *self.k.stride()[:3], *self.v.stride()[:3])
+        pos, doc = self.pos_q is not None, self.doc_q is not None
+        self.tail = (ptr(self.slope), ptr(self.pos_q), ptr(self.pos_k), self.pos_q.stride(0) if pos else 0,
+                     self.pos_k.stride(0) if pos else 0, ptr(self.doc_q), ptr(self.doc_k), self.doc_q.stride(0) if doc else 0,
+                     self.doc_k.stride(0) if doc else 0, ptr(self.prefix))
 
     def set_out(self, out, lse):
         self.out, self.lse = out, lse
-        self.a.out, self.a.o_stride, self.a.lse = ptr(out), _stride3(out), ptr(lse)
+        self.a = _lib.Attention()
+        _PACK_ATTENTION.pack_into(self.a, 0, *self.head, *out.stride()[:3], self.q.data_ptr(), self.k.data_ptr(), self.v.data_ptr(),
+                                  out.data_ptr(), ptr(lse), *self.tail)
 
 
 def _like_heads(t: torch.Tensor) -> torch.Tensor:
@@ -143,8 +143,8 @@ def _like_heads(t: torch.Tensor) -> torch.Tensor:
     it) where its model is, head by head otherwise."""
     B, H, L, D = t.shape
     if t.stride(1) < t.stride(2):
-        return torch.empty(B, L, H, D, dtype=t.dtype, device=t.device).transpose(1, 2)
-    return torch.empty(B, H, L, D, dtype=t.dtype, device=t.device)
+        return torch.empty_strided((B, H, L, D), (L * H * D, D, H * D, 1), dtype=t.dtype, device=t.device)
+    return torch.empty_strided((B, H, L, D), (H * L * D, L * D, D, 1), dtype=t.dtype, device=t.device)
 
 
 def _forward(call: _Call, want_lse: bool):
@@ -154,10 +154,10 @@ def _forward(call: _Call, want_lse: bool):
     call.set_out(out, lse)
     if out.numel():
         lib = _lib.load()
-        need = lib.dgl_attention_forward_workspace_floats(ctypes.byref(call.a))
-        with _on(q.device):
-            ws = torch.empty(need, dtype=torch.float32, device=q.device) if need > 0 else None
-            check(lib.dgl_attention_forward(ctypes.byref(call.a), ptr(ws), _stream(q.device)), "dgl_attention_forward")
+        a = ctypes.byref(call.a)
+        need = lib.dgl_attention_forward_workspace_floats(a)
+        ws = torch.empty(need, dtype=torch.float32, device=q.device) if need > 0 else None
+        _launch(q.device, lib.dgl_attention_forward, a, ptr(ws), what="dgl_attention_forward")
     return out, lse
 
 
@@ -172,13 +172,11 @@ def _backward(call: _Call, dout: torch.Tensor, want_slope: bool):
     if q.shape[0] == 0:
         return dq, dk, dv, None if dslope is None else dslope.zero_()
     g = _lib.AttentionGrad()
-    g.dout, g.dq, g.dk, g.dv, g.dslope = ptr(dout), ptr(dq), ptr(dk), ptr(dv), ptr(dslope)
-    g.dout_stride, g.dq_stride, g.dk_stride, g.dv_stride = _stride3(dout), _stride3(dq), _stride3(dk), _stride3(dv)
-    need = lib.dgl_attention_backward_workspace_floats(ctypes.byref(call.a))
-    with _on(q.device):
-        ws = torch.empty(max(need, 1), dtype=torch.float32, device=q.device)
-        check(lib.dgl_attention_backward(ctypes.byref(call.a), ctypes.byref(g), ptr(ws), _stream(q.device)),
-              "dgl_attention_backward")
+    _PACK_GRAD.pack_into(g, 0, dout.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), *dout.stride()[:3], *dq.stride()[:3],
+                         *dk.stride()[:3], *dv.stride()[:3], ptr(dslope))
+    a = ctypes.byref(call.a)
+    ws = torch.empty(max(lib.dgl_attention_backward_workspace_floats(a), 1), dtype=torch.float32, device=q.device)
+    _launch(q.device, lib.dgl_attention_backward, a, ctypes.byref(g), ws.data_ptr(), what="dgl_attention_backward")
     return dq, dk, dv, dslope
 
 
@@ -243,14 +241,17 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, scale: Optio
     Under graph capture, leaves that collect gradients are refused: a leaf's accumulation belongs to the stream on which
     it was first used, and a captured backward pass that meets an eager graph of the same leaf ends the process.  Capture
     attention_forward and attention_backward instead."""
-    if torch.is_grad_enabled() and torch.cuda.is_available() and torch.cuda.is_current_stream_capturing():
-        for t in (q, k, v, slope):
-            if t is not None and t.requires_grad and t.is_leaf:
-                raise RuntimeError("attention: a leaf that requires grad inside a graph capture; capture attention_forward "
-                                   "and attention_backward, or pass a tensor computed from the leaf")
+    if torch.is_grad_enabled():
+        leaves = [t for t in (q, k, v, slope) if t is not None and t.requires_grad and t.is_leaf]
+        if leaves and q.is_cuda and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("attention: a leaf that requires grad inside a graph capture; capture attention_forward "
+                               "and attention_backward, or pass a tensor computed from the leaf")
     for name, t in (("pos_q", pos_q), ("pos_k", pos_k)):
         if t is not None and t.requires_grad and torch.is_grad_enabled():
             raise ValueError(f"{name} requires grad: the operator is not differentiable in the coordinates")
+    if not torch.is_grad_enabled() or not (q.requires_grad or k.requires_grad or v.requires_grad or
+                                           (slope is not None and slope.requires_grad)):
+        return _forward(_Call(q, k, v, scale, cap, slope, pos_q, pos_k, doc_q, doc_k, causal, prefix), False)[0]
     return _Attention.apply(q, k, v, slope, scale, cap, pos_q, pos_k, doc_q, doc_k, causal, prefix)
 
 
@@ -313,7 +314,8 @@ class PagedCache:
         c = self.struct = _lib.KVCache()
         c.dtype, c.B, c.Hkv, c.D = _DTYPES[self.dtype], self.batch, k_pages.shape[1], k_pages.shape[3]
         c.page_size, c.max_pages, c.num_pages = self.page_size, table.shape[1], k_pages.shape[0]
-        c.k_stride, c.v_stride, c.table_stride = _stride3(k_pages), _stride3(v_pages), table.stride(0)
+        c.k_stride = (ctypes.c_int64 * 3)(*k_pages.stride()[:3])
+        c.v_stride, c.table_stride = (ctypes.c_int64 * 3)(*v_pages.stride()[:3]), table.stride(0)
         c.k_pages, c.v_pages, c.table, c.lengths = ptr(k_pages), ptr(v_pages), ptr(table), ptr(lengths)
 
     # ---- pages of a pool ------------------------------------------------------------------
@@ -358,9 +360,10 @@ class PagedCache:
             k_new, v_new = _usable(k_new), _usable(v_new)
             counts = _side(counts, "counts", (self.batch,), torch.int32, self.device)
             start = self.lengths if start is None else _side(start, "start", (self.batch,), torch.int32, self.device)
-            with _on(self.device):
-                check(_lib.load().dgl_cache_append(ctypes.byref(c), ptr(k_new), ptr(v_new), _stride3(k_new), _stride3(v_new), want[2],
-                                                   ptr(start), ptr(counts), ptr(self.lengths), _stream(self.device)), "dgl_cache_append")
+            strides = (ctypes.c_int64 * 6)(*k_new.stride()[:3], *v_new.stride()[:3])
+            _launch(self.device, _lib.load().dgl_cache_append, ctypes.byref(c), k_new.data_ptr(), v_new.data_ptr(),
+                    ctypes.addressof(strides), ctypes.addressof(strides) + 24, want[2], start.data_ptr(), ptr(counts),
+                    self.lengths.data_ptr(), what="dgl_cache_append")
 
 
 def attention_step(q: torch.Tensor, cache: PagedCache, *, rows_per_instance: int = 1, scale: Optional[float] = None,
@@ -382,13 +385,8 @@ def attention_step(q: torch.Tensor, cache: PagedCache, *, rows_per_instance: int
         R, H, D = q.shape
         out = torch.empty(R, H, D, dtype=q.dtype, device=dev)
         lse = torch.empty(R, H, dtype=torch.float32, device=dev) if return_lse else None
-        a = _lib.AttentionStep()
-        a.cache, a.rows_per_instance, a.Hq, a.cap = c, rows_per_instance, H, float(cap)
-        a.scale = D ** -0.5 if scale is None else float(scale)
-        a.q_stride, a.o_stride = (ctypes.c_int64 * 2)(*q.stride()[:2]), (ctypes.c_int64 * 2)(H * D, D)
-        a.q, a.out, a.lse = ptr(q), ptr(out), ptr(lse)
         slope = _side(slope, "slope", (H,), torch.float32, dev)
-        a.slope = ptr(slope)
+        n = pos_stride = words = bits_stride = 0
         if pos_q is not None:
             pos_q = _side(pos_q, "pos_q", (R, 2), torch.float32, dev)
             if pos_q.stride(0) != 2:             # rows of one wide tensor, or one row for all
@@ -397,16 +395,21 @@ def attention_step(q: torch.Tensor, cache: PagedCache, *, rows_per_instance: int
             pos_k = _side(pos_k, "pos_k", (cache.batch, n, 2), torch.float32, dev)
             if pos_k.data_ptr() % 8 or pos_k.stride(0) % 2:
                 pos_k = pos_k.clone(memory_format=torch.contiguous_format)
-            a.pos_q, a.pos_k, a.pos_k_stride, a.pos_rows = ptr(pos_q), ptr(pos_k), pos_k.stride(0), n
+            pos_stride = pos_k.stride(0)
         if blocked is not None:
             if blocked.dim() != 2 or blocked.shape[0] != R or blocked.dtype != torch.int64 or blocked.device != dev:
                 raise ValueError(f"blocked is {tuple(blocked.shape)} {blocked.dtype}: int64 words [{R}, n] on {dev} are expected")
-            if blocked.shape[1] > 1 and blocked.stride(1) != 1:
+            words = blocked.shape[1]
+            if words > 1 and blocked.stride(1) != 1:
                 blocked = blocked.contiguous()
-            a.blocked, a.words, a.blocked_stride = ptr(blocked), blocked.shape[1], blocked.stride(0)
-        lib = _lib.load()
-        need = lib.dgl_attention_step_workspace_floats(ctypes.byref(a))
-        with _on(dev):
-            ws = torch.empty(need, dtype=torch.float32, device=dev) if need > 0 else None
-            check(lib.dgl_attention_step(ctypes.byref(a), ptr(ws), _stream(dev)), "dgl_attention_step")
+            bits_stride = blocked.stride(0)
+        a = _lib.AttentionStep()
+        a.cache = c
+        _PACK_STEP.pack_into(a, _STEP_AT, rows_per_instance, H, D ** -0.5 if scale is None else float(scale), float(cap),
+                             *q.stride()[:2], H * D, D, q.data_ptr(), out.data_ptr(), ptr(lse), ptr(slope), ptr(pos_q),
+                             ptr(pos_k), pos_stride, n, words, ptr(blocked), bits_stride)
+        lib, ref = _lib.load(), ctypes.byref(a)
+        need = lib.dgl_attention_step_workspace_floats(ref)
+        ws = torch.empty(need, dtype=torch.float32, device=dev) if need > 0 else None
+        _launch(dev, lib.dgl_attention_step, ref, ptr(ws), what="dgl_attention_step")
         return (out, lse) if return_lse else out

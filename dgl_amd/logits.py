@@ -7,16 +7,19 @@ hold them."""
 from __future__ import annotations
 
 import ctypes
+import struct
 from dataclasses import dataclass
 from typing import Optional, Tuple, Union
 
 import torch
 
 from . import _lib
-from ._lib import check, ptr
-from .attention import _DTYPES, _on, _side, _stream
+from ._lib import ptr
+from .attention import _DTYPES, _launch, _side
 
 PerRow = Union[float, torch.Tensor]
+_PACK = struct.Struct("@4iPqPq2iPqPq4P4fPqP")
+assert _PACK.size == ctypes.sizeof(_lib.Logits)
 
 
 @dataclass
@@ -58,21 +61,17 @@ def process_logits(logits: torch.Tensor, *, blocked: Optional[torch.Tensor] = No
             raise ValueError("no actions")
         if logits.stride(1) != 1 and A > 1:
             logits = logits.contiguous()
-        a = _lib.Logits()
-        a.dtype, a.R, a.A, a.period = _DTYPES[logits.dtype], R, A, A if period is None else int(period)
-        a.logits, a.logits_stride, a.temperature = ptr(logits), logits.stride(0), float(temperature)
-        keep = []
+        words = bits_stride = cols = history_stride = bias_stride = 0
         if blocked is not None:
             if blocked.dim() != 2 or blocked.shape[0] != R or blocked.dtype != torch.int64 or blocked.device != dev:
                 raise ValueError(f"blocked is {tuple(blocked.shape)} {blocked.dtype}: int64 words [{R}, n] on {dev} are expected")
-            if blocked.shape[1] > 1 and blocked.stride(1) != 1:
+            words = blocked.shape[1]
+            if words > 1 and blocked.stride(1) != 1:
                 blocked = blocked.contiguous()
-            keep.append(blocked)
-            a.blocked, a.blocked_stride, a.words = ptr(blocked), blocked.stride(0), blocked.shape[1]
+            bits_stride = blocked.stride(0)
         if bias is not None:
             bias = _side(bias, "bias", (A,) if bias.dim() == 1 else (R, A), torch.float32, dev)
-            keep.append(bias)
-            a.bias, a.bias_stride = ptr(bias), 0 if bias.dim() == 1 else bias.stride(0)
+            bias_stride = 0 if bias.dim() == 1 else bias.stride(0)
         if history_len is not None and history is None:
             raise ValueError("history_len without a history")
         if history is not None:
@@ -80,26 +79,23 @@ def process_logits(logits: torch.Tensor, *, blocked: Optional[torch.Tensor] = No
                 raise ValueError(f"history has shape {tuple(history.shape)}: [{R}, n] is expected")
             history = _side(history, "history", (R, history.shape[1]), torch.int32, dev)
             history_len = _side(history_len, "history_len", (R,), torch.int32, dev)
-            keep += [history, history_len]
-            a.history, a.history_stride, a.history_cols = ptr(history), history.stride(0), history.shape[1]
-            a.history_len = ptr(history_len)
-            if a.history is None or not history.numel():
-                a.history = None
-        for name, x in (("repetition", repetition), ("presence", presence), ("frequency", frequency)):
-            if isinstance(x, torch.Tensor):
-                x = _side(x, name, (R,), torch.float32, dev)
-                keep.append(x)
-                setattr(a, name, ptr(x))
-            else:
-                setattr(a, name + "_all", float(x))
-        out = torch.empty(R, A, dtype=torch.float32, device=dev)
+            cols, history_stride = history.shape[1], history.stride(0)
+        rows, numbers = [], []
+        for name, x, neutral in (("repetition", repetition, 1.0), ("presence", presence, 0.0), ("frequency", frequency, 0.0)):
+            per_row = isinstance(x, torch.Tensor)
+            rows.append(_side(x, name, (R,), torch.float32, dev) if per_row else None)
+            numbers.append(neutral if per_row else float(x))
+        out = torch.empty((R, A), dtype=torch.float32, device=dev)
         selected = torch.empty(R, dtype=torch.int32, device=dev)
         if R == 0:
             return out, selected
-        a.log_probs, a.out_stride, a.selected = ptr(out), A, ptr(selected)
-        lib = _lib.load()
-        need = lib.dgl_logits_workspace_floats(ctypes.byref(a))
-        with _on(dev):
-            ws = torch.empty(need, dtype=torch.float32, device=dev) if need > 0 else None
-            check(lib.dgl_logits_process(ctypes.byref(a), ptr(ws), _stream(dev)), "dgl_logits_process")
+        a = _lib.Logits()
+        _PACK.pack_into(a, 0, _DTYPES[logits.dtype], R, A, A if period is None else int(period), logits.data_ptr(), logits.stride(0),
+                        ptr(blocked), bits_stride, words, cols, ptr(bias), bias_stride, ptr(history) if cols else 0, history_stride,
+                        ptr(history_len), ptr(rows[0]), ptr(rows[1]), ptr(rows[2]), *numbers, float(temperature), out.data_ptr(), A,
+                        selected.data_ptr())
+        lib, ref = _lib.load(), ctypes.byref(a)
+        need = lib.dgl_logits_workspace_floats(ref)
+        ws = torch.empty(need, dtype=torch.float32, device=dev) if need > 0 else None
+        _launch(dev, lib.dgl_logits_process, ref, ptr(ws), what="dgl_logits_process")
         return out, selected
