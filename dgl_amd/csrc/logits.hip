@@ -4,8 +4,8 @@
 //   c = occurrences of a in the history;  c > 0:  x = (x > 0 ? x / repetition : x repetition) - presence - frequency c
 //   x = (x + bias) / temperature;  blocked: x = -inf;   log_prob = x - log sum exp x;   pick = lowest index of the maximum
 //
-// Bound by reading the logits and writing the log-probabilities once.  Up to 32 values per thread a row stays in the
-// registers of one workgroup between the two (a row of the policy's actions always does); longer rows are cut into tiles of
+// Bound by reading the logits and writing the log-probabilities once.  Up to 24576 actions a row stays in the registers of
+// one workgroup between the two (the policy's rows up to CVRP-12000 do); longer rows are cut into tiles of
 // 8192 actions, one launch for the tiles' maxima and sums, a second one that computes the values again - reading the
 // logits twice costs less than writing and reading back binary32 values in between.
 // Occurrences are counted in LDS per row (or tile), with integer atomics: their order does not matter.
@@ -31,7 +31,8 @@ struct LogitsArgs {
     int64_t hs;
     int cols;
     const float *rep, *pres, *freq;
-    float rep_all, pres_all, freq_all, temperature;
+    float rep_all, pres_all, freq_all, temperature, inv_temperature;
+    int bits_together;                // V neighbouring actions share a word of bits
     float *out;
     int64_t os;
     int *selected;
@@ -47,17 +48,13 @@ template <int TYPE> __device__ __forceinline__ float logit_float(typename LogitE
     else return __uint_as_float((unsigned)x << 16);
 }
 
-// V consecutive values (V = 4: one access of 16 or 8 bytes)
+// V consecutive values by one access
 template <int TYPE, int V> __device__ __forceinline__ void load_logits(float (&x)[V], const typename LogitElem<TYPE>::raw *p) {
-    if constexpr (V == 1) {
-        x[0] = logit_float<TYPE>(p[0]);
-    } else if constexpr (TYPE == 0) {
-        const float4 v = *reinterpret_cast<const float4 *>(p);
-        x[0] = v.x; x[1] = v.y; x[2] = v.z; x[3] = v.w;
-    } else {
-        const ushort4 v = *reinterpret_cast<const ushort4 *>(p);
-        x[0] = logit_float<TYPE>(v.x); x[1] = logit_float<TYPE>(v.y); x[2] = logit_float<TYPE>(v.z); x[3] = logit_float<TYPE>(v.w);
-    }
+    typedef typename LogitElem<TYPE>::raw raw;
+    struct alignas(sizeof(raw) * V) Pack { raw e[V]; };
+    const Pack v = *reinterpret_cast<const Pack *>(p);
+#pragma unroll
+    for (int e = 0; e < V; ++e) x[e] = logit_float<TYPE>(v.e[e]);
 }
 
 struct RowParams {
@@ -78,172 +75,278 @@ __device__ __forceinline__ unsigned bit_of(const LogitsArgs &a, unsigned act) {
     if (r >= (unsigned)a.period) r -= (unsigned)a.period;
     return r;
 }
-// the value of action `act` of row r; count: its occurrences (0 without a history).  Every operation rounds once, as written
-__device__ __forceinline__ float process(const LogitsArgs &a, const RowParams &p, int r, int act, float x, unsigned count) {
-    if (count != 0) {
-        x = __fsub_rn(x > 0.0f ? __fdiv_rn(x, p.rep) : __fmul_rn(x, p.rep), p.pres);
-        x = __fsub_rn(x, __fmul_rn(p.freq, (float)count));
-    }
-    if (a.bias != nullptr) x = __fadd_rn(x, a.bias[r * a.bias_s + act]);
-    if (a.temperature != 1.0f) x = __fdiv_rn(x, a.temperature);
-    if (a.blocked != nullptr) {
-        const unsigned bit = bit_of(a, (unsigned)act);
-        if ((int)(bit >> 5) < a.halves && ((a.blocked[r * a.bs + (bit >> 5)] >> (bit & 31)) & 1)) x = -__builtin_inff();
-    }
-    return x;
+// The value of an action that occurs c > 0 times in the history
+__device__ __forceinline__ float penalised(const RowParams &p, float x, unsigned c) {
+    const float y = __fsub_rn(x > 0.0f ? __fdiv_rn(x, p.rep) : __fmul_rn(x, p.rep), p.pres);
+    return __fsub_rn(y, __fmul_rn(p.freq, (float)c));
 }
 
-// counts of the actions first .. first + n - 1 of row r, by THREADS threads (a barrier on either side for more than a wave)
-template <int THREADS> __device__ __forceinline__ void count_history(unsigned *count, const LogitsArgs &a, int r, int first, int n, int tid) {
-    for (int i = tid; i < n; i += THREADS) count[i] = 0;
-    __syncthreads();
-    const int len = min(a.history_len != nullptr ? a.history_len[r] : a.cols, a.cols);
-    const int *h = a.history + r * a.hs;
-    for (int i = tid; i < len; i += THREADS) {
-        const int x = h[i] - first;
-        if (x >= 0 && x < n) atomicAdd(&count[x], 1u);
-    }
-    __syncthreads();
-}
-
-struct Best {
-    float value;
-    int index;                                   // INT_MAX: none
+// Occurrences in LDS, two 16-bit fields to a word while a history has fewer than 65536 entries (a CVRP-10000 row's fields
+// then leave room for several workgroups), else one 32-bit counter.
+struct Counts {
+    unsigned *word;
+    bool narrow;
+    __device__ __forceinline__ unsigned at(int i) const { return narrow ? (word[i >> 1] >> (16 * (i & 1))) & 0xffffu : word[i]; }
 };
-__device__ __forceinline__ Best better(Best a, Best b) { return b.value > a.value || (b.value == a.value && b.index < a.index) ? b : a; }
+// Counts the actions first .. first + n - 1 in row r's history.  (Computing the penalised values here, by the threads that
+// hold history entries, so that the values' owners only look them up, was 9 us slower at 256 x 131072 with 2048 entries.)
+template <int THREADS> __device__ __forceinline__ void count_history(const Counts &c, const LogitsArgs &a, int r, int first, int n, int tid) {
+    constexpr int EARLY = 4;                     // entries requested before the fields are cleared
+    const int words = c.narrow ? (n + 1) / 2 : n;
+    const int *h = a.history + r * a.hs;
+    int early[EARLY];
+#pragma unroll
+    for (int k = 0; k < EARLY; ++k) early[k] = tid + k * THREADS < a.cols ? h[tid + k * THREADS] : -1;
+    const int len = min(a.history_len != nullptr ? a.history_len[r] : a.cols, a.cols);
+    for (int i = tid; i < words; i += THREADS) c.word[i] = 0;
+    __syncthreads();
+    auto add = [&](int action) {
+        const int x = action - first;
+        if (x >= 0 && x < n) atomicAdd(&c.word[c.narrow ? x >> 1 : x], c.narrow ? 1u << (16 * (x & 1)) : 1u);
+    };
+#pragma unroll
+    for (int k = 0; k < EARLY; ++k)
+        if (tid + k * THREADS < len) add(early[k]);
+    for (int i = tid + EARLY * THREADS; i < len; i += THREADS) add(h[i]);
+    __syncthreads();
+}
+
 __device__ __forceinline__ float shifted_exp(float x, float shift) { return __builtin_amdgcn_exp2f((x - shift) * 1.4426950408889634f); }
 
-// maximum with its lowest index over the workgroup, in every thread
-template <int THREADS> __device__ __forceinline__ Best block_best(Best v, Best *slots, int tid) {
+// maximum / lowest index / sum over the workgroup, in every thread; `slots` of each are their own
+template <int THREADS> __device__ __forceinline__ float block_max(float v, float *slots, int tid) {
 #pragma unroll
-    for (int d = 1; d < 64; d <<= 1) v = better(v, Best{__shfl_xor(v.value, d), __shfl_xor(v.index, d)});
+    for (int d = 1; d < 64; d <<= 1) v = fmaxf(v, __shfl_xor(v, d));
     if constexpr (THREADS > 64) {
         if ((tid & 63) == 0) slots[tid >> 6] = v;
         __syncthreads();
         v = slots[0];
 #pragma unroll
-        for (int w = 1; w < THREADS / 64; ++w) v = better(v, slots[w]);
+        for (int w = 1; w < THREADS / 64; ++w) v = fmaxf(v, slots[w]);
     }
     return v;
 }
-template <int THREADS> __device__ __forceinline__ float block_sum(float v, float *slots, int tid) {
+// sum and lowest index together: one exchange
+template <int THREADS> __device__ __forceinline__ void block_sum_index(float &v, int &index, float *slots, int *index_slots, int tid) {
 #pragma unroll
-    for (int d = 1; d < 64; d <<= 1) v += __shfl_xor(v, d);
+    for (int d = 1; d < 64; d <<= 1) {
+        v += __shfl_xor(v, d);
+        index = min(index, __shfl_xor(index, d));
+    }
     if constexpr (THREADS > 64) {
-        if ((tid & 63) == 0) slots[tid >> 6] = v;
+        if ((tid & 63) == 0) {
+            slots[tid >> 6] = v;
+            index_slots[tid >> 6] = index;
+        }
         __syncthreads();
         v = 0.0f;
+        index = INT_MAX;
 #pragma unroll
-        for (int w = 0; w < THREADS / 64; ++w) v += slots[w];
+        for (int w = 0; w < THREADS / 64; ++w) {
+            v += slots[w];
+            index = min(index, index_slots[w]);
+        }
     }
-    return v;
 }
 
-// values of chunks tid, tid + THREADS, ... of V actions each from action `first` on, at most N chunks; dead places are -inf
-// and their index INT_MAX
+// Values of chunks tid, tid + THREADS, ... of V actions each from action `first` on, at most N chunks; dead places are -inf.
+// Returns the thread's maximum.  The logits are requested first and arrive while the history is counted.  One uniform branch
+// per control around all of a thread's values; every operation rounds once, as the header writes it.  Selections are bit
+// operations on masks: a comparison into a scalar register and a v_cndmask from it cost five times as much here.
 template <int TYPE, int THREADS, int N, int V>
-__device__ __forceinline__ Best load_values(float (&x)[N][V], const LogitsArgs &a, int r, int first, int n, const unsigned *count, int tid) {
+__device__ __forceinline__ float load_values(float (&x)[N][V], const LogitsArgs &a, int r, int first, int n, unsigned *count_words, int tid) {
     typedef typename LogitElem<TYPE>::raw raw;
     const raw *row = reinterpret_cast<const raw *>(a.logits) + r * a.ls + first;
-    const RowParams p = row_params(a, r);
-    Best best = {-__builtin_inff(), INT_MAX};
 #pragma unroll
     for (int k = 0; k < N; ++k) {
         const int at = (k * THREADS + tid) * V;
         if (at < n) load_logits<TYPE, V>(x[k], row + at);
+        else
+#pragma unroll
+            for (int e = 0; e < V; ++e) x[k][e] = -__builtin_inff();
     }
+    if (a.history != nullptr) {
+        const Counts count = {count_words, a.cols < 65536};
+        count_history<THREADS>(count, a, r, first, n, tid);
+        const RowParams p = row_params(a, r);
 #pragma unroll
-    for (int k = 0; k < N; ++k) {
-        const int at = (k * THREADS + tid) * V;
+        for (int k = 0; k < N; ++k) {
+            const int at = (k * THREADS + tid) * V;
+            if (at >= n) continue;
+            unsigned c[V], some = 0;
 #pragma unroll
-        for (int e = 0; e < V; ++e) {
-            if (at >= n) {
-                x[k][e] = -__builtin_inff();
-                continue;
-            }
-            x[k][e] = process(a, p, r, first + at + e, x[k][e], count != nullptr ? count[at + e] : 0u);
-            if (x[k][e] > best.value) best = Best{x[k][e], first + at + e};
+            for (int e = 0; e < V; ++e) some |= c[e] = count.at(at + e);
+            if (some == 0) continue;
+#pragma unroll
+            for (int e = 0; e < V; ++e)
+                if (c[e] != 0) x[k][e] = penalised(p, x[k][e], c[e]);
         }
     }
-    return best;
+    if (a.bias != nullptr) {
+        const float *b = a.bias + r * a.bias_s + first;
+#pragma unroll
+        for (int k = 0; k < N; ++k) {
+            const int at = (k * THREADS + tid) * V;
+            if (at >= n) continue;
+#pragma unroll
+            for (int e = 0; e < V; ++e) x[k][e] = __fadd_rn(x[k][e], b[at + e]);
+        }
+    }
+    if (a.temperature != 1.0f) {
+        // x / t, correctly rounded: with y the rounded reciprocal, q = x y is within an ulp, x - q t is exact, and one more
+        // multiply-add rounds correctly (Markstein) while nothing over- or underflows.  A thread with a value outside 1e-15 ..
+        // 1e15 (dead places apart), and every temperature outside that or with a significand of ones, divides.
+        float small = 1.0f, large = 1.0f;
+#pragma unroll
+        for (int k = 0; k < N; ++k) {
+            if ((k * THREADS + tid) * V >= n) continue;
+#pragma unroll
+            for (int e = 0; e < V; ++e) {
+                small = fminf(small, fabsf(x[k][e]));
+                large = fmaxf(large, fabsf(x[k][e]));
+            }
+        }
+        if (a.inv_temperature != 0.0f && small > 1.0e-15f && large < 1.0e15f) {
+#pragma unroll
+            for (int k = 0; k < N; ++k) {
+                if ((k * THREADS + tid) * V >= n) continue;
+#pragma unroll
+                for (int e = 0; e < V; ++e) {
+                    const float q = x[k][e] * a.inv_temperature;
+                    x[k][e] = fmaf(fmaf(-q, a.temperature, x[k][e]), a.inv_temperature, q);
+                }
+            }
+        } else {
+#pragma unroll
+            for (int k = 0; k < N; ++k)
+#pragma unroll
+                for (int e = 0; e < V; ++e) x[k][e] = __fdiv_rn(x[k][e], a.temperature);
+        }
+    }
+    if (a.blocked != nullptr) {
+        const unsigned *bits = a.blocked + r * a.bs;
+#pragma unroll
+        for (int k = 0; k < N; ++k) {
+            const int at = (k * THREADS + tid) * V;
+            if (at >= n) continue;
+            // V actions share a word where V divides the period (they start at a multiple of V)
+            const unsigned bit = bit_of(a, (unsigned)(first + at));
+            unsigned word = (int)(bit >> 5) < a.halves ? bits[bit >> 5] >> (bit & 31) : 0u;
+#pragma unroll
+            for (int e = 0; e < V; ++e) {
+                if (V > 1 && !a.bits_together && e > 0) {
+                    const unsigned one = bit_of(a, (unsigned)(first + at + e));
+                    word = ((int)(one >> 5) < a.halves ? bits[one >> 5] >> (one & 31) : 0u) << e;
+                }
+                const unsigned mask = (unsigned)((int)(word << (31 - e)) >> 31);
+                x[k][e] = __uint_as_float((__float_as_uint(x[k][e]) & ~mask) | (0xff800000u & mask));
+            }
+        }
+    }
+    float top = -__builtin_inff();
+#pragma unroll
+    for (int k = 0; k < N; ++k)
+#pragma unroll
+        for (int e = 0; e < V; ++e) top = fmaxf(top, x[k][e]);
+    return top;
+}
+// the lowest index of the maximum among a thread's values
+template <int THREADS, int N, int V> __device__ __forceinline__ int lowest_index(const float (&x)[N][V], float top, int first, int tid) {
+    int index = INT_MAX;
+#pragma unroll
+    for (int k = N - 1; k >= 0; --k)
+#pragma unroll
+        for (int e = V - 1; e >= 0; --e)
+            if (x[k][e] == top) index = first + (k * THREADS + tid) * V + e;
+    return index;
 }
 template <int THREADS, int N, int V>
 __device__ __forceinline__ void store_values(const float (&x)[N][V], float lse, float *row, int n, int tid) {
+    const bool finite = lse - lse == 0.0f;
 #pragma unroll
     for (int k = 0; k < N; ++k) {
         const int at = (k * THREADS + tid) * V;
         if (at >= n) continue;
         float y[V];
 #pragma unroll
-        for (int e = 0; e < V; ++e) y[e] = x[k][e] == -__builtin_inff() ? x[k][e] : x[k][e] - lse;
-        if constexpr (V == 4) *reinterpret_cast<float4 *>(row + at) = float4{y[0], y[1], y[2], y[3]};
-        else row[at] = y[0];
+        for (int e = 0; e < V; ++e) {
+            y[e] = x[k][e] - lse;
+            if (!finite && x[k][e] == -__builtin_inff()) y[e] = x[k][e];      // (a row of NaN: what is blocked stays -inf)
+        }
+        struct alignas(4 * V) Pack { float e[V]; };
+        Pack w;
+#pragma unroll
+        for (int e = 0; e < V; ++e) w.e[e] = y[e];
+        *reinterpret_cast<Pack *>(row + at) = w;
     }
 }
 
 // one workgroup per row, the row in registers
 template <int TYPE, int THREADS, int N, int V> __global__ __launch_bounds__(THREADS) void logits_row_kernel(LogitsArgs a) {
-    extern __shared__ unsigned count[];
-    __shared__ Best best_slots[THREADS / 64];
-    __shared__ float sum_slots[THREADS / 64];
+    extern __shared__ unsigned count_words[];
+    __shared__ float max_slots[THREADS / 64], sum_slots[THREADS / 64];
+    __shared__ int index_slots[THREADS / 64];
     const int r = blockIdx.x, tid = threadIdx.x;
-    if (a.history != nullptr) count_history<THREADS>(count, a, r, 0, a.A, tid);
     float x[N][V];
-    Best best = load_values<TYPE, THREADS, N, V>(x, a, r, 0, a.A, a.history != nullptr ? count : nullptr, tid);
-    best = block_best<THREADS>(best, best_slots, tid);
-    const float shift = best.value == -__builtin_inff() ? 0.0f : best.value;
+    const float own = load_values<TYPE, THREADS, N, V>(x, a, r, 0, a.A, count_words, tid);
+    const float top = block_max<THREADS>(own, max_slots, tid), shift = top == -__builtin_inff() ? 0.0f : top;
+    int index = INT_MAX;
+    if (own == top && top != -__builtin_inff()) index = lowest_index<THREADS, N, V>(x, top, 0, tid);
     float sum = 0.0f;
 #pragma unroll
     for (int k = 0; k < N; ++k)
 #pragma unroll
         for (int e = 0; e < V; ++e) sum += shifted_exp(x[k][e], shift);
-    sum = block_sum<THREADS>(sum, sum_slots, tid);
-    if (a.selected != nullptr && tid == 0) a.selected[r] = best.index == INT_MAX ? -1 : best.index;
-    if (a.out != nullptr) store_values<THREADS, N, V>(x, shift + logf(sum), a.out + r * a.os, a.A, tid);
+    block_sum_index<THREADS>(sum, index, sum_slots, index_slots, tid);
+    if (a.selected != nullptr && tid == 0) a.selected[r] = index == INT_MAX ? -1 : index;
+    if (a.out != nullptr) store_values<THREADS, N, V>(x, top == -__builtin_inff() ? 0.0f : shift + logf(sum), a.out + r * a.os, a.A, tid);
 }
 
-// long rows: one workgroup per tile; `write` = second launch
+// long rows: one workgroup per tile; WRITE = second launch
 template <int TYPE, int V, bool WRITE> __global__ __launch_bounds__(LOGITS_TILE_THREADS) void logits_tile_kernel(LogitsArgs a) {
     constexpr int THREADS = LOGITS_TILE_THREADS, N = LOGITS_TILE / THREADS / V;
-    extern __shared__ unsigned count[];
-    __shared__ Best best_slots[THREADS / 64];
-    __shared__ float sum_slots[THREADS / 64];
+    extern __shared__ unsigned count_words[];
+    __shared__ float max_slots[THREADS / 64], sum_slots[THREADS / 64];
+    __shared__ int index_slots[THREADS / 64];
     const int r = blockIdx.x / a.tiles, t = blockIdx.x % a.tiles, tid = threadIdx.x;
     const int first = t * LOGITS_TILE, n = min(LOGITS_TILE, a.A - first);
-    float lse = 0.0f;
+    float x[N][V];
     if constexpr (WRITE) {
         // the row's maximum and sum from its tiles', in a fixed order
         const float *p = a.part + (int64_t)r * a.tiles * 4;
-        Best best = {-__builtin_inff(), INT_MAX};
-        for (int i = tid; i < a.tiles; i += THREADS) best = better(best, Best{p[4 * i], __float_as_int(p[4 * i + 2])});
-        best = block_best<THREADS>(best, best_slots, tid);
-        const float shift = best.value == -__builtin_inff() ? 0.0f : best.value;
+        float top = -__builtin_inff();
+        for (int i = tid; i < a.tiles; i += THREADS) top = fmaxf(top, p[4 * i]);
+        top = block_max<THREADS>(top, max_slots, tid);
+        const float shift = top == -__builtin_inff() ? 0.0f : top;
         float sum = 0.0f;
-        for (int i = tid; i < a.tiles; i += THREADS) sum = fmaf(p[4 * i + 1], shifted_exp(p[4 * i] == -__builtin_inff() ? shift : p[4 * i], shift), sum);
-        sum = block_sum<THREADS>(sum, sum_slots, tid);
-        lse = shift + logf(sum);
-        if (a.selected != nullptr && t == 0 && tid == 0) a.selected[r] = best.index == INT_MAX ? -1 : best.index;
+        int index = INT_MAX;
+        for (int i = tid; i < a.tiles; i += THREADS) {
+            const float m = p[4 * i];
+            sum = fmaf(p[4 * i + 1], m == -__builtin_inff() ? 1.0f : shifted_exp(m, shift), sum);
+            if (m == top) index = min(index, __float_as_int(p[4 * i + 2]));
+        }
+        block_sum_index<THREADS>(sum, index, sum_slots, index_slots, tid);
+        const float lse = top == -__builtin_inff() ? 0.0f : shift + logf(sum);
+        if (a.selected != nullptr && t == 0 && tid == 0) a.selected[r] = index == INT_MAX ? -1 : index;
         if (a.out == nullptr) return;
-    }
-    if (a.history != nullptr) count_history<THREADS>(count, a, r, first, n, tid);
-    float x[N][V];
-    Best best = load_values<TYPE, THREADS, N, V>(x, a, r, first, n, a.history != nullptr ? count : nullptr, tid);
-    if constexpr (WRITE) {
+        load_values<TYPE, THREADS, N, V>(x, a, r, first, n, count_words, tid);
         store_values<THREADS, N, V>(x, lse, a.out + r * a.os + first, n, tid);
     } else {
-        best = block_best<THREADS>(best, best_slots, tid);
-        const float shift = best.value == -__builtin_inff() ? 0.0f : best.value;
+        const float own = load_values<TYPE, THREADS, N, V>(x, a, r, first, n, count_words, tid);
+        const float top = block_max<THREADS>(own, max_slots, tid), shift = top == -__builtin_inff() ? 0.0f : top;
+        int index = INT_MAX;
+        if (own == top && top != -__builtin_inff()) index = lowest_index<THREADS, N, V>(x, top, first, tid);
         float sum = 0.0f;
 #pragma unroll
         for (int k = 0; k < N; ++k)
 #pragma unroll
             for (int e = 0; e < V; ++e) sum += shifted_exp(x[k][e], shift);
-        sum = block_sum<THREADS>(sum, sum_slots, tid);
+        block_sum_index<THREADS>(sum, index, sum_slots, index_slots, tid);
         if (tid == 0) {
             float *p = a.part + ((int64_t)r * a.tiles + t) * 4;
-            p[0] = best.value;
+            p[0] = top;
             p[1] = sum;
-            p[2] = __int_as_float(best.index);
+            p[2] = __int_as_float(index);
         }
     }
 }
@@ -261,24 +364,26 @@ int check_logits(const dgl_logits_t *p) {
     DGL_CHECK_ARG(p->history == nullptr || p->repetition != nullptr || p->repetition_all > 0.0f, "repetition %g", (double)p->repetition_all);
     return DGL_OK;
 }
-#define LOGITS_ROW_MAX 32768           // 1024 threads x 32 values
+#define LOGITS_ROW_MAX 24576           // 512 threads x 48 values
 bool in_tiles(const dgl_logits_t *p) { return p->A > LOGITS_ROW_MAX; }
 
+int count_bytes(const LogitsArgs &a, int n) { return a.history == nullptr ? 0 : a.cols < 65536 ? (n + 1) / 2 * 4 : n * 4; }
 template <int TYPE, int THREADS, int N, int V> void launch_row(const LogitsArgs &a, hipStream_t s) {
-    const int lds = a.history != nullptr ? a.A * 4 : 0;
+    const int lds = count_bytes(a, a.A);
     if (lds > 48 * 1024) dgl_max_dynamic_lds(reinterpret_cast<const void *>(&logits_row_kernel<TYPE, THREADS, N, V>), LOGITS_ROW_MAX * 4);
     hipLaunchKernelGGL((logits_row_kernel<TYPE, THREADS, N, V>), dim3(a.R), dim3(THREADS), lds, s, a);
 }
-// The smallest workgroup that holds a row at 4 to 32 values a thread (V = 1: rows that 16-byte accesses cannot take)
+// The smallest workgroup that holds a row at 4 to 48 values a thread; several share a compute unit, so that one row's loads
+// run beside another's reductions and stores
 template <int TYPE, int V> int launch_logits(const LogitsArgs &a, hipStream_t s) {
     if (a.A <= 256) launch_row<TYPE, 64, 4 / V, V>(a, s);
     else if (a.A <= 1024) launch_row<TYPE, 256, 4 / V, V>(a, s);
     else if (a.A <= 4096) launch_row<TYPE, 256, 16 / V, V>(a, s);
-    else if (a.A <= 8192) launch_row<TYPE, 1024, 8 / V, V>(a, s);
-    else if (a.A <= 16384) launch_row<TYPE, 1024, 16 / V, V>(a, s);
-    else if (a.A <= LOGITS_ROW_MAX) launch_row<TYPE, 1024, 32 / V, V>(a, s);
+    else if (a.A <= 8192) launch_row<TYPE, 512, 16 / V, V>(a, s);
+    else if (a.A <= 16384) launch_row<TYPE, 512, 32 / V, V>(a, s);
+    else if (a.A <= LOGITS_ROW_MAX) launch_row<TYPE, 512, 48 / V, V>(a, s);
     else {
-        const int lds = a.history != nullptr ? LOGITS_TILE * 4 : 0;
+        const int lds = count_bytes(a, LOGITS_TILE);
         const dim3 grid((unsigned)((int64_t)a.R * a.tiles));
         hipLaunchKernelGGL((logits_tile_kernel<TYPE, V, false>), grid, dim3(LOGITS_TILE_THREADS), lds, s, a);
         DGL_CHECK_LAUNCH("dgl_logits_process (statistics)");
@@ -309,11 +414,22 @@ extern "C" int dgl_logits_process(const dgl_logits_t *p, float *ws, dgl_stream_t
     a.tiles = (p->A + LOGITS_TILE - 1) / LOGITS_TILE; a.part = ws;
     DGL_CHECK_ARG(!in_tiles(p) || ws != nullptr, "a workspace is needed");
     DGL_CHECK_ARG((int64_t)a.R * a.tiles < (1ll << 31), "too many rows");
+    // penalties that change nothing need no counts
+    if (a.rep == nullptr && a.pres == nullptr && a.freq == nullptr && a.rep_all == 1.0f && a.pres_all == 0.0f && a.freq_all == 0.0f) a.history = nullptr;
+    const bool all_ones = (__builtin_bit_cast(unsigned, a.temperature) & 0x7fffffu) == 0x7fffffu;
+    a.inv_temperature = all_ones || a.temperature < 1.0e-15f || a.temperature > 1.0e15f ? 0.0f : 1.0f / a.temperature;
+    // the widest access that every row of the logits and of the result can take
     const int bytes = p->dtype == DGL_DTYPE_F32 ? 4 : 2;
-    const bool four = p->A % 4 == 0 && p->logits_stride % 4 == 0 && p->out_stride % 4 == 0 &&
-                      (reinterpret_cast<uintptr_t>(p->logits) & (4 * bytes - 1)) == 0 && (reinterpret_cast<uintptr_t>(p->log_probs) & 15) == 0;
+    auto fits = [&](int v) {
+        return p->A % v == 0 && p->logits_stride % v == 0 && p->out_stride % v == 0 &&
+               (reinterpret_cast<uintptr_t>(p->logits) & (v * bytes - 1)) == 0 && (reinterpret_cast<uintptr_t>(p->log_probs) & (4 * v - 1)) == 0;
+    };
+    const int v = fits(4) ? 4 : fits(2) ? 2 : 1;
+    a.bits_together = a.period % v == 0;
     hipStream_t s = (hipStream_t)stream;
-    if (p->dtype == DGL_DTYPE_F32) return four ? launch_logits<0, 4>(a, s) : launch_logits<0, 1>(a, s);
-    if (p->dtype == DGL_DTYPE_F16) return four ? launch_logits<1, 4>(a, s) : launch_logits<1, 1>(a, s);
-    return four ? launch_logits<2, 4>(a, s) : launch_logits<2, 1>(a, s);
+#define LOGITS_CASE(T) \
+    if (p->dtype == T) return v == 4 ? launch_logits<T, 4>(a, s) : v == 2 ? launch_logits<T, 2>(a, s) : launch_logits<T, 1>(a, s);
+    LOGITS_CASE(0) LOGITS_CASE(1) LOGITS_CASE(2)
+#undef LOGITS_CASE
+    return dgl_set_error(DGL_ERR_INVALID_ARGUMENT, "unknown element type %d", p->dtype);
 }

@@ -98,6 +98,22 @@ def test_penalties(device, A):
     check(x, history=hist[:, :0])
 
 
+@pytest.mark.parametrize("temperature", [0.7, 1.0 / 3.0, 1.9999998807907104, 1e-3, 37.5, 1e35])
+def test_temperature_divides_exactly(device, temperature):
+    """Equal quotients tie, so a pick depends on the division's last bit: 200 000 values in 100 rows of near-ties."""
+    g = torch.Generator(device=device).manual_seed(6)
+    x = 1.0 + torch.randint(0, 8, (100, 2000), device=device, generator=g) * 2.0 ** -23
+    x = x * torch.exp2(torch.randint(-60, 60, (100, 1), device=device, generator=g).float())
+    check(x, temperature=temperature)
+
+
+def test_many_repeats_count_in_full(device):
+    """Histories of 65536 entries and more count in 32 bits."""
+    x, g = rnd(2, 300, torch.float32, 8)
+    for n in (65535, 65536, 70000):
+        check(x, history=torch.full((2, n), 17, device=device, dtype=torch.int32), frequency=1e-4)
+
+
 def test_equal_logits_go_to_the_lowest_action(device):
     for A in (7, 1000, 5000, 50000):
         x = torch.zeros(3, A, device=device)
