@@ -158,19 +158,24 @@ template <int TYPE> __device__ __forceinline__ void store_wide(typename Elem<TYP
     else if constexpr (TYPE == ATTN_F16) o[d] = __builtin_bit_cast(unsigned short, (_Float16)x);
     else o[d] = __builtin_bit_cast(unsigned short, (__bf16)x);
 }
-template <int TYPE>
-__device__ void careful_forward_row(const AttnArgs &a, const ScoreParams &sp, int b, int h, int i, float m, float l) {
+template <int TYPE> __device__ void careful_forward_row(const AttnArgs &a, const ScoreParams &sp, int b, int h, int i) {
     typedef typename Elem<TYPE>::raw raw;
     const int lane = threadIdx.x & 63, hk = h / a.G, limit = row_limit(a, b, i);
     const raw *q = reinterpret_cast<const raw *>(a.q) + b * a.qs[0] + h * a.qs[1] + i * a.qs[2];
     const raw *k = reinterpret_cast<const raw *>(a.k) + b * a.ks[0] + hk * a.ks[1];
     const raw *v = reinterpret_cast<const raw *>(a.v) + b * a.vs[0] + hk * a.vs[1];
-    float acc0 = 0.0f, acc1 = 0.0f;
+    float m = -attn_inf(), l = 0.0f, acc0 = 0.0f, acc1 = 0.0f, th;
+    for (int j = lane; j < limit; j += 64)
+        if (pair_allowed(a, b, i, j, limit)) m = fmaxf(m, pair_score<TYPE>(a, sp, b, i, j, q, k + j * a.ks[2], th));
+#pragma unroll
+    for (int x = 1; x < 64; x <<= 1) m = fmaxf(m, __shfl_xor(m, x));
+    if (m == -attn_inf()) m = 0.0f;
     for (int base = 0; base < limit; base += 64) {
         const int j = base + lane;
         const bool ok = pair_allowed(a, b, i, j, limit);
-        float p = 0.0f, th;
+        float p = 0.0f;
         if (ok) p = __builtin_amdgcn_exp2f(pair_score<TYPE>(a, sp, b, i, j, q, k + j * a.ks[2], th) - m);
+        l += p;
         for (unsigned long long w = __ballot(ok); w != 0; w &= w - 1) {
             const int jj = __ffsll((long long)w) - 1;
             const float pj = __shfl(p, jj);
@@ -179,24 +184,27 @@ __device__ void careful_forward_row(const AttnArgs &a, const ScoreParams &sp, in
             if (lane + 64 < a.D) acc1 = fmaf(pj, elem_to_float<TYPE>(vr[lane + 64]), acc1);
         }
     }
+#pragma unroll
+    for (int x = 1; x < 64; x <<= 1) l += __shfl_xor(l, x);
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
     raw *o = reinterpret_cast<raw *>(a.out) + b * a.os[0] + h * a.os[1] + i * a.os[2];
     if (lane < a.D) store_wide<TYPE>(o, lane, acc0 * inv);
     if (lane + 64 < a.D) store_wide<TYPE>(o, lane + 64, acc1 * inv);
+    if (a.lse != nullptr && lane == 0)
+        a.lse[((int64_t)b * a.Hq + h) * a.Lq + i] = l == 0.0f ? -attn_inf() : (m + __builtin_amdgcn_logf(l)) * ATTN_LN2;
 }
 
 template <int TYPE, int DP, int NQ>
 __global__ __launch_bounds__(ATTN_THREADS, TYPE == ATTN_F32 && DP == 128 ? 1 : 2) void attn_fwd_kernel(AttnArgs a) {
     typedef Shape<TYPE, DP> S;
     typedef typename Elem<TYPE>::raw raw;
-    // KB: blocks of 16 keys whose scores are held at once (two for wide heads: 256 registers at two waves per SIMD)
-    constexpr int ROWS = 64 * NQ, UNITS = (2 * S::units + ATTN_THREADS - 1) / ATTN_THREADS, KB = DP == 128 ? 2 : 4;
-    __shared__ __align__(16) char lds[S::row_bytes + (S::wide ? S::row_bytes : S::t_bytes)];
+    // KB: blocks of 16 keys whose scores are held at once.  Two where that fits another wave on a SIMD: heads of 128 (256
+    // registers for two waves) and binary32 heads of 16 (168 for three: nodes of 1000, 551 -> 475 us)
+    constexpr int ROWS = 64 * NQ, KB = DP == 128 || (TYPE == ATTN_F32 && DP <= 32) ? 2 : 4;
+    __shared__ __align__(16) char Kt[S::bytes], Vt[S::bytes];
     __shared__ __align__(16) float key_pos[2 * ATTN_ROWS];
     __shared__ __align__(16) int key_doc[ATTN_ROWS];
     __shared__ TileMap map_store;
-    raw *Kt = reinterpret_cast<raw *>(lds), *Vt = reinterpret_cast<raw *>(lds + S::row_bytes);
-
     int work = xcd_work();
     if (work >= a.B * a.Hq * a.tiles * a.splits) return;
     const int split = work % a.splits;
@@ -216,9 +224,8 @@ __global__ __launch_bounds__(ATTN_THREADS, TYPE == ATTN_F32 && DP == 128 ? 1 : 2
         map = &map_store;
         build_tile_map(map_store, a.doc_q + b * a.dqs, row0, ROWS, a.Lq, docs, a.Lk);
     }
-    zero_padding<TYPE, DP>(Kt);
-
-    Frag<TYPE, DP> qf[NQ];
+    
+    ColFrag<TYPE, DP> qf[NQ];
     f32x4 o[NQ][S::dt];
     float m[NQ], l[NQ], qx[NQ], qy[NQ];
     int limit[NQ], doc[NQ];
@@ -226,7 +233,10 @@ __global__ __launch_bounds__(ATTN_THREADS, TYPE == ATTN_F32 && DP == 128 ? 1 : 2
 #pragma unroll
     for (int n = 0; n < NQ; ++n) {
         const int i = wrow0 + 16 * n + c;
-        frag_from_global<TYPE, DP>(qf[n], q + (int64_t)i * a.qs[2], i < a.Lq, a.D, g);
+        Eight<TYPE> q8[S::chunks];
+#pragma unroll
+        for (int k8 = 0; k8 < S::chunks; ++k8) q8[k8] = load_eight<TYPE>(q + (int64_t)i * a.qs[2], frag_d<DP>(k8, g), i < a.Lq && frag_d<DP>(k8, g) < a.D);
+        col_frag<TYPE, DP>(qf[n], q8, g);
         m[n] = -attn_inf();
         l[n] = 0.0f;
         limit[n] = row_limit(a, b, i);
@@ -247,26 +257,14 @@ __global__ __launch_bounds__(ATTN_THREADS, TYPE == ATTN_F32 && DP == 128 ? 1 : 2
     const int tiles = (row_limit(a, b, min(row0 + ROWS, a.Lq) - 1) + ATTN_ROWS - 1) / ATTN_ROWS;
     const int per = (tiles + a.splits - 1) / a.splits, end = min(tiles, (split + 1) * per);
 
-    UnitPlan plan[UNITS];
-#pragma unroll
-    for (int x = 0; x < UNITS; ++x) {
-        const int u = tid + x * ATTN_THREADS;
-        plan[x] = u < S::units ? unit_plan<TYPE, DP>(u, a.ks[2], a.D) : unit_plan<TYPE, DP>(u - S::units, a.vs[2], a.D);
-    }
-    Unit un[UNITS];
-    UnitIds ids[UNITS];
+    Stager<TYPE, DP> stage;
+    stage.init(a.ks[2], a.vs[2], a.D);
     float stage_pos = 0.0f;
     int stage_doc = -1;
     auto load = [&](int tile) {
         const int base = tile * ATTN_ROWS, left = a.Lk - base;
         const char *kt = k + base * a.ks[2] * Elem<TYPE>::bytes, *vt = v + base * a.vs[2] * Elem<TYPE>::bytes;
-#pragma unroll
-        for (int x = 0; x < UNITS; ++x) {
-            const int u = tid + x * ATTN_THREADS;
-            if (u < S::units) unit_load(un[x], plan[x], kt, left);
-            else if (u < 2 * S::units) unit_load(un[x], plan[x], vt, left);
-            if (map != nullptr && u < 2 * S::units) unit_load_ids(ids[x], plan[x], docs + base, left);
-        }
+        stage.load(kt, vt, left, map != nullptr ? docs + base : nullptr);
         if (a.bias == 2 && tid < 2 * ATTN_ROWS) stage_pos = tid < 2 * left ? a.pos_k[b * a.pks + 2 * (int64_t)base + tid] : 0.0f;
         if (map != nullptr && tid < ATTN_ROWS) stage_doc = doc_of_key(a, b, base + tid);
     };
@@ -274,13 +272,7 @@ __global__ __launch_bounds__(ATTN_THREADS, TYPE == ATTN_F32 && DP == 128 ? 1 : 2
     if (tile < end) load(tile);
     while (tile < end) {
         __syncthreads();
-#pragma unroll
-        for (int x = 0; x < UNITS; ++x) {
-            const int u = tid + x * ATTN_THREADS;
-            if (map != nullptr && u < 2 * S::units) unit_skip(un[x], ids[x]);
-            if (u < S::units) unit_write<TYPE, DP, true, false>(un[x], u, Kt, nullptr);
-            else if (u < 2 * S::units) unit_write<TYPE, DP, false, true>(un[x], u - S::units, Vt, Vt);
-        }
+        stage.write(Kt, Vt, map != nullptr);
         if (a.bias == 2 && tid < 2 * ATTN_ROWS) key_pos[tid] = stage_pos;
         if (map != nullptr && tid < ATTN_ROWS) key_doc[tid] = stage_doc;
         const int here = tile, base = here * ATTN_ROWS;
@@ -295,8 +287,8 @@ __global__ __launch_bounds__(ATTN_THREADS, TYPE == ATTN_F32 && DP == 128 ? 1 : 2
             f32x4 s[KB][NQ];
 #pragma unroll
             for (int t = 0; t < KB; ++t) {
-                Frag<TYPE, DP> kf;
-                frag_from_lds<TYPE, DP>(kf, Kt, 16 * (kb + t) + c, g);
+                RowFrag<TYPE, DP> kf;
+                row_frag<TYPE, DP>(kf, Kt, 16 * (kb + t) + c, g);
 #pragma unroll
                 for (int n = 0; n < NQ; ++n) s[t][n] = dot_block<TYPE, DP>(kf, qf[n]);
             }
@@ -350,7 +342,7 @@ __global__ __launch_bounds__(ATTN_THREADS, TYPE == ATTN_F32 && DP == 128 ? 1 : 2
 #pragma unroll
                     for (int t = 0; t < KB; ++t)
 #pragma unroll
-                        for (int r = 0; r < 4; ++r) s[t][n][r] = 16 * t + r < left ? s[t][n][r] : -attn_inf();
+                        for (int r = 0; r < 4; ++r) s[t][n][r] = keep_or(mask_below(16 * t + r, left), s[t][n][r], -attn_inf());
                 }
             }
             if (by_doc) {
@@ -360,7 +352,7 @@ __global__ __launch_bounds__(ATTN_THREADS, TYPE == ATTN_F32 && DP == 128 ? 1 : 2
 #pragma unroll
                     for (int n = 0; n < NQ; ++n)
 #pragma unroll
-                        for (int r = 0; r < 4; ++r) s[t][n][r] = kd[r] == doc[n] ? s[t][n][r] : -attn_inf();
+                        for (int r = 0; r < 4; ++r) s[t][n][r] = keep_or(mask_equal(kd[r], doc[n]), s[t][n][r], -attn_inf());
                 }
             }
 #pragma unroll
@@ -389,7 +381,7 @@ __global__ __launch_bounds__(ATTN_THREADS, TYPE == ATTN_F32 && DP == 128 ? 1 : 2
                     }
             }
 #pragma unroll
-            for (int t = 0; t < KB; t += 2) accumulate<TYPE, DP, NQ>(o, Vt, Vt, (kb + t) / 2, s[t], s[t + 1], g, c);
+            for (int t = 0; t < KB; t += 2) accumulate<TYPE, DP, NQ>(o, Vt, (kb + t) / 2, s[t], s[t + 1], g, c);
         }
     }
 
@@ -423,8 +415,7 @@ __global__ __launch_bounds__(ATTN_THREADS, TYPE == ATTN_F32 && DP == 128 ? 1 : 2
         unsigned long long bad = __ballot(!fine && i < a.Lq);
         bad = (bad | bad >> 16 | bad >> 32 | bad >> 48) & 0xffff;
         for (; bad != 0; bad &= bad - 1) {
-            const int cc = __ffsll((long long)bad) - 1;
-            careful_forward_row<TYPE>(a, sp, b, h, wrow0 + 16 * n + cc, __shfl(shift, cc), __shfl(total, cc));
+            careful_forward_row<TYPE>(a, sp, b, h, wrow0 + 16 * n + __ffsll((long long)bad) - 1);
         }
     }
 }
@@ -456,7 +447,7 @@ template <int TYPE> __global__ __launch_bounds__(ATTN_THREADS) void attn_fwd_joi
     if (lane + 64 < a.D) store_wide<TYPE>(o, lane + 64, acc1 * inv);
     if (a.lse != nullptr && lane == 0) a.lse[row] = total == 0.0f ? -attn_inf() : (shift + __builtin_amdgcn_logf(total)) * ATTN_LN2;
     if (__any((acc0 + acc1) * 0.0f != 0.0f))
-        careful_forward_row<TYPE>(a, score_params(a.scale, a.cap, a.bias, a.slope, h), b, h, i, shift, total);
+        careful_forward_row<TYPE>(a, score_params(a.scale, a.cap, a.bias, a.slope, h), b, h, i);
 }
 
 // ---------------------------------------------------------------------------------------------------------- backward
@@ -465,8 +456,9 @@ template <int TYPE> __global__ __launch_bounds__(ATTN_THREADS) void attn_fwd_joi
 //   in   s = q.k,  dp = do.v - delta (the subtraction is the matrix instruction's initial accumulator), e = lse in units of
 //        log2 (infinite for rows without a key), dist
 //   out  s = p,  dp = ds = p (dp - delta)
-// slack is 1 - tanh^2 = 4 (r - r^2) without its 4 (undo_factor), and undefined without a cap.
-template <int N>
+// slack is 1 - tanh^2 = 4 (r - r^2) without its 4 (undo_factor).  FOLD: it goes into dp (which then ends as du); else it is
+// returned, undefined without a cap (the slope's gradient needs ds itself).
+template <int N, bool FOLD>
 __device__ __forceinline__ void pair_probability(const ScoreParams &sp, f32x4 (&s)[2][N], f32x4 (&dp)[2][N], f32x4 (&slack)[2][N],
                                                  const f32x4 (&dist)[2][N], const f32x4 (&e)[2][N]) {
     if (sp.cap == CAP_NONE) {
@@ -492,7 +484,8 @@ __device__ __forceinline__ void pair_probability(const ScoreParams &sp, f32x4 (&
                     k[r] = fmaf(-y, y, y);
                 }
                 s[t][n] = x;
-                slack[t][n] = k;
+                if constexpr (FOLD) dp[t][n] = dp[t][n] * k;
+                else slack[t][n] = k;
             }
     } else {
 #pragma unroll
@@ -507,7 +500,8 @@ __device__ __forceinline__ void pair_probability(const ScoreParams &sp, f32x4 (&
                     k[r] = 0.25f * fmaf(-th, th, 1.0f);
                 }
                 s[t][n] = x;
-                slack[t][n] = k;
+                if constexpr (FOLD) dp[t][n] = dp[t][n] * k;
+                else slack[t][n] = k;
             }
     }
     if (sp.bias) {
@@ -581,15 +575,12 @@ template <int TYPE, int DP, int NQ>
 __global__ __launch_bounds__(ATTN_THREADS, DP <= 64 ? 2 : 1) void attn_bwd_q_kernel(AttnArgs a) {
     typedef Shape<TYPE, DP> S;
     typedef typename Elem<TYPE>::raw raw;
-    constexpr int ROWS = 64 * NQ, UNITS = (2 * S::units + ATTN_THREADS - 1) / ATTN_THREADS;
-    __shared__ __align__(16) char lds[2 * S::row_bytes + S::t_bytes];
+    constexpr int ROWS = 64 * NQ, HALVES = DP <= 32 ? 2 : 1;     // (unrolled, the halves of a tile of wide heads spill)
+    __shared__ __align__(16) char Kt[S::bytes], Vt[S::bytes];
     __shared__ __align__(16) float key_pos[2 * ATTN_ROWS];
     __shared__ __align__(16) int key_doc[ATTN_ROWS];
     __shared__ TileMap map_store;
     __shared__ float part[4];
-    raw *Kt = reinterpret_cast<raw *>(lds), *Vt = reinterpret_cast<raw *>(lds + S::row_bytes);
-    raw *KT = reinterpret_cast<raw *>(lds + 2 * S::row_bytes);
-
     const int work = xcd_work();
     if (work >= a.B * a.Hq * a.tiles) return;
     const int bh = work / a.tiles, qt = a.tiles - 1 - work % a.tiles;
@@ -609,10 +600,8 @@ __global__ __launch_bounds__(ATTN_THREADS, DP <= 64 ? 2 : 1) void attn_bwd_q_ker
         map = &map_store;
         build_tile_map(map_store, a.doc_q + b * a.dqs, row0, ROWS, a.Lq, docs, a.Lk);
     }
-    zero_padding<TYPE, DP>(Kt);
-    zero_padding<TYPE, DP>(Vt);
-
-    Frag<TYPE, DP> qf[NQ], of[NQ];
+    
+    ColFrag<TYPE, DP> qf[NQ], of[NQ];
     f32x4 dq[NQ][S::dt];
     float lse2[NQ], delta[NQ], rs[NQ], qx[NQ], qy[NQ], excess[NQ], pd[NQ], dsl[NQ];
     int limit[NQ], doc[NQ];
@@ -621,26 +610,23 @@ __global__ __launch_bounds__(ATTN_THREADS, DP <= 64 ? 2 : 1) void attn_bwd_q_ker
     for (int n = 0; n < NQ; ++n) {
         const int i = wrow0 + 16 * n + c;
         const bool live = i < a.Lq;
-        frag_from_global<TYPE, DP>(qf[n], q + (int64_t)i * a.qs[2], live, a.D, g);
-        frag_from_global<TYPE, DP>(of[n], go + (int64_t)i * a.dos[2], live, a.D, g);
-        Frag<TYPE, DP> ff;
-        frag_from_global<TYPE, DP>(ff, fo + (int64_t)i * a.os[2], live, a.D, g);
+        Eight<TYPE> q8[S::chunks], g8[S::chunks];
         float dot = 0.0f, amax = 0.0f;
 #pragma unroll
-        for (int x = 0; x < S::chunks; ++x)
+        for (int k8 = 0; k8 < S::chunks; ++k8) {
+            const int d = frag_d<DP>(k8, g);
+            q8[k8] = load_eight<TYPE>(q + (int64_t)i * a.qs[2], d, live && d < a.D);
+            g8[k8] = load_eight<TYPE>(go + (int64_t)i * a.dos[2], d, live && d < a.D);
+            const Eight<TYPE> o8 = load_eight<TYPE>(fo + (int64_t)i * a.os[2], d, live && d < a.D && frag_counts<DP>(g));
 #pragma unroll
-            for (int w = 0; w < 4; ++w) {
-                if constexpr (S::wide) {
-                    dot = fmaf(__uint_as_float(of[n].c[x][w]), __uint_as_float(ff.c[x][w]), dot);
-                } else {
-#pragma unroll
-                    for (int half = 0; half < 2; ++half) {
-                        const float e = elem_to_float<TYPE>((unsigned short)(of[n].c[x][w] >> (16 * half)));
-                        dot = fmaf(e, elem_to_float<TYPE>((unsigned short)(ff.c[x][w] >> (16 * half))), dot);
-                        amax = fmaxf(amax, fabsf(e));
-                    }
-                }
+            for (int e = 0; e < 8; ++e) {
+                const float x = eight_at<TYPE>(g8[k8], e);
+                if (frag_counts<DP>(g)) dot = fmaf(x, eight_at<TYPE>(o8, e), dot);
+                amax = fmaxf(amax, fabsf(x));
             }
+        }
+        col_frag<TYPE, DP>(qf[n], q8, g);
+        col_frag<TYPE, DP>(of[n], g8, g);
         delta[n] = group_sum(dot);
         const int64_t at = ((int64_t)b * a.Hq + h) * a.Lq + i;
         const float lse = live ? a.lse[at] : -attn_inf();
@@ -673,26 +659,14 @@ __global__ __launch_bounds__(ATTN_THREADS, DP <= 64 ? 2 : 1) void attn_bwd_q_ker
     const int end = (row_limit(a, b, min(row0 + ROWS, a.Lq) - 1) + ATTN_ROWS - 1) / ATTN_ROWS;
     const bool want_slope = a.dslope_part != nullptr;
 
-    UnitPlan plan[UNITS];
-#pragma unroll
-    for (int x = 0; x < UNITS; ++x) {
-        const int u = tid + x * ATTN_THREADS;
-        plan[x] = u < S::units ? unit_plan<TYPE, DP>(u, a.ks[2], a.D) : unit_plan<TYPE, DP>(u - S::units, a.vs[2], a.D);
-    }
-    Unit un[UNITS];
-    UnitIds ids[UNITS];
+    Stager<TYPE, DP> stage;
+    stage.init(a.ks[2], a.vs[2], a.D);
     float stage_pos = 0.0f;
     int stage_doc = -1;
     auto load = [&](int tile) {
         const int base = tile * ATTN_ROWS, left = a.Lk - base;
         const char *kt = k + base * a.ks[2] * Elem<TYPE>::bytes, *vt = v + base * a.vs[2] * Elem<TYPE>::bytes;
-#pragma unroll
-        for (int x = 0; x < UNITS; ++x) {
-            const int u = tid + x * ATTN_THREADS;
-            if (u < S::units) unit_load(un[x], plan[x], kt, left);
-            else if (u < 2 * S::units) unit_load(un[x], plan[x], vt, left);
-            if (map != nullptr && u < 2 * S::units) unit_load_ids(ids[x], plan[x], docs + base, left);
-        }
+        stage.load(kt, vt, left, map != nullptr ? docs + base : nullptr);
         if (a.bias == 2 && tid < 2 * ATTN_ROWS) stage_pos = tid < 2 * left ? a.pos_k[b * a.pks + 2 * (int64_t)base + tid] : 0.0f;
         if (map != nullptr && tid < ATTN_ROWS) stage_doc = doc_of_key(a, b, base + tid);
     };
@@ -700,13 +674,7 @@ __global__ __launch_bounds__(ATTN_THREADS, DP <= 64 ? 2 : 1) void attn_bwd_q_ker
     if (tile < end) load(tile);
     while (tile < end) {
         __syncthreads();
-#pragma unroll
-        for (int x = 0; x < UNITS; ++x) {
-            const int u = tid + x * ATTN_THREADS;
-            if (map != nullptr && u < 2 * S::units) unit_skip(un[x], ids[x]);
-            if (u < S::units) unit_write<TYPE, DP, true, true>(un[x], u, Kt, KT);
-            else if (u < 2 * S::units) unit_write<TYPE, DP, true, false>(un[x], u - S::units, Vt, nullptr);
-        }
+        stage.write(Kt, Vt, map != nullptr);
         if (a.bias == 2 && tid < 2 * ATTN_ROWS) key_pos[tid] = stage_pos;
         if (map != nullptr && tid < ATTN_ROWS) key_doc[tid] = stage_doc;
         const int here = tile, base = here * ATTN_ROWS;
@@ -716,16 +684,16 @@ __global__ __launch_bounds__(ATTN_THREADS, DP <= 64 ? 2 : 1) void attn_bwd_q_ker
         if (base >= wave_limit) continue;
         const bool by_doc = !tile_same(map, here), masked = by_doc || base + ATTN_ROWS > wave_full;
 
-#pragma unroll
+#pragma unroll HALVES
         for (int tp = 0; tp < 2; ++tp) {
             f32x4 s[2][NQ], dp[2][NQ], slack[2][NQ] = {}, dist[2][NQ] = {};
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
-                Frag<TYPE, DP> f;
-                frag_from_lds<TYPE, DP>(f, Kt, 32 * tp + 16 * t + c, g);
+                RowFrag<TYPE, DP> f;
+                row_frag<TYPE, DP>(f, Kt, 32 * tp + 16 * t + c, g);
 #pragma unroll
                 for (int n = 0; n < NQ; ++n) s[t][n] = dot_block<TYPE, DP>(f, qf[n]);
-                frag_from_lds<TYPE, DP>(f, Vt, 32 * tp + 16 * t + c, g);
+                row_frag<TYPE, DP>(f, Vt, 32 * tp + 16 * t + c, g);
 #pragma unroll
                 for (int n = 0; n < NQ; ++n) dp[t][n] = dot_block<TYPE, DP>(f, of[n], f32x4{-delta[n], -delta[n], -delta[n], -delta[n]});
             }
@@ -755,7 +723,7 @@ __global__ __launch_bounds__(ATTN_THREADS, DP <= 64 ? 2 : 1) void attn_bwd_q_ker
             f32x4 e[2][NQ];
 #pragma unroll
             for (int n = 0; n < NQ; ++n) e[0][n] = e[1][n] = f32x4{lse2[n], lse2[n], lse2[n], lse2[n]};
-            pair_probability<NQ>(sp, s, dp, slack, dist, e);
+            pair_probability<NQ, false>(sp, s, dp, slack, dist, e);
             if (masked) {
 #pragma unroll
                 for (int t = 0; t < 2; ++t) {
@@ -767,10 +735,10 @@ __global__ __launch_bounds__(ATTN_THREADS, DP <= 64 ? 2 : 1) void attn_bwd_q_ker
                         f32x4 p = s[t][n], ds = dp[t][n], away = dist[t][n];
 #pragma unroll
                         for (int r = 0; r < 4; ++r) {
-                            const bool ok = (16 * t + r < left) & (kd[r] == own);
-                            p[r] = ok ? p[r] : 0.0f;
-                            ds[r] = ok ? ds[r] : 0.0f;
-                            away[r] = ok ? away[r] : 0.0f;                   // (a masked key's coordinates may be NaN)
+                            const unsigned ok = mask_below(16 * t + r, left) & mask_equal(kd[r], own);
+                            p[r] = keep_or_zero(ok, p[r]);
+                            ds[r] = keep_or_zero(ok, ds[r]);
+                            away[r] = keep_or_zero(ok, away[r]);             // (a masked key's coordinates may be NaN)
                         }
                         s[t][n] = p;
                         dp[t][n] = ds;
@@ -796,7 +764,7 @@ __global__ __launch_bounds__(ATTN_THREADS, DP <= 64 ? 2 : 1) void attn_bwd_q_ker
 #pragma unroll
                     for (int n = 0; n < NQ; ++n) dp[t][n] = dp[t][n] * slack[t][n];
             }
-            accumulate<TYPE, DP, NQ>(dq, Kt, KT, tp, dp[0], dp[1], g, c);
+            accumulate<TYPE, DP, NQ>(dq, Kt, tp, dp[0], dp[1], g, c);
         }
     }
 
@@ -910,15 +878,12 @@ template <int TYPE, int DP, int NK>
 __global__ __launch_bounds__(ATTN_THREADS, DP <= 64 ? 2 : 1) void attn_bwd_kv_kernel(AttnArgs a) {
     typedef Shape<TYPE, DP> S;
     typedef typename Elem<TYPE>::raw raw;
-    constexpr int ROWS = 64 * NK, UNITS = (2 * S::units + ATTN_THREADS - 1) / ATTN_THREADS;
-    __shared__ __align__(16) char lds[2 * S::row_bytes + 2 * S::t_bytes];
+    constexpr int ROWS = 64 * NK, HALVES = DP <= 32 ? 2 : 1;
+    __shared__ __align__(16) char Qt[S::bytes], Ot[S::bytes];
     __shared__ __align__(16) float row_lse[ATTN_ROWS], row_delta[ATTN_ROWS], row_x[ATTN_ROWS], row_y[ATTN_ROWS];
     __shared__ __align__(16) int row_lim[ATTN_ROWS], row_doc[ATTN_ROWS];
     __shared__ TileMap map_store;
     __shared__ unsigned least_scale;
-    raw *Qt = reinterpret_cast<raw *>(lds), *Ot = reinterpret_cast<raw *>(lds + S::row_bytes);
-    raw *QT = reinterpret_cast<raw *>(lds + 2 * S::row_bytes), *OT = reinterpret_cast<raw *>(lds + 2 * S::row_bytes + S::t_bytes);
-
     const int parts = a.head_parts * a.splits;
     int work = xcd_work();
     if (work >= a.B * a.Hkv * a.tiles * parts) return;
@@ -939,10 +904,8 @@ __global__ __launch_bounds__(ATTN_THREADS, DP <= 64 ? 2 : 1) void attn_bwd_kv_ke
         map = &map_store;
         build_tile_map(map_store, a.doc_k + b * a.dks, row0, ROWS, a.Lk, docs, a.Lq);
     }
-    zero_padding<TYPE, DP>(Qt);
-    zero_padding<TYPE, DP>(Ot);
 
-    Frag<TYPE, DP> kf[NK], vf[NK];
+    ColFrag<TYPE, DP> kf[NK], vf[NK];
     f32x4 dk[NK][S::dt], dv[NK][S::dt];
     float kx[NK], ky[NK];
     int doc[NK];
@@ -950,8 +913,15 @@ __global__ __launch_bounds__(ATTN_THREADS, DP <= 64 ? 2 : 1) void attn_bwd_kv_ke
     for (int n = 0; n < NK; ++n) {
         const int j = wrow0 + 16 * n + c;
         const bool live = j < a.Lk;
-        frag_from_global<TYPE, DP>(kf[n], k + (int64_t)j * a.ks[2], live, a.D, g);
-        frag_from_global<TYPE, DP>(vf[n], v + (int64_t)j * a.vs[2], live, a.D, g);
+        Eight<TYPE> k8[S::chunks], v8[S::chunks];
+#pragma unroll
+        for (int x = 0; x < S::chunks; ++x) {
+            const int d = frag_d<DP>(x, g);
+            k8[x] = load_eight<TYPE>(k + (int64_t)j * a.ks[2], d, live && d < a.D);
+            v8[x] = load_eight<TYPE>(v + (int64_t)j * a.vs[2], d, live && d < a.D);
+        }
+        col_frag<TYPE, DP>(kf[n], k8, g);
+        col_frag<TYPE, DP>(vf[n], v8, g);
         doc[n] = map != nullptr ? doc_of_key(a, b, j) : 0;
         kx[n] = ky[n] = 0.0f;
         if (a.bias == 1) kx[n] = (float)j;
@@ -988,31 +958,19 @@ __global__ __launch_bounds__(ATTN_THREADS, DP <= 64 ? 2 : 1) void attn_bwd_kv_ke
     }
     const float gmul = TYPE == ATTN_F16 ? gscale * exp2_of(-F16_P_EXPONENT) : 1.0f;
 
-    UnitPlan plan[UNITS];
-#pragma unroll
-    for (int x = 0; x < UNITS; ++x) {
-        const int u = tid + x * ATTN_THREADS;
-        plan[x] = u < S::units ? unit_plan<TYPE, DP>(u, a.qs[2], a.D) : unit_plan<TYPE, DP>(u - S::units, a.dos[2], a.D);
-    }
+    Stager<TYPE, DP> stage;
+    stage.init(a.qs[2], a.dos[2], a.D);
     for (int h = h0; h < h1; ++h) {
         const char *q = a.q + (b * a.qs[0] + h * a.qs[1]) * Elem<TYPE>::bytes;
         const char *go = a.dout + (b * a.dos[0] + h * a.dos[1]) * Elem<TYPE>::bytes;
         const float *lse = a.lse + ((int64_t)b * a.Hq + h) * a.Lq, *del = a.delta + ((int64_t)b * a.Hq + h) * a.Lq;
         const ScoreParams sp = score_params(a.scale, a.cap, a.bias, a.slope, h);
-        Unit un[UNITS];
-        UnitIds ids[UNITS];
         float st_lse = 0.0f, st_delta = 0.0f, st_x = 0.0f, st_y = 0.0f;
         int st_lim = 0, st_doc = -2;
         auto load = [&](int tile) {
             const int base = tile * ATTN_ROWS, left = a.Lq - base;
             const char *qt = q + base * a.qs[2] * Elem<TYPE>::bytes, *ot = go + base * a.dos[2] * Elem<TYPE>::bytes;
-#pragma unroll
-            for (int x = 0; x < UNITS; ++x) {
-                const int u = tid + x * ATTN_THREADS;
-                if (u < S::units) unit_load(un[x], plan[x], qt, left);
-                else if (u < 2 * S::units) unit_load(un[x], plan[x], ot, left);
-                if (map != nullptr && u < 2 * S::units) unit_load_ids(ids[x], plan[x], docs + base, left);
-            }
+            stage.load(qt, ot, left, map != nullptr ? docs + base : nullptr);
             if (tid < ATTN_ROWS) {
                 const int i = base + tid;
                 const bool live = i < a.Lq;
@@ -1033,13 +991,7 @@ __global__ __launch_bounds__(ATTN_THREADS, DP <= 64 ? 2 : 1) void attn_bwd_kv_ke
         if (tile < end) load(tile);
         while (tile < end) {
             __syncthreads();
-#pragma unroll
-            for (int x = 0; x < UNITS; ++x) {
-                const int u = tid + x * ATTN_THREADS;
-                if (map != nullptr && u < 2 * S::units) unit_skip(un[x], ids[x]);
-                if (u < S::units) unit_write<TYPE, DP, true, true>(un[x], u, Qt, QT);
-                else if (u < 2 * S::units) unit_write<TYPE, DP, true, true>(un[x], u - S::units, Ot, OT);
-            }
+            stage.write(Qt, Ot, map != nullptr);
             if (tid < ATTN_ROWS) {
                 row_lse[tid] = st_lse;
                 row_delta[tid] = st_delta;
@@ -1055,18 +1007,18 @@ __global__ __launch_bounds__(ATTN_THREADS, DP <= 64 ? 2 : 1) void attn_bwd_kv_ke
             if (base + ATTN_ROWS <= wave_first || wrow0 >= a.Lk) continue;
             const bool by_doc = !tile_same(map, here), masked = by_doc || tail || base < wave_all || base + ATTN_ROWS > a.Lq;
 
-#pragma unroll
+#pragma unroll HALVES
             for (int tp = 0; tp < 2; ++tp) {
                 f32x4 s[2][NK], dp[2][NK], slack[2][NK] = {}, dist[2][NK] = {}, e[2][NK];
 #pragma unroll
                 for (int t = 0; t < 2; ++t) {
                     const int at = 32 * tp + 16 * t;
-                    Frag<TYPE, DP> f;
-                    frag_from_lds<TYPE, DP>(f, Qt, at + c, g);
+                    RowFrag<TYPE, DP> f;
+                    row_frag<TYPE, DP>(f, Qt, at + c, g);
 #pragma unroll
                     for (int n = 0; n < NK; ++n) s[t][n] = dot_block<TYPE, DP>(f, kf[n]);
                     const f32x4 minus_delta = *reinterpret_cast<const f32x4 *>(row_delta + at + 4 * g);
-                    frag_from_lds<TYPE, DP>(f, Ot, at + c, g);
+                    row_frag<TYPE, DP>(f, Ot, at + c, g);
 #pragma unroll
                     for (int n = 0; n < NK; ++n) dp[t][n] = dot_block<TYPE, DP>(f, vf[n], minus_delta);
                     const f32x4 lse2 = *reinterpret_cast<const f32x4 *>(row_lse + at + 4 * g);
@@ -1094,7 +1046,7 @@ __global__ __launch_bounds__(ATTN_THREADS, DP <= 64 ? 2 : 1) void attn_bwd_kv_ke
                         }
                     }
                 }
-                pair_probability<NK>(sp, s, dp, slack, dist, e);
+                pair_probability<NK, true>(sp, s, dp, slack, dist, e);
                 if (masked) {
 #pragma unroll
                     for (int t = 0; t < 2; ++t) {
@@ -1107,29 +1059,23 @@ __global__ __launch_bounds__(ATTN_THREADS, DP <= 64 ? 2 : 1) void attn_bwd_kv_ke
                             f32x4 p = s[t][n], ds = dp[t][n];
 #pragma unroll
                             for (int r = 0; r < 4; ++r) {
-                                const bool ok = (j < lim[r]) & (qd[r] == own);
-                                p[r] = ok ? p[r] : 0.0f;
-                                ds[r] = ok ? ds[r] : 0.0f;
+                                const unsigned ok = mask_below(j, lim[r]) & mask_equal(qd[r], own);
+                                p[r] = keep_or_zero(ok, p[r]);
+                                ds[r] = keep_or_zero(ok, ds[r]);
                             }
                             s[t][n] = p;
                             dp[t][n] = ds;
                         }
                     }
                 }
-                accumulate<TYPE, DP, NK>(dv, Ot, OT, tp, s[0], s[1], g, c);
-                if (sp.cap) {
-#pragma unroll
-                    for (int t = 0; t < 2; ++t)
-#pragma unroll
-                        for (int n = 0; n < NK; ++n) dp[t][n] = dp[t][n] * slack[t][n];
-                }
+                accumulate<TYPE, DP, NK>(dv, Ot, tp, s[0], s[1], g, c);
                 if (TYPE == ATTN_F16) {
 #pragma unroll
                     for (int t = 0; t < 2; ++t)
 #pragma unroll
                         for (int n = 0; n < NK; ++n) dp[t][n] = dp[t][n] * gmul;
                 }
-                accumulate<TYPE, DP, NK>(dk, Qt, QT, tp, dp[0], dp[1], g, c);
+                accumulate<TYPE, DP, NK>(dk, Qt, tp, dp[0], dp[1], g, c);
             }
         }
     }
@@ -1264,9 +1210,14 @@ void plan_forward(AttnArgs &a, int dtype, int &n) {
     a.splits = a.tiles > 0 ? ranges((int64_t)a.B * a.Hq * a.tiles, a.Lk) : 1;
 }
 void plan_keys(AttnArgs &a, int dtype, int &n) {
-    // (the heads of a group and ranges of 512 query rows can be dealt out as well, so two blocks of keys fill the chip earlier)
+    // The heads of a group and ranges of 512 query rows can be dealt out as well, so two blocks of keys fill the chip earlier.
+    // Not with documents: a range of rows may hold none of the block's documents, and the work is badly dealt (8 heads of 64
+    // numbers, 6000 rows in 9 documents, fp16: 168 us with one block and no ranges, 237 us with two and ranges; 2 x 16 heads over
+    // 4 of 64 numbers, 2047 causal rows behind a prefix, bf16: 146 us and 130 us).
     const int64_t pairs = (int64_t)a.B * a.Hq * ((a.Lk + 127) / 128) * ((a.Lq + 511) / 512);
-    n = two_fit(KERNEL_BWD_KV, dtype, padded(a.D)) && pairs >= 512 ? 2 : 1;
+    const bool two = a.doc_k != nullptr ? two_blocks(KERNEL_BWD_KV, dtype, a, a.Lk, a.Hkv)
+                                        : two_fit(KERNEL_BWD_KV, dtype, padded(a.D)) && pairs >= 512;
+    n = two ? 2 : 1;
     a.tiles = (a.Lk + 64 * n - 1) / (64 * n);
     const int64_t blocks = (int64_t)a.B * a.Hkv * (a.tiles > 0 ? a.tiles : 1);
     const int64_t want = blocks >= 768 ? 1 : (768 + blocks - 1) / blocks;       // (two or three workgroups fit a unit)

@@ -39,6 +39,41 @@ struct StepArgs {
     float *part;                  // [B Hkv][splits][M][D + 2]: sum of p v, maximum, sum of p
 };
 
+// ---- operands straight from memory: binary32 on the binary32 matrix instructions (the operation waits for memory, and a
+// split into bfloat16 terms would cost vector work), 16-bit types as they are ------------------------------------------
+template <int TYPE, int DP> struct DirectShape {
+    static constexpr bool wide = TYPE == ATTN_F32;
+    static constexpr int chunks = wide ? DP / 16 : DP < 32 ? 1 : DP / 32;   // operand register sets over the head size
+    static constexpr int dt = DP / 16;
+};
+template <int TYPE, int DP> struct Frag {
+    u32x4 c[DirectShape<TYPE, DP>::chunks];
+};
+// lane (g, c) of a block whose row c starts at `row`: binary32 takes d = 16 k + 4 g + i, 16-bit d = 32 k + 8 g + i
+template <int TYPE, int DP>
+__device__ __forceinline__ void frag_from_global(Frag<TYPE, DP> &f, const typename Elem<TYPE>::raw *row, bool live, int D, int g) {
+    typedef DirectShape<TYPE, DP> S;
+#pragma unroll
+    for (int k = 0; k < S::chunks; ++k) {
+        const int d = S::wide ? 16 * k + 4 * g : 32 * k + 8 * g;
+        f.c[k] = live && d < D ? *reinterpret_cast<const u32x4 *>(row + d) : u32x4{0, 0, 0, 0};
+    }
+}
+template <int TYPE, int DP> __device__ __forceinline__ f32x4 dot_block(const Frag<TYPE, DP> &a, const Frag<TYPE, DP> &b) {
+    f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int k = 0; k < DirectShape<TYPE, DP>::chunks; ++k) {
+        if constexpr (TYPE == ATTN_F32) {
+            const f32x4 x = __builtin_bit_cast(f32x4, a.c[k]), y = __builtin_bit_cast(f32x4, b.c[k]);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(x[i], y[i], acc, 0, 0, 0);
+        } else {
+            acc = mfma32<TYPE>(a.c[k], b.c[k], acc);
+        }
+    }
+    return acc;
+}
+
 __device__ __forceinline__ int live_length(const StepArgs &a, int b) {
     return max(0, min(a.lengths[b], a.max_pages << a.shift));
 }
@@ -93,7 +128,7 @@ template <int TYPE> __device__ void careful_step_row(const StepArgs &a, int b, i
 }
 
 template <int TYPE, int DP> struct StepShape {
-    typedef Shape<TYPE, DP> S;
+    typedef DirectShape<TYPE, DP> S;
     static constexpr int vw = S::wide ? (S::dt < 4 ? S::dt : 4) : (S::dt < 8 ? S::dt : 8);   // elements of V a lane reads at once
     static constexpr int vb = S::dt / vw;                                                     // such reads per key
     static constexpr int words = (vw * Elem<TYPE>::bytes + 3) / 4;                            // 32-bit registers of one
@@ -190,7 +225,7 @@ __device__ __forceinline__ void step_accumulate(f32x4 (&o)[NQ][DP / 16], const S
                                   __builtin_amdgcn_perm(t.v[1][1][y][w], t.v[1][0][y][w], pick),
                                   __builtin_amdgcn_perm(t.v[1][3][y][w], t.v[1][2][y][w], pick)};
 #pragma unroll
-                for (int n = 0; n < NQ; ++n) o[n][V::vw * y + i] = mfma16<TYPE>(av, b[n], o[n][V::vw * y + i]);
+                for (int n = 0; n < NQ; ++n) o[n][V::vw * y + i] = mfma32<TYPE>(av, b[n], o[n][V::vw * y + i]);
             }
     }
 }
@@ -198,7 +233,7 @@ __device__ __forceinline__ void step_accumulate(f32x4 (&o)[NQ][DP / 16], const S
 template <int TYPE, int DP, int NQ>
 __global__ __launch_bounds__(64 * STEP_WAVES) void attn_step_kernel(StepArgs a) {
     typedef typename Elem<TYPE>::raw raw;
-    typedef Shape<TYPE, DP> S;
+    typedef DirectShape<TYPE, DP> S;
     typedef StepShape<TYPE, DP> V;
     constexpr int LD = 16 * S::dt + 4;           // floats of one query's partial result in LDS (sum, maximum, sum of p)
     __shared__ __align__(16) float join[STEP_WAVES / 2][16 * NQ][LD];

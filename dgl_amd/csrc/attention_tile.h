@@ -43,6 +43,24 @@ __device__ __forceinline__ float group_sum(float x) {
 // NaN.  (A NaN score makes its row NaN through the sum, whatever the maximum is.)
 __device__ __forceinline__ float fast_max(float a, float b) { return __builtin_amdgcn_fmed3f(a, b, __builtin_inff()); }
 
+// Selections by masks of bits (all ones: keep).  A comparison into a scalar register and a v_cndmask from it take 27 cycles
+// of a wave here, a subtraction, a shift and a v_bfi 15.
+// (the shift is written in assembly: the compiler would turn it back into the comparison)
+__device__ __forceinline__ unsigned mask_below(int x, int limit) {       // x < limit
+    unsigned m;
+    asm("v_ashrrev_i32 %0, 31, %1" : "=v"(m) : "v"(x - limit));
+    return m;
+}
+__device__ __forceinline__ unsigned mask_equal(int a, int b) {
+    unsigned d;
+    asm("v_min_u32 %0, 1, %1" : "=v"(d) : "v"(a ^ b));
+    return d - 1u;
+}
+__device__ __forceinline__ float keep_or(unsigned mask, float x, float other) {
+    return __uint_as_float((__float_as_uint(x) & mask) | (__float_as_uint(other) & ~mask));
+}
+__device__ __forceinline__ float keep_or_zero(unsigned mask, float x) { return __uint_as_float(__float_as_uint(x) & mask); }
+
 // tanh to about 4 ulp: 1 - 2 / (e^{2y} + 1) away from zero, its odd series (to y^11) near it, where the difference would cancel
 __device__ __forceinline__ float attn_tanh(float y) {
     const float e = __builtin_amdgcn_exp2f(y * (2.0f * ATTN_LOG2E));
@@ -110,201 +128,295 @@ template <int TYPE> __device__ __forceinline__ void store4(typename Elem<TYPE>::
     else *reinterpret_cast<bf16x4 *>(p) = __builtin_convertvector(v, bf16x4);
 }
 
-// Shape of a tile of ATTN_ROWS rows of DP (padded head size) elements.
+template <int TYPE> __device__ __forceinline__ f32x4 mfma32(u32x4 a, u32x4 b, f32x4 acc) {      // 32 reduction slots
+    if constexpr (TYPE == ATTN_F16)
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), acc, 0, 0, 0);
+    else
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), acc, 0, 0, 0);
+}
+
+// ---- binary32 operands as three bfloat16 terms ----------------------------------------------------------------------
+// x = hi + mid + lo exactly (8 significand bits each, by truncation); a product is hh + hm + mh + hl + lh + mm, what is left
+// out is below 2^-23 of it.  Six bfloat16 products of 17 cycles replace eight binary32 ones of 32 per 16 x 16 x 32 block -
+// and the binary32 matrix instructions of gfx950 hold the vector ALU back for their whole duration (measured: a stream of
+// them beside vector work takes the sum of both times), the bfloat16 ones for two thirds of theirs.
+struct Split3 {
+    float hi, mid, lo;             // bfloat16 values in binary32 (lo: its upper half counts)
+};
+__device__ __forceinline__ Split3 split3(float x) {
+    Split3 s;
+    s.hi = __uint_as_float(__float_as_uint(x) & 0xffff0000u);
+    const float r = x - s.hi;
+    s.mid = __uint_as_float(__float_as_uint(r) & 0xffff0000u);
+    s.lo = r - s.mid;
+    return s;
+}
+__device__ __forceinline__ unsigned pack_upper(float a, float b) {       // upper halves: a in the low half of the word
+    return __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302u);
+}
+
+// Shape of a tile of ATTN_ROWS rows of DP (padded head size) elements in LDS: one plane of 16-bit elements, or three of a
+// binary32 tile's terms.  A plane's rows are DP / 8 pieces of 16 bytes; pieces are permuted so that the access
+// patterns spread over all 64 banks: 16 rows at one piece (operand reads, staging writes) and 16 rows at two neighbouring
+// pieces (transposing reads).
 template <int TYPE, int DP> struct Shape {
     typedef typename Elem<TYPE>::raw raw;
-    static constexpr bool wide = TYPE == ATTN_F32;
-    static constexpr int vec = 16 / Elem<TYPE>::bytes;               // elements of a 16-byte access
-    // rows are padded by 16 bytes: the 16-byte reads of 8 neighbouring rows then fall on different banks
-    static constexpr int dk = wide ? DP : (DP < 32 ? 32 : DP);       // reduction length over the head size (16-bit: multiples of 32)
-    static constexpr int ld = dk + vec;                              // row stride, elements
-    static constexpr int ldt = ATTN_ROWS + 8;                        // row stride of a transposed 16-bit tile
-    static constexpr int chunks = wide ? DP / 16 : dk / 32;          // operand registers sets over the head size
+    static constexpr int terms = TYPE == ATTN_F32 ? 3 : 1;
+    static constexpr int mma = TYPE == ATTN_F16 ? ATTN_F16 : ATTN_BF16;
+    static constexpr int vec = 16 / Elem<TYPE>::bytes;               // elements of a 16-byte global access
+    static constexpr int pieces = DP / 8;                            // 16-byte pieces of a plane's row
+    static constexpr int chunks = DP < 32 ? 1 : DP / 32;             // reductions of 32 over the head size
     static constexpr int dt = DP / 16;                               // 16-row tiles over the head size
-    static constexpr int row_bytes = ATTN_ROWS * ld * Elem<TYPE>::bytes;
-    static constexpr int t_bytes = wide ? 0 : DP * ldt * 2;          // transposed copy (binary32 reads columns in place)
-    static constexpr int per_row = DP / vec;                         // 16-byte pieces of a row
+    static constexpr int plane = ATTN_ROWS * DP * 2, bytes = terms * plane;
+    static constexpr int per_row = DP / vec;                         // 16-byte global pieces of a row
     static constexpr int units = ATTN_ROWS / 4 * per_row;            // pieces of 4 rows x 16 bytes
+    // operands of one 16-row block: A from LDS, B in registers.  Heads of 16 fill half of the 32 slots; binary32 puts two
+    // terms side by side there: A [h m], [h l] against B [h m], [m h], [l h] are the six products in three instructions.
+    static constexpr int a_regs = DP < 32 && terms == 3 ? 2 : terms * chunks, b_regs = terms * chunks;
 };
-
-// operand registers of one 16-row block over the head size
-template <int TYPE, int DP> struct Frag {
-    u32x4 c[Shape<TYPE, DP>::chunks];
-};
-
-// lane (g, c) of a block whose row c starts at `row`: binary32 takes d = 16 k + 4 g + i, 16-bit d = 32 k + 8 g + i
-template <int TYPE, int DP>
-__device__ __forceinline__ void frag_from_lds(Frag<TYPE, DP> &f, const typename Elem<TYPE>::raw *tile, int row, int g) {
-    typedef Shape<TYPE, DP> S;
-#pragma unroll
-    for (int k = 0; k < S::chunks; ++k)
-        f.c[k] = *reinterpret_cast<const u32x4 *>(tile + row * S::ld + (S::wide ? 16 * k + 4 * g : 32 * k + 8 * g));
+// (the permutation looks at the row within its block of 16 alone: blocks differ by a constant, which an LDS access adds free)
+template <int TYPE, int DP> __device__ __forceinline__ unsigned piece_at(int row, int piece) {
+    constexpr int P = Shape<TYPE, DP>::pieces, SH = P == 2 ? 3 : P == 4 ? 2 : P == 8 ? 1 : 0;
+    const int low = row & 15;
+    return (unsigned)((row >> 4) * 16 * P + low * P + (piece ^ ((low >> SH) & (P - 1)))) * 16u;
 }
-template <int TYPE, int DP>
-__device__ __forceinline__ void frag_from_global(Frag<TYPE, DP> &f, const typename Elem<TYPE>::raw *row, bool live, int D, int g) {
+
+template <int TYPE, int DP> struct RowFrag { u32x4 c[Shape<TYPE, DP>::a_regs]; };     // A: 16 rows of a tile
+template <int TYPE, int DP> struct ColFrag { u32x4 c[Shape<TYPE, DP>::b_regs]; };     // B: 16 rows kept in registers
+
+template <int TYPE, int DP> __device__ __forceinline__ void row_frag(RowFrag<TYPE, DP> &f, const char *tile, int row, int g) {
+    typedef Shape<TYPE, DP> S;
+    if constexpr (DP < 32) {
+        const char *at = tile + piece_at<TYPE, DP>(row, g & 1);
+        if constexpr (S::terms == 3) {
+            f.c[0] = *reinterpret_cast<const u32x4 *>(at + (g >> 1) * S::plane);
+            f.c[1] = *reinterpret_cast<const u32x4 *>(at + (g >> 1) * 2 * S::plane);
+        } else {
+            f.c[0] = *reinterpret_cast<const u32x4 *>(at);           // (the upper slots meet zeros)
+        }
+    } else {
+#pragma unroll
+        for (int k = 0; k < S::chunks; ++k)
+#pragma unroll
+            for (int p = 0; p < S::terms; ++p)
+                f.c[k * S::terms + p] = *reinterpret_cast<const u32x4 *>(tile + p * S::plane + piece_at<TYPE, DP>(row, 4 * k + g));
+    }
+}
+
+// eight elements of a row in global memory from element d on; zeros beyond the head size
+template <int TYPE> struct Eight { u32x4 w[Elem<TYPE>::bytes / 2]; };
+template <int TYPE> __device__ __forceinline__ Eight<TYPE> load_eight(const typename Elem<TYPE>::raw *row, int d, bool live) {
+    Eight<TYPE> x;
+#pragma unroll
+    for (int i = 0; i < Elem<TYPE>::bytes / 2; ++i)
+        x.w[i] = live ? *reinterpret_cast<const u32x4 *>(row + d + i * (16 / Elem<TYPE>::bytes)) : u32x4{0, 0, 0, 0};
+    return x;
+}
+template <int TYPE> __device__ __forceinline__ float eight_at(const Eight<TYPE> &x, int i) {
+    if constexpr (TYPE == ATTN_F32) return __uint_as_float(x.w[i >> 2][i & 3]);
+    else return elem_to_float<TYPE>((unsigned short)(x.w[0][i >> 1] >> (16 * (i & 1))));
+}
+// the first element that lane group g holds of chunk k, and whether it is the group that counts it (heads of 16: two groups
+// hold the same)
+template <int DP> __device__ __forceinline__ int frag_d(int k, int g) { return DP < 32 ? 8 * (g & 1) : 32 * k + 8 * g; }
+template <int DP> __device__ __forceinline__ bool frag_counts(int g) { return DP >= 32 || g < 2; }
+
+template <int TYPE, int DP> __device__ __forceinline__ void col_frag(ColFrag<TYPE, DP> &f, const Eight<TYPE> (&x)[Shape<TYPE, DP>::chunks], int g) {
     typedef Shape<TYPE, DP> S;
 #pragma unroll
     for (int k = 0; k < S::chunks; ++k) {
-        const int d = S::wide ? 16 * k + 4 * g : 32 * k + 8 * g;
-        f.c[k] = live && d < D ? *reinterpret_cast<const u32x4 *>(row + d) : u32x4{0, 0, 0, 0};
-    }
-}
-
-template <int TYPE> __device__ __forceinline__ f32x4 mfma16(u32x4 a, u32x4 b, f32x4 acc) {
-    if constexpr (TYPE == ATTN_F32) {
-        const f32x4 x = __builtin_bit_cast(f32x4, a), y = __builtin_bit_cast(f32x4, b);
+        if constexpr (S::terms == 1) {
+            f.c[k] = x[k].w[0];
+            if (DP < 32 && g >= 2) f.c[k] = u32x4{0, 0, 0, 0};
+        } else {
+            u32x4 t[3];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(x[i], y[i], acc, 0, 0, 0);
-        return acc;
-    } else if constexpr (TYPE == ATTN_F16) {
-        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), acc, 0, 0, 0);
-    } else {
-        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), acc, 0, 0, 0);
+            for (int i = 0; i < 4; ++i) {
+                const Split3 a = split3(eight_at<TYPE>(x[k], 2 * i)), b = split3(eight_at<TYPE>(x[k], 2 * i + 1));
+                t[0][i] = pack_upper(a.hi, b.hi);
+                t[1][i] = pack_upper(a.mid, b.mid);
+                t[2][i] = pack_upper(a.lo, b.lo);
+            }
+            if constexpr (DP < 32) {
+                f.c[0] = g < 2 ? t[0] : t[1];
+                f.c[1] = g < 2 ? t[1] : t[0];
+                f.c[2] = g < 2 ? t[2] : t[0];
+            } else {
+#pragma unroll
+                for (int p = 0; p < 3; ++p) f.c[3 * k + p] = t[p];
+            }
+        }
     }
 }
 
-// acc[row 4g+r][column c] += (tile rows 16 t ..) . (block whose operand registers are b)
+// accumulator + (16 tile rows) . (16 register rows): rows 4 g + r, column c
 template <int TYPE, int DP>
-__device__ __forceinline__ f32x4 dot_block(const Frag<TYPE, DP> &a, const Frag<TYPE, DP> &b, f32x4 acc = f32x4{0.0f, 0.0f, 0.0f, 0.0f}) {
+__device__ __forceinline__ f32x4 dot_block(const RowFrag<TYPE, DP> &a, const ColFrag<TYPE, DP> &b, f32x4 acc = f32x4{0.0f, 0.0f, 0.0f, 0.0f}) {
+    typedef Shape<TYPE, DP> S;
+    if constexpr (S::terms == 1) {
 #pragma unroll
-    for (int k = 0; k < Shape<TYPE, DP>::chunks; ++k) acc = mfma16<TYPE>(a.c[k], b.c[k], acc);
+        for (int k = 0; k < S::chunks; ++k) acc = mfma32<S::mma>(a.c[k], b.c[k], acc);
+    } else if constexpr (DP < 32) {
+        acc = mfma32<S::mma>(a.c[1], b.c[2], acc);
+        acc = mfma32<S::mma>(a.c[0], b.c[1], acc);
+        acc = mfma32<S::mma>(a.c[0], b.c[0], acc);
+    } else {
+#pragma unroll
+        for (int k = 0; k < S::chunks; ++k) {        // the small products first
+            acc = mfma32<S::mma>(a.c[3 * k], b.c[3 * k + 2], acc);
+            acc = mfma32<S::mma>(a.c[3 * k + 2], b.c[3 * k], acc);
+            acc = mfma32<S::mma>(a.c[3 * k + 1], b.c[3 * k + 1], acc);
+            acc = mfma32<S::mma>(a.c[3 * k], b.c[3 * k + 1], acc);
+            acc = mfma32<S::mma>(a.c[3 * k + 1], b.c[3 * k], acc);
+            acc = mfma32<S::mma>(a.c[3 * k], b.c[3 * k], acc);
+        }
+    }
     return acc;
 }
 
-// The second product of a chain: out[d][column] += sum over the rows of a pair of 16-row blocks 2 tp, 2 tp + 1 of
-// tile[row][d] * w[row][column]; w0 / w1 are accumulators of dot_block for the two blocks.  Binary32 reads the row-major
-// tile by columns; 16-bit types read the transposed copy, whose rows are stored in the order 8 g + 4 (t mod 2) + r of
-// every 32, so that a lane's eight reduction slots are one 16-byte read.
+// The second product of a chain: out[d][column] += sum over the rows of two 16-row blocks 2 tp, 2 tp + 1 of
+// tile[row][d] * w[row][column]; w0 / w1 are results of dot_block for the two blocks (probabilities, score gradients),
+// rounded to 16 bits here - or split into three terms.  The tile is read transposed: ds_read_b64_tr_b16 gives lane c of a
+// 16-lane group element c mod 4 of the addresses of lanes c / 4 + 4 j, so lane s points at four elements of row s / 4.
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ u32x2 read_transposed(const char *p) {
+    return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *)p));
+}
 template <int TYPE, int DP, int N, int DT>
-__device__ __forceinline__ void accumulate(f32x4 (&out)[N][DT], const typename Elem<TYPE>::raw *tile,
-                                           const typename Elem<TYPE>::raw *tile_t, int tp, const f32x4 (&w0)[N],
-                                           const f32x4 (&w1)[N], int g, int c) {
+__device__ __forceinline__ void accumulate(f32x4 (&out)[N][DT], const char *tile, int tp, const f32x4 (&w0)[N], const f32x4 (&w1)[N], int g, int c) {
     typedef Shape<TYPE, DP> S;
     static_assert(DT == S::dt, "accumulators of another head size");
-    if constexpr (S::wide) {
+    u32x4 b[N][S::terms];
 #pragma unroll
-        for (int t = 0; t < 2; ++t)
+    for (int n = 0; n < N; ++n) {
+        if constexpr (TYPE == ATTN_F16) {
+            const u32x2 lo = __builtin_bit_cast(u32x2, __builtin_convertvector(w0[n], f16x4)), hi = __builtin_bit_cast(u32x2, __builtin_convertvector(w1[n], f16x4));
+            b[n][0] = u32x4{lo[0], lo[1], hi[0], hi[1]};
+        } else if constexpr (TYPE == ATTN_BF16) {
+            const u32x2 lo = __builtin_bit_cast(u32x2, __builtin_convertvector(w0[n], bf16x4)), hi = __builtin_bit_cast(u32x2, __builtin_convertvector(w1[n], bf16x4));
+            b[n][0] = u32x4{lo[0], lo[1], hi[0], hi[1]};
+        } else {
 #pragma unroll
-            for (int r = 0; r < 4; ++r)
-#pragma unroll
-                for (int d = 0; d < S::dt; ++d) {
-                    const float a = tile[(32 * tp + 16 * t + 4 * g + r) * S::ld + 16 * d + c];
-#pragma unroll
-                    for (int n = 0; n < N; ++n)
-                        out[n][d] = __builtin_amdgcn_mfma_f32_16x16x4f32(a, t ? w1[n][r] : w0[n][r], out[n][d], 0, 0, 0);
-                }
-    } else {
-        u32x4 b[N];
-#pragma unroll
-        for (int n = 0; n < N; ++n) {
-            u32x2 lo, hi;
-            if constexpr (TYPE == ATTN_F16) {
-                lo = __builtin_bit_cast(u32x2, __builtin_convertvector(w0[n], f16x4));
-                hi = __builtin_bit_cast(u32x2, __builtin_convertvector(w1[n], f16x4));
-            } else {
-                lo = __builtin_bit_cast(u32x2, __builtin_convertvector(w0[n], bf16x4));
-                hi = __builtin_bit_cast(u32x2, __builtin_convertvector(w1[n], bf16x4));
+            for (int i = 0; i < 4; ++i) {
+                const Split3 x = split3(i < 2 ? w0[n][2 * i] : w1[n][2 * i - 4]), y = split3(i < 2 ? w0[n][2 * i + 1] : w1[n][2 * i - 3]);
+                b[n][0][i] = pack_upper(x.hi, y.hi);
+                b[n][1][i] = pack_upper(x.mid, y.mid);
+                b[n][2][i] = pack_upper(x.lo, y.lo);
             }
-            b[n] = u32x4{lo[0], lo[1], hi[0], hi[1]};
+        }
+    }
+#pragma unroll
+    for (int d = 0; d < S::dt; ++d) {
+        u32x4 a[S::terms];
+#pragma unroll
+        for (int p = 0; p < S::terms; ++p) {
+            const char *at = tile + piece_at<TYPE, DP>(4 * g + (c >> 2), 2 * d + ((c >> 1) & 1)) + 8 * (c & 1) + p * S::plane + 64 * DP * tp;
+            const u32x2 lo = read_transposed(at), hi = read_transposed(at + 32 * DP);
+            a[p] = u32x4{lo[0], lo[1], hi[0], hi[1]};
         }
 #pragma unroll
-        for (int d = 0; d < S::dt; ++d) {
-            const u32x4 a = *reinterpret_cast<const u32x4 *>(tile_t + (16 * d + c) * S::ldt + 32 * tp + 8 * g);
-#pragma unroll
-            for (int n = 0; n < N; ++n) out[n][d] = mfma16<TYPE>(a, b[n], out[n][d]);
+        for (int n = 0; n < N; ++n) {
+            if constexpr (S::terms == 3) {
+                out[n][d] = mfma32<S::mma>(a[0], b[n][2], out[n][d]);
+                out[n][d] = mfma32<S::mma>(a[2], b[n][0], out[n][d]);
+                out[n][d] = mfma32<S::mma>(a[1], b[n][1], out[n][d]);
+                out[n][d] = mfma32<S::mma>(a[0], b[n][1], out[n][d]);
+                out[n][d] = mfma32<S::mma>(a[1], b[n][0], out[n][d]);
+            }
+            out[n][d] = mfma32<S::mma>(a[0], b[n][0], out[n][d]);
         }
     }
 }
 
 // ---- staging ------------------------------------------------------------------------------------------------------
-// One unit = 4 consecutive rows x 16 bytes, held by one thread between its global loads and its LDS writes.
-struct Unit {
-    u32x4 r[4];
-};
-
-template <int TYPE, int DP> __device__ __forceinline__ void unit_place(int u, int &grp, int &piece) {
+// Two [rows][D] matrices pass through LDS tile by tile, in units of rows grp, grp + 16, + 32, + 48 x 16 bytes that one thread
+// holds between its global loads and its LDS writes.  Where a matrix has fewer than 256 units, whole waves take one matrix
+// or the other; else every thread takes the same units of both.  Row strides are scalars and a unit's offset from the tile is
+// below 2^32 (the launcher's check), so that a load is a scalar address plus a 32-bit offset.
+template <int TYPE, int DP> struct Stager {
     typedef Shape<TYPE, DP> S;
-    if constexpr (S::wide) {
-        piece = u % S::per_row;
-        grp = u / S::per_row;
-    } else {           // neighbouring threads take neighbouring row groups: their transposed 8-byte writes are contiguous
-        grp = u % (ATTN_ROWS / 4);
-        piece = u / (ATTN_ROWS / 4);
-    }
-}
+    static constexpr bool both = S::units >= 256;
+    static constexpr int plans = both ? S::units / 256 : 1, second = S::units < 64 ? 64 : S::units;   // first thread of the second matrix
+    u32x4 r[both ? 2 : 1][plans][4];
+    int id[plans][4];
+    unsigned off[both ? 2 : 1][plans], at[plans];
+    int grp[plans];
+    bool in[plans];
+    int which;                                   // !both: the wave's matrix
+    unsigned rb0, rb1;                           // bytes between rows
 
-// What a thread knows about its unit of every tile: byte offsets of the four rows from the tile's first (below 2^32 by the
-// launcher's check, so that a load is a scalar address plus a 32-bit offset)
-struct UnitPlan {
-    unsigned off, row_bytes;
-    int grp;
-    bool in;                                   // the piece lies within the head size
-};
-template <int TYPE, int DP> __device__ __forceinline__ UnitPlan unit_plan(int u, int64_t stride, int D) {
-    UnitPlan p;
-    int piece;
-    unit_place<TYPE, DP>(u, p.grp, piece);
-    p.row_bytes = (unsigned)(stride * Elem<TYPE>::bytes);
-    p.off = 4u * (unsigned)p.grp * p.row_bytes + 16u * (unsigned)piece;
-    p.in = piece * Shape<TYPE, DP>::vec < D;
-    return p;
-}
-// the rows of a tile that starts at `tile` with `rows` rows left; rows beyond are zero
-__device__ __forceinline__ void unit_load(Unit &un, const UnitPlan &p, const char *tile, int rows) {
-    if (rows >= ATTN_ROWS) {
+    __device__ __forceinline__ void init(int64_t stride0, int64_t stride1, int D) {
+        const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+        which = !both && wave >= second / 64;
+        rb0 = (unsigned)(stride0 * Elem<TYPE>::bytes);
+        rb1 = (unsigned)(stride1 * Elem<TYPE>::bytes);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) un.r[i] = p.in ? *reinterpret_cast<const u32x4 *>(tile + (p.off + i * p.row_bytes)) : u32x4{0, 0, 0, 0};
-    } else {
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-            un.r[i] = p.in && 4 * p.grp + i < rows ? *reinterpret_cast<const u32x4 *>(tile + (p.off + i * p.row_bytes)) : u32x4{0, 0, 0, 0};
-    }
-}
-// rows of padding (document id < 0) may hold anything: they are staged as zeros, so that a NaN among them does not send the
-// whole tile down the careful path
-struct UnitIds {
-    int id[4];
-};
-__device__ __forceinline__ void unit_load_ids(UnitIds &ids, const UnitPlan &p, const int *tile, int rows) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) ids.id[i] = 4 * p.grp + i < rows ? tile[4 * p.grp + i] : -1;
-}
-__device__ __forceinline__ void unit_skip(Unit &un, const UnitIds &ids) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int w = 0; w < 4; ++w) un.r[i][w] = ids.id[i] >= 0 ? un.r[i][w] : 0u;
-}
-
-template <int TYPE, int DP, bool ROWMAJOR, bool TRANSPOSED>
-__device__ __forceinline__ void unit_write(const Unit &un, int u, typename Elem<TYPE>::raw *tile, typename Elem<TYPE>::raw *tile_t) {
-    typedef Shape<TYPE, DP> S;
-    int grp, piece;
-    unit_place<TYPE, DP>(u, grp, piece);
-    if constexpr (ROWMAJOR || S::wide) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) *reinterpret_cast<u32x4 *>(tile + (4 * grp + i) * S::ld + piece * S::vec) = un.r[i];
-    }
-    if constexpr (TRANSPOSED && !S::wide) {
-        const int t = grp >> 2, at = 32 * (t >> 1) + 8 * (grp & 3) + 4 * (t & 1);
-#pragma unroll
-        for (int w = 0; w < 4; ++w) {
-            typename Elem<TYPE>::raw *p = tile_t + (piece * 8 + 2 * w) * S::ldt + at;
-            *reinterpret_cast<u32x2 *>(p) = u32x2{__builtin_amdgcn_perm(un.r[1][w], un.r[0][w], 0x05040100u),
-                                                  __builtin_amdgcn_perm(un.r[3][w], un.r[2][w], 0x05040100u)};
-            *reinterpret_cast<u32x2 *>(p + S::ldt) = u32x2{__builtin_amdgcn_perm(un.r[1][w], un.r[0][w], 0x07060302u),
-                                                           __builtin_amdgcn_perm(un.r[3][w], un.r[2][w], 0x07060302u)};
+        for (int x = 0; x < plans; ++x) {
+            const int u = (int)threadIdx.x + 256 * x - (which ? second : 0), piece = u % S::per_row;
+            grp[x] = u / S::per_row;
+            in[x] = u < S::units && piece * S::vec < D;
+            if constexpr (both) {
+                off[0][x] = (unsigned)grp[x] * rb0 + 16u * (unsigned)piece;
+                off[1][x] = (unsigned)grp[x] * rb1 + 16u * (unsigned)piece;
+            } else {
+                off[0][x] = (unsigned)grp[x] * (which ? rb1 : rb0) + 16u * (unsigned)piece;
+            }
+            at[x] = S::terms == 1 ? piece_at<TYPE, DP>(grp[x], piece) : piece_at<TYPE, DP>(grp[x], piece >> 1) + 8 * (piece & 1);
+            if (u >= S::units) grp[x] = -1;      // (no unit: nothing is written)
         }
     }
-}
-
-// 16-bit row-major tiles of heads below 32: the columns beyond the head size multiply zero operands and have to be finite
-template <int TYPE, int DP> __device__ __forceinline__ void zero_padding(typename Elem<TYPE>::raw *tile) {
-    typedef Shape<TYPE, DP> S;
-    if constexpr (!S::wide && DP < 32) {
-        for (int i = threadIdx.x; i < ATTN_ROWS * (32 - DP) / 8; i += blockDim.x) {
-            const int per = (32 - DP) / 8;
-            *reinterpret_cast<u32x4 *>(tile + (i / per) * S::ld + DP + 8 * (i % per)) = u32x4{0, 0, 0, 0};
+    // the tiles that start at t0 / t1 with `rows` rows left (rows beyond are zero); ids: the rows' document ids or nullptr
+    __device__ __forceinline__ void load(const char *t0, const char *t1, int rows, const int *ids) {
+#pragma unroll
+        for (int m = 0; m < (both ? 2 : 1); ++m) {
+            const char *t = both ? (m ? t1 : t0) : (which ? t1 : t0);
+            const unsigned rb = both ? (m ? rb1 : rb0) : (which ? rb1 : rb0);
+#pragma unroll
+            for (int x = 0; x < plans; ++x)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const bool live = in[x] && (rows >= ATTN_ROWS || grp[x] + 16 * i < rows);
+                    r[m][x][i] = live ? *reinterpret_cast<const u32x4 *>(t + (uint64_t)(16u * i * rb) + off[m][x]) : u32x4{0, 0, 0, 0};
+                }
+        }
+        if (ids != nullptr) {
+#pragma unroll
+            for (int x = 0; x < plans; ++x)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) id[x][i] = grp[x] >= 0 && grp[x] + 16 * i < rows ? ids[grp[x] + 16 * i] : -1;
         }
     }
-}
+    // Rows of padding (document id < 0) may hold anything: they are staged as zeros, so that a NaN among them does not send
+    // the whole tile down the careful path.
+    __device__ __forceinline__ void write(char *l0, char *l1, bool skip) {
+#pragma unroll
+        for (int x = 0; x < plans; ++x) {
+            if (!both && grp[x] < 0) continue;
+#pragma unroll
+            for (int m = 0; m < (both ? 2 : 1); ++m) {
+                char *l = (both ? (m ? l1 : l0) : (which ? l1 : l0)) + at[x];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    u32x4 v = r[m][x][i];
+                    if (skip) {
+                        unsigned keep;
+                        asm("v_ashrrev_i32 %0, 31, %1" : "=v"(keep) : "v"(id[x][i]));
+#pragma unroll
+                        for (int w = 0; w < 4; ++w) v[w] &= ~keep;
+                    }
+                    char *to = l + 256 * S::pieces * i;
+                    if constexpr (S::terms == 1) {
+                        *reinterpret_cast<u32x4 *>(to) = v;
+                    } else {                     // four binary32 elements are half a piece of each plane
+                        Split3 y[4];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) y[e] = split3(__uint_as_float(v[e]));
+                        *reinterpret_cast<u32x2 *>(to) = u32x2{pack_upper(y[0].hi, y[1].hi), pack_upper(y[2].hi, y[3].hi)};
+                        *reinterpret_cast<u32x2 *>(to + S::plane) = u32x2{pack_upper(y[0].mid, y[1].mid), pack_upper(y[2].mid, y[3].mid)};
+                        *reinterpret_cast<u32x2 *>(to + 2 * S::plane) = u32x2{pack_upper(y[0].lo, y[1].lo), pack_upper(y[2].lo, y[3].lo)};
+                    }
+                }
+            }
+        }
+    }
+};
