@@ -63,7 +63,7 @@ class Attention(Structure):
                 ("q", c_void_p), ("k", c_void_p), ("v", c_void_p), ("out", c_void_p), ("lse", c_void_p),
                 ("slope", c_void_p), ("pos_q", c_void_p), ("pos_k", c_void_p), ("pos_q_stride", c_int64),
                 ("pos_k_stride", c_int64), ("doc_q", c_void_p), ("doc_k", c_void_p), ("doc_q_stride", c_int64),
-                ("doc_k_stride", c_int64), ("prefix", c_void_p)]
+                ("doc_k_stride", c_int64), ("prefix", c_void_p), ("out_rest", c_void_p)]
 
 
 class AttentionGrad(Structure):

@@ -25,7 +25,7 @@ _VEC = {torch.float32: 4, torch.float16: 8, torch.bfloat16: 8}      # elements o
 
 # A call of a few microseconds on the device is lost in a host path that sets ctypes fields one by one: the ABI structs are
 # packed in one go (the formats restate include/dgl_amd.h; a wrong size fails here, at import).
-_PACK_ATTENTION = struct.Struct("@8i2f12q5P3P2q2P2qP")
+_PACK_ATTENTION = struct.Struct("@8i2f12q5P3P2q2P2q2P")
 _PACK_GRAD = struct.Struct("@4P12qP")
 _PACK_STEP = struct.Struct("@2i2f4q6Pq2iPq")
 _STEP_AT = _lib.AttentionStep.rows_per_instance.offset
@@ -99,7 +99,8 @@ def _side(t: Optional[torch.Tensor], name, shape, dtype, device) -> Optional[tor
 
 class _Call:
     """Arguments of one operator call: the tensors the kernels can address, and the ABI struct over them."""
-    __slots__ = ("q", "k", "v", "slope", "pos_q", "pos_k", "doc_q", "doc_k", "prefix", "head", "tail", "a", "out", "lse")
+    __slots__ = ("q", "k", "v", "slope", "pos_q", "pos_k", "doc_q", "doc_k", "prefix", "head", "tail", "a", "out", "lse",
+                 "rest")
 
     def __init__(self, q, k, v, scale, cap, slope, pos_q, pos_k, doc_q, doc_k, causal, prefix):
         _check_qkv(q, k, v)
@@ -131,11 +132,11 @@ class _Call:
                      self.pos_k.stride(0) if pos else 0, ptr(self.doc_q), ptr(self.doc_k), self.doc_q.stride(0) if doc else 0,
                      self.doc_k.stride(0) if doc else 0, ptr(self.prefix))
 
-    def set_out(self, out, lse):
-        self.out, self.lse = out, lse
+    def set_out(self, out, lse, rest=None):
+        self.out, self.lse, self.rest = out, lse, rest
         self.a = _lib.Attention()
         _PACK_ATTENTION.pack_into(self.a, 0, *self.head, *out.stride()[:3], self.q.data_ptr(), self.k.data_ptr(), self.v.data_ptr(),
-                                  out.data_ptr(), ptr(lse), *self.tail)
+                                  out.data_ptr(), ptr(lse), *self.tail, ptr(rest))
 
 
 def _like_heads(t: torch.Tensor) -> torch.Tensor:
@@ -147,11 +148,12 @@ def _like_heads(t: torch.Tensor) -> torch.Tensor:
     return torch.empty_strided((B, H, L, D), (H * L * D, L * D, D, 1), dtype=t.dtype, device=t.device)
 
 
-def _forward(call: _Call, want_lse: bool):
+def _forward(call: _Call, want_lse: bool, want_rest: bool = False):
     q = call.q
     out = _like_heads(q)
+    rest = torch.empty_like(out) if want_rest and q.dtype != torch.float32 else None
     lse = torch.empty(q.shape[:3], dtype=torch.float32, device=q.device) if want_lse else None
-    call.set_out(out, lse)
+    call.set_out(out, lse, rest)
     if out.numel():
         lib = _lib.load()
         a = ctypes.byref(call.a)
@@ -183,7 +185,8 @@ def _backward(call: _Call, dout: torch.Tensor, want_slope: bool):
 def attention_forward(q, k, v, *, scale=None, cap=0.0, slope=None, pos_q=None, pos_k=None, doc_q=None, doc_k=None,
                       causal=False, prefix=None) -> Tuple[torch.Tensor, torch.Tensor]:
     """(out, lse) without autograd: the pair of calls to use where the backward pass is driven by hand, for instance
-    inside a captured graph."""
+    inside a captured graph.  (In 16 bits the differentiable call also keeps what the rounding of ``out`` left off; here the
+    backward pass works with the rounded output.)"""
     with torch.no_grad():
         return _forward(_Call(q, k, v, scale, cap, slope, pos_q, pos_k, doc_q, doc_k, causal, prefix), True)
 
@@ -206,20 +209,20 @@ class _Attention(torch.autograd.Function):
     def forward(ctx, q, k, v, slope, scale, cap, pos_q, pos_k, doc_q, doc_k, causal, prefix):
         call = _Call(q, k, v, scale, cap, slope, pos_q, pos_k, doc_q, doc_k, causal, prefix)
         need = any(ctx.needs_input_grad[:4])
-        out, lse = _forward(call, need)
+        out, lse = _forward(call, need, need)
         if need:
             # (the saved inputs are the caller's: autograd notices a change in place between the two passes)
-            ctx.save_for_backward(q, k, v, slope, pos_q, pos_k, doc_q, doc_k, prefix, out, lse)
+            ctx.save_for_backward(q, k, v, slope, pos_q, pos_k, doc_q, doc_k, prefix, out, lse, call.rest)
             ctx.scalars = (scale, cap, causal)
         return out
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dout):
-        q, k, v, slope, pos_q, pos_k, doc_q, doc_k, prefix, out, lse = ctx.saved_tensors
+        q, k, v, slope, pos_q, pos_k, doc_q, doc_k, prefix, out, lse, rest = ctx.saved_tensors
         scale, cap, causal = ctx.scalars
         call = _Call(q, k, v, scale, cap, slope, pos_q, pos_k, doc_q, doc_k, causal, prefix)
-        call.set_out(out, lse)
+        call.set_out(out, lse, rest)
         dq, dk, dv, dslope = _backward(call, dout, slope is not None and ctx.needs_input_grad[3])
         if dslope is not None and slope.dtype != torch.float32:
             dslope = dslope.to(slope.dtype)

@@ -104,7 +104,7 @@ __device__ __forceinline__ float score_of(const ScoreParams &p, float dot, float
 }
 
 // ---- element types -----------------------------------------------------------------------------------------------
-// F32: binary32 matrix instructions (FMA chains: no operand is rounded).  F16 / BF16: the tile operands are the inputs
+// F32: operands as three bfloat16 terms (below), so none is rounded.  F16 / BF16: the tile operands are the inputs
 // as they are, probabilities and score gradients are rounded to the type (relative error 2^-11 / 2^-8 each, independent
 // from term to term), accumulation is binary32.
 enum { ATTN_F32 = 0, ATTN_F16 = 1, ATTN_BF16 = 2 };
@@ -126,6 +126,20 @@ template <int TYPE> __device__ __forceinline__ void store4(typename Elem<TYPE>::
     if constexpr (TYPE == ATTN_F32) *reinterpret_cast<f32x4 *>(p) = v;
     else if constexpr (TYPE == ATTN_F16) *reinterpret_cast<f16x4 *>(p) = __builtin_convertvector(v, f16x4);
     else *reinterpret_cast<bf16x4 *>(p) = __builtin_convertvector(v, bf16x4);
+}
+
+// the value that a store of x leaves
+template <int TYPE> __device__ __forceinline__ f32x4 rounded4(f32x4 x) {
+    if constexpr (TYPE == ATTN_F32) return x;
+    else if constexpr (TYPE == ATTN_F16) {
+        const u32x2 h = __builtin_bit_cast(u32x2, __builtin_convertvector(x, f16x4));
+        return f32x4{elem_to_float<TYPE>((unsigned short)h[0]), elem_to_float<TYPE>((unsigned short)(h[0] >> 16)),
+                     elem_to_float<TYPE>((unsigned short)h[1]), elem_to_float<TYPE>((unsigned short)(h[1] >> 16))};
+    } else {
+        const u32x2 h = __builtin_bit_cast(u32x2, __builtin_convertvector(x, bf16x4));
+        return f32x4{__uint_as_float(h[0] << 16), __uint_as_float(h[0] & 0xffff0000u), __uint_as_float(h[1] << 16),
+                     __uint_as_float(h[1] & 0xffff0000u)};
+    }
 }
 
 template <int TYPE> __device__ __forceinline__ f32x4 mfma32(u32x4 a, u32x4 b, f32x4 acc) {      // 32 reduction slots

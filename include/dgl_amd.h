@@ -394,6 +394,8 @@ typedef struct {
     const int32_t *doc_q, *doc_k;           /* [B][Lq], [B][Lk] or both NULL */
     int64_t doc_q_stride, doc_k_stride;     /* ids between batch entries */
     const int32_t *prefix;     /* [B] or NULL */
+    void *out_rest;            /* 16-bit types: like out (its strides), or NULL.  Written forward: what out's rounding left off,
+                                  rounded to the type; read backward, where the rows' dout.out is taken from both. */
 } dgl_attention_t;
 
 typedef struct {

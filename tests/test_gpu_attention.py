@@ -324,3 +324,36 @@ def test_gradients_keep_their_types(device):
     out = attention(q, q, q, slope=slope)
     out.sum().backward()
     assert q.grad.dtype == torch.bfloat16 and slope.grad.dtype == torch.bfloat16
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("H,K,L,M,D", [(2, 2, 70, 70, 24), (2, 1, 5, 3000, 16), (4, 1, 300, 130, 128), (16, 16, 2100, 65, 64)])
+def test_autograd_in_16_bits(device, dtype, H, K, L, M, D):
+    """The differentiable call keeps what the output's rounding left off for its backward pass: one block of rows per wave
+    and two, ranges of keys that are joined, head sizes behind the padding."""
+    from dgl_amd.attention import attention
+    t, kw = inputs(2, H, K, L, M, D, TYPES[dtype], 31, bias="index")
+    leaves = [t[n].clone().requires_grad_() for n in "qkv"]
+    out = attention(*leaves, **kw)
+    out.backward(t["dout"])
+    want = reference(t["q"], t["k"], t["v"], t["dout"], **kw)
+    assert_within(out.detach(), want["out"], "out")
+    for x, n in zip(leaves, ("dq", "dk", "dv")):
+        assert_within(x.grad, want[n], n)
+
+
+def test_rounding_of_the_output_does_not_reach_the_gradients(device):
+    """A steep slope: few keys carry a row, and with the output's rounding delta is off by 2^-9 of its terms, as much as the
+    score gradients' own rounding (both: sqrt(2) times the error of one); the rest of the output takes that away."""
+    from dgl_amd.attention import attention, attention_backward, attention_forward
+    t, kw = inputs(2, 4, 4, 512, 512, 64, torch.bfloat16, 37)
+    kw["slope"] = torch.full((4,), 0.7, device=device)
+    want = reference(t["q"], t["k"], t["v"], t["dout"], **kw)
+    leaves = [t[n].clone().requires_grad_() for n in "qkv"]
+    attention(*leaves, **kw).backward(t["dout"])
+    out, lse = attention_forward(t["q"], t["k"], t["v"], **kw)
+    by_hand = attention_backward(t["dout"], t["q"], t["k"], t["v"], out, lse, **kw)
+    for n, x, y in zip(("dq", "dk"), leaves, by_hand):
+        value = want[n][0]
+        error = [((z.double() - value).norm() / value.norm()).item() for z in (x.grad, y)]
+        assert error[0] < 0.9 * error[1], (n, error)
