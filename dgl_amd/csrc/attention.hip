@@ -154,6 +154,11 @@ __device__ __forceinline__ bool finite4(const f32x4 &v) {
 // One workgroup = 4 waves x NQ blocks of 16 queries of one (batch, head); keys and values pass through LDS in tiles of 64,
 // the next tile's loads in flight while the current one is computed.  Lane (g, c) holds query c of its blocks and, per
 // 16 keys, the scores against keys 4 g + r.
+//
+// The running maximum follows the scores only when one rises 2^SOFTMAX_RISE above it: sums and probabilities are binary32,
+// or have room for 2^8 in 16 bits, and a row's sums are rescaled a few times instead of at every new maximum.  Scores come
+// out of the cap (or the scaling) relative to it, which saves the subtraction.
+#define SOFTMAX_RISE 8.0f
 template <int TYPE> __device__ __forceinline__ void store_wide(typename Elem<TYPE>::raw *o, int d, float x) {
     if constexpr (TYPE == ATTN_F32) o[d] = x;
     else if constexpr (TYPE == ATTN_F16) o[d] = __builtin_bit_cast(unsigned short, (_Float16)x);
@@ -244,7 +249,7 @@ __global__ __launch_bounds__(ATTN_THREADS, TYPE == ATTN_F32 && DP == 128 ? 1 : 2
     
     ColFrag<TYPE, DP> qf[NQ];
     f32x4 o[NQ][S::dt];
-    float m[NQ], l[NQ], qx[NQ], qy[NQ];
+    float w[NQ], rise[NQ], l[NQ], qx[NQ], qy[NQ];     // what scores are taken relative to, and how far above it they may be
     int limit[NQ], doc[NQ];
     int wave_limit = 0, wave_full = INT_MAX;          // keys some row / every row of the wave sees
 #pragma unroll
@@ -253,8 +258,9 @@ __global__ __launch_bounds__(ATTN_THREADS, TYPE == ATTN_F32 && DP == 128 ? 1 : 2
         Eight<TYPE> q8[S::chunks];
 #pragma unroll
         for (int k8 = 0; k8 < S::chunks; ++k8) q8[k8] = load_eight<TYPE>(q + (int64_t)i * a.qs[2], frag_d<DP>(k8, g), i < a.Lq && frag_d<DP>(k8, g) < a.D);
-        col_frag<TYPE, DP>(qf[n], q8, g);
-        m[n] = -attn_inf();
+        col_frag<TYPE, DP>(qf[n], q8, g, score_factor(sp));
+        w[n] = 0.0f;
+        rise[n] = -attn_inf();
         l[n] = 0.0f;
         limit[n] = row_limit(a, b, i);
         doc[n] = map != nullptr ? doc_of_query(a, b, i) : 0;
@@ -313,21 +319,25 @@ __global__ __launch_bounds__(ATTN_THREADS, TYPE == ATTN_F32 && DP == 128 ? 1 : 2
 #pragma unroll
                 for (int t = 0; t < KB; ++t)
 #pragma unroll
-                    for (int n = 0; n < NQ; ++n) s[t][n] = s[t][n] * sp.mul;
-            } else if (sp.cap == CAP_FAST) {
-#pragma unroll
-                for (int t = 0; t < KB; ++t)
-#pragma unroll
                     for (int n = 0; n < NQ; ++n)
 #pragma unroll
-                        for (int r = 0; r < 4; ++r) s[t][n][r] = fmaf(-2.0f * sp.cap2, cap_r(s[t][n][r] * sp.mul2), sp.cap2);
+                        for (int r = 0; r < 4; ++r) s[t][n][r] = TYPE == ATTN_F32 ? s[t][n][r] - w[n] : fmaf(s[t][n][r], sp.mul, -w[n]);
+            } else if (sp.cap == CAP_FAST) {
+#pragma unroll
+                for (int n = 0; n < NQ; ++n) {
+                    const float high = sp.cap2 - w[n];
+#pragma unroll
+                    for (int t = 0; t < KB; ++t)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) s[t][n][r] = fmaf(-2.0f * sp.cap2, cap_r(scaled<TYPE>(s[t][n][r], sp.mul2)), high);
+                }
             } else {
 #pragma unroll
                 for (int t = 0; t < KB; ++t)
 #pragma unroll
                     for (int n = 0; n < NQ; ++n)
 #pragma unroll
-                        for (int r = 0; r < 4; ++r) s[t][n][r] = sp.cap2 * attn_tanh(s[t][n][r] * sp.mul);
+                        for (int r = 0; r < 4; ++r) s[t][n][r] = fmaf(sp.cap2, attn_tanh(scaled<TYPE>(s[t][n][r], sp.mul)), -w[n]);
             }
             if (sp.bias == 1) {
                 const float k0 = (float)(base + 16 * kb + 4 * g);
@@ -379,21 +389,24 @@ __global__ __launch_bounds__(ATTN_THREADS, TYPE == ATTN_F32 && DP == 128 ? 1 : 2
                 for (int t = 0; t < KB; ++t)
 #pragma unroll
                     for (int r = 0; r < 4; ++r) top = fast_max(top, s[t][n][r]);
-                top = fast_max(group_max(top), m[n]);
-                if (__any(top > m[n])) {
-                    const float shift = top == -attn_inf() ? 0.0f : top;
-                    const float f = __builtin_amdgcn_exp2f(m[n] - shift);
+                if (__any(top > rise[n])) {
+                    top = group_max(top);
+                    const bool up = top > rise[n];
+                    const float next = up ? w[n] + top : w[n], by = next - w[n];
+                    const float f = rise[n] == -attn_inf() ? 1.0f : __builtin_amdgcn_exp2f(-by);     // (nothing summed yet: 1)
                     l[n] *= f;
 #pragma unroll
                     for (int d = 0; d < S::dt; ++d) o[n][d] = o[n][d] * f;
-                    m[n] = top;
+                    w[n] = next;
+                    if (up) rise[n] = SOFTMAX_RISE;
+#pragma unroll
+                    for (int t = 0; t < KB; ++t) s[t][n] = s[t][n] - f32x4{by, by, by, by};
                 }
-                const float shift = m[n] == -attn_inf() ? 0.0f : m[n];
 #pragma unroll
                 for (int t = 0; t < KB; ++t)
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
-                        s[t][n][r] = __builtin_amdgcn_exp2f(s[t][n][r] - shift);
+                        s[t][n][r] = __builtin_amdgcn_exp2f(s[t][n][r]);
                         l[n] += s[t][n][r];
                     }
             }
@@ -406,14 +419,13 @@ __global__ __launch_bounds__(ATTN_THREADS, TYPE == ATTN_F32 && DP == 128 ? 1 : 2
     for (int n = 0; n < NQ; ++n) {
         const int i = wrow0 + 16 * n + c;
         const float total = group_sum(l[n]);
-        const float shift = m[n] == -attn_inf() ? 0.0f : m[n];
         if (a.splits > 1) {
             if (i < a.Lq) {
                 float *to = a.part + (((int64_t)bh * a.splits + split) * a.Lq + i) * (a.D + 4);
 #pragma unroll
                 for (int d = 0; d < S::dt; ++d)
                     if (16 * d + 4 * g < a.D) *reinterpret_cast<f32x4 *>(to + 16 * d + 4 * g) = o[n][d];
-                if (g == 0) *reinterpret_cast<f32x2 *>(to + a.D) = f32x2{m[n], total};
+                if (g == 0) *reinterpret_cast<f32x2 *>(to + a.D) = f32x2{rise[n] == -attn_inf() ? -attn_inf() : w[n], total};
             }
             continue;
         }
@@ -427,7 +439,7 @@ __global__ __launch_bounds__(ATTN_THREADS, TYPE == ATTN_F32 && DP == 128 ? 1 : 2
             for (int d = 0; d < S::dt; ++d)
                 if (16 * d + 4 * g < a.D) store_out4<TYPE>(a, out + 16 * d, o[n][d] * inv);
             if (a.lse != nullptr && g == 0)
-                a.lse[((int64_t)b * a.Hq + h) * a.Lq + i] = total == 0.0f ? -attn_inf() : (shift + __builtin_amdgcn_logf(total)) * ATTN_LN2;
+                a.lse[((int64_t)b * a.Hq + h) * a.Lq + i] = total == 0.0f ? -attn_inf() : (w[n] + __builtin_amdgcn_logf(total)) * ATTN_LN2;
         }
         unsigned long long bad = __ballot(!fine && i < a.Lq);
         bad = (bad | bad >> 16 | bad >> 32 | bad >> 48) & 0xffff;
@@ -475,7 +487,7 @@ template <int TYPE> __global__ __launch_bounds__(ATTN_THREADS) void attn_fwd_joi
 //   out  s = p,  dp = ds = p (dp - delta)
 // slack is 1 - tanh^2 = 4 (r - r^2) without its 4 (undo_factor).  FOLD: it goes into dp (which then ends as du); else it is
 // returned, undefined without a cap (the slope's gradient needs ds itself).
-template <int N, bool FOLD>
+template <int TYPE, int N, bool FOLD>
 __device__ __forceinline__ void pair_probability(const ScoreParams &sp, f32x4 (&s)[2][N], f32x4 (&dp)[2][N], f32x4 (&slack)[2][N],
                                                  const f32x4 (&dist)[2][N], const f32x4 (&e)[2][N]) {
     if (sp.cap == CAP_NONE) {
@@ -485,7 +497,7 @@ __device__ __forceinline__ void pair_probability(const ScoreParams &sp, f32x4 (&
             for (int n = 0; n < N; ++n) {
                 f32x4 x = s[t][n];
 #pragma unroll
-                for (int r = 0; r < 4; ++r) x[r] = fmaf(x[r], sp.mul, -e[t][n][r]);
+                for (int r = 0; r < 4; ++r) x[r] = TYPE == ATTN_F32 ? x[r] - e[t][n][r] : fmaf(x[r], sp.mul, -e[t][n][r]);
                 s[t][n] = x;
             }
     } else if (sp.cap == CAP_FAST) {
@@ -496,7 +508,7 @@ __device__ __forceinline__ void pair_probability(const ScoreParams &sp, f32x4 (&
                 f32x4 x = s[t][n], k = x;
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
-                    const float y = cap_r(x[r] * sp.mul2);
+                    const float y = cap_r(scaled<TYPE>(x[r], sp.mul2));
                     x[r] = fmaf(-2.0f * sp.cap2, y, sp.cap2 - e[t][n][r]);
                     k[r] = fmaf(-y, y, y);
                 }
@@ -512,7 +524,7 @@ __device__ __forceinline__ void pair_probability(const ScoreParams &sp, f32x4 (&
                 f32x4 x = s[t][n], k = x;
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
-                    const float th = attn_tanh(x[r] * sp.mul);
+                    const float th = attn_tanh(scaled<TYPE>(x[r], sp.mul));
                     x[r] = fmaf(sp.cap2, th, -e[t][n][r]);
                     k[r] = 0.25f * fmaf(-th, th, 1.0f);
                 }
@@ -648,7 +660,7 @@ __global__ __launch_bounds__(ATTN_THREADS, DP <= 64 ? 2 : 1) void attn_bwd_q_ker
                 for (int e = 0; e < 8; ++e) dot = fmaf(eight_at<TYPE>(g8[k8], e), eight_at<TYPE>(r8, e), dot);
             }
         }
-        col_frag<TYPE, DP>(qf[n], q8, g);
+        col_frag<TYPE, DP>(qf[n], q8, g, score_factor(sp));
         col_frag<TYPE, DP>(of[n], g8, g);
         delta[n] = group_sum(dot);
         const int64_t at = ((int64_t)b * a.Hq + h) * a.Lq + i;
@@ -746,7 +758,7 @@ __global__ __launch_bounds__(ATTN_THREADS, DP <= 64 ? 2 : 1) void attn_bwd_q_ker
             f32x4 e[2][NQ];
 #pragma unroll
             for (int n = 0; n < NQ; ++n) e[0][n] = e[1][n] = f32x4{lse2[n], lse2[n], lse2[n], lse2[n]};
-            pair_probability<NQ, false>(sp, s, dp, slack, dist, e);
+            pair_probability<TYPE, NQ, false>(sp, s, dp, slack, dist, e);
             if (masked) {
 #pragma unroll
                 for (int t = 0; t < 2; ++t) {
@@ -928,6 +940,7 @@ __global__ __launch_bounds__(ATTN_THREADS, DP <= 64 ? 2 : 1) void attn_bwd_kv_ke
         build_tile_map(map_store, a.doc_k + b * a.dks, row0, ROWS, a.Lk, docs, a.Lq);
     }
 
+    const float factor = score_factor(score_params(a.scale, a.cap, 0, nullptr, 0));      // (the same for all heads)
     ColFrag<TYPE, DP> kf[NK], vf[NK];
     f32x4 dk[NK][S::dt], dv[NK][S::dt];
     float kx[NK], ky[NK];
@@ -943,7 +956,7 @@ __global__ __launch_bounds__(ATTN_THREADS, DP <= 64 ? 2 : 1) void attn_bwd_kv_ke
             k8[x] = load_eight<TYPE>(k + (int64_t)j * a.ks[2], d, live && d < a.D);
             v8[x] = load_eight<TYPE>(v + (int64_t)j * a.vs[2], d, live && d < a.D);
         }
-        col_frag<TYPE, DP>(kf[n], k8, g);
+        col_frag<TYPE, DP>(kf[n], k8, g, factor);
         col_frag<TYPE, DP>(vf[n], v8, g);
         doc[n] = map != nullptr ? doc_of_key(a, b, j) : 0;
         kx[n] = ky[n] = 0.0f;
@@ -1069,7 +1082,7 @@ __global__ __launch_bounds__(ATTN_THREADS, DP <= 64 ? 2 : 1) void attn_bwd_kv_ke
                         }
                     }
                 }
-                pair_probability<NK, true>(sp, s, dp, slack, dist, e);
+                pair_probability<TYPE, NK, true>(sp, s, dp, slack, dist, e);
                 if (masked) {
 #pragma unroll
                     for (int t = 0; t < 2; ++t) {

@@ -149,6 +149,11 @@ template <int TYPE> __device__ __forceinline__ f32x4 mfma32(u32x4 a, u32x4 b, f3
         return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), acc, 0, 0, 0);
 }
 
+// Binary32 operands are split into terms when they are loaded: the score's factor goes into the one that stays in registers
+// (one more rounding of 2^-24 per element, as the split's own), and scaled() leaves the products as they are.
+__device__ __forceinline__ float score_factor(const ScoreParams &p) { return p.cap == CAP_FAST ? p.mul2 : p.mul; }
+template <int TYPE> __device__ __forceinline__ float scaled(float dot, float factor) { return TYPE == ATTN_F32 ? dot : dot * factor; }
+
 // ---- binary32 operands as three bfloat16 terms ----------------------------------------------------------------------
 // x = hi + mid + lo exactly (8 significand bits each, by truncation); a product is hh + hm + mh + hl + lh + mm, what is left
 // out is below 2^-23 of it.  Six bfloat16 products of 17 cycles replace eight binary32 ones of 32 per 16 x 16 x 32 block -
@@ -235,7 +240,8 @@ template <int TYPE> __device__ __forceinline__ float eight_at(const Eight<TYPE> 
 template <int DP> __device__ __forceinline__ int frag_d(int k, int g) { return DP < 32 ? 8 * (g & 1) : 32 * k + 8 * g; }
 template <int DP> __device__ __forceinline__ bool frag_counts(int g) { return DP >= 32 || g < 2; }
 
-template <int TYPE, int DP> __device__ __forceinline__ void col_frag(ColFrag<TYPE, DP> &f, const Eight<TYPE> (&x)[Shape<TYPE, DP>::chunks], int g) {
+// (`factor` only for binary32 operands: score_factor)
+template <int TYPE, int DP> __device__ __forceinline__ void col_frag(ColFrag<TYPE, DP> &f, const Eight<TYPE> (&x)[Shape<TYPE, DP>::chunks], int g, float factor = 1.0f) {
     typedef Shape<TYPE, DP> S;
 #pragma unroll
     for (int k = 0; k < S::chunks; ++k) {
@@ -246,7 +252,7 @@ template <int TYPE, int DP> __device__ __forceinline__ void col_frag(ColFrag<TYP
             u32x4 t[3];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const Split3 a = split3(eight_at<TYPE>(x[k], 2 * i)), b = split3(eight_at<TYPE>(x[k], 2 * i + 1));
+                const Split3 a = split3(factor * eight_at<TYPE>(x[k], 2 * i)), b = split3(factor * eight_at<TYPE>(x[k], 2 * i + 1));
                 t[0][i] = pack_upper(a.hi, b.hi);
                 t[1][i] = pack_upper(a.mid, b.mid);
                 t[2][i] = pack_upper(a.lo, b.lo);
