@@ -32,7 +32,6 @@ struct LogitsArgs {
     int cols;
     const float *rep, *pres, *freq;
     float rep_all, pres_all, freq_all, temperature, inv_temperature;
-    int bits_together;                // V neighbouring actions share a word of bits
     float *out;
     int64_t os;
     int *selected;
@@ -111,12 +110,58 @@ template <int THREADS> __device__ __forceinline__ void count_history(const Count
     __syncthreads();
 }
 
+// Blocked bits in LDS, one per action from `first` on, whatever the period: 32 of them are gathered from two neighbouring words
+// (more only where the period ends among them).  The first ones are requested before the logits.  (Words read from memory for each
+// thread's actions, after the logits: 22 us in place of 16 at 512 x 20002 with odd periods, where two words were needed per action.)
+struct Window {
+    unsigned bit, lo, hi;
+};
+__device__ __forceinline__ unsigned bits_at(const LogitsArgs &a, const unsigned *bits, int i) { return i < a.halves ? bits[i] : 0u; }
+__device__ __forceinline__ Window request_bits(const LogitsArgs &a, int r, int first, int n, int w) {
+    Window x = {0, 0, 0};
+    if (32 * w >= n) return x;
+    const unsigned *bits = a.blocked + r * a.bs;
+    x.bit = bit_of(a, (unsigned)(first + 32 * w));
+    x.lo = bits_at(a, bits, (int)(x.bit >> 5));
+    x.hi = bits_at(a, bits, (int)(x.bit >> 5) + 1);
+    return x;
+}
+__device__ __forceinline__ unsigned gather_bits(const LogitsArgs &a, int r, const Window &x) {
+    unsigned v = __builtin_amdgcn_alignbit(x.hi, x.lo, x.bit & 31), filled = (unsigned)a.period - x.bit;
+    const unsigned *bits = a.blocked + r * a.bs;
+    while (filled < 32) {                        // the period starts again
+        v &= (1u << filled) - 1;
+        const unsigned next = __builtin_amdgcn_alignbit(bits_at(a, bits, 1), bits_at(a, bits, 0), 0);
+        v |= next << filled;
+        filled += min((unsigned)a.period, 32u);
+    }
+    return v;
+}
+
 __device__ __forceinline__ float shifted_exp(float x, float shift) { return __builtin_amdgcn_exp2f((x - shift) * 1.4426950408889634f); }
 
-// maximum / lowest index / sum over the workgroup, in every thread; `slots` of each are their own
+// Exchanges inside a wave by lane permutations of the vector unit: a shuffle takes the LDS pipe, and 18 of them per wave took
+// 2 of 54 us at 256 x 131072 bf16 without controls.
+template <int CTRL> __device__ __forceinline__ float permuted(float x) {
+    return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), CTRL, 0xf, 0xf, true));
+}
+#define DPP_SWAP_1 0xb1            // quad_perm(1, 0, 3, 2)
+#define DPP_SWAP_2 0x4e            // quad_perm(2, 3, 0, 1)
+#define DPP_HALF_MIRROR 0x141
+#define DPP_MIRROR 0x140
+template <typename F> __device__ __forceinline__ float wave_reduce(float x, F f) {
+    x = f(x, permuted<DPP_SWAP_1>(x));
+    x = f(x, permuted<DPP_SWAP_2>(x));
+    x = f(x, permuted<DPP_HALF_MIRROR>(x));
+    x = f(x, permuted<DPP_MIRROR>(x));
+    auto p = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    x = f(__uint_as_float(p[0]), __uint_as_float(p[1]));
+    p = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return f(__uint_as_float(p[0]), __uint_as_float(p[1]));
+}
+// maximum / sum over the workgroup, in every thread; `slots` of each are their own
 template <int THREADS> __device__ __forceinline__ float block_max(float v, float *slots, int tid) {
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) v = fmaxf(v, __shfl_xor(v, d));
+    v = wave_reduce(v, [](float x, float y) { return fmaxf(x, y); });
     if constexpr (THREADS > 64) {
         if ((tid & 63) == 0) slots[tid >> 6] = v;
         __syncthreads();
@@ -126,27 +171,15 @@ template <int THREADS> __device__ __forceinline__ float block_max(float v, float
     }
     return v;
 }
-// sum and lowest index together: one exchange
-template <int THREADS> __device__ __forceinline__ void block_sum_index(float &v, int &index, float *slots, int *index_slots, int tid) {
+// The sum, and the lowest of the indexes that threads have put into *index before (behind a barrier that set it to INT_MAX)
+template <int THREADS> __device__ __forceinline__ float block_sum(float v, float *slots, int tid) {
+    v = wave_reduce(v, [](float x, float y) { return x + y; });
+    if ((tid & 63) == 0) slots[tid >> 6] = v;
+    __syncthreads();
+    v = 0.0f;
 #pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        v += __shfl_xor(v, d);
-        index = min(index, __shfl_xor(index, d));
-    }
-    if constexpr (THREADS > 64) {
-        if ((tid & 63) == 0) {
-            slots[tid >> 6] = v;
-            index_slots[tid >> 6] = index;
-        }
-        __syncthreads();
-        v = 0.0f;
-        index = INT_MAX;
-#pragma unroll
-        for (int w = 0; w < THREADS / 64; ++w) {
-            v += slots[w];
-            index = min(index, index_slots[w]);
-        }
-    }
+    for (int w = 0; w < THREADS / 64; ++w) v += slots[w];
+    return v;
 }
 
 // Values of chunks tid, tid + THREADS, ... of V actions each from action `first` on, at most N chunks; dead places are -inf.
@@ -154,8 +187,11 @@ template <int THREADS> __device__ __forceinline__ void block_sum_index(float &v,
 // per control around all of a thread's values; every operation rounds once, as the header writes it.  Selections are bit
 // operations on masks: a comparison into a scalar register and a v_cndmask from it cost five times as much here.
 template <int TYPE, int THREADS, int N, int V>
-__device__ __forceinline__ float load_values(float (&x)[N][V], const LogitsArgs &a, int r, int first, int n, unsigned *count_words, int tid) {
+__device__ __forceinline__ float load_values(float (&x)[N][V], const LogitsArgs &a, int r, int first, int n, unsigned *words, int tid) {
     typedef typename LogitElem<TYPE>::raw raw;
+    unsigned *blocked_words = words, *count_words = words + (a.blocked != nullptr ? (n + 31) / 32 : 0);
+    Window window = {0, 0, 0};
+    if (a.blocked != nullptr) window = request_bits(a, r, first, n, tid);
     const raw *row = reinterpret_cast<const raw *>(a.logits) + r * a.ls + first;
 #pragma unroll
     for (int k = 0; k < N; ++k) {
@@ -164,6 +200,11 @@ __device__ __forceinline__ float load_values(float (&x)[N][V], const LogitsArgs 
         else
 #pragma unroll
             for (int e = 0; e < V; ++e) x[k][e] = -__builtin_inff();
+    }
+    if (a.blocked != nullptr) {
+        if (32 * tid < n) blocked_words[tid] = gather_bits(a, r, window);
+        for (int w = tid + THREADS; 32 * w < n; w += THREADS) blocked_words[w] = gather_bits(a, r, request_bits(a, r, first, n, w));
+        if (a.history == nullptr) __syncthreads();
     }
     if (a.history != nullptr) {
         const Counts count = {count_words, a.cols < 65536};
@@ -224,20 +265,13 @@ __device__ __forceinline__ float load_values(float (&x)[N][V], const LogitsArgs 
         }
     }
     if (a.blocked != nullptr) {
-        const unsigned *bits = a.blocked + r * a.bs;
 #pragma unroll
         for (int k = 0; k < N; ++k) {
             const int at = (k * THREADS + tid) * V;
             if (at >= n) continue;
-            // V actions share a word where V divides the period (they start at a multiple of V)
-            const unsigned bit = bit_of(a, (unsigned)(first + at));
-            unsigned word = (int)(bit >> 5) < a.halves ? bits[bit >> 5] >> (bit & 31) : 0u;
+            const unsigned word = blocked_words[at >> 5] >> (at & 31);       // (V divides 32)
 #pragma unroll
             for (int e = 0; e < V; ++e) {
-                if (V > 1 && !a.bits_together && e > 0) {
-                    const unsigned one = bit_of(a, (unsigned)(first + at + e));
-                    word = ((int)(one >> 5) < a.halves ? bits[one >> 5] >> (one & 31) : 0u) << e;
-                }
                 const unsigned mask = (unsigned)((int)(word << (31 - e)) >> 31);
                 x[k][e] = __uint_as_float((__float_as_uint(x[k][e]) & ~mask) | (0xff800000u & mask));
             }
@@ -283,21 +317,21 @@ __device__ __forceinline__ void store_values(const float (&x)[N][V], float lse, 
 
 // one workgroup per row, the row in registers
 template <int TYPE, int THREADS, int N, int V> __global__ __launch_bounds__(THREADS) void logits_row_kernel(LogitsArgs a) {
-    extern __shared__ unsigned count_words[];
+    extern __shared__ unsigned words[];
     __shared__ float max_slots[THREADS / 64], sum_slots[THREADS / 64];
-    __shared__ int index_slots[THREADS / 64];
+    __shared__ int index;
     const int r = blockIdx.x, tid = threadIdx.x;
     float x[N][V];
-    const float own = load_values<TYPE, THREADS, N, V>(x, a, r, 0, a.A, count_words, tid);
+    if (tid == 0) index = INT_MAX;
+    const float own = load_values<TYPE, THREADS, N, V>(x, a, r, 0, a.A, words, tid);
     const float top = block_max<THREADS>(own, max_slots, tid), shift = top == -__builtin_inff() ? 0.0f : top;
-    int index = INT_MAX;
-    if (own == top && top != -__builtin_inff()) index = lowest_index<THREADS, N, V>(x, top, 0, tid);
+    if (own == top && top != -__builtin_inff()) atomicMin(&index, lowest_index<THREADS, N, V>(x, top, 0, tid));
     float sum = 0.0f;
 #pragma unroll
     for (int k = 0; k < N; ++k)
 #pragma unroll
         for (int e = 0; e < V; ++e) sum += shifted_exp(x[k][e], shift);
-    block_sum_index<THREADS>(sum, index, sum_slots, index_slots, tid);
+    sum = block_sum<THREADS>(sum, sum_slots, tid);
     if (a.selected != nullptr && tid == 0) a.selected[r] = index == INT_MAX ? -1 : index;
     if (a.out != nullptr) store_values<THREADS, N, V>(x, top == -__builtin_inff() ? 0.0f : shift + logf(sum), a.out + r * a.os, a.A, tid);
 }
@@ -305,12 +339,13 @@ template <int TYPE, int THREADS, int N, int V> __global__ __launch_bounds__(THRE
 // long rows: one workgroup per tile; WRITE = second launch
 template <int TYPE, int V, bool WRITE> __global__ __launch_bounds__(LOGITS_TILE_THREADS) void logits_tile_kernel(LogitsArgs a) {
     constexpr int THREADS = LOGITS_TILE_THREADS, N = LOGITS_TILE / THREADS / V;
-    extern __shared__ unsigned count_words[];
+    extern __shared__ unsigned words[];
     __shared__ float max_slots[THREADS / 64], sum_slots[THREADS / 64];
-    __shared__ int index_slots[THREADS / 64];
+    __shared__ int index;
     const int r = blockIdx.x / a.tiles, t = blockIdx.x % a.tiles, tid = threadIdx.x;
     const int first = t * LOGITS_TILE, n = min(LOGITS_TILE, a.A - first);
     float x[N][V];
+    if (tid == 0) index = INT_MAX;
     if constexpr (WRITE) {
         // the row's maximum and sum from its tiles', in a fixed order
         const float *p = a.part + (int64_t)r * a.tiles * 4;
@@ -319,29 +354,27 @@ template <int TYPE, int V, bool WRITE> __global__ __launch_bounds__(LOGITS_TILE_
         top = block_max<THREADS>(top, max_slots, tid);
         const float shift = top == -__builtin_inff() ? 0.0f : top;
         float sum = 0.0f;
-        int index = INT_MAX;
         for (int i = tid; i < a.tiles; i += THREADS) {
             const float m = p[4 * i];
             sum = fmaf(p[4 * i + 1], m == -__builtin_inff() ? 1.0f : shifted_exp(m, shift), sum);
-            if (m == top) index = min(index, __float_as_int(p[4 * i + 2]));
+            if (m == top) atomicMin(&index, __float_as_int(p[4 * i + 2]));
         }
-        block_sum_index<THREADS>(sum, index, sum_slots, index_slots, tid);
+        sum = block_sum<THREADS>(sum, sum_slots, tid);
         const float lse = top == -__builtin_inff() ? 0.0f : shift + logf(sum);
         if (a.selected != nullptr && t == 0 && tid == 0) a.selected[r] = index == INT_MAX ? -1 : index;
         if (a.out == nullptr) return;
-        load_values<TYPE, THREADS, N, V>(x, a, r, first, n, count_words, tid);
+        load_values<TYPE, THREADS, N, V>(x, a, r, first, n, words, tid);
         store_values<THREADS, N, V>(x, lse, a.out + r * a.os + first, n, tid);
     } else {
-        const float own = load_values<TYPE, THREADS, N, V>(x, a, r, first, n, count_words, tid);
+        const float own = load_values<TYPE, THREADS, N, V>(x, a, r, first, n, words, tid);
         const float top = block_max<THREADS>(own, max_slots, tid), shift = top == -__builtin_inff() ? 0.0f : top;
-        int index = INT_MAX;
-        if (own == top && top != -__builtin_inff()) index = lowest_index<THREADS, N, V>(x, top, first, tid);
+        if (own == top && top != -__builtin_inff()) atomicMin(&index, lowest_index<THREADS, N, V>(x, top, first, tid));
         float sum = 0.0f;
 #pragma unroll
         for (int k = 0; k < N; ++k)
 #pragma unroll
             for (int e = 0; e < V; ++e) sum += shifted_exp(x[k][e], shift);
-        block_sum_index<THREADS>(sum, index, sum_slots, index_slots, tid);
+        sum = block_sum<THREADS>(sum, sum_slots, tid);
         if (tid == 0) {
             float *p = a.part + ((int64_t)r * a.tiles + t) * 4;
             p[0] = top;
@@ -367,10 +400,13 @@ int check_logits(const dgl_logits_t *p) {
 #define LOGITS_ROW_MAX 24576           // 512 threads x 48 values
 bool in_tiles(const dgl_logits_t *p) { return p->A > LOGITS_ROW_MAX; }
 
-int count_bytes(const LogitsArgs &a, int n) { return a.history == nullptr ? 0 : a.cols < 65536 ? (n + 1) / 2 * 4 : n * 4; }
+// LDS of n actions: blocked bits, then counters
+int word_bytes(const LogitsArgs &a, int n) {
+    return (a.blocked == nullptr ? 0 : (n + 31) / 32 * 4) + (a.history == nullptr ? 0 : a.cols < 65536 ? (n + 1) / 2 * 4 : n * 4);
+}
 template <int TYPE, int THREADS, int N, int V> void launch_row(const LogitsArgs &a, hipStream_t s) {
-    const int lds = count_bytes(a, a.A);
-    if (lds > 48 * 1024) dgl_max_dynamic_lds(reinterpret_cast<const void *>(&logits_row_kernel<TYPE, THREADS, N, V>), LOGITS_ROW_MAX * 4);
+    const int lds = word_bytes(a, a.A);
+    if (lds > 48 * 1024) dgl_max_dynamic_lds(reinterpret_cast<const void *>(&logits_row_kernel<TYPE, THREADS, N, V>), LOGITS_ROW_MAX * 4 + LOGITS_ROW_MAX / 8);
     hipLaunchKernelGGL((logits_row_kernel<TYPE, THREADS, N, V>), dim3(a.R), dim3(THREADS), lds, s, a);
 }
 // The smallest workgroup that holds a row at 4 to 48 values a thread; several share a compute unit, so that one row's loads
@@ -383,7 +419,7 @@ template <int TYPE, int V> int launch_logits(const LogitsArgs &a, hipStream_t s)
     else if (a.A <= 16384) launch_row<TYPE, 512, 32 / V, V>(a, s);
     else if (a.A <= LOGITS_ROW_MAX) launch_row<TYPE, 512, 48 / V, V>(a, s);
     else {
-        const int lds = count_bytes(a, LOGITS_TILE);
+        const int lds = word_bytes(a, LOGITS_TILE);
         const dim3 grid((unsigned)((int64_t)a.R * a.tiles));
         hipLaunchKernelGGL((logits_tile_kernel<TYPE, V, false>), grid, dim3(LOGITS_TILE_THREADS), lds, s, a);
         DGL_CHECK_LAUNCH("dgl_logits_process (statistics)");
@@ -425,7 +461,6 @@ extern "C" int dgl_logits_process(const dgl_logits_t *p, float *ws, dgl_stream_t
                (reinterpret_cast<uintptr_t>(p->logits) & (v * bytes - 1)) == 0 && (reinterpret_cast<uintptr_t>(p->log_probs) & (4 * v - 1)) == 0;
     };
     const int v = fits(4) ? 4 : fits(2) ? 2 : 1;
-    a.bits_together = a.period % v == 0;
     hipStream_t s = (hipStream_t)stream;
 #define LOGITS_CASE(T) \
     if (p->dtype == T) return v == 4 ? launch_logits<T, 4>(a, s) : v == 2 ? launch_logits<T, 2>(a, s) : launch_logits<T, 1>(a, s);

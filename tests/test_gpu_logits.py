@@ -201,3 +201,15 @@ def test_refusals(device):
     with pytest.raises(ValueError):
         process_logits(x.cpu())
     assert process_logits(x[:0])[0].shape == (0, 10)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("A,period", [(70, 7), (33, 33), (96, 3), (4095, 45), (24570, 819), (24576, 24576), (40000, 10000), (49149, 16383)])
+def test_bits_of_any_period(device, dtype, A, period):
+    """Periods that end inside a word, in the middle of a tile, and several times within 32 actions; bits beyond the words
+    that are given are clear; with a history beside them."""
+    x, g = rnd(4, A, TYPES[dtype], A + period)
+    blocked = words(4, period, g)
+    check(x, blocked=blocked, period=period)
+    hist = torch.randint(0, A, (4, 70), device=device, generator=g).to(torch.int32)
+    check(x, blocked=blocked[:, : max(1, blocked.shape[1] // 2)], period=period, history=hist, presence=0.5, frequency=0.25)
