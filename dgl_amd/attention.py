@@ -27,17 +27,20 @@ _VEC = {torch.float32: 4, torch.float16: 8, torch.bfloat16: 8}      # elements o
 # packed in one go (the formats restate include/dgl_amd.h; a wrong size fails here, at import).
 _PACK_ATTENTION = struct.Struct("@8i2f12q5P3P2q2P2q2P")
 _PACK_GRAD = struct.Struct("@4P12qP")
+_PACK_CACHE = struct.Struct("@7i7q4P")
 _PACK_STEP = struct.Struct("@2i2f4q6Pq2iPq")
 _STEP_AT = _lib.AttentionStep.rows_per_instance.offset
 assert _PACK_ATTENTION.size == ctypes.sizeof(_lib.Attention) and _PACK_GRAD.size == ctypes.sizeof(_lib.AttentionGrad)
+assert _PACK_CACHE.size == ctypes.sizeof(_lib.KVCache)
 assert _STEP_AT == ctypes.sizeof(_lib.KVCache) and _STEP_AT + _PACK_STEP.size == ctypes.sizeof(_lib.AttentionStep)
 _raw_stream = torch._C._cuda_getCurrentRawStream
+_current_device = torch._C._cuda_getDevice
 
 
 def _launch(device, function, *args, what: str) -> None:
     """An entry point on the device's current stream, with that device current."""
     index = device.index
-    if index == torch.cuda.current_device():
+    if index == _current_device():              # (a tensor on the device is there: nothing is left to initialise)
         code = function(*args, _raw_stream(index))
     else:
         with torch.cuda.device(index):
@@ -315,11 +318,10 @@ class PagedCache:
         self.device, self.dtype = dev, k_pages.dtype
         self.page_size, self.batch = k_pages.shape[2], table.shape[0]
         c = self.struct = _lib.KVCache()
-        c.dtype, c.B, c.Hkv, c.D = _DTYPES[self.dtype], self.batch, k_pages.shape[1], k_pages.shape[3]
-        c.page_size, c.max_pages, c.num_pages = self.page_size, table.shape[1], k_pages.shape[0]
-        c.k_stride = (ctypes.c_int64 * 3)(*k_pages.stride()[:3])
-        c.v_stride, c.table_stride = (ctypes.c_int64 * 3)(*v_pages.stride()[:3]), table.stride(0)
-        c.k_pages, c.v_pages, c.table, c.lengths = ptr(k_pages), ptr(v_pages), ptr(table), ptr(lengths)
+        pages, heads, page_size, size = k_pages.shape
+        _PACK_CACHE.pack_into(c, 0, _DTYPES[self.dtype], self.batch, heads, size, page_size, table.shape[1], pages,
+                              *k_pages.stride()[:3], *v_pages.stride()[:3], table.stride(0), k_pages.data_ptr(),
+                              v_pages.data_ptr(), table.data_ptr(), lengths.data_ptr())
 
     # ---- pages of a pool ------------------------------------------------------------------
     def _pool(self):
@@ -376,43 +378,42 @@ def attention_step(q: torch.Tensor, cache: PagedCache, *, rows_per_instance: int
     rows_per_instance).  ``cap`` / ``slope`` as in ``attention``; coordinates ``pos_q`` [R, 2] and ``pos_k`` [batch, n, 2]
     (n at least the live lengths), or, without them, the distance lengths[b] - 1 - j.  ``blocked`` int64 [R, words]: bit j of
     word j // 64 set = key j is not seen, as the states' visited words.  A row that sees nothing is zeros (lse -inf)."""
-    with torch.no_grad():
-        c, dev = cache.struct, cache.device
-        if q.dim() != 3 or q.shape[0] != cache.batch * rows_per_instance or q.shape[2] != c.D or q.shape[1] % c.Hkv or q.shape[1] < 1:
-            raise ValueError(f"q has shape {tuple(q.shape)}: expected [{cache.batch} x {rows_per_instance}, a multiple of {c.Hkv}, {c.D}]")
-        if q.dtype != cache.dtype or q.device != dev:
-            raise ValueError(f"q is {q.dtype} on {q.device}, the cache {cache.dtype} on {dev}")
-        if (pos_q is None) != (pos_k is None) or (pos_q is not None and slope is None):
-            raise ValueError("coordinates are given for both sides and with a slope")
-        q = _usable(q)
-        R, H, D = q.shape
-        out = torch.empty(R, H, D, dtype=q.dtype, device=dev)
-        lse = torch.empty(R, H, dtype=torch.float32, device=dev) if return_lse else None
-        slope = _side(slope, "slope", (H,), torch.float32, dev)
-        n = pos_stride = words = bits_stride = 0
-        if pos_q is not None:
-            pos_q = _side(pos_q, "pos_q", (R, 2), torch.float32, dev)
-            if pos_q.stride(0) != 2:             # rows of one wide tensor, or one row for all
-                pos_q = pos_q.clone(memory_format=torch.contiguous_format)
-            n = pos_k.shape[1] if pos_k.dim() == 3 else -1
-            pos_k = _side(pos_k, "pos_k", (cache.batch, n, 2), torch.float32, dev)
-            if pos_k.data_ptr() % 8 or pos_k.stride(0) % 2:
-                pos_k = pos_k.clone(memory_format=torch.contiguous_format)
-            pos_stride = pos_k.stride(0)
-        if blocked is not None:
-            if blocked.dim() != 2 or blocked.shape[0] != R or blocked.dtype != torch.int64 or blocked.device != dev:
-                raise ValueError(f"blocked is {tuple(blocked.shape)} {blocked.dtype}: int64 words [{R}, n] on {dev} are expected")
-            words = blocked.shape[1]
-            if words > 1 and blocked.stride(1) != 1:
-                blocked = blocked.contiguous()
-            bits_stride = blocked.stride(0)
-        a = _lib.AttentionStep()
-        a.cache = c
-        _PACK_STEP.pack_into(a, _STEP_AT, rows_per_instance, H, D ** -0.5 if scale is None else float(scale), float(cap),
-                             *q.stride()[:2], H * D, D, q.data_ptr(), out.data_ptr(), ptr(lse), ptr(slope), ptr(pos_q),
-                             ptr(pos_k), pos_stride, n, words, ptr(blocked), bits_stride)
-        lib, ref = _lib.load(), ctypes.byref(a)
-        need = lib.dgl_attention_step_workspace_floats(ref)
-        ws = torch.empty(need, dtype=torch.float32, device=dev) if need > 0 else None
-        _launch(dev, lib.dgl_attention_step, ref, ptr(ws), what="dgl_attention_step")
-        return (out, lse) if return_lse else out
+    c, dev = cache.struct, cache.device
+    if q.dim() != 3 or q.shape[0] != cache.batch * rows_per_instance or q.shape[2] != c.D or q.shape[1] % c.Hkv or q.shape[1] < 1:
+        raise ValueError(f"q has shape {tuple(q.shape)}: expected [{cache.batch} x {rows_per_instance}, a multiple of {c.Hkv}, {c.D}]")
+    if q.dtype != cache.dtype or q.device != dev:
+        raise ValueError(f"q is {q.dtype} on {q.device}, the cache {cache.dtype} on {dev}")
+    if (pos_q is None) != (pos_k is None) or (pos_q is not None and slope is None):
+        raise ValueError("coordinates are given for both sides and with a slope")
+    q = _usable(q)
+    R, H, D = q.shape
+    out = torch.empty(R, H, D, dtype=q.dtype, device=dev)
+    lse = torch.empty(R, H, dtype=torch.float32, device=dev) if return_lse else None
+    slope = _side(slope, "slope", (H,), torch.float32, dev)
+    n = pos_stride = words = bits_stride = 0
+    if pos_q is not None:
+        pos_q = _side(pos_q, "pos_q", (R, 2), torch.float32, dev)
+        if pos_q.stride(0) != 2:             # rows of one wide tensor, or one row for all
+            pos_q = pos_q.clone(memory_format=torch.contiguous_format)
+        n = pos_k.shape[1] if pos_k.dim() == 3 else -1
+        pos_k = _side(pos_k, "pos_k", (cache.batch, n, 2), torch.float32, dev)
+        if pos_k.data_ptr() % 8 or pos_k.stride(0) % 2:
+            pos_k = pos_k.clone(memory_format=torch.contiguous_format)
+        pos_stride = pos_k.stride(0)
+    if blocked is not None:
+        if blocked.dim() != 2 or blocked.shape[0] != R or blocked.dtype != torch.int64 or blocked.device != dev:
+            raise ValueError(f"blocked is {tuple(blocked.shape)} {blocked.dtype}: int64 words [{R}, n] on {dev} are expected")
+        words = blocked.shape[1]
+        if words > 1 and blocked.stride(1) != 1:
+            blocked = blocked.contiguous()
+        bits_stride = blocked.stride(0)
+    a = _lib.AttentionStep()
+    a.cache = c
+    _PACK_STEP.pack_into(a, _STEP_AT, rows_per_instance, H, D ** -0.5 if scale is None else float(scale), float(cap),
+                         *q.stride()[:2], H * D, D, q.data_ptr(), out.data_ptr(), ptr(lse), ptr(slope), ptr(pos_q),
+                         ptr(pos_k), pos_stride, n, words, ptr(blocked), bits_stride)
+    lib, ref = _lib.load(), ctypes.byref(a)
+    need = lib.dgl_attention_step_workspace_floats(ref)
+    ws = torch.empty(need, dtype=torch.float32, device=dev) if need > 0 else None
+    _launch(dev, lib.dgl_attention_step, ref, ptr(ws), what="dgl_attention_step")
+    return (out, lse) if return_lse else out

@@ -242,7 +242,10 @@ __global__ __launch_bounds__(64 * STEP_WAVES) void attn_step_kernel(StepArgs a) 
     if (work >= a.B * a.Hkv * a.splits * a.chunks) return;
     const int chunk = work % a.chunks, split = work / a.chunks % a.splits, bh = work / (a.chunks * a.splits);
     const int b = bh / a.Hkv, hk = bh % a.Hkv;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g = lane >> 4, c = lane & 15;
+    const int tid = threadIdx.x, lane = tid & 63, g = lane >> 4, c = lane & 15;
+    // (in a scalar register, so that the pages are looked up by scalar loads: a vector load among the tiles' would be waited for
+    // with all the loads before it)
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int n_keys = live_length(a, b);
     const int tiles = (n_keys + STEP_TILE - 1) / STEP_TILE, per = (tiles + a.splits - 1) / a.splits;
     const int end = min(tiles, (split + 1) * per);
@@ -496,7 +499,8 @@ template <int TYPE> __global__ __launch_bounds__(256) void attn_step_join_kernel
     for (int x = 1; x < 64; x <<= 1) top = fmaxf(top, __shfl_xor(top, x));
     const float shift = top == -attn_inf() ? 0.0f : top;
     float total = 0.0f, acc0 = 0.0f, acc1 = 0.0f;
-    for (int s = 0; s < a.splits; ++s) {
+#pragma unroll 8
+    for (int s = 0; s < a.splits; ++s) {             // (unrolled: the ranges' loads are in flight together)
         const float *x = from + s * stride;
         const float f = __builtin_amdgcn_exp2f(x[a.D] - shift);
         total = fmaf(x[a.D + 1], f, total);

@@ -51,51 +51,50 @@ def process_logits(logits: torch.Tensor, *, blocked: Optional[torch.Tensor] = No
     where bit (a mod ``period``) of ``blocked`` [R, words] is set (``period``: default A; CVRP's direct and via-depot moves
     share N + 1 bits).  log_probs is the log-softmax of what is left, ``selected`` its lowest greatest action (-1 and -inf
     throughout where all is blocked).  Penalties are numbers or float tensors [R]."""
-    with torch.no_grad():
-        if logits.dim() != 2 or logits.dtype not in _DTYPES or not logits.is_cuda:
-            raise ValueError(f"logits are {tuple(logits.shape)} {logits.dtype} on {logits.device}: [rows, actions] of float32, "
-                             "float16 or bfloat16 on a GPU are expected")
-        R, A = logits.shape
-        dev = logits.device
-        if A < 1:
-            raise ValueError("no actions")
-        if logits.stride(1) != 1 and A > 1:
-            logits = logits.contiguous()
-        words = bits_stride = cols = history_stride = bias_stride = 0
-        if blocked is not None:
-            if blocked.dim() != 2 or blocked.shape[0] != R or blocked.dtype != torch.int64 or blocked.device != dev:
-                raise ValueError(f"blocked is {tuple(blocked.shape)} {blocked.dtype}: int64 words [{R}, n] on {dev} are expected")
-            words = blocked.shape[1]
-            if words > 1 and blocked.stride(1) != 1:
-                blocked = blocked.contiguous()
-            bits_stride = blocked.stride(0)
-        if bias is not None:
-            bias = _side(bias, "bias", (A,) if bias.dim() == 1 else (R, A), torch.float32, dev)
-            bias_stride = 0 if bias.dim() == 1 else bias.stride(0)
-        if history_len is not None and history is None:
-            raise ValueError("history_len without a history")
-        if history is not None:
-            if history.dim() != 2:
-                raise ValueError(f"history has shape {tuple(history.shape)}: [{R}, n] is expected")
-            history = _side(history, "history", (R, history.shape[1]), torch.int32, dev)
-            history_len = _side(history_len, "history_len", (R,), torch.int32, dev)
-            cols, history_stride = history.shape[1], history.stride(0)
-        rows, numbers = [], []
-        for name, x, neutral in (("repetition", repetition, 1.0), ("presence", presence, 0.0), ("frequency", frequency, 0.0)):
-            per_row = isinstance(x, torch.Tensor)
-            rows.append(_side(x, name, (R,), torch.float32, dev) if per_row else None)
-            numbers.append(neutral if per_row else float(x))
-        out = torch.empty((R, A), dtype=torch.float32, device=dev)
-        selected = torch.empty(R, dtype=torch.int32, device=dev)
-        if R == 0:
-            return out, selected
-        a = _lib.Logits()
-        _PACK.pack_into(a, 0, _DTYPES[logits.dtype], R, A, A if period is None else int(period), logits.data_ptr(), logits.stride(0),
-                        ptr(blocked), bits_stride, words, cols, ptr(bias), bias_stride, ptr(history) if cols else 0, history_stride,
-                        ptr(history_len), ptr(rows[0]), ptr(rows[1]), ptr(rows[2]), *numbers, float(temperature), out.data_ptr(), A,
-                        selected.data_ptr())
-        lib, ref = _lib.load(), ctypes.byref(a)
-        need = lib.dgl_logits_workspace_floats(ref)
-        ws = torch.empty(need, dtype=torch.float32, device=dev) if need > 0 else None
-        _launch(dev, lib.dgl_logits_process, ref, ptr(ws), what="dgl_logits_process")
+    if logits.dim() != 2 or logits.dtype not in _DTYPES or not logits.is_cuda:
+        raise ValueError(f"logits are {tuple(logits.shape)} {logits.dtype} on {logits.device}: [rows, actions] of float32, "
+                         "float16 or bfloat16 on a GPU are expected")
+    R, A = logits.shape
+    dev = logits.device
+    if A < 1:
+        raise ValueError("no actions")
+    if logits.stride(1) != 1 and A > 1:
+        logits = logits.contiguous()
+    words = bits_stride = cols = history_stride = bias_stride = 0
+    if blocked is not None:
+        if blocked.dim() != 2 or blocked.shape[0] != R or blocked.dtype != torch.int64 or blocked.device != dev:
+            raise ValueError(f"blocked is {tuple(blocked.shape)} {blocked.dtype}: int64 words [{R}, n] on {dev} are expected")
+        words = blocked.shape[1]
+        if words > 1 and blocked.stride(1) != 1:
+            blocked = blocked.contiguous()
+        bits_stride = blocked.stride(0)
+    if bias is not None:
+        bias = _side(bias, "bias", (A,) if bias.dim() == 1 else (R, A), torch.float32, dev)
+        bias_stride = 0 if bias.dim() == 1 else bias.stride(0)
+    if history_len is not None and history is None:
+        raise ValueError("history_len without a history")
+    if history is not None:
+        if history.dim() != 2:
+            raise ValueError(f"history has shape {tuple(history.shape)}: [{R}, n] is expected")
+        history = _side(history, "history", (R, history.shape[1]), torch.int32, dev)
+        history_len = _side(history_len, "history_len", (R,), torch.int32, dev)
+        cols, history_stride = history.shape[1], history.stride(0)
+    rows, numbers = [], []
+    for name, x, neutral in (("repetition", repetition, 1.0), ("presence", presence, 0.0), ("frequency", frequency, 0.0)):
+        per_row = isinstance(x, torch.Tensor)
+        rows.append(_side(x, name, (R,), torch.float32, dev) if per_row else None)
+        numbers.append(neutral if per_row else float(x))
+    out = torch.empty((R, A), dtype=torch.float32, device=dev)
+    selected = torch.empty(R, dtype=torch.int32, device=dev)
+    if R == 0:
         return out, selected
+    a = _lib.Logits()
+    _PACK.pack_into(a, 0, _DTYPES[logits.dtype], R, A, A if period is None else int(period), logits.data_ptr(), logits.stride(0),
+                    ptr(blocked), bits_stride, words, cols, ptr(bias), bias_stride, ptr(history) if cols else 0, history_stride,
+                    ptr(history_len), ptr(rows[0]), ptr(rows[1]), ptr(rows[2]), *numbers, float(temperature), out.data_ptr(), A,
+                    selected.data_ptr())
+    lib, ref = _lib.load(), ctypes.byref(a)
+    need = lib.dgl_logits_workspace_floats(ref)
+    ws = torch.empty(need, dtype=torch.float32, device=dev) if need > 0 else None
+    _launch(dev, lib.dgl_logits_process, ref, ptr(ws), what="dgl_logits_process")
+    return out, selected
