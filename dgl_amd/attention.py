@@ -251,7 +251,7 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, scale: Optio
         leaves = [t for t in (q, k, v, slope) if t is not None and t.requires_grad and t.is_leaf]
         if leaves and q.is_cuda and torch.cuda.is_current_stream_capturing():
             raise RuntimeError("attention: a leaf that requires grad inside a graph capture; capture attention_forward "
-                               "and attention_backward, or pass a tensor computed from the leaf")
+                               "and attention_backward instead")
     for name, t in (("pos_q", pos_q), ("pos_k", pos_k)):
         if t is not None and t.requires_grad and torch.is_grad_enabled():
             raise ValueError(f"{name} requires grad: the operator is not differentiable in the coordinates")

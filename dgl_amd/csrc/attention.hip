@@ -15,6 +15,16 @@
 // A pair that is masked contributes nothing, whatever its operands hold: the products of the matrix instructions would
 // carry a NaN or infinity of a masked row into its tile neighbours (0 * NaN), so a result that is not finite at the end is
 // recomputed pair by pair (careful_*), which costs nothing where all is finite.
+//
+// Bound by the issue of vector instructions, not by memory (a head's keys are read by all its row blocks from L2): a pair of
+// a forward pass takes 15 simple operations and 4 of exp / rcp / sqrt with a cap and coordinates in binary32 (a third of the
+// simple ones split probabilities into terms), 7 and 3 with a cap in 16 bits, and the 16-bit matrix instructions hold the
+// vector unit back for two thirds of their 17 cycles.  Measured, per launch:
+//   forward, 64 x 8 heads of 16, 1000 nodes, cap and coordinates, binary32                423 us  77 TFLOP/s
+//   forward, 32 heads over 8 of 128, 8192 causal rows, cap, bf16                           905 us  608 TFLOP/s
+//   2 x 16 heads over 4 of 64, 2047 causal rows behind a prefix, slopes, bf16     forward 79, rows 96, keys 113 + 13 us
+//   8 heads of 64, 6000 rows in 9 documents, fp16                                 forward 91, rows 117, keys 169 us
+//   8 x 8 heads of 16, 1001 rows in 4 documents, cap and coordinates, binary32    forward 91, rows 109, keys 121 us
 #include "attention_tile.h"
 
 #include <cfloat>
@@ -221,7 +231,7 @@ __global__ __launch_bounds__(ATTN_THREADS, TYPE == ATTN_F32 && DP == 128 ? 1 : 2
     typedef Shape<TYPE, DP> S;
     typedef typename Elem<TYPE>::raw raw;
     // KB: blocks of 16 keys whose scores are held at once.  Two where that fits another wave on a SIMD: heads of 128 (256
-    // registers for two waves) and binary32 heads of 16 (168 for three: nodes of 1000, 551 -> 475 us)
+    // registers for two waves) and binary32 heads of 16 (168 for three: 14 % less for nodes of 1000)
     constexpr int ROWS = 64 * NQ, KB = DP == 128 || (TYPE == ATTN_F32 && DP <= 32) ? 2 : 4;
     __shared__ __align__(16) char Kt[S::bytes], Vt[S::bytes];
     __shared__ __align__(16) float key_pos[2 * ATTN_ROWS];

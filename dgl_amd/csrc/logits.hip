@@ -9,6 +9,11 @@
 // 8192 actions, one launch for the tiles' maxima and sums, a second one that computes the values again - reading the
 // logits twice costs less than writing and reading back binary32 values in between.
 // Occurrences are counted in LDS per row (or tile), with integer atomics: their order does not matter.
+//
+// Measured, per launch: 512 rows x 1000 with blocked bits 3.9 us; 512 x 20002 with bits shared by two moves, biases, penalties
+// and a temperature, binary32, 25 us = 3.3 TB/s (14 us = 5.9 TB/s without controls); 256 x 131072, bf16, bits, penalties over a
+// history of 2048, temperature: 44 us for the statistics and 47 us for the values (27 and 27 without controls, of which
+// writing the result takes 20), 12 of each for counting the history once more per tile.
 #include "common.h"
 
 #include <cfloat>

@@ -204,6 +204,7 @@ class TspEngine:
         self.overflow = torch.zeros(1, dtype=torch.int32, device=dev)      # set by the split-f16 kernel (range guard)
         self.t = 0
         self.tile_t = -1                 # step count the neighbourhood buffers (idx, tile) belong to
+        self.linked = False              # the last step's nodes are in the back-pointer history only
         self._beam_bufs = None
 
     def _alloc_outputs(self) -> None:
@@ -254,12 +255,14 @@ class TspEngine:
         check(self.lib.dgl_tsp_reset(ctypes.byref(self.state["struct"]), stream_ptr()), "dgl_tsp_reset")
         self.t = 0
         self.tile_t = -1
+        self.linked = False
 
     @on_own_device
     def step(self, selected: torch.Tensor, want_knn: bool = True) -> None:
         """Apply ``selected`` (int32 [R]) and, unless the tour is complete, build the next neighbourhood."""
         assert selected.dtype == torch.int32 and selected.is_cuda and selected.numel() == self.R
         self.t += 1
+        self.linked = False
         more = want_knn and self.t < self.N
         check(self.lib.dgl_tsp_step(ctypes.byref(self.state["struct"]), ptr(selected), self.t, self.knn,
                                     ptr(self.idx) if more else 0, ptr(self.tile) if more else 0, stream_ptr()),
@@ -380,7 +383,8 @@ class TspEngine:
         if slope is not None:
             if self.t < 1:
                 raise ValueError("no current node before the first step")
-            cur = self.state["tour"][:, self.t - 1].long()
+            # (steps along back-pointers leave the nodes to the history until they are traced back)
+            cur = (self.hist_node[self.t - 1] if self.linked else self.state["tour"][:, self.t - 1]).long()
             pos_q = self.xy[torch.arange(self.R, device=self.device) // self.rpi, cur]
         return attention_step(q, cache, rows_per_instance=self.rpi, scale=scale, cap=cap, slope=slope, pos_q=pos_q,
                               pos_k=self.xy if slope is not None else None, blocked=self.state["visited"], return_lse=return_lse)
@@ -395,6 +399,7 @@ class TspEngine:
             self.hist_parent = torch.zeros(self.N, self.R, dtype=torch.int32, device=self.device)
         src, dst = self.bufs[self.cur], self.bufs[1 - self.cur]
         self.t += 1
+        self.linked = True
         more = self.t < self.N
         check(self.lib.dgl_tsp_step_beam(ctypes.byref(src["struct"]), ctypes.byref(dst["struct"]), ptr(prev_k), beam,
                                          ptr(selected), self.t, self.knn, ptr(self.idx) if more else 0,
@@ -478,6 +483,7 @@ class CvrpEngine:
         self.overflow = torch.zeros(1, dtype=torch.int32, device=dev)      # set by the split-f16 kernel (range guard)
         self.t = 0
         self.tile_t = -1
+        self.linked = False
 
     def _alloc_outputs(self) -> None:
         w = max(MAX_TOKENS, self.ntok_max)
@@ -533,11 +539,13 @@ class CvrpEngine:
         check(self.lib.dgl_cvrp_reset(ctypes.byref(self.state["struct"]), stream_ptr()), "dgl_cvrp_reset")
         self.t = 0
         self.tile_t = -1
+        self.linked = False
 
     @on_own_device
     def step(self, action: torch.Tensor, want_knn: bool = True) -> None:
         assert action.dtype == torch.int32 and action.is_cuda and action.numel() == self.R
         self.t += 1
+        self.linked = False
         more = want_knn and self.t < self.N
         check(self.lib.dgl_cvrp_step(ctypes.byref(self.state["struct"]), ptr(action), self.t, self.knn, self.depot_knn,
                                      ptr(self.idx_last) if more else 0, ptr(self.idx_dep) if more else 0,
@@ -639,7 +647,11 @@ class CvrpEngine:
         if slope is not None:
             if self.t < 1:
                 raise ValueError("no current node before the first step")
-            cur = self.state["nodes"][:, self.t - 1].long()
+            if self.linked:                      # (as TspEngine.attend; the history holds actions)
+                cur = self.hist_action[self.t - 1].long()
+                cur = torch.where(cur > self.N, cur - (self.N + 1), cur)
+            else:
+                cur = self.state["nodes"][:, self.t - 1].long()
             pos_q = self.xy[torch.arange(self.R, device=self.device) // self.rpi, cur]
         return attention_step(q, cache, rows_per_instance=self.rpi, scale=scale, cap=cap, slope=slope, pos_q=pos_q,
                               pos_k=self.xy if slope is not None else None, blocked=self.state["visited"], return_lse=return_lse)
@@ -654,6 +666,7 @@ class CvrpEngine:
             self.hist_parent = torch.zeros(self.N, self.R, dtype=torch.int32, device=self.device)
         src, dst = self.bufs[self.cur], self.bufs[1 - self.cur]
         self.t += 1
+        self.linked = True
         more = self.t < self.N
         check(self.lib.dgl_cvrp_step_beam(ctypes.byref(src["struct"]), ctypes.byref(dst["struct"]), ptr(prev_k), beam,
                                           ptr(action), self.t, self.knn, self.depot_knn,

@@ -210,3 +210,41 @@ def test_training_and_serving_agree_on_a_causal_encoder(device):
     for a, b in ((w.grad, w64.grad), (slope.grad, s64.grad)):
         # binary32 products of lengths 60 and 32 before and after the operator: 1e-5 of the gradient's size
         assert float((a.double() - b).norm()) <= 1e-5 * float(b.norm())
+
+
+@pytest.mark.parametrize("problem", ["tsp", "cvrp"])
+def test_attention_between_steps_along_back_pointers(device, problem):
+    """The current node of a row after a fused beam step, whose tours are only traced back at the end, and after a plain step
+    that follows another rollout."""
+    from dgl_amd.attention import PagedCache, attention_step
+    B, N, beam, H, D = 3, 30, 4, 4, 16
+    eng, pol, start = (tsp if problem == "tsp" else cvrp)(device, B=B, N=N, rpi=beam)
+    nodes = eng.xy.shape[1]
+    q, k, v = encoder(eng.xy, H, D, 3)
+    cache = PagedCache(B, H, D, nodes, page_size=16, device=device)
+    cache.append(k, v)
+    slope = 1.0 + torch.rand(H, device=device)
+    rows = torch.randn(eng.R, H, D, device=device)
+    seq = torch.arange(eng.R, device=device) // beam
+    at = {"node": start.long() if problem == "tsp" else start.long() - (N + 1)}
+
+    def check_attend():
+        want = attention_step(rows, cache, rows_per_instance=beam, slope=slope, pos_q=eng.xy[seq, at["node"]], pos_k=eng.xy,
+                              blocked=eng.state["visited"])
+        assert torch.equal(eng.attend(rows, cache, slope=slope), want)
+    eng.reset()
+    eng.step(start)
+    check_attend()
+    scores = torch.zeros(B, beam, device=device)
+    prev_k, action = (torch.zeros(B, beam, dtype=torch.int32, device=device) for _ in range(2))
+    for t in range(1, 6):
+        eng.forward(pol, want_logits=False)
+        eng.beam_advance(scores, beam, t, prev_k, action)
+        eng.step_beam(prev_k.view(-1), action.view(-1), beam)
+        chosen = action.view(-1).long()
+        at["node"] = torch.where(chosen > N, chosen - (N + 1), chosen) if problem == "cvrp" else chosen
+        check_attend()
+    eng.reset()
+    eng.step(start)
+    at["node"] = start.long() if problem == "tsp" else start.long() - (N + 1)
+    check_attend()
