@@ -89,6 +89,8 @@ def _side(t: Optional[torch.Tensor], name, shape, dtype, device) -> Optional[tor
     if t.dtype != dtype:
         if dtype == torch.int32 and t.is_floating_point() or dtype == torch.float32 and not t.is_floating_point():
             raise ValueError(f"{name} is {t.dtype}, expected {dtype}")
+        if t.dtype == torch.int64:               # (2^32 + 5 is no 5: what does not fit stays beyond every bound)
+            t = t.clamp(-(1 << 31), (1 << 31) - 1)
         t = t.to(dtype)
     if t.is_contiguous():
         return t

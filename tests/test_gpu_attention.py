@@ -357,3 +357,16 @@ def test_rounding_of_the_output_does_not_reach_the_gradients(device):
         value = want[n][0]
         error = [((z.double() - value).norm() / value.norm()).item() for z in (x.grad, y)]
         assert error[0] < 0.9 * error[1], (n, error)
+
+
+def test_wide_ids_and_prefixes_keep_their_sign(device):
+    from dgl_amd.attention import attention
+    t, _ = inputs(1, 2, 2, 40, 40, 16, torch.float32, 43)
+    ids = torch.zeros(1, 40, dtype=torch.int64, device=device)
+    ids[:, 30:] = -2 ** 40
+    out = attention(t["q"], t["k"], t["v"], doc_q=ids, doc_k=ids)
+    assert torch.equal(out, attention(t["q"], t["k"], t["v"], doc_q=ids.clamp(-1).int(), doc_k=ids.clamp(-1).int()))
+    assert not out[:, :, 30:].any() and bool(out[:, :, :30].any())
+    far = torch.tensor([2 ** 40], device=device)
+    assert torch.equal(attention(t["q"], t["k"], t["v"], causal=True, prefix=far),
+                       attention(t["q"], t["k"], t["v"], causal=True, prefix=far.clamp(max=40).int()))

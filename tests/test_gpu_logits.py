@@ -213,3 +213,12 @@ def test_bits_of_any_period(device, dtype, A, period):
     check(x, blocked=blocked, period=period)
     hist = torch.randint(0, A, (4, 70), device=device, generator=g).to(torch.int32)
     check(x, blocked=blocked[:, : max(1, blocked.shape[1] // 2)], period=period, history=hist, presence=0.5, frequency=0.25)
+
+
+def test_wide_history_entries_are_no_actions(device):
+    from dgl_amd.logits import process_logits
+    x, g = rnd(2, 100, torch.float32, 3)
+    history = torch.tensor([[5, 7, 2 ** 32 + 5, -2 ** 33 + 9], [2 ** 31, 2 ** 40, -1, 3]], device=device)
+    narrow = torch.tensor([[5, 7, -1, -1], [-1, -1, -1, 3]], device=device, dtype=torch.int32)
+    for a, b in zip(process_logits(x, history=history, presence=1.0), process_logits(x, history=narrow, presence=1.0)):
+        assert torch.equal(a, b)
