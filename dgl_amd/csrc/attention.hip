@@ -21,8 +21,8 @@
 // simple ones split probabilities into terms), 7 and 3 with a cap in 16 bits, and the 16-bit matrix instructions hold the
 // vector unit back for two thirds of their 17 cycles.  Measured, per launch:
 //   forward, 64 x 8 heads of 16, 1000 nodes, cap and coordinates, binary32                423 us  77 TFLOP/s
-//   forward, 32 heads over 8 of 128, 8192 causal rows, cap, bf16                           905 us  608 TFLOP/s
-//   2 x 16 heads over 4 of 64, 2047 causal rows behind a prefix, slopes, bf16     forward 79, rows 96, keys 113 + 13 us
+//   forward, 32 heads over 8 of 128, 8192 causal rows, cap, bf16                           860 us  640 TFLOP/s
+//   2 x 16 heads over 4 of 64, 2047 causal rows behind a prefix, slopes, bf16     forward 72, rows 86, keys 114 + 13 us
 //   8 heads of 64, 6000 rows in 9 documents, fp16                                 forward 91, rows 117, keys 169 us
 //   8 x 8 heads of 16, 1001 rows in 4 documents, cap and coordinates, binary32    forward 91, rows 109, keys 121 us
 #include "attention_tile.h"
@@ -61,6 +61,24 @@ struct AttnArgs {
 // Blocks are dealt to the 8 XCDs in turn; giving every XCD a contiguous range of the work keeps the row blocks of one
 // head, which read the same keys and values, on one L2.
 __device__ __forceinline__ int xcd_work() { return (int)(blockIdx.x % 8) * (int)(gridDim.x / 8) + (int)(blockIdx.x / 8); }
+
+// The workgroup's unit (a head, or a part of one) and the rank of its block among the unit's `tiles`, longest first.  Blocks of
+// a causal call differ in length: there the longest blocks of all the heads of an XCD start before any shorter one, or the last
+// head's long blocks would run on a chip that is otherwise idle (32 heads of 128, 8192 rows: 883 -> 856 us; 2 x 16 heads of 64, 2047
+// rows: forward 78 -> 72, query rows' gradients 96 -> 86.  The keys' gradients, cut finer, gain nothing and keep their order).
+struct Work {
+    int unit, rank;                              // rank >= tiles: nothing to do
+};
+__device__ __forceinline__ Work deal(bool uneven, int units, int tiles) {
+    const int i = blockIdx.x;
+    if (!uneven) {
+        const int work = xcd_work();
+        return {work / tiles, work < units * tiles ? work % tiles : tiles};
+    }
+    if (units % 8 != 0) return {i % units, i / units};
+    const int per = units / 8, l = i / 8;
+    return {i % 8 * per + l % per, l / per};
+}
 
 // keys a query row sees: j < limit (and the document test)
 __device__ __forceinline__ int row_limit(const AttnArgs &a, int b, int i) {
@@ -237,11 +255,9 @@ __global__ __launch_bounds__(ATTN_THREADS, TYPE == ATTN_F32 && DP == 128 ? 1 : 2
     __shared__ __align__(16) float key_pos[2 * ATTN_ROWS];
     __shared__ __align__(16) int key_doc[ATTN_ROWS];
     __shared__ TileMap map_store;
-    int work = xcd_work();
-    if (work >= a.B * a.Hq * a.tiles * a.splits) return;
-    const int split = work % a.splits;
-    work /= a.splits;
-    const int bh = work / a.tiles, qt = a.tiles - 1 - work % a.tiles;        // (causal: the longest rows first)
+    const Work work = deal(a.causal, a.B * a.Hq * a.splits, a.tiles);
+    if (work.rank >= a.tiles) return;
+    const int split = work.unit % a.splits, bh = work.unit / a.splits, qt = a.tiles - 1 - work.rank;      // (the last rows see most)
     const int b = bh / a.Hq, h = bh % a.Hq, hk = h / a.G;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g = lane >> 4, c = lane & 15;
     const int row0 = qt * ROWS, wrow0 = row0 + wave * 16 * NQ;
@@ -620,9 +636,9 @@ __global__ __launch_bounds__(ATTN_THREADS, DP <= 64 ? 2 : 1) void attn_bwd_q_ker
     __shared__ __align__(16) int key_doc[ATTN_ROWS];
     __shared__ TileMap map_store;
     __shared__ float part[4];
-    const int work = xcd_work();
-    if (work >= a.B * a.Hq * a.tiles) return;
-    const int bh = work / a.tiles, qt = a.tiles - 1 - work % a.tiles;
+    const Work work = deal(a.causal, a.B * a.Hq, a.tiles);
+    if (work.rank >= a.tiles) return;
+    const int bh = work.unit, qt = a.tiles - 1 - work.rank;
     const int b = bh / a.Hq, h = bh % a.Hq, hk = h / a.G;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g = lane >> 4, c = lane & 15;
     const int row0 = qt * ROWS, wrow0 = row0 + wave * 16 * NQ;
