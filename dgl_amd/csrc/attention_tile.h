@@ -188,7 +188,6 @@ template <int TYPE, int DP> struct Shape {
     static constexpr int dt = DP / 16;                               // 16-row tiles over the head size
     static constexpr int plane = ATTN_ROWS * DP * 2, bytes = terms * plane;
     static constexpr int per_row = DP / vec;                         // 16-byte global pieces of a row
-    static constexpr int units = ATTN_ROWS / 4 * per_row;            // pieces of 4 rows x 16 bytes
     // operands of one 16-row block: A from LDS, B in registers.  Heads of 16 fill half of the 32 slots; binary32 puts two
     // terms side by side there: A [h m], [h l] against B [h m], [m h], [l h] are the six products in three instructions.
     static constexpr int a_regs = DP < 32 && terms == 3 ? 2 : terms * chunks, b_regs = terms * chunks;
@@ -349,16 +348,19 @@ __device__ __forceinline__ void accumulate(f32x4 (&out)[N][DT], const char *tile
 }
 
 // ---- staging ------------------------------------------------------------------------------------------------------
-// Two [rows][D] matrices pass through LDS tile by tile, in units of rows grp, grp + 16, + 32, + 48 x 16 bytes that one thread
-// holds between its global loads and its LDS writes.  Where a matrix has fewer than 256 units, whole waves take one matrix
-// or the other; else every thread takes the same units of both.  Row strides are scalars and a unit's offset from the tile is
-// below 2^32 (the launcher's check), so that a load is a scalar address plus a 32-bit offset.
+// Two [rows][D] matrices pass through LDS tile by tile, in pieces of 16 bytes that a thread holds between its global loads and its
+// LDS writes: `held` rows, `step` apart, of one piece (two for the widest rows) of both matrices, so that every thread has the
+// same share of the work - binary32 pieces are split into their terms here.  The narrowest rows have 128 pieces: two waves take
+// one matrix, two the other.  Row strides are scalars and a piece's offset from the tile is below 2^32 (the launcher's check), so
+// that a load is a scalar address plus a 32-bit offset.
 template <int TYPE, int DP> struct Stager {
     typedef Shape<TYPE, DP> S;
-    static constexpr bool both = S::units >= 256;
-    static constexpr int plans = both ? S::units / 256 : 1, second = S::units < 64 ? 64 : S::units;   // first thread of the second matrix
-    u32x4 r[both ? 2 : 1][plans][4];
-    int id[plans][4];
+    static constexpr int held = S::per_row >= 16 ? 4 : S::per_row >= 8 ? 2 : 1, step = ATTN_ROWS / held, units = step * S::per_row;
+    static constexpr bool both = units >= 256;
+    static constexpr int plans = both ? units / 256 : 1;
+    static_assert(step % 16 == 0 && (both || units == 128), "a thread's rows share their permutation");
+    u32x4 r[both ? 2 : 1][plans][held];
+    int id[plans][held];
     unsigned off[both ? 2 : 1][plans], at[plans];
     int grp[plans];
     bool in[plans];
@@ -367,14 +369,14 @@ template <int TYPE, int DP> struct Stager {
 
     __device__ __forceinline__ void init(int64_t stride0, int64_t stride1, int D) {
         const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
-        which = !both && wave >= second / 64;
+        which = !both && wave >= 2;
         rb0 = (unsigned)(stride0 * Elem<TYPE>::bytes);
         rb1 = (unsigned)(stride1 * Elem<TYPE>::bytes);
 #pragma unroll
         for (int x = 0; x < plans; ++x) {
-            const int u = (int)threadIdx.x + 256 * x - (which ? second : 0), piece = u % S::per_row;
+            const int u = (int)threadIdx.x + 256 * x - (which ? 128 : 0), piece = u % S::per_row;
             grp[x] = u / S::per_row;
-            in[x] = u < S::units && piece * S::vec < D;
+            in[x] = piece * S::vec < D;
             if constexpr (both) {
                 off[0][x] = (unsigned)grp[x] * rb0 + 16u * (unsigned)piece;
                 off[1][x] = (unsigned)grp[x] * rb1 + 16u * (unsigned)piece;
@@ -382,7 +384,6 @@ template <int TYPE, int DP> struct Stager {
                 off[0][x] = (unsigned)grp[x] * (which ? rb1 : rb0) + 16u * (unsigned)piece;
             }
             at[x] = S::terms == 1 ? piece_at<TYPE, DP>(grp[x], piece) : piece_at<TYPE, DP>(grp[x], piece >> 1) + 8 * (piece & 1);
-            if (u >= S::units) grp[x] = -1;      // (no unit: nothing is written)
         }
     }
     // the tiles that start at t0 / t1 with `rows` rows left (rows beyond are zero); ids: the rows' document ids or nullptr
@@ -394,16 +395,16 @@ template <int TYPE, int DP> struct Stager {
 #pragma unroll
             for (int x = 0; x < plans; ++x)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const bool live = in[x] && (rows >= ATTN_ROWS || grp[x] + 16 * i < rows);
-                    r[m][x][i] = live ? *reinterpret_cast<const u32x4 *>(t + (uint64_t)(16u * i * rb) + off[m][x]) : u32x4{0, 0, 0, 0};
+                for (int i = 0; i < held; ++i) {
+                    const bool live = in[x] && (rows >= ATTN_ROWS || grp[x] + step * i < rows);
+                    r[m][x][i] = live ? *reinterpret_cast<const u32x4 *>(t + (uint64_t)((unsigned)(step * i) * rb) + off[m][x]) : u32x4{0, 0, 0, 0};
                 }
         }
         if (ids != nullptr) {
 #pragma unroll
             for (int x = 0; x < plans; ++x)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) id[x][i] = grp[x] >= 0 && grp[x] + 16 * i < rows ? ids[grp[x] + 16 * i] : -1;
+                for (int i = 0; i < held; ++i) id[x][i] = grp[x] + step * i < rows ? ids[grp[x] + step * i] : -1;
         }
     }
     // Rows of padding (document id < 0) may hold anything: they are staged as zeros, so that a NaN among them does not send
@@ -411,12 +412,11 @@ template <int TYPE, int DP> struct Stager {
     __device__ __forceinline__ void write(char *l0, char *l1, bool skip) {
 #pragma unroll
         for (int x = 0; x < plans; ++x) {
-            if (!both && grp[x] < 0) continue;
 #pragma unroll
             for (int m = 0; m < (both ? 2 : 1); ++m) {
                 char *l = (both ? (m ? l1 : l0) : (which ? l1 : l0)) + at[x];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
+                for (int i = 0; i < held; ++i) {
                     u32x4 v = r[m][x][i];
                     if (skip) {
                         unsigned keep;
@@ -424,7 +424,7 @@ template <int TYPE, int DP> struct Stager {
 #pragma unroll
                         for (int w = 0; w < 4; ++w) v[w] &= ~keep;
                     }
-                    char *to = l + 256 * S::pieces * i;
+                    char *to = l + 16 * S::pieces * step * i;
                     if constexpr (S::terms == 1) {
                         *reinterpret_cast<u32x4 *>(to) = v;
                     } else {                     // four binary32 elements are half a piece of each plane
