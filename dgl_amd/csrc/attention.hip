@@ -55,6 +55,7 @@ struct AttnArgs {
     char *dq, *dk, *dv;
     int64_t dos[3], dqst[3], dkst[3], dvst[3];
     float *delta, *rowscale, *dslope_part, *dslope;
+    int *many;                                   // per row: all ones, or 0 where it sees a single key
     int head_parts;                              // key kernel: parts of the heads that share a key head
 };
 
@@ -660,7 +661,7 @@ __global__ __launch_bounds__(ATTN_THREADS, DP <= 64 ? 2 : 1) void attn_bwd_q_ker
     ColFrag<TYPE, DP> qf[NQ], of[NQ];
     f32x4 dq[NQ][S::dt];
     float lse2[NQ], delta[NQ], rs[NQ], qx[NQ], qy[NQ], excess[NQ], pd[NQ], dsl[NQ];
-    int limit[NQ], doc[NQ];
+    int limit[NQ], doc[NQ], seen[NQ];            // seen: how many of the lane's keys the row sees
     int wave_limit = 0, wave_full = INT_MAX;
 #pragma unroll
     for (int n = 0; n < NQ; ++n) {
@@ -705,6 +706,7 @@ __global__ __launch_bounds__(ATTN_THREADS, DP <= 64 ? 2 : 1) void attn_bwd_q_ker
         limit[n] = row_limit(a, b, i);
         doc[n] = map != nullptr ? doc_of_query(a, b, i) : 0;
         qx[n] = qy[n] = excess[n] = pd[n] = dsl[n] = 0.0f;
+        seen[n] = 0;
         if (a.bias == 1) qx[n] = (float)(i + a.Lk - a.Lq);
         if (a.bias == 2 && live) {
             qx[n] = a.pos_q[b * a.pqs + 2 * (int64_t)i];
@@ -797,6 +799,7 @@ __global__ __launch_bounds__(ATTN_THREADS, DP <= 64 ? 2 : 1) void attn_bwd_q_ker
 #pragma unroll
                         for (int r = 0; r < 4; ++r) {
                             const unsigned ok = mask_below(16 * t + r, left) & mask_equal(kd[r], own);
+                            seen[n] -= (int)ok;
                             p[r] = keep_or_zero(ok, p[r]);
                             ds[r] = keep_or_zero(ok, ds[r]);
                             away[r] = keep_or_zero(ok, away[r]);             // (a masked key's coordinates may be NaN)
@@ -806,6 +809,9 @@ __global__ __launch_bounds__(ATTN_THREADS, DP <= 64 ? 2 : 1) void attn_bwd_q_ker
                         dist[t][n] = away;
                     }
                 }
+            } else {
+#pragma unroll
+                for (int n = 0; n < NQ; ++n) seen[n] += 8;
             }
             if (want_slope) {
 #pragma unroll
@@ -838,14 +844,18 @@ __global__ __launch_bounds__(ATTN_THREADS, DP <= 64 ? 2 : 1) void attn_bwd_q_ker
         const float inv_rs = 1.0f / rs[n], undo = undo_factor(a) * inv_rs;
 #pragma unroll
         for (int d = 0; d < S::dt; ++d) fine = fine && finite4(dq[n][d]);
+        unsigned long long bad = __ballot(!fine && live);
+        bad = (bad | bad >> 16 | bad >> 32 | bad >> 48) & 0xffff;
+        // A single key has the probability 1 whatever its score: the row's score gradients are zero, and not what the rounding
+        // of dp and delta leaves of their difference.  (Such a row is never in a tile without masks, here or below.)
+        const bool single = group_sum((float)min(seen[n], 64)) == 1.0f && (bad >> c & 1) == 0;
         if (live) {
             raw *out = reinterpret_cast<raw *>(a.dq) + b * a.dqst[0] + h * a.dqst[1] + (int64_t)i * a.dqst[2];
 #pragma unroll
             for (int d = 0; d < S::dt; ++d)
-                if (16 * d + 4 * g < a.D) store4<TYPE>(out + 16 * d + 4 * g, dq[n][d] * undo);
+                if (16 * d + 4 * g < a.D) store4<TYPE>(out + 16 * d + 4 * g, single ? f32x4{0.0f, 0.0f, 0.0f, 0.0f} : dq[n][d] * undo);
+            if (g == 0) a.many[((int64_t)b * a.Hq + h) * a.Lq + i] = single ? 0 : -1;
         }
-        unsigned long long bad = __ballot(!fine && live);
-        bad = (bad | bad >> 16 | bad >> 32 | bad >> 48) & 0xffff;
         for (; bad != 0; bad &= bad - 1) {
             const int cc = __ffsll((long long)bad) - 1;
             const int64_t at = ((int64_t)b * a.Hq + h) * a.Lq + wrow0 + 16 * n + cc;
@@ -853,7 +863,7 @@ __global__ __launch_bounds__(ATTN_THREADS, DP <= 64 ? 2 : 1) void attn_bwd_q_ker
         }
         if (want_slope) {
             const float e = group_sum(excess[n]) * inv_rs, x = group_sum(pd[n]) * inv_rs, y = group_sum(dsl[n]) * inv_rs;
-            slope_sum += live ? fmaf(-e, x, y) : 0.0f;
+            slope_sum += live && !single ? fmaf(-e, x, y) : 0.0f;
         }
     }
     if (want_slope) {
@@ -942,7 +952,7 @@ __global__ __launch_bounds__(ATTN_THREADS, DP <= 64 ? 2 : 1) void attn_bwd_kv_ke
     constexpr int ROWS = 64 * NK, HALVES = DP <= 32 ? 2 : 1;
     __shared__ __align__(16) char Qt[S::bytes], Ot[S::bytes];
     __shared__ __align__(16) float row_lse[ATTN_ROWS], row_delta[ATTN_ROWS], row_x[ATTN_ROWS], row_y[ATTN_ROWS];
-    __shared__ __align__(16) int row_lim[ATTN_ROWS], row_doc[ATTN_ROWS];
+    __shared__ __align__(16) int row_lim[ATTN_ROWS], row_doc[ATTN_ROWS], row_many[ATTN_ROWS];
     __shared__ TileMap map_store;
     __shared__ unsigned least_scale;
     const int parts = a.head_parts * a.splits;
@@ -1026,9 +1036,10 @@ __global__ __launch_bounds__(ATTN_THREADS, DP <= 64 ? 2 : 1) void attn_bwd_kv_ke
         const char *q = a.q + (b * a.qs[0] + h * a.qs[1]) * Elem<TYPE>::bytes;
         const char *go = a.dout + (b * a.dos[0] + h * a.dos[1]) * Elem<TYPE>::bytes;
         const float *lse = a.lse + ((int64_t)b * a.Hq + h) * a.Lq, *del = a.delta + ((int64_t)b * a.Hq + h) * a.Lq;
+        const int *many = a.many + ((int64_t)b * a.Hq + h) * a.Lq;
         const ScoreParams sp = score_params(a.scale, a.cap, a.bias, a.slope, h);
         float st_lse = 0.0f, st_delta = 0.0f, st_x = 0.0f, st_y = 0.0f;
-        int st_lim = 0, st_doc = -2;
+        int st_lim = 0, st_doc = -2, st_many = 0;
         auto load = [&](int tile) {
             const int base = tile * ATTN_ROWS, left = a.Lq - base;
             const char *qt = q + base * a.qs[2] * Elem<TYPE>::bytes, *ot = go + base * a.dos[2] * Elem<TYPE>::bytes;
@@ -1040,6 +1051,7 @@ __global__ __launch_bounds__(ATTN_THREADS, DP <= 64 ? 2 : 1) void attn_bwd_kv_ke
                 st_lse = e == -attn_inf() ? attn_inf() : e * ATTN_LOG2E;
                 if (TYPE == ATTN_F16) st_lse -= (float)F16_P_EXPONENT;
                 st_delta = live ? -del[i] : 0.0f;
+                st_many = live ? many[i] : 0;
                 st_lim = row_limit(a, b, i);
                 if (map != nullptr) st_doc = doc_of_query(a, b, i);
                 if (a.bias == 1) st_x = (float)(i + a.Lk - a.Lq);
@@ -1059,6 +1071,7 @@ __global__ __launch_bounds__(ATTN_THREADS, DP <= 64 ? 2 : 1) void attn_bwd_kv_ke
                 row_delta[tid] = st_delta;
                 row_lim[tid] = st_lim;
                 row_doc[tid] = st_doc;
+                row_many[tid] = st_many;
                 row_x[tid] = st_x;
                 row_y[tid] = st_y;
             }
@@ -1113,6 +1126,7 @@ __global__ __launch_bounds__(ATTN_THREADS, DP <= 64 ? 2 : 1) void attn_bwd_kv_ke
 #pragma unroll
                     for (int t = 0; t < 2; ++t) {
                         const i32x4 lim = *reinterpret_cast<const i32x4 *>(row_lim + 32 * tp + 16 * t + 4 * g);
+                        const i32x4 more = *reinterpret_cast<const i32x4 *>(row_many + 32 * tp + 16 * t + 4 * g);
                         i32x4 qd = {0, 0, 0, 0};
                         if (by_doc) qd = *reinterpret_cast<const i32x4 *>(row_doc + 32 * tp + 16 * t + 4 * g);
 #pragma unroll
@@ -1123,7 +1137,7 @@ __global__ __launch_bounds__(ATTN_THREADS, DP <= 64 ? 2 : 1) void attn_bwd_kv_ke
                             for (int r = 0; r < 4; ++r) {
                                 const unsigned ok = mask_below(j, lim[r]) & mask_equal(qd[r], own);
                                 p[r] = keep_or_zero(ok, p[r]);
-                                ds[r] = keep_or_zero(ok, ds[r]);
+                                ds[r] = keep_or_zero(ok & (unsigned)more[r], ds[r]);
                             }
                             s[t][n] = p;
                             dp[t][n] = ds;
@@ -1369,13 +1383,13 @@ extern "C" int dgl_attention_forward(const dgl_attention_t *p, float *ws, dgl_st
     return by_type<LaunchFwd>(a, p->dtype, n, (hipStream_t)stream);
 }
 
-// Workspace of the backward pass: delta and (half precision) the row scales, the slopes' partial sums, the parts of dk / dv
+// Workspace of the backward pass: delta, (half precision) the row scales, the rows' flags, the slopes' partial sums, the parts of dk / dv
 int64_t backward_rows(const dgl_attention_t *p) { return ((int64_t)p->B * p->Hq * p->Lq + 3) / 4 * 4; }
 int64_t backward_slopes(const dgl_attention_t *p) { return ((int64_t)p->B * p->Hq * ((p->Lq + 63) / 64) + 3) / 4 * 4; }
 
 extern "C" int64_t dgl_attention_backward_workspace_floats(const dgl_attention_t *p) {
     if (check_attention(p) != DGL_OK) return -1;
-    return 2 * backward_rows(p) + backward_slopes(p) + keys_floats(attention_args(p), p->dtype) + 4;
+    return 3 * backward_rows(p) + backward_slopes(p) + keys_floats(attention_args(p), p->dtype) + 4;
 }
 
 extern "C" int dgl_attention_backward(const dgl_attention_t *p, const dgl_attention_grad_t *g, float *ws, dgl_stream_t stream) {
@@ -1395,8 +1409,9 @@ extern "C" int dgl_attention_backward(const dgl_attention_t *p, const dgl_attent
     }
     a.delta = ws;
     a.rowscale = ws + backward_rows(p);
-    a.dslope_part = g->dslope != nullptr ? ws + 2 * backward_rows(p) : nullptr;
-    a.part = ws + 2 * backward_rows(p) + backward_slopes(p);
+    a.many = reinterpret_cast<int *>(ws + 2 * backward_rows(p));
+    a.dslope_part = g->dslope != nullptr ? ws + 3 * backward_rows(p) : nullptr;
+    a.part = ws + 3 * backward_rows(p) + backward_slopes(p);
     hipStream_t s = (hipStream_t)stream;
     if (p->Lq > 0) {
         const int n = two_blocks(KERNEL_BWD_Q, p->dtype, a, a.Lq, a.Hq) ? 2 : 1;

@@ -370,3 +370,32 @@ def test_wide_ids_and_prefixes_keep_their_sign(device):
     far = torch.tensor([2 ** 40], device=device)
     assert torch.equal(attention(t["q"], t["k"], t["v"], causal=True, prefix=far),
                        attention(t["q"], t["k"], t["v"], causal=True, prefix=far.clamp(max=40).int()))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("L,kind", [(1, "one"), (1, "causal"), (5, "documents"), (200, "documents"), (130, "pairs")])
+def test_a_single_key_leaves_no_score_gradient(device, dtype, L, kind):
+    """A row with one key has the probability 1 whatever its score: dq, dk and dslope are exactly zero where all rows are such,
+    dv is dout; beside rows with more keys only they get a gradient."""
+    from dgl_amd.attention import attention
+    for D, H, K in ((16, 4, 2), (64, 2, 2), (128, 2, 1)):
+        t, kw = inputs(2, H, K, L, L, D, TYPES[dtype], L, bias="coords")
+        causal = kind == "causal"
+        if kind in ("documents", "pairs"):
+            ids = torch.arange(L, device=device, dtype=torch.int32).expand(2, L).contiguous()
+            if kind == "pairs":
+                ids[:, 100:] //= 2
+            kw["doc_q"] = kw["doc_k"] = ids
+        leaves = [t[n].clone().requires_grad_() for n in "qkv"] + [kw["slope"].clone().requires_grad_()]
+        attention(*leaves[:3], **dict(kw, slope=leaves[3], causal=causal, cap=5.0)).backward(t["dout"])
+        ids = kw.get("doc_q", torch.zeros(2, L, device=device))[0]
+        single = (ids[:, None] == ids[None]).sum(1) == 1           # (halved ids meet some of the first hundred)
+        assert not leaves[0].grad[:, :, single].any() and not leaves[1].grad[:, :, single].any()
+        assert int(single.sum()) == (85 if kind == "pairs" else L)
+        if kind == "pairs":
+            assert bool(leaves[0].grad[:, :, ~single].any()) and bool(leaves[1].grad[:, :, ~single].any())
+        else:
+            assert not leaves[3].grad.any()
+        want = reference(t["q"], t["k"], t["v"], t["dout"], cap=5.0, causal=causal, **kw)
+        for x, n in zip(leaves, ("dq", "dk", "dv")):
+            assert_within(x.grad, want[n], n)
