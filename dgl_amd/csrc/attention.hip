@@ -356,7 +356,8 @@ __global__ __launch_bounds__(ATTN_THREADS, TYPE == ATTN_F32 && DP == 128 ? 1 : 2
 #pragma unroll
                     for (int t = 0; t < KB; ++t)
 #pragma unroll
-                        for (int r = 0; r < 4; ++r) s[t][n][r] = fmaf(-2.0f * sp.cap2, cap_r(scaled<TYPE>(s[t][n][r], sp.mul2)), high);
+                        for (int r = 0; r < 4; ++r) s[t][n][r] = TYPE == ATTN_F32 ? fmaf(2.0f * sp.cap2, cap_h(s[t][n][r]), -w[n])
+                                                          : fmaf(-2.0f * sp.cap2, cap_r(s[t][n][r] * sp.mul2), high);
                 }
             } else {
 #pragma unroll
@@ -535,9 +536,15 @@ __device__ __forceinline__ void pair_probability(const ScoreParams &sp, f32x4 (&
                 f32x4 x = s[t][n], k = x;
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
-                    const float y = cap_r(scaled<TYPE>(x[r], sp.mul2));
-                    x[r] = fmaf(-2.0f * sp.cap2, y, sp.cap2 - e[t][n][r]);
-                    k[r] = fmaf(-y, y, y);
+                    if constexpr (TYPE == ATTN_F32) {
+                        const float y = cap_h(x[r]);
+                        x[r] = fmaf(2.0f * sp.cap2, y, -e[t][n][r]);
+                        k[r] = fmaf(-y, y, 0.25f);
+                    } else {
+                        const float y = cap_r(x[r] * sp.mul2);
+                        x[r] = fmaf(-2.0f * sp.cap2, y, sp.cap2 - e[t][n][r]);
+                        k[r] = fmaf(-y, y, y);
+                    }
                 }
                 s[t][n] = x;
                 if constexpr (FOLD) dp[t][n] = dp[t][n] * k;

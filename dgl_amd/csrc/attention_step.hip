@@ -300,7 +300,7 @@ __global__ __launch_bounds__(64 * STEP_WAVES) void attn_step_kernel(StepArgs a) 
 #pragma unroll
                 for (int n = 0; n < NQ; ++n)
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) s[x][n][r] = fmaf(-2.0f * sp.cap2, cap_r(s[x][n][r] * sp.mul2), sp.cap2);
+                    for (int r = 0; r < 4; ++r) s[x][n][r] = 2.0f * sp.cap2 * cap_h(s[x][n][r] * sp.mul2);
         } else {
 #pragma unroll
             for (int x = 0; x < 2; ++x)

@@ -73,12 +73,19 @@ __device__ __forceinline__ float attn_tanh(float y) {
     const float near = fmaf(y * z, p, y);
     return z < 0.16f ? near : far;
 }
-// A capped score cap tanh(x / cap) is cap - 2 cap r with r = 1 / (e^{2x/cap} + 1): off by about cap 2^-24 absolutely, no
-// more than a binary32 score of that size is anyhow, in 11 issue slots instead of 23.  Above CAP_PRECISE the relative error
-// of small scores would count (4e-6 at 64): there tanh is taken to a few ulp.  In both, 1 - tanh^2 = 4 (r - r^2).
+// A capped score cap tanh(x / cap) is cap - 2 cap r with r = 1 / (e^{2x/cap} + 1), in 11 issue slots instead of 23: off by up to
+// 3 cap 2^-24 absolutely, which 16-bit operands and probabilities drown.  Binary32 takes 2 cap h with h = tanh / 2 =
+// (e^{2x/cap} / 2 - 1/2) / (e^{2x/cap} + 1): the difference is exact near zero, what remains is a quarter of that, for three more
+// operations.  Above CAP_PRECISE the relative error of small scores would count (4e-6 at 64): there tanh is taken to a few ulp.
+// 1 - tanh^2 = 4 (r - r^2) = 4 (1/4 - h^2).
 #define CAP_PRECISE 64.0f
 enum { CAP_NONE = 0, CAP_FAST = 1, CAP_EXACT = 2 };
 __device__ __forceinline__ float cap_r(float y2) { return __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(y2) + 1.0f); }
+
+__device__ __forceinline__ float cap_h(float y2) {
+    const float e = __builtin_amdgcn_exp2f(__builtin_amdgcn_fmed3f(y2, -__builtin_inff(), 60.0f));      // (infinity / infinity)
+    return fmaf(e, 0.5f, -0.5f) * __builtin_amdgcn_rcpf(e + 1.0f);
+}
 
 // the scalar part of a score, in units of log2
 struct ScoreParams {
@@ -99,7 +106,7 @@ __device__ __forceinline__ ScoreParams score_params(float scale, float cap, int 
 __device__ __forceinline__ float score_of(const ScoreParams &p, float dot, float &th) {
     th = 0.0f;
     if (p.cap == CAP_NONE) return dot * p.mul;
-    th = p.cap == CAP_FAST ? fmaf(-2.0f, cap_r(dot * p.mul2), 1.0f) : attn_tanh(dot * p.mul);
+    th = p.cap == CAP_FAST ? 2.0f * cap_h(dot * p.mul2) : attn_tanh(dot * p.mul);
     return p.cap2 * th;
 }
 
