@@ -17,14 +17,14 @@
 // recomputed pair by pair (careful_*), which costs nothing where all is finite.
 //
 // Bound by the issue of vector instructions, not by memory (a head's keys are read by all its row blocks from L2): a pair of
-// a forward pass takes 15 simple operations and 4 of exp / rcp / sqrt with a cap and coordinates in binary32 (a third of the
+// a forward pass takes 18 simple operations and 4 of exp / rcp / sqrt with a cap and coordinates in binary32 (a third of the
 // simple ones split probabilities into terms), 7 and 3 with a cap in 16 bits, and the 16-bit matrix instructions hold the
 // vector unit back for two thirds of their 17 cycles.  Measured, per launch:
-//   forward, 64 x 8 heads of 16, 1000 nodes, cap and coordinates, binary32                423 us  77 TFLOP/s
+//   forward, 64 x 8 heads of 16, 1000 nodes, cap and coordinates, binary32                447 us  73 TFLOP/s
 //   forward, 32 heads over 8 of 128, 8192 causal rows, cap, bf16                           860 us  640 TFLOP/s
-//   2 x 16 heads over 4 of 64, 2047 causal rows behind a prefix, slopes, bf16     forward 72, rows 86, keys 114 + 13 us
-//   8 heads of 64, 6000 rows in 9 documents, fp16                                 forward 91, rows 117, keys 169 us
-//   8 x 8 heads of 16, 1001 rows in 4 documents, cap and coordinates, binary32    forward 91, rows 109, keys 121 us
+//   2 x 16 heads over 4 of 64, 2047 causal rows behind a prefix, slopes, bf16     forward 71, rows 86, keys 111 + 13 us
+//   8 heads of 64, 6000 rows in 9 documents, fp16                                 forward 88, rows 114, keys 160 us
+//   8 x 8 heads of 16, 1001 rows in 4 documents, cap and coordinates, binary32    forward 89, rows 116, keys 121 us
 #include "attention_tile.h"
 
 #include <cfloat>
