@@ -83,7 +83,8 @@ enum { CAP_NONE = 0, CAP_FAST = 1, CAP_EXACT = 2 };
 __device__ __forceinline__ float cap_r(float y2) { return __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(y2) + 1.0f); }
 
 __device__ __forceinline__ float cap_h(float y2) {
-    const float e = __builtin_amdgcn_exp2f(__builtin_amdgcn_fmed3f(y2, -__builtin_inff(), 60.0f));      // (infinity / infinity)
+    // limited from above, or infinity / infinity would follow; v_minimum3_f32 leaves a NaN what it is (fmin and the median drop it)
+    const float e = __builtin_amdgcn_exp2f(__builtin_elementwise_minimum(y2, 60.0f));
     return fmaf(e, 0.5f, -0.5f) * __builtin_amdgcn_rcpf(e + 1.0f);
 }
 
