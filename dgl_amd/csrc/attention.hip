@@ -598,6 +598,9 @@ __device__ __forceinline__ int gradient_exponent(float amax) {
     return max(-100, min(100, 3 - ((int)(__float_as_uint(amax) >> 23) - 127)));
 }
 __device__ __forceinline__ float exp2_of(int e) { return __uint_as_float((unsigned)(127 + e) << 23); }
+// The scale of a row whose score gradients are zero - no gradient of its own, no key or a single one - or not finite, which the
+// careful path deals with: larger than every other, so that it never is the least
+#define NO_SCALE 0x1p127f
 
 // ---- query rows: dq of NQ x 16 rows per wave, with delta_i = do_i . o_i on the way (kept for the kernel that owns the
 // keys) and the rows' share of dslope.  sum_j ds_ij is zero by definition; what it is with the delta at hand (o may have
@@ -701,14 +704,17 @@ __global__ __launch_bounds__(ATTN_THREADS, DP <= 64 ? 2 : 1) void attn_bwd_q_ker
         const float lse = live ? a.lse[at] : -attn_inf();
         lse2[n] = lse == -attn_inf() ? attn_inf() : lse * ATTN_LOG2E;
         rs[n] = 1.0f;
+        float key_scale = NO_SCALE;
         if constexpr (TYPE == ATTN_F16) {          // probabilities carry the row's scale through their exponent
-            const int e = gradient_exponent(group_max(amax));
+            amax = group_max(amax);
+            const int e = gradient_exponent(amax);
             rs[n] = exp2_of(e);
+            if (amax > 0.0f && amax < attn_inf() && lse2[n] != attn_inf()) key_scale = rs[n];
             lse2[n] -= (float)e;
         }
         if (live && g == 0) {
             a.delta[at] = delta[n];
-            if (TYPE == ATTN_F16) a.rowscale[at] = rs[n];
+            if (TYPE == ATTN_F16) a.rowscale[at] = key_scale;
         }
         limit[n] = row_limit(a, b, i);
         doc[n] = map != nullptr ? doc_of_query(a, b, i) : 0;
@@ -861,7 +867,10 @@ __global__ __launch_bounds__(ATTN_THREADS, DP <= 64 ? 2 : 1) void attn_bwd_q_ker
 #pragma unroll
             for (int d = 0; d < S::dt; ++d)
                 if (16 * d + 4 * g < a.D) store4<TYPE>(out + 16 * d + 4 * g, single ? f32x4{0.0f, 0.0f, 0.0f, 0.0f} : dq[n][d] * undo);
-            if (g == 0) a.many[((int64_t)b * a.Hq + h) * a.Lq + i] = single ? 0 : -1;
+            if (g == 0) {
+                a.many[((int64_t)b * a.Hq + h) * a.Lq + i] = single ? 0 : -1;
+                if (TYPE == ATTN_F16 && single) a.rowscale[((int64_t)b * a.Hq + h) * a.Lq + i] = NO_SCALE;
+            }
         }
         for (; bad != 0; bad &= bad - 1) {
             const int cc = __ffsll((long long)bad) - 1;
@@ -1024,16 +1033,17 @@ __global__ __launch_bounds__(ATTN_THREADS, DP <= 64 ? 2 : 1) void attn_bwd_kv_ke
 
     float gscale = 1.0f;
     if constexpr (TYPE == ATTN_F16) {               // one scale for all rows: that of the largest gradient among them
-        unsigned least = 0x7f000000u;
+        const unsigned none = __float_as_uint(NO_SCALE);
+        unsigned least = none;
         for (int h = h0; h < h1; ++h)
             for (int x = tid; x < a.Lq; x += ATTN_THREADS) least = min(least, __float_as_uint(a.rowscale[((int64_t)b * a.Hq + h) * a.Lq + x]));
 #pragma unroll
         for (int x = 1; x < 64; x <<= 1) least = min(least, (unsigned)__shfl_xor((int)least, x));
-        if (tid == 0) least_scale = 0x7f000000u;
+        if (tid == 0) least_scale = none;
         __syncthreads();
         if (lane == 0) atomicMin(&least_scale, least);
         __syncthreads();
-        gscale = __uint_as_float(least_scale);
+        gscale = least_scale == none ? 1.0f : __uint_as_float(least_scale);
     }
     const float gmul = TYPE == ATTN_F16 ? gscale * exp2_of(-F16_P_EXPONENT) : 1.0f;
 
