@@ -8,7 +8,6 @@ from __future__ import annotations
 
 import ctypes
 import functools
-import math
 import os
 from typing import Dict, Optional
 
@@ -152,12 +151,22 @@ def forward_range_guarded(engine, policy: "PackedPolicy") -> None:
             engine.arithmetic = _lib.ARITH_SPLIT_F16
 
 
+# Log-probabilities under controls: an offered action's least, everything else's; a hypothesis' sum that holds one of the
+# latter, or the -1e20 that a beam's first expansion has for all rows but the first (utils/beamsearch.py:68-69).  1e10 decisions
+# at LEAST_OFFERED are still above LOST.
+LEAST_OFFERED, NOT_OFFERED, LOST = -1e9, -1e25, -1e19
+
+
 def controlled_log_probs(engine, controls):
     """Dense log-probabilities [R, A] of the last forward() under a search's controls (dgl_amd/logits.py), and the greedy
     pick per row.  Only actions the policy itself offers can be taken: non-candidates (1e-20 in the dense tensor) and
     infeasible moves (the floor, 1e-7) stay out whatever the controls add.  A row whose controls leave nothing keeps the
-    policy's own probabilities.  Values below log 1e-20 are that, as in the dense tensor of the reference
-    (TSP/TSPModel.py:328-337), so that a beam wider than its candidates behaves as without controls."""
+    policy's own probabilities.
+
+    What is not offered is NOT_OFFERED, so far below everything that is (LEAST_OFFERED at the least) that no sum of a
+    hypothesis' values makes up for it: a beam wider than its candidates is filled with hypotheses at or below LOST, which
+    beam_rollout gives an infinite length.  (The 1e-20 of the reference's dense tensor, TSP/TSPModel.py:328-337, is a value
+    that a cold temperature or a bias reaches with an offered action.)"""
     from .logits import process_logits
     dense = engine.dense_probs()
     lp = torch.where(dense > 1.0000001e-7, dense.log(), float("-inf"))
@@ -165,8 +174,9 @@ def controlled_log_probs(engine, controls):
                               history=controls.history, history_len=controls.history_len, repetition=controls.repetition,
                               presence=controls.presence, frequency=controls.frequency)
     none = sel < 0
-    out = torch.where(none[:, None], lp, out).clamp_min_(math.log(1e-20))
-    return out, torch.where(none, engine.selected, sel)
+    out = torch.where(none[:, None], lp, out)
+    return (torch.where(out > float("-inf"), out.clamp_min(LEAST_OFFERED), NOT_OFFERED),
+            torch.where(none, engine.selected, sel))
 
 
 def dense_beam_advance(engine, controls, scores, beam, step, prev_k, action, actions):
@@ -174,6 +184,11 @@ def dense_beam_advance(engine, controls, scores, beam, step, prev_k, action, act
     lp, _ = controlled_log_probs(engine, controls)
     check(engine.lib.dgl_beam_advance(ptr(lp), ptr(scores), engine.R // beam, beam, actions, step, ptr(prev_k), ptr(action),
                                       stream_ptr()), "dgl_beam_advance")
+
+
+def lengths_that_count(engine, length):
+    """Lengths of the last rollout's rows; infinite for beams under controls that were filled with actions nobody offered."""
+    return length if engine.lost is None else length.masked_fill(engine.lost, float("inf"))
 
 
 class TspEngine:
@@ -205,6 +220,7 @@ class TspEngine:
         self.t = 0
         self.tile_t = -1                 # step count the neighbourhood buffers (idx, tile) belong to
         self.linked = False              # the last step's nodes are in the back-pointer history only
+        self.lost = None                 # rows of a beam rollout under controls that hold no valid solution
         self._beam_bufs = None
 
     def _alloc_outputs(self) -> None:
@@ -256,6 +272,7 @@ class TspEngine:
         self.t = 0
         self.tile_t = -1
         self.linked = False
+        self.lost = None
 
     @on_own_device
     def step(self, selected: torch.Tensor, want_knn: bool = True) -> None:
@@ -421,7 +438,8 @@ class TspEngine:
         """Beam-search decode (TSP/TSPTester.py:145-199) on the compact state: per step the policy, the beam
         expansion over beam*k candidates and one pass over the state that follows the back-pointers while it
         updates; the tours are rebuilt from the back-pointer history at the end.  Nothing returns to the host.
-        ``controls`` (dgl_amd.logits.LogitControls) steer every expansion, over dense log-probabilities."""
+        ``controls`` (dgl_amd.logits.LogitControls) steer every expansion, over dense log-probabilities; rows that hold no
+        tour because a beam had fewer candidates than rows have an infinite length."""
         assert self.rpi % beam == 0 and len(self.bufs) == 2
         G = self.R // beam
         dev = self.device
@@ -442,7 +460,8 @@ class TspEngine:
         if self.N >= 2:
             self.backtrack(2)
         self.beam_scores = scores
-        return self.tour_length()
+        self.lost = None if controls is None else scores.view(-1) <= LOST
+        return lengths_that_count(self, self.tour_length())
 
 
 class CvrpEngine:
@@ -484,6 +503,7 @@ class CvrpEngine:
         self.t = 0
         self.tile_t = -1
         self.linked = False
+        self.lost = None
 
     def _alloc_outputs(self) -> None:
         w = max(MAX_TOKENS, self.ntok_max)
@@ -540,6 +560,7 @@ class CvrpEngine:
         self.t = 0
         self.tile_t = -1
         self.linked = False
+        self.lost = None
 
     @on_own_device
     def step(self, action: torch.Tensor, want_knn: bool = True) -> None:
@@ -688,7 +709,7 @@ class CvrpEngine:
     def beam_rollout(self, policy: PackedPolicy, start_action: torch.Tensor, beam: int, controls=None) -> torch.Tensor:
         """Beam-search decode (CVRP/CVRPTester.py:147-227) on the compact state; the step follows the
         back-pointers while it updates, nodes and flags are rebuilt from the history at the end.  ``controls``
-        (dgl_amd.logits.LogitControls) steer every expansion, over dense log-probabilities."""
+        (dgl_amd.logits.LogitControls) steer every expansion, over dense log-probabilities (as TspEngine.beam_rollout)."""
         assert self.rpi % beam == 0 and len(self.bufs) == 2
         G = self.R // beam
         dev = self.device
@@ -709,4 +730,5 @@ class CvrpEngine:
         if self.N >= 2:
             self.backtrack(2)
         self.beam_scores = scores
-        return self.route_length()
+        self.lost = None if controls is None else scores.view(-1) <= LOST
+        return lengths_that_count(self, self.route_length())

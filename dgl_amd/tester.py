@@ -15,6 +15,7 @@ import torch
 from . import distributed as D
 from .beamsearch import Beamsearch
 from .cvrp import CVRPEnv, CVRPModel
+from .engine import lengths_that_count
 from .tsp import TSPEnv, TSPModel
 from .weights import load_checkpoint
 
@@ -161,7 +162,7 @@ class TSPTester(_TesterBase):
             length = eng.beam_rollout(policy, sel, beam_size, controls=controls)
         env.selected_count = eng.t
         if getattr(env, "_orig_xy", None) is not None:             # aug_test: lengths on the original coordinates
-            length = env._get_travel_distance()
+            length = lengths_that_count(eng, env._get_travel_distance())
         shortest, index = self._summarise(length, beam_size)
         self.last_tours = env.selected_node_list
         self.last_lengths = length
@@ -250,7 +251,7 @@ class CVRPTester(_TesterBase):
                   eng.beam_rollout(policy, sel, beam_size, controls=controls))
         env.selected_count = eng.t
         if getattr(env, "_orig_xy", None) is not None:             # aug_test: lengths on the original coordinates
-            length = env.cal_length()
+            length = lengths_that_count(eng, env.cal_length())
         shortest, index = self._summarise(length, beam_size)
         self.last_tours = env.selected_node_list
         self.last_flags = env.step_state.selected_flag

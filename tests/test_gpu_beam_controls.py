@@ -1,0 +1,106 @@
+"""Beam search under controls expands what the policy offers and nothing else, however far the controls push it."""
+import math
+
+import pytest
+import torch
+
+from test_gpu_search_controls import cvrp, tsp
+
+pytestmark = pytest.mark.gpu
+
+
+def check_tsp(eng, length):
+    """Every row whose length counts is a tour; every group has such a row."""
+    fin = length.isfinite()
+    tours = eng.state["tour"].long()
+    whole = (tours.sort(1)[0] == torch.arange(eng.N, device=tours.device)).all(1)
+    assert bool(whole[fin].all()), f"{int((fin & ~whole).sum())} of {len(fin)} rows are no tours and have a length"
+    return fin
+
+
+def check_cvrp(eng, length):
+    """... visits every customer once within the capacity."""
+    fin = length.isfinite()
+    nodes = eng.state["nodes"].long()
+    whole = (nodes.sort(1)[0] == torch.arange(1, eng.N + 1, device=nodes.device)).all(1)
+    seq = torch.arange(eng.R, device=nodes.device) // eng.rpi
+    demand = eng.demand[seq].double().gather(1, nodes)
+    load = torch.zeros(eng.R, device=nodes.device, dtype=torch.float64)
+    ok = whole.clone()
+    for t in range(eng.N):
+        load = torch.where(eng.state["flags"][:, t] == 1, demand[:, t], load + demand[:, t])
+        ok &= load <= 1 + 1e-5
+    assert bool(ok[fin].all()), f"{int((fin & ~ok).sum())} of {len(fin)} rows break the rules and have a length"
+    return fin
+
+
+def controls(kind, R, actions, device):
+    from dgl_amd.logits import LogitControls
+    if kind == "cold":
+        return LogitControls(temperature=0.1)
+    if kind == "bias":
+        bias = torch.zeros(actions, device=device)
+        bias[::2] = -60.0
+        return LogitControls(bias=bias)
+    if kind == "far bias":
+        return LogitControls(bias=torch.where(torch.arange(actions, device=device) % 3 == 0, 0.0, -1e30))
+    if kind == "presence":
+        every = torch.arange(0, actions, 2, device=device, dtype=torch.int32).expand(R, -1)
+        return LogitControls(history=every, presence=200.0)
+    blocked = torch.zeros(R, (actions + 63) // 64, dtype=torch.int64, device=device)
+    blocked[:, 0] = 0x5555_5555_5555
+    return LogitControls(blocked=blocked, temperature=0.3)
+
+
+KINDS = ["cold", "bias", "far bias", "presence", "blocked"]
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("knn,beam", [(5, 4), (5, 16), (20, 4), (2, 8)])
+def test_tsp_rows_that_count_are_tours(device, kind, knn, beam):
+    for weights in ("trained", "random"):
+        eng, pol, start = tsp(device, B=4, N=30, rpi=beam, knn=knn, weights=weights)
+        length = eng.beam_rollout(pol, start, beam, controls=controls(kind, eng.R, eng.N, device))
+        assert bool(check_tsp(eng, length).view(-1, beam).any(1).all())
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("knn,beam", [(4, 4), (4, 16), (10, 4), (1, 8)])
+def test_cvrp_rows_that_count_keep_the_rules(device, kind, knn, beam):
+    for weights in ("trained", "random"):
+        eng, pol, start = cvrp(device, B=4, N=24, rpi=beam, knn=knn, weights=weights)
+        length = eng.beam_rollout(pol, start, beam, controls=controls(kind, eng.R, 2 * (eng.N + 1), device))
+        assert bool(check_cvrp(eng, length).view(-1, beam).any(1).all())
+
+
+def test_multi_starts_and_a_rollout_without_controls_afterwards(device):
+    from dgl_amd.logits import LogitControls
+    eng, pol, start = tsp(device, B=3, N=30, rpi=8, knn=3)
+    start = (start + torch.arange(8, device=device).repeat_interleave(4)[: 8].repeat(3)).to(torch.int32)   # two starts of four beams
+    length = eng.beam_rollout(pol, start, 4, controls=LogitControls(temperature=0.05))
+    assert bool(check_tsp(eng, length).view(-1, 4).any(1).all())
+    assert eng.beam_rollout(pol, start, 4).isfinite().all()          # lengths as before without controls
+
+
+def test_tester_under_augmentation(device):
+    """Lengths measured again on the original coordinates keep the rows that do not count out."""
+    import os
+    import tempfile
+    from conftest import GOLDEN
+    from dgl_amd import TSPTester, formats
+    from dgl_amd.logits import LogitControls
+    tp = {"use_cuda": True, "cuda_device_num": 0, "knn": 2, "test_batch_size": 2, "beam_size": 16, "problem_size": 20,
+          "test_episodes": 2, "test_episodes_all": 2, "model_load": {"enable": True, "path": GOLDEN, "file": "ckpt_tsp_nn.pt"},
+          "logit_controls": LogitControls(temperature=0.1)}
+    model = {"mode": "test", "embedding_dim": 128, "head_num": 8, "qkv_dim": 16, "ff_hidden_dim": 512, "decoder_layer_num": 3}
+    with tempfile.TemporaryDirectory() as d:
+        path = os.path.join(d, "x.txt")
+        formats.write_tsp_instances(path, torch.rand(2, 20, 2, generator=torch.Generator().manual_seed(0)))
+        for mode, aug in (("pomo_test", 1), ("aug_test", 8)):
+            env = {"mode": "test", "test_mode": mode, "aug_size": aug, "data_path": path, "baseline_path": ""}
+            t = TSPTester(env_params=env, model_params=dict(model), tester_params=dict(tp))
+            t.run()
+            assert math.isfinite(t.score)
+            fin = t.last_lengths.isfinite()
+            whole = (t.last_tours.long().sort(1)[0] == torch.arange(20, device=t.last_tours.device)).all(1)
+            assert bool(whole[fin].all())
