@@ -159,8 +159,8 @@ LEAST_OFFERED, NOT_OFFERED, LOST = -1e9, -1e25, -1e19
 
 def controlled_log_probs(engine, controls):
     """Dense log-probabilities [R, A] of the last forward() under a search's controls (dgl_amd/logits.py), and the greedy
-    pick per row.  Only actions the policy itself offers can be taken: non-candidates (1e-20 in the dense tensor) and
-    infeasible moves (the floor, 1e-7) stay out whatever the controls add.  A row whose controls leave nothing keeps the
+    pick per row.  Only actions the policy itself offers can be taken: the feasible ones among the candidates of this decision;
+    all others stay out whatever the controls add.  A row whose controls leave nothing keeps the
     policy's own probabilities.
 
     What is not offered is NOT_OFFERED, so far below everything that is (LEAST_OFFERED at the least) that no sum of a
@@ -168,8 +168,7 @@ def controlled_log_probs(engine, controls):
     beam_rollout gives an infinite length.  (The 1e-20 of the reference's dense tensor, TSP/TSPModel.py:328-337, is a value
     that a cold temperature or a bias reaches with an offered action.)"""
     from .logits import process_logits
-    dense = engine.dense_probs()
-    lp = torch.where(dense > 1.0000001e-7, dense.log(), float("-inf"))
+    lp = engine.offered_log_probs()
     out, sel = process_logits(lp, blocked=controls.blocked, bias=controls.bias, temperature=controls.temperature,
                               history=controls.history, history_len=controls.history_len, repetition=controls.repetition,
                               presence=controls.presence, frequency=controls.frequency)
@@ -310,6 +309,12 @@ class TspEngine:
         check(self.lib.dgl_policy_scatter_probs(ctypes.byref(io), ptr(self.prob), ptr(out), self.N, stream_ptr()),
               "dgl_policy_scatter_probs")
         return out
+
+    @on_own_device
+    def offered_log_probs(self) -> torch.Tensor:
+        """Log-probabilities [R, N] of the last forward() at its candidates, -inf elsewhere."""
+        out = torch.full((self.R, self.N), float("-inf"), device=self.device)
+        return out.scatter_(1, self.idx[:, :self.k].long(), self.prob[:, :self.k].log())
 
     @on_own_device
     def permute(self, prev_k: torch.Tensor, beam: int) -> None:
@@ -604,6 +609,17 @@ class CvrpEngine:
         check(self.lib.dgl_policy_scatter_probs(ctypes.byref(io), ptr(self.prob), ptr(out), A, stream_ptr()),
               "dgl_policy_scatter_probs")
         return out
+
+    @on_own_device
+    def offered_log_probs(self) -> torch.Tensor:
+        """Log-probabilities [R, 2 (N + 1)] of the last forward() at its candidates - direct moves where they are feasible -
+        and -inf elsewhere.  (The probabilities do not tell: an infeasible move has the floor's 1e-7, which a feasible one
+        below 1e-14 has as well.)"""
+        kl, kd = self.kl, self.kd
+        out = torch.full((self.R, 2 * (self.N + 1)), float("-inf"), device=self.device)
+        near = self.prob[:, :kl].log().masked_fill(self.infeasible[:, :kl] != 0, float("-inf"))
+        out.scatter_(1, self.idx_last[:, :kl].long(), near)
+        return out.scatter_(1, self.idx_dep[:, :kd].long() + (self.N + 1), self.prob[:, kl + 1:kl + 1 + kd].log())
 
     @on_own_device
     def permute(self, prev_k: torch.Tensor, beam: int) -> None:

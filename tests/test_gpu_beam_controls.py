@@ -104,3 +104,61 @@ def test_tester_under_augmentation(device):
             fin = t.last_lengths.isfinite()
             whole = (t.last_tours.long().sort(1)[0] == torch.arange(20, device=t.last_tours.device)).all(1)
             assert bool(whole[fin].all())
+
+
+@pytest.mark.parametrize("problem", ["tsp", "cvrp"])
+def test_decisions_offer_candidates_alone(device, problem):
+    """One decision: what is above the floor are the policy's feasible candidates, with the softmax of the controlled values."""
+    from dgl_amd.engine import controlled_log_probs
+    from dgl_amd.logits import LogitControls
+    eng, pol, start = (tsp if problem == "tsp" else cvrp)(device, B=6, N=30, knn=7)
+    eng.reset()
+    eng.step(start)
+    for t in range(1, 12):
+        eng.forward(pol, want_logits=False)
+        bias = torch.randn(eng.N if problem == "tsp" else 2 * (eng.N + 1), device=device) * 40
+        lp, sel = controlled_log_probs(eng, LogitControls(bias=bias, temperature=0.2))
+        dense = eng.dense_probs().double()
+        offered = dense > 1e-19
+        if problem == "cvrp":
+            near = eng.idx_last[:, :eng.kl].long()
+            offered.scatter_(1, near, offered.gather(1, near) & (eng.infeasible[:, :eng.kl] == 0))
+        x = torch.where(offered, (dense.log() + bias.double()) / 0.2, -math.inf)
+        want = torch.log_softmax(x, 1)
+        assert torch.equal(lp > -1e19, offered)
+        # binary32: the logarithm, the bias and the division round values of up to 1e3 by 2^-24 each, the sum adds 1e-5
+        size = x[offered].abs().max()
+        assert (lp.double() - want)[offered].abs().max() <= 8 * 2.0 ** -24 * size + 1e-5
+        assert torch.equal(sel.long(), lp.argmax(1))
+        eng.step(sel)
+
+
+@pytest.mark.parametrize("problem", ["tsp", "cvrp"])
+def test_improbable_candidates_are_candidates(device, problem):
+    """A policy that is certain of one candidate (the others' softmax is below 1e-14, their probability the floor): with that
+    one blocked another candidate is taken, not the blocked one."""
+    from dgl_amd.logits import LogitControls
+    from dgl_amd.engine import PackedPolicy, controlled_log_probs
+    eng, pol, start = (tsp if problem == "tsp" else cvrp)(device, B=6, N=30, knn=7, weights="random")
+    sd = {n: x.clone() for n, x in pol.sd.items()}
+    sd["decoder.Linear_final.weight"] *= 3e4
+    pol = PackedPolicy(sd, pol.problem, device)
+    eng.reset()
+    eng.step(start)
+    saw = 0
+    for t in range(1, 20):
+        eng.forward(pol, want_logits=False)
+        own = eng.selected.clone().long()
+        near = eng.offered_log_probs()
+        offered = near > -math.inf
+        alone = (near > math.log(2e-7)).sum(1) == 1                # the rest at the floor
+        actions = near.shape[1]
+        bits = torch.zeros(eng.R, (actions + 63) // 64, dtype=torch.int64, device=device)
+        bits.scatter_(1, (own // 64)[:, None], (torch.ones_like(own) << (own % 64))[:, None])
+        lp, sel = controlled_log_probs(eng, LogitControls(blocked=bits))
+        more = offered.sum(1) > 1
+        assert bool(offered.gather(1, sel.long()[:, None]).all())
+        assert bool((sel.long() != own)[more].all()) and bool((sel.long() == own)[~more].all())
+        saw += int((alone & more).sum())
+        eng.step(sel)
+    assert saw > 0
