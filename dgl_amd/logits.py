@@ -27,9 +27,14 @@ class LogitControls:
     """What ``process_logits`` applies at every decision of a rollout (TspEngine / CvrpEngine.greedy_rollout and
     beam_rollout; the testers' ``tester_params['logit_controls']``), on top of the states' own masks.
 
-    ``bias`` [actions] or [rows, actions]; ``temperature``; ``blocked`` int64 words [rows, n], actions never taken while
-    another one is left; ``history`` int32 [rows, n] with ``history_len`` [rows] live entries, actions to penalise - for
-    instance the first moves of solutions found earlier."""
+    ``bias`` [actions] or [rows, actions]; ``temperature``; ``blocked`` int64 words [rows, n], actions never taken while the
+    policy offers another one - its feasible candidates at that decision, not every node that is left: a row whose candidates
+    are all blocked takes the policy's own choice; ``history`` int32 [rows, n] with ``history_len`` [rows] live entries, actions
+    to penalise - for instance the first moves of solutions found earlier.
+
+    They apply to the policy's log-probabilities, which are never positive: a repetition penalty always multiplies.  Row-wise
+    controls belong to the engine's rows and stay with them.  In a beam rollout a row is a slot of its beam, which hypotheses
+    enter and leave: give all slots of a beam the same."""
     bias: Optional[torch.Tensor] = None
     temperature: float = 1.0
     repetition: PerRow = 1.0

@@ -162,3 +162,30 @@ def test_improbable_candidates_are_candidates(device, problem):
         saw += int((alone & more).sum())
         eng.step(sel)
     assert saw > 0
+
+
+@pytest.mark.parametrize("problem", ["tsp", "cvrp"])
+def test_only_candidates_count_for_blocked_actions(device, problem):
+    """Small neighbourhoods whose candidates are all blocked: the policy's own choice, though nodes outside are not blocked; and
+    a penalty for repetitions multiplies log-probabilities."""
+    from dgl_amd.engine import controlled_log_probs
+    from dgl_amd.logits import LogitControls
+    eng, pol, start = (tsp if problem == "tsp" else cvrp)(device, B=6, N=30, knn=3)
+    eng.reset()
+    eng.step(start)
+    eng.forward(pol, want_logits=False)
+    near = eng.offered_log_probs()
+    offered = near > -math.inf
+    assert bool((offered.sum(1) <= 6).all())
+    at = torch.arange(near.shape[1], device=device)
+    words = torch.zeros(eng.R, 1, dtype=torch.int64, device=device)
+    for r in range(eng.R):
+        for a in at[offered[r]].tolist():
+            words[r, 0] |= 1 << a if a < 63 else -1 << 63
+    lp, sel = controlled_log_probs(eng, LogitControls(blocked=words))
+    assert torch.equal(sel, eng.selected) and torch.equal(lp > -1e19, offered)
+    best = near.argmax(1)
+    lp, _ = controlled_log_probs(eng, LogitControls(history=best.to(torch.int32)[:, None], repetition=3.0))
+    x = near.double()
+    x.scatter_(1, best[:, None], 3.0 * x.gather(1, best[:, None]))
+    assert (lp.double() - torch.log_softmax(x, 1))[offered].abs().max() <= 1e-5
