@@ -143,6 +143,9 @@ SIGNATURES = {
     "dgl_attention_forward_workspace_floats": (c_int64, [POINTER(Attention)]),
     "dgl_attention_backward": (c_int32, [POINTER(Attention), POINTER(AttentionGrad), c_void_p, c_void_p]),
     "dgl_attention_backward_workspace_floats": (c_int64, [POINTER(Attention)]),
+    "dgl_document_ids": (c_int32, [c_int32, c_int32, c_int32, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_void_p,
+                                   c_void_p]),
+    "dgl_document_ids_workspace_floats": (c_int64, [c_int32, c_int32]),
     "dgl_cache_append": (c_int32, [POINTER(KVCache), c_void_p, c_void_p, c_void_p, c_void_p, c_int32, c_void_p, c_void_p,
                                    c_void_p, c_void_p]),
     "dgl_attention_step": (c_int32, [POINTER(AttentionStep), c_void_p, c_void_p]),

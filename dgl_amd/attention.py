@@ -21,6 +21,7 @@ from . import _lib
 from ._lib import check, ptr
 
 _DTYPES = {torch.float32: _lib.DTYPE_F32, torch.float16: _lib.DTYPE_F16, torch.bfloat16: _lib.DTYPE_BF16}
+_WIDE = (torch.int64, torch.uint32)                                 # integers that int32 does not hold
 _VEC = {torch.float32: 4, torch.float16: 8, torch.bfloat16: 8}      # elements of 16 bytes
 
 # A call of a few microseconds on the device is lost in a host path that sets ctypes fields one by one: the ABI structs are
@@ -79,7 +80,7 @@ def _check_qkv(q, k, v):
 
 
 def _side(t: Optional[torch.Tensor], name, shape, dtype, device) -> Optional[torch.Tensor]:
-    """A float32 / int32 side input, broadcast over the batch where it may be, inner axes consecutive."""
+    """A float32 / int32 / int64 side input, broadcast over the batch where it may be, inner axes consecutive."""
     if t is None:
         return None
     if t.device != device:
@@ -87,10 +88,10 @@ def _side(t: Optional[torch.Tensor], name, shape, dtype, device) -> Optional[tor
     if t.shape != shape:
         raise ValueError(f"{name} has shape {tuple(t.shape)}, expected {tuple(shape)}")
     if t.dtype != dtype:
-        if dtype == torch.int32 and t.is_floating_point() or dtype == torch.float32 and not t.is_floating_point():
+        if t.is_floating_point() != (dtype == torch.float32) or t.is_complex() or t.dtype == torch.uint64:
             raise ValueError(f"{name} is {t.dtype}, expected {dtype}")
-        if t.dtype == torch.int64:               # (2^32 + 5 is no 5: what does not fit stays beyond every bound)
-            t = t.clamp(-(1 << 31), (1 << 31) - 1)
+        if t.dtype in _WIDE and dtype == torch.int32:      # (2^32 + 5 is no 5: what does not fit stays beyond every bound)
+            t = t.to(torch.int64).clamp(-(1 << 31), (1 << 31) - 1)
         t = t.to(dtype)
     if t.is_contiguous():
         return t
@@ -100,6 +101,20 @@ def _side(t: Optional[torch.Tensor], name, shape, dtype, device) -> Optional[tor
             return t.contiguous()
         n *= size
     return t.contiguous() if len(shape) == 1 else t
+
+
+def _documents(doc_q, doc_k, B: int, L: int, M: int, device):
+    """Both sides' document ids as int32.  Ids of wider types are mapped to small ones that are equal where they are."""
+    if doc_q is None or not (doc_q.dtype in _WIDE or doc_k.dtype in _WIDE):
+        return _side(doc_q, "doc_q", (B, L), torch.int32, device), _side(doc_k, "doc_k", (B, M), torch.int32, device)
+    doc_q, doc_k = _side(doc_q, "doc_q", (B, L), torch.int64, device), _side(doc_k, "doc_k", (B, M), torch.int64, device)
+    ids_q, ids_k = (torch.empty((B, n), dtype=torch.int32, device=device) for n in (L, M))
+    if B:
+        lib = _lib.load()
+        ws = torch.empty(max(lib.dgl_document_ids_workspace_floats(B, M), 2), dtype=torch.float32, device=device)
+        _launch(device, lib.dgl_document_ids, B, L, M, doc_q.data_ptr(), doc_q.stride(0), doc_k.data_ptr(), doc_k.stride(0),
+                ids_q.data_ptr(), ids_k.data_ptr(), ws.data_ptr(), what="dgl_document_ids")
+    return ids_q, ids_k
 
 
 class _Call:
@@ -127,8 +142,7 @@ class _Call:
         self.slope = _side(slope, "slope", (H,), torch.float32, dev)
         self.pos_q = _side(pos_q, "pos_q", (B, L, 2), torch.float32, dev)
         self.pos_k = _side(pos_k, "pos_k", (B, M, 2), torch.float32, dev)
-        self.doc_q = _side(doc_q, "doc_q", (B, L), torch.int32, dev)
-        self.doc_k = _side(doc_k, "doc_k", (B, M), torch.int32, dev)
+        self.doc_q, self.doc_k = _documents(doc_q, doc_k, B, L, M, dev)
         self.prefix = _side(prefix, "prefix", (B,), torch.int32, dev)
         self.head = (_DTYPES[q.dtype], B, H, K, L, M, D, 1 if causal else 0, D ** -0.5 if scale is None else float(scale), cap,
                      *self.q.stride()[:3], *self.k.stride()[:3], *self.v.stride()[:3])
@@ -244,7 +258,7 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, scale: Optio
     ``scale``: default D ** -0.5.  ``cap`` > 0: scores pass through cap tanh(. / cap).  ``slope`` [H]: bias -slope dist,
     between the coordinates ``pos_q`` [B, Lq, 2] and ``pos_k`` [B, Lk, 2], or, without them, between positions
     (|i + Lk - Lq - j|).  ``doc_q`` [B, Lq] / ``doc_k`` [B, Lk]: whole numbers; tokens see their own document, negative ids
-    are padding (such rows give zeros).  ``causal``: j <= i + Lk - Lq, and in front of ``prefix`` [B] everything.
+    are padding (such rows give zeros); int64 ids cost three launches of a few microseconds, int32 ones none.  ``causal``: j <= i + Lk - Lq, and in front of ``prefix`` [B] everything.
 
     Under graph capture, leaves that collect gradients are refused: a leaf's accumulation belongs to the stream on which
     it was first used, and a captured backward pass that meets an eager graph of the same leaf ends the process.  Capture

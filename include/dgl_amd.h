@@ -421,6 +421,16 @@ DGL_API int dgl_attention_backward(const dgl_attention_t *a, const dgl_attention
 /* Floats of workspace dgl_attention_backward needs for `a` (-1: invalid arguments; beside TSP/TSPModel.py:420-441). */
 DGL_API int64_t dgl_attention_backward_workspace_floats(const dgl_attention_t *a);
 
+/* Document ids of 64 bits to the 32-bit ones above: ids_k[b][j] is the first position among doc_k[b] that has the id of j,
+ * ids_q[b][i] that of doc_q[b][i] (dense [B][Lk], [B][Lq]); -1 for a negative id, and for a row whose id no key has.  Strides in
+ * ids between batch entries.  ws: dgl_document_ids_workspace_floats floats, 8-byte aligned.  (The reference has one
+ * instance per row, TSP/TSPModel.py:420-441.) */
+DGL_API int dgl_document_ids(int32_t B, int32_t Lq, int32_t Lk, const int64_t *doc_q, int64_t doc_q_stride, const int64_t *doc_k,
+                             int64_t doc_k_stride, int32_t *ids_q, int32_t *ids_k, float *ws, dgl_stream_t stream);
+
+/* Floats of workspace dgl_document_ids needs (-1: invalid arguments; beside TSP/TSPModel.py:420-441). */
+DGL_API int64_t dgl_document_ids_workspace_floats(int32_t B, int32_t Lk);
+
 /* ------------------------------------------------------------------ paged key-value cache
  * Keys and values of B sequences (the nodes of an instance, or the tokens decoded so far) in pages of page_size tokens: token
  * j of sequence b lies in slot j % page_size of page table[b][j / page_size]; lengths[b] tokens are live.  The reference
