@@ -117,6 +117,13 @@ def _documents(doc_q, doc_k, B: int, L: int, M: int, device):
     return ids_q, ids_k
 
 
+def _both(a, b):
+    """Addresses of a pair of side inputs.  An empty tensor has none, and NULL says "not given": nothing of it is read, so the
+    other's stands in."""
+    a, b = ptr(a), ptr(b)
+    return a or b, b or a
+
+
 class _Call:
     """Arguments of one operator call: the tensors the kernels can address, and the ABI struct over them."""
     __slots__ = ("q", "k", "v", "slope", "pos_q", "pos_k", "doc_q", "doc_k", "prefix", "head", "tail", "a", "out", "lse",
@@ -147,8 +154,8 @@ class _Call:
         self.head = (_DTYPES[q.dtype], B, H, K, L, M, D, 1 if causal else 0, D ** -0.5 if scale is None else float(scale), cap,
                      *self.q.stride()[:3], *self.k.stride()[:3], *self.v.stride()[:3])
         pos, doc = self.pos_q is not None, self.doc_q is not None
-        self.tail = (ptr(self.slope), ptr(self.pos_q), ptr(self.pos_k), self.pos_q.stride(0) if pos else 0,
-                     self.pos_k.stride(0) if pos else 0, ptr(self.doc_q), ptr(self.doc_k), self.doc_q.stride(0) if doc else 0,
+        self.tail = (ptr(self.slope), *_both(self.pos_q, self.pos_k), self.pos_q.stride(0) if pos else 0,
+                     self.pos_k.stride(0) if pos else 0, *_both(self.doc_q, self.doc_k), self.doc_q.stride(0) if doc else 0,
                      self.doc_k.stride(0) if doc else 0, ptr(self.prefix))
 
     def set_out(self, out, lse, rest=None):
