@@ -15,7 +15,7 @@ import torch
 
 from . import _lib
 from ._lib import ptr
-from .attention import _DTYPES, _launch, _side
+from .attention import _DTYPES, _launch, _side, no_derivatives
 
 PerRow = Union[float, torch.Tensor]
 _PACK = struct.Struct("@4iPqPq2iPqPq4P4fPqP")
@@ -55,7 +55,11 @@ def process_logits(logits: torch.Tensor, *, blocked: Optional[torch.Tensor] = No
     x = (x > 0 ? x / repetition : x * repetition) - presence - frequency * c.  Then x = (x + bias) / temperature, and -inf
     where bit (a mod ``period``) of ``blocked`` [R, words] is set (``period``: default A; CVRP's direct and via-depot moves
     share N + 1 bits).  log_probs is the log-softmax of what is left, ``selected`` its lowest greatest action (-1 and -inf
-    throughout where all is blocked).  Penalties are numbers or float tensors [R]."""
+    throughout where all is blocked).  Penalties are numbers or float tensors [R].  For decisions: inputs that require grad are
+    refused."""
+    no_derivatives("process_logits", logits=logits, bias=bias,
+                   **{n: x for n, x in (("repetition", repetition), ("presence", presence), ("frequency", frequency))
+                      if isinstance(x, torch.Tensor)})
     if logits.dim() != 2 or logits.dtype not in _DTYPES or not logits.is_cuda:
         raise ValueError(f"logits are {tuple(logits.shape)} {logits.dtype} on {logits.device}: [rows, actions] of float32, "
                          "float16 or bfloat16 on a GPU are expected")
