@@ -363,13 +363,15 @@ class PagedCache:
                               v_pages.data_ptr(), table.data_ptr(), lengths.data_ptr())
 
     # ---- pages of a pool ------------------------------------------------------------------
-    def _pool(self):
+    def _pool(self, sequence: int):
         if self._free is None:
             raise ValueError("the pages of this cache are managed by their owner")
+        if not 0 <= sequence < self.batch:
+            raise ValueError(f"sequence {sequence}: the cache holds {self.batch}")
 
     def reserve(self, sequence: int, tokens: int) -> None:
         """Give ``sequence`` the pages for ``tokens`` tokens (those it has stay)."""
-        self._pool()
+        self._pool(sequence)
         need = (tokens + self.page_size - 1) // self.page_size
         if need > self.table.shape[1]:
             raise ValueError(f"{tokens} tokens: a sequence holds at most {self.table.shape[1] * self.page_size}")
@@ -383,7 +385,7 @@ class PagedCache:
 
     def release(self, sequence: int) -> None:
         """Return the pages of ``sequence`` to the pool; it is empty afterwards."""
-        self._pool()
+        self._pool(sequence)
         self._free.extend(reversed(self._owned[sequence]))
         self._owned[sequence] = []
         self.table[sequence].fill_(-1)
