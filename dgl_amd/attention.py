@@ -396,7 +396,7 @@ class PagedCache:
                start: Optional[torch.Tensor] = None) -> None:
         """Write new tokens [batch, kv heads, tokens, head size] behind each sequence (or from position ``start`` [batch]
         on) and set the lengths to their end.  ``counts`` [batch]: only the first counts[b] of a ragged batch.  Tokens
-        beyond a sequence's pages are dropped.  No gradient passes through a cache: tokens that require one are refused."""
+        beyond a sequence's pages are dropped, and its length ends before the first of them.  No gradient passes through a cache: tokens that require one are refused."""
         no_derivatives("PagedCache.append", k_new=k_new, v_new=v_new)
         with torch.no_grad():
             c = self.struct

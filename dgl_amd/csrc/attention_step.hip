@@ -538,6 +538,20 @@ struct AppendArgs {
     const int *table, *start, *counts;
     int *lengths_out;
 };
+// The length after an append: the end of its tokens, or the first of them whose page is absent.  (A token that was not stored
+// must not count: once the sequence gets the page, whatever lies there would be read as that token.)  Called by whole waves.
+__device__ __forceinline__ int end_of_append(const AppendArgs &a, int b, int first, int count) {
+    const int64_t capacity = (int64_t)a.max_pages << a.shift, stop = (int64_t)first + count;
+    const int lo = max(first, 0), hi = (int)min(stop, capacity);
+    const int lane = threadIdx.x & 63;
+    for (int p = lo >> a.shift; lo < hi && p <= (hi - 1) >> a.shift; p += 64) {
+        const int at = p + lane;
+        const int page = at <= (hi - 1) >> a.shift ? a.table[b * a.ts + at] : 0;
+        const unsigned long long absent = __ballot(page < 0 || page >= a.num_pages);
+        if (absent != 0) return max(lo, (p + __ffsll((long long)absent) - 1) << a.shift);
+    }
+    return (int)max((int64_t)0, min(stop, capacity));
+}
 // `blocks` workgroups per sequence copy 16-byte pieces; one workgroup per sequence may also store the new length (it is
 // the only one that reads the old one)
 __global__ __launch_bounds__(256) void cache_append_kernel(AppendArgs a) {
@@ -545,6 +559,9 @@ __global__ __launch_bounds__(256) void cache_append_kernel(AppendArgs a) {
     const int first = a.start[b];
     const int count = max(0, min(a.counts != nullptr ? a.counts[b] : a.T, a.T));
     const int64_t total = (int64_t)count * a.Hkv * a.pieces;
+    const bool store = a.lengths_out != nullptr && a.blocks == 1;
+    int end = 0;
+    if (store && threadIdx.x < 64) end = end_of_append(a, b, first, count);
     for (int64_t x = (int64_t)part * 256 + threadIdx.x; x < total; x += (int64_t)a.blocks * 256) {
         const int piece = (int)(x % a.pieces), hk = (int)(x / a.pieces % a.Hkv), t = (int)(x / ((int64_t)a.pieces * a.Hkv));
         const int64_t at = (int64_t)first + t;
@@ -557,16 +574,17 @@ __global__ __launch_bounds__(256) void cache_append_kernel(AppendArgs a) {
         *reinterpret_cast<u32x4 *>(a.v + page * a.vs[0] + hk * a.vs[1] + slot * a.vs[2] + 16 * piece) =
             *reinterpret_cast<const u32x4 *>(a.v_new + b * a.vn[0] + hk * a.vn[1] + t * a.vn[2] + 16 * piece);
     }
-    if (a.lengths_out != nullptr && a.blocks == 1) {
+    if (store) {
         __syncthreads();                         // every thread has read the old length
-        if (threadIdx.x == 0) a.lengths_out[b] = (int)max((int64_t)0, min((int64_t)first + count, (int64_t)a.max_pages << a.shift));
+        if (threadIdx.x == 0) a.lengths_out[b] = end;
     }
 }
-__global__ __launch_bounds__(256) void cache_lengths_kernel(AppendArgs a) {
-    const int b = blockIdx.x * 256 + threadIdx.x;
+__global__ __launch_bounds__(256) void cache_lengths_kernel(AppendArgs a) {      // one wave per sequence
+    const int b = blockIdx.x * 4 + (threadIdx.x >> 6);
     if (b >= a.B) return;
     const int count = max(0, min(a.counts != nullptr ? a.counts[b] : a.T, a.T));
-    a.lengths_out[b] = (int)max((int64_t)0, min((int64_t)a.start[b] + count, (int64_t)a.max_pages << a.shift));
+    const int end = end_of_append(a, b, a.start[b], count);
+    if ((threadIdx.x & 63) == 0) a.lengths_out[b] = end;
 }
 
 // ------------------------------------------------------------------------------------------------------------ launch
@@ -714,7 +732,7 @@ extern "C" int dgl_cache_append(const dgl_kv_cache_t *c, const void *k_new, cons
     hipLaunchKernelGGL(cache_append_kernel, dim3((unsigned)(a.B * a.blocks)), dim3(256), 0, (hipStream_t)stream, a);
     DGL_CHECK_LAUNCH("dgl_cache_append");
     if (lengths_out != nullptr && a.blocks > 1) {
-        hipLaunchKernelGGL(cache_lengths_kernel, dim3((a.B + 255) / 256), dim3(256), 0, (hipStream_t)stream, a);
+        hipLaunchKernelGGL(cache_lengths_kernel, dim3((a.B + 3) / 4), dim3(256), 0, (hipStream_t)stream, a);
         DGL_CHECK_LAUNCH("dgl_cache_append (lengths)");
     }
     return DGL_OK;

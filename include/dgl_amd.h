@@ -455,8 +455,9 @@ typedef struct {
 
 /* Writes T new tokens per sequence: token t < counts[b] (NULL: T) of k_new / v_new goes to position start[b] + t (strides in
  * elements {sequence, head, token}).  Positions outside the table's capacity and absent pages are skipped.  lengths_out
- * (may be NULL; may be the array behind `start`) receives start[b] + counts[b], within the capacity.  Beside
- * TSP/TSPModel.py:174-231, whose keys and values are recomputed at every step. */
+ * (may be NULL; may be the array behind `start`) receives start[b] + counts[b], within the capacity, or the first position
+ * among the new ones whose page is absent: what was not stored does not count.  Beside TSP/TSPModel.py:174-231, whose keys and
+ * values are recomputed at every step. */
 DGL_API int dgl_cache_append(const dgl_kv_cache_t *c, const void *k_new, const void *v_new, const int64_t *k_new_stride,
                              const int64_t *v_new_stride, int32_t T, const int32_t *start, const int32_t *counts,
                              int32_t *lengths_out, dgl_stream_t stream);
