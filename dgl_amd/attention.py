@@ -134,6 +134,13 @@ def _documents(doc_q, doc_k, B: int, L: int, M: int, device):
     return ids_q, ids_k
 
 
+def _cap(cap) -> float:
+    cap = float(cap)
+    if not 0.0 <= cap < float("inf") or 0.0 < cap < 2.0 ** -126:       # (what binary32 rounds to 0 would be no cap)
+        raise ValueError(f"cap {cap}: a number >= 0 is expected (0: no cap; else at least 2^-126)")
+    return cap
+
+
 def _both(a, b):
     """Addresses of a pair of side inputs.  An empty tensor has none, and NULL says "not given": nothing of it is read, so the
     other's stands in."""
@@ -151,9 +158,7 @@ class _Call:
         B, H, L, D = q.shape
         _, K, M, _ = k.shape
         dev = q.device
-        cap = float(cap)
-        if not 0.0 <= cap < float("inf"):
-            raise ValueError(f"cap {cap}: a number >= 0 is expected (0: no cap)")
+        cap = _cap(cap)
         if (pos_q is None) != (pos_k is None) or (doc_q is None) != (doc_k is None):
             raise ValueError("coordinates and document ids are given for both sides or for neither")
         if pos_q is not None and slope is None:
@@ -453,7 +458,7 @@ def attention_step(q: torch.Tensor, cache: PagedCache, *, rows_per_instance: int
         bits_stride = blocked.stride(0)
     a = _lib.AttentionStep()
     a.cache = c
-    _PACK_STEP.pack_into(a, _STEP_AT, rows_per_instance, H, D ** -0.5 if scale is None else float(scale), float(cap),
+    _PACK_STEP.pack_into(a, _STEP_AT, rows_per_instance, H, D ** -0.5 if scale is None else float(scale), _cap(cap),
                          *q.stride()[:2], H * D, D, q.data_ptr(), out.data_ptr(), ptr(lse), ptr(slope), ptr(pos_q),
                          ptr(pos_k), pos_stride, n, words, ptr(blocked), bits_stride)
     lib, ref = _lib.load(), ctypes.byref(a)

@@ -1251,7 +1251,7 @@ int check_attention(const dgl_attention_t *p) {
     DGL_CHECK_ARG(p->Hq % p->Hkv == 0, "%d query heads over %d key heads", p->Hq, p->Hkv);
     DGL_CHECK_ARG(p->D >= 8 && p->D <= 128 && p->D % 8 == 0, "head size %d (a multiple of 8, at most 128)", p->D);
     DGL_CHECK_ARG(p->Lq <= DGL_ATTENTION_MAX_LENGTH && p->Lk <= DGL_ATTENTION_MAX_LENGTH, "length above %d", DGL_ATTENTION_MAX_LENGTH);
-    DGL_CHECK_ARG(p->scale == p->scale && p->cap >= 0.0f && p->cap < 3.0e38f, "scale %g, cap %g", (double)p->scale, (double)p->cap);
+    DGL_CHECK_ARG(score_params_fit(p->scale, p->cap), "scale %g, cap %g", (double)p->scale, (double)p->cap);
     DGL_CHECK_ARG((p->pos_q == nullptr) == (p->pos_k == nullptr), "coordinates of one side only");
     DGL_CHECK_ARG(p->pos_q == nullptr || p->slope != nullptr, "coordinates without a slope");
     DGL_CHECK_ARG((p->doc_q == nullptr) == (p->doc_k == nullptr), "document ids of one side only");

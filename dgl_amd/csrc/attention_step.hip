@@ -621,7 +621,7 @@ int check_step(const dgl_attention_step_t *p) {
     if (int e = check_cache(&p->cache)) return e;
     DGL_CHECK_ARG(p->rows_per_instance >= 1 && p->Hq >= 1 && p->Hq % p->cache.Hkv == 0, "rows %d, %d query heads over %d key heads",
                   p->rows_per_instance, p->Hq, p->cache.Hkv);
-    DGL_CHECK_ARG(p->scale == p->scale && p->cap >= 0.0f && p->cap < 3.0e38f, "scale %g, cap %g", (double)p->scale, (double)p->cap);
+    DGL_CHECK_ARG(score_params_fit(p->scale, p->cap), "scale %g, cap %g", (double)p->scale, (double)p->cap);
     DGL_CHECK_ARG(p->q != nullptr && p->out != nullptr, "q or out is NULL");
     DGL_CHECK_ARG((p->pos_q == nullptr) == (p->pos_k == nullptr), "coordinates of one side only");
     DGL_CHECK_ARG(p->pos_q == nullptr || (p->slope != nullptr && p->pos_rows >= 1), "coordinates without a slope or without rows");

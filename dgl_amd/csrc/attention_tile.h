@@ -88,6 +88,12 @@ __device__ __forceinline__ float cap_h(float y2) {
     return fmaf(e, 0.5f, -0.5f) * __builtin_amdgcn_rcpf(e + 1.0f);
 }
 
+// scale, 2 log2(e) scale / cap and the cap itself have to be ordinary binary32 numbers (a cap that underflows would be none)
+inline bool score_params_fit(float scale, float cap) {
+    const float s = scale < 0.0f ? -scale : scale;
+    return s <= 1e38f && (cap == 0.0f || (cap >= 0x1p-126f && cap < 3.0e38f && s / cap <= 1e38f));
+}
+
 // the scalar part of a score, in units of log2
 struct ScoreParams {
     float mul, mul2, cap2, slope2;     // factor of the dot product; 2 log2(e) scale / cap; cap log2(e); slope log2(e)

@@ -371,6 +371,7 @@ DGL_API int dgl_adam_step(float *params, const float *grads, float *exp_avg, flo
  * Query head h reads key head h / (Hq / Hkv).  A masked pair contributes nothing, whatever its operands hold (NaN and
  * infinities included).  Tensors are addressed by strides in elements {batch, head, token}, the head's D elements are
  * consecutive; pointers and strides are multiples of 16 bytes, tokens less than 64 MiB apart, strides may be 0 for inputs.
+ * |scale| and |scale| / cap are at most 1e38, a cap is 0 or at least 2^-126.
  * D is a multiple of 8, at most 128; lengths may be 0 and are at most DGL_ATTENTION_MAX_LENGTH.  Scores, softmax and sums are binary32 for every
  * element type; for the 16-bit types probabilities (and, backward, score gradients) are rounded to the type before they
  * multiply v (k, q, dout). */
