@@ -35,8 +35,10 @@ _STEP_AT = _lib.AttentionStep.rows_per_instance.offset
 assert _PACK_ATTENTION.size == ctypes.sizeof(_lib.Attention) and _PACK_GRAD.size == ctypes.sizeof(_lib.AttentionGrad)
 assert _PACK_CACHE.size == ctypes.sizeof(_lib.KVCache)
 assert _STEP_AT == ctypes.sizeof(_lib.KVCache) and _STEP_AT + _PACK_STEP.size == ctypes.sizeof(_lib.AttentionStep)
-_raw_stream = torch._C._cuda_getCurrentRawStream
-_current_device = torch._C._cuda_getDevice
+# The short ways to the current stream and device are not torch's documented ones (they save 1.2 of a call's 14 us): without them the
+# documented ones serve.
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", lambda index: torch.cuda.current_stream(index).cuda_stream)
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 
 
 def _launch(device, function, *args, what: str) -> None:
