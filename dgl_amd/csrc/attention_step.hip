@@ -640,13 +640,16 @@ int padded_size(int D) { return D <= 16 ? 16 : D <= 32 ? 32 : D <= 64 ? 64 : 128
 struct StepPlan {
     int nq, chunks, splits;
 };
+// the most blocks of 16 queries whose operands and sums fit a wave's registers
+constexpr int most_blocks(int dtype, int DP) { return DP <= 32 ? 4 : DP == 128 && dtype == ATTN_F32 ? 1 : 2; }
 // Queries of one key head are taken 16 NQ at a time (two blocks per wave from 17 queries on, four for small heads from 33
 // on: the cache is read once per chunk).  A sequence is cut so that the workgroups cover the 256 compute units twice, but
 // a range keeps at least four tiles for each of its 8 waves - below that the second launch costs more than it brings.
 StepPlan step_plan(const dgl_attention_step_t *p) {
     StepPlan s;
     const int M = p->rows_per_instance * (p->Hq / p->cache.Hkv), DP = padded_size(p->cache.D);
-    s.nq = M <= 16 || (DP == 128 && p->cache.dtype == DGL_DTYPE_F32) ? 1 : M <= 32 || DP > 32 ? 2 : 4;
+    const int wanted = M <= 16 ? 1 : M <= 32 ? 2 : 4, most_nq = most_blocks(p->cache.dtype, DP);
+    s.nq = wanted < most_nq ? wanted : most_nq;
     s.chunks = (M + 16 * s.nq - 1) / (16 * s.nq);
     const int64_t units = (int64_t)p->cache.B * p->cache.Hkv * s.chunks;
     const int64_t tiles = ((int64_t)p->cache.max_pages * p->cache.page_size + STEP_TILE - 1) / STEP_TILE;
@@ -657,13 +660,14 @@ StepPlan step_plan(const dgl_attention_step_t *p) {
     return s;
 }
 
-template <int T, int DP> int launch_step(const StepArgs &a, int nq, hipStream_t s) {
+template <int T, int DP, int NQ = most_blocks(T, DP)> void launch_blocks(const StepArgs &a, int nq, hipStream_t s) {
+    if constexpr (NQ > 1)
+        if (nq < NQ) return launch_blocks<T, DP, NQ / 2>(a, nq, s);
     const int64_t work = (int64_t)a.B * a.Hkv * a.splits * a.chunks;
-    const dim3 grid((unsigned)((work + 7) / 8 * 8)), block(64 * STEP_WAVES);
-    if (nq == 1) hipLaunchKernelGGL((attn_step_kernel<T, DP, 1>), grid, block, 0, s, a);
-    else if constexpr (DP == 128 && T == ATTN_F32) return dgl_set_error(DGL_ERR_UNSUPPORTED, "no such plan");
-    else if (nq == 2) hipLaunchKernelGGL((attn_step_kernel<T, DP, 2>), grid, block, 0, s, a);
-    else if constexpr (DP <= 32) hipLaunchKernelGGL((attn_step_kernel<T, DP, 4>), grid, block, 0, s, a);
+    hipLaunchKernelGGL((attn_step_kernel<T, DP, NQ>), dim3((unsigned)((work + 7) / 8 * 8)), dim3(64 * STEP_WAVES), 0, s, a);
+}
+template <int T, int DP> int launch_step(const StepArgs &a, int nq, hipStream_t s) {
+    launch_blocks<T, DP>(a, nq, s);
     DGL_CHECK_LAUNCH("dgl_attention_step");
     if (a.splits > 1) {
         const int64_t rows = (int64_t)a.B * a.Hkv * a.M;
