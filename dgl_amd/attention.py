@@ -289,7 +289,7 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, scale: Optio
     ``scale``: default D ** -0.5.  ``cap`` > 0: scores pass through cap tanh(. / cap).  ``slope`` [H]: bias -slope dist,
     between the coordinates ``pos_q`` [B, Lq, 2] and ``pos_k`` [B, Lk, 2], or, without them, between positions
     (|i + Lk - Lq - j|).  ``doc_q`` [B, Lq] / ``doc_k`` [B, Lk]: whole numbers; tokens see their own document, negative ids
-    are padding (such rows give zeros); int64 ids cost three launches of a few microseconds, int32 ones none.  ``causal``: j <= i + Lk - Lq, and in front of ``prefix`` [B] everything.
+    are padding (such rows give zeros); int64 ids are mapped to those in 15 us, int32 ones are taken as they are.  ``causal``: j <= i + Lk - Lq, and in front of ``prefix`` [B] everything.
 
     Under graph capture, leaves that collect gradients are refused: a leaf's accumulation belongs to the stream on which
     it was first used, and a captured backward pass that meets an eager graph of the same leaf ends the process.  Capture

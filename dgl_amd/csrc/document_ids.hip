@@ -4,8 +4,8 @@
 //
 // One hash table per sequence, twice as many slots as keys, probed linearly: the keys' ids go in by compare-and-swap - only
 // from the first token of a run of equal ids, where a first position has to be - and the least position of each by an integer
-// minimum, so the result does not depend on the order.  Then both sides look theirs up.  Three launches of some microseconds, bound
-// by launching at the lengths of a batch; no value returns to the host.
+// minimum, so the result does not depend on the order.  Then both sides look theirs up.  No value returns to the host.  Bound by
+// three launches: 15-16 us a call, from 6000 ids to 64 x 1001 and 200000 on either side.
 #include "common.h"
 
 namespace {
