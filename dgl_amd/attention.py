@@ -53,17 +53,27 @@ def _launch(device, function, *args, what: str) -> None:
         check(code, what)
 
 
+def forward_mode() -> bool:
+    """Inside a dual level, where inputs may have tangents."""
+    return getattr(forward_ad, "_current_level", 0) >= 0
+
+
+def derivatives(*inputs) -> bool:
+    """Whether some input (a tensor or None) may have a gradient or a tangent to pass on: the quick question of every call."""
+    if torch.is_grad_enabled():
+        for t in inputs:
+            if t is not None and t.requires_grad:
+                return True
+    return forward_mode()
+
+
 def no_derivatives(what: str, **inputs) -> None:
     """Refuse inputs whose gradient or tangent the call would drop without a word."""
     if torch.is_grad_enabled():
         for name, t in inputs.items():
             if t is not None and t.requires_grad:
                 raise ValueError(f"{what}: {name} requires grad, but no gradient passes here: detach it, or call under no_grad")
-    no_tangents(what, **inputs)
-
-
-def no_tangents(what: str, **inputs) -> None:
-    if getattr(forward_ad, "_current_level", 0) >= 0:        # (inside a dual level)
+    if forward_mode():
         for name, t in inputs.items():
             if t is not None and forward_ad.unpack_dual(t).tangent is not None:
                 raise ValueError(f"{what}: {name} has a tangent, but forward-mode derivatives do not pass here")
@@ -299,8 +309,10 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, scale: Optio
         if leaves and q.is_cuda and torch.cuda.is_current_stream_capturing():
             raise RuntimeError("attention: a leaf that requires grad inside a graph capture; capture attention_forward "
                                "and attention_backward instead")
-    no_derivatives("attention", pos_q=pos_q, pos_k=pos_k)
-    no_tangents("attention", q=q, k=k, v=v, slope=slope)
+    if derivatives(pos_q, pos_k):
+        no_derivatives("attention", pos_q=pos_q, pos_k=pos_k)
+        with torch.no_grad():                    # (q, k, v and slope: in reverse mode only)
+            no_derivatives("attention", q=q, k=k, v=v, slope=slope)
     if not torch.is_grad_enabled() or not (q.requires_grad or k.requires_grad or v.requires_grad or
                                            (slope is not None and slope.requires_grad)):
         return _forward(_Call(q, k, v, scale, cap, slope, pos_q, pos_k, doc_q, doc_k, causal, prefix), False)[0]
@@ -404,7 +416,8 @@ class PagedCache:
         """Write new tokens [batch, kv heads, tokens, head size] behind each sequence (or from position ``start`` [batch]
         on) and set the lengths to their end.  ``counts`` [batch]: only the first counts[b] of a ragged batch.  Tokens
         beyond a sequence's pages are dropped, and its length ends before the first of them.  No gradient passes through a cache: tokens that require one are refused."""
-        no_derivatives("PagedCache.append", k_new=k_new, v_new=v_new)
+        if derivatives(k_new, v_new):
+            no_derivatives("PagedCache.append", k_new=k_new, v_new=v_new)
         with torch.no_grad():
             c = self.struct
             want = (self.batch, c.Hkv, k_new.shape[2] if k_new.dim() == 4 else -1, c.D)
@@ -428,7 +441,8 @@ def attention_step(q: torch.Tensor, cache: PagedCache, *, rows_per_instance: int
     (n at least the live lengths), or, without them, the distance lengths[b] - 1 - j.  ``blocked`` int64 [R, words]: bit j of
     word j // 64 set = key j is not seen, as the states' visited words.  A row that sees nothing is zeros (lse -inf).  For
     serving: inputs that require grad are refused."""
-    no_derivatives("attention_step", q=q, slope=slope, pos_q=pos_q, pos_k=pos_k)
+    if derivatives(q, slope, pos_q, pos_k):
+        no_derivatives("attention_step", q=q, slope=slope, pos_q=pos_q, pos_k=pos_k)
     c, dev = cache.struct, cache.device
     if q.dim() != 3 or q.shape[0] != cache.batch * rows_per_instance or q.shape[2] != c.D or q.shape[1] % c.Hkv or q.shape[1] < 1:
         raise ValueError(f"q has shape {tuple(q.shape)}: expected [{cache.batch} x {rows_per_instance}, a multiple of {c.Hkv}, {c.D}]")

@@ -15,7 +15,7 @@ import torch
 
 from . import _lib
 from ._lib import ptr
-from .attention import _DTYPES, _launch, _side, no_derivatives
+from .attention import _DTYPES, _launch, _side, derivatives, no_derivatives
 
 PerRow = Union[float, torch.Tensor]
 _PACK = struct.Struct("@4iPqPq2iPqPq4P4fPqP")
@@ -57,9 +57,10 @@ def process_logits(logits: torch.Tensor, *, blocked: Optional[torch.Tensor] = No
     share N + 1 bits).  log_probs is the log-softmax of what is left, ``selected`` its lowest greatest action (-1 and -inf
     throughout where all is blocked).  Penalties are numbers or float tensors [R].  For decisions: inputs that require grad are
     refused."""
-    no_derivatives("process_logits", logits=logits, bias=bias,
-                   **{n: x for n, x in (("repetition", repetition), ("presence", presence), ("frequency", frequency))
-                      if isinstance(x, torch.Tensor)})
+    penalties = [x if isinstance(x, torch.Tensor) else None for x in (repetition, presence, frequency)]
+    if derivatives(logits, bias, *penalties):
+        no_derivatives("process_logits", logits=logits, bias=bias, repetition=penalties[0], presence=penalties[1],
+                       frequency=penalties[2])
     if logits.dim() != 2 or logits.dtype not in _DTYPES or not logits.is_cuda:
         raise ValueError(f"logits are {tuple(logits.shape)} {logits.dtype} on {logits.device}: [rows, actions] of float32, "
                          "float16 or bfloat16 on a GPU are expected")
@@ -89,10 +90,10 @@ def process_logits(logits: torch.Tensor, *, blocked: Optional[torch.Tensor] = No
         history_len = _side(history_len, "history_len", (R,), torch.int32, dev)
         cols, history_stride = history.shape[1], history.stride(0)
     rows, numbers = [], []
-    for name, x, neutral in (("repetition", repetition, 1.0), ("presence", presence, 0.0), ("frequency", frequency, 0.0)):
-        per_row = isinstance(x, torch.Tensor)
-        rows.append(_side(x, name, (R,), torch.float32, dev) if per_row else None)
-        numbers.append(neutral if per_row else float(x))
+    for name, x, t, neutral in (("repetition", repetition, penalties[0], 1.0), ("presence", presence, penalties[1], 0.0),
+                                ("frequency", frequency, penalties[2], 0.0)):
+        rows.append(_side(t, name, (R,), torch.float32, dev))
+        numbers.append(float(x) if t is None else neutral)
     out = torch.empty((R, A), dtype=torch.float32, device=dev)
     selected = torch.empty(R, dtype=torch.int32, device=dev)
     if R == 0:
