@@ -16,15 +16,18 @@
 // carry a NaN or infinity of a masked row into its tile neighbours (0 * NaN), so a result that is not finite at the end is
 // recomputed pair by pair (careful_*), which costs nothing where all is finite.
 //
-// Bound by the issue of vector instructions, not by memory (a head's keys are read by all its row blocks from L2): a pair of
+// Bound by vector instructions, not by memory (a head's keys are read by all its row blocks from L2): a pair of
 // a forward pass takes 18 simple operations and 4 of exp / rcp / sqrt with a cap and coordinates in binary32 (a third of the
 // simple ones split probabilities into terms), 7 and 3 with a cap in 16 bits, and the 16-bit matrix instructions hold the
-// vector unit back for two thirds of their 17 cycles.  Measured, per launch:
-//   forward, 64 x 8 heads of 16, 1000 nodes, cap and coordinates, binary32                447 us  73 TFLOP/s
+// vector unit back for two thirds of their 17 cycles.  Their issue fills the binary32 forward pass (vector unit busy 1.00 of its
+// cycles).  Heads of 128 leave both units free (vector 0.57, matrix 0.26): two waves a SIMD wait for each other's results a third of
+// the time.  The backward kernels and documents have 1.2-1.9 waves a SIMD on average, their blocks being uneven (vector 0.25-0.6,
+// matrix 0.09-0.15).  Measured, per launch:
+//   forward, 64 x 8 heads of 16, 1000 nodes, cap and coordinates, binary32                431 us  76 TFLOP/s
 //   forward, 32 heads over 8 of 128, 8192 causal rows, cap, bf16                           860 us  640 TFLOP/s
 //   2 x 16 heads over 4 of 64, 2047 causal rows behind a prefix, slopes, bf16     forward 71, rows 86, keys 111 + 13 us
-//   8 heads of 64, 6000 rows in 9 documents, fp16                                 forward 88, rows 114, keys 160 us
-//   8 x 8 heads of 16, 1001 rows in 4 documents, cap and coordinates, binary32    forward 89, rows 116, keys 121 us
+//   8 heads of 64, 6000 rows in 9 documents, fp16                                 forward 88, rows 117, keys 162 us
+//   8 x 8 heads of 16, 1001 rows in 4 documents, cap and coordinates, binary32    forward 89, rows 114, keys 120 us
 #include "attention_tile.h"
 
 #include <cfloat>
