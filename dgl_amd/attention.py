@@ -299,7 +299,8 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, scale: Optio
     ``scale``: default D ** -0.5.  ``cap`` > 0: scores pass through cap tanh(. / cap).  ``slope`` [H]: bias -slope dist,
     between the coordinates ``pos_q`` [B, Lq, 2] and ``pos_k`` [B, Lk, 2], or, without them, between positions
     (|i + Lk - Lq - j|).  ``doc_q`` [B, Lq] / ``doc_k`` [B, Lk]: whole numbers; tokens see their own document, negative ids
-    are padding (such rows give zeros); int64 ids are mapped to those in 15 us, int32 ones are taken as they are.  ``causal``: j <= i + Lk - Lq, and in front of ``prefix`` [B] everything.
+    are padding (such rows give zeros); int32 ids are taken as they are, int64 ones mapped to those in 15 us.  ``causal``: j <= i +
+    Lk - Lq, and in front of ``prefix`` [B] everything.
 
     Under graph capture, leaves that collect gradients are refused: a leaf's accumulation belongs to the stream on which
     it was first used, and a captured backward pass that meets an eager graph of the same leaf ends the process.  Capture
@@ -415,7 +416,8 @@ class PagedCache:
                start: Optional[torch.Tensor] = None) -> None:
         """Write new tokens [batch, kv heads, tokens, head size] behind each sequence (or from position ``start`` [batch]
         on) and set the lengths to their end.  ``counts`` [batch]: only the first counts[b] of a ragged batch.  Tokens
-        beyond a sequence's pages are dropped, and its length ends before the first of them.  No gradient passes through a cache: tokens that require one are refused."""
+        beyond a sequence's pages are dropped, and its length ends before the first of them.  No gradient passes through a
+        cache: tokens that require one are refused."""
         if derivatives(k_new, v_new):
             no_derivatives("PagedCache.append", k_new=k_new, v_new=v_new)
         with torch.no_grad():

@@ -160,8 +160,7 @@ LEAST_OFFERED, NOT_OFFERED, LOST = -1e9, -1e25, -1e19
 def controlled_log_probs(engine, controls):
     """Dense log-probabilities [R, A] of the last forward() under a search's controls (dgl_amd/logits.py), and the greedy
     pick per row.  Only actions the policy itself offers can be taken: the feasible ones among the candidates of this decision;
-    all others stay out whatever the controls add.  A row whose controls leave nothing keeps the
-    policy's own probabilities.
+    all others stay out whatever the controls add.  A row whose controls leave nothing keeps the policy's own probabilities.
 
     What is not offered is NOT_OFFERED, so far below everything that is (LEAST_OFFERED at the least) that no sum of a
     hypothesis' values makes up for it: a beam wider than its candidates is filled with hypotheses at or below LOST, which
